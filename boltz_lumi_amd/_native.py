@@ -22,6 +22,9 @@ F32, BF16 = 0, 1
 _P = c_void_p
 _I64P = ctypes.POINTER(c_int64)
 
+_NORM_ROPE = [_P, _P, c_int, _I64P, _I64P, _P, _P, c_int, _P, _P, c_int, _P, c_int, c_int64, c_int, c_float]
+_RELATIVE = [_P, c_int, c_int64, c_int64, _P, _P, c_int] + [c_int64] * 5 + [_P, c_int, c_int]
+
 # name -> (restype, argtypes); mirrors include/bmx.h
 SIGNATURES = {
     "bmx_last_error": (ctypes.c_char_p, []),
@@ -81,6 +84,12 @@ SIGNATURES = {
                                          + [c_int, c_int, c_float, _P, _P, c_size_t, _P]),
     "bmx_seq_attention_x3_batched_split_fwd": (c_int, [_P, _P, _P, _P, _P, _P] + [c_int64] * 10
                                                + [c_int, c_int, c_float, _P, _P, c_size_t, _P]),
+    "bmx_qk_norm_rope_fwd": (c_int, _NORM_ROPE + [_P, _P, _P]),
+    "bmx_qk_norm_rope_workspace_bytes": (c_size_t, [c_int64]),
+    "bmx_qk_norm_rope_bwd": (c_int, _NORM_ROPE + [_P] * 7 + [c_size_t, _P]),
+    "bmx_relative_bias_fwd": (c_int, _RELATIVE + [_P, _P]),
+    "bmx_relative_bias_workspace_bytes": (c_size_t, [c_int] + [c_int64] * 5),
+    "bmx_relative_bias_bwd": (c_int, _RELATIVE + [_P, _P, c_size_t, _P]),
 }
 
 

@@ -1,13 +1,15 @@
 """Torch-facing wrappers of the libbmx C ABI.
 
-Two groups:
+Three groups:
 
 * the reference's native operator set, same names and argument meaning as
   the reference's extension functions (``norm``, ``gate``, ``split``,
   ``pack``, ``silu_mul``, ``epilogue``, ``ordered_softmax``), each raising
   ``RuntimeError`` on bad input like the reference's ``TORCH_CHECK``s;
 * the fused hot-path modules (``trimul``, ``triattn``, ``pair_transition``,
-  ``adaln``) that take a module with Boltz's parameter names.
+  ``adaln``) that take a module with Boltz's parameter names;
+* sequence operators with gradients (``qk_norm_rope``, ``relative_bias``) for
+  an encoder / decoder beside the pair stack.
 
 Every call launches on torch's current stream of the input's device, allocates
 outputs and workspaces through torch's caching allocator and never
@@ -19,8 +21,11 @@ from __future__ import annotations
 
 import ctypes
 import os
+from contextlib import nullcontext
+from functools import lru_cache
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
 
@@ -1140,3 +1145,248 @@ def adaln_modulate(a, scale, shift, eps):
         N.call("bmx_adaln_strided", a.data_ptr(), scale.data_ptr(), shift.data_ptr(), ld, out.data_ptr(),
                _code(a.dtype), rows, d, float(eps), _stream(a))
     return out
+
+
+# ------------------------------------------------------ sequence operators
+#
+# Differentiable (torch.autograd; one backward pass, no double backward).  A
+# call that needs no gradient does not go through autograd.  In a captured
+# graph make the leaves inside or before the capture and take the gradients
+# with torch.autograd.grad, as for torch's own operators.
+
+
+def _at_device(t):
+    """The context a launch on ``t``'s device needs: none on the current device."""
+    return nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+def _needs_grad(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _head_rows(x):
+    """``x`` [B, T, H, D] with a dense last axis, outer strides of multiples of
+    four elements and four-element alignment: itself, or a dense copy."""
+    ok = x.stride(3) == 1 and x.data_ptr() % (4 * x.element_size()) == 0
+    if not ok or any(x.stride(i) % 4 for i in range(3) if x.shape[i] > 1):
+        x = x.contiguous()
+        return x if x.data_ptr() % (4 * x.element_size()) == 0 else x.clone()
+    return x
+
+
+def _strides(x, axes):
+    """Strides of the leading ``axes`` axes; those of single elements, which nothing steps, as 0."""
+    return [x.stride(i) if x.shape[i] > 1 else 0 for i in range(axes)]
+
+
+def _positions(pos, tokens, batch, like, what):
+    """Checked positions: int32 / int64 [tokens] or [batch, tokens], dense; their batch stride."""
+    _check(isinstance(pos, torch.Tensor) and pos.dtype in (torch.int32, torch.int64),
+           f"expected int32 or int64 {what}")
+    _check(pos.shape in ((tokens,), (batch, tokens)), f"expected {what} of shape [tokens] or [batch, tokens]")
+    _cuda(like, pos)
+    pos = pos.contiguous()
+    return pos, tokens if pos.dim() == 2 else 0
+
+
+def _qk_norm_rope_args(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved):
+    b, m, h, d = q.shape
+    n, hk = (k.shape[1], k.shape[2]) if k is not None else (0, 0)
+    q_pos, q_sb = q_pos
+    k_pos, k_sb = k_pos
+    shape = N.int64_array([b, m, n, h, hk, d])
+    strides = N.int64_array(_strides(q, 3) + (_strides(k, 3) if k is not None else [0, 0, 0]) + [q_sb, k_sb])
+    w = q_weight if q_weight is not None else k_weight
+    return (q.data_ptr(), _ptr(k), _code(q.dtype), shape, strides, _ptr(q_weight), _ptr(k_weight),
+            _code(w.dtype if w is not None else q.dtype), _ptr(q_pos), _ptr(k_pos),
+            int(q_pos is not None and q_pos.dtype == torch.int64), _ptr(inv_freq),
+            int(inv_freq is not None and inv_freq.dtype == torch.float64),
+            inv_freq.numel() if inv_freq is not None else 0, int(interleaved), eps)
+
+
+def _qk_norm_rope_fwd(q, k, *args):
+    q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    k_out = torch.empty(k.shape, device=k.device, dtype=k.dtype) if k is not None else None
+    with _at_device(q):
+        N.call("bmx_qk_norm_rope_fwd", *_qk_norm_rope_args(q, k, *args), q_out.data_ptr(), _ptr(k_out), _stream(q))
+    return q_out, k_out
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved):
+        ctx.save_for_backward(q, k, q_weight, k_weight, q_pos[0], k_pos[0], inv_freq)
+        ctx.rest = q_pos[1], k_pos[1], eps, interleaved
+        ctx.set_materialize_grads(False)
+        return _qk_norm_rope_fwd(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k, q_weight, k_weight, q_pos, k_pos, inv_freq = ctx.saved_tensors
+        q_sb, k_sb, eps, interleaved = ctx.rest
+        # A tensor whose result got no gradient takes no part: no tokens of it.
+        q_in, k_in = dq_out is not None, dk_out is not None
+        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if q_in else None
+        dk = torch.empty(k.shape, device=k.device, dtype=k.dtype) if k_in else None
+        dqw = torch.empty_like(q_weight) if q_in and ctx.needs_input_grad[2] else None
+        dkw = torch.empty_like(k_weight) if k_in and ctx.needs_input_grad[3] else None
+        if q_in or k_in:
+            d = q.shape[3]
+            ws = None
+            if dqw is not None or dkw is not None:
+                ws = _workspace(N.lib().bmx_qk_norm_rope_workspace_bytes(d), q.device)
+            args = _qk_norm_rope_args(q if q_in else q[:, :0], k if k_in else None, q_weight, k_weight, (q_pos, q_sb),
+                                      (k_pos, k_sb), inv_freq, eps, interleaved)
+            dq_out = _aligned(dq_out.contiguous()) if q_in else None
+            dk_out = _aligned(dk_out.contiguous()) if k_in else None
+            with _at_device(q):
+                N.call("bmx_qk_norm_rope_bwd", *args, _ptr(dq_out), _ptr(dk_out), _ptr(dq), _ptr(dk), _ptr(dqw),
+                       _ptr(dkw), _ptr(ws), 0 if ws is None else ws.numel(), _stream(q))
+        return dq, dk, dqw, dkw, None, None, None, None, None
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps=1e-6, interleaved=False):
+    """RMS norm of every query and key head and the rotation by position, one
+    pass (``bmx_qk_norm_rope_fwd``): ``R(pos) (x / sqrt(mean(x^2) + eps) * weight)``.
+
+    q [B, M, H, D] and k [B, N, Hk, D] (or None: queries alone) are fp32 or bf16
+    with D a multiple of 8 in [8, 256], in any strides (column slices of one
+    projection are read in place; layouts that the kernel cannot read are
+    copied).  Weights are [D] fp32 or in q's type, or None.  q_pos [M] or
+    [B, M] and k_pos [N] or [B, N] are int32 / int64.  inv_freq (fp32 / fp64,
+    a multiple of 4 of at most D / 2 values) turns channels (i, R + i) by
+    ``pos * inv_freq[i]``, R = len(inv_freq) (``interleaved``: channels
+    (2 i, 2 i + 1)); channels past 2 R are only normalised.  With inv_freq None
+    nothing turns and the positions may be None.  Returns dense (q', k');
+    gradients reach q, k and the weights."""
+    _check(q.dim() == 4 and (k is None or k.dim() == 4), "expected q and k of shape [B, tokens, heads, D]")
+    _cuda(q, *(t for t in (k, q_weight, k_weight, inv_freq) if t is not None))
+    b, m, _, d = q.shape
+    _code(q.dtype)
+    _check(8 <= d <= 256 and d % 8 == 0, "head dim must be a multiple of 8 in [8, 256]")
+    _check(k is None or (k.shape[0] == b and k.shape[3] == d and k.dtype == q.dtype),
+           "k must match q's batch, head dim and dtype")
+    _check(k is not None or k_weight is None, "k_weight needs k")
+    for w in (q_weight, k_weight):
+        _check(w is None or (w.shape == (d,) and w.dtype in (torch.float32, q.dtype)),
+               "expected weights of [D] in fp32 or q's dtype")
+    _check(q_weight is None or k_weight is None or q_weight.dtype == k_weight.dtype, "the weights must share a dtype")
+    _check(eps > 0, "eps must be positive")
+    if inv_freq is None:
+        q_pos, k_pos = (None, 0), (None, 0)
+    else:
+        _check(inv_freq.dim() == 1 and inv_freq.dtype in (torch.float32, torch.float64) and inv_freq.numel() > 0
+               and inv_freq.numel() % 4 == 0 and 2 * inv_freq.numel() <= d,
+               "expected fp32 or fp64 inv_freq, a multiple of 4 of at most D / 2 values")
+        _check(not inv_freq.requires_grad, "inv_freq takes no gradient")
+        inv_freq = inv_freq.contiguous()
+        q_pos = _positions(q_pos, m, b, q, "q_pos")
+        k_pos = _positions(k_pos, k.shape[1], b, q, "k_pos") if k is not None else (None, 0)
+        _check(k is None or q_pos[0].dtype == k_pos[0].dtype, "the positions must share a dtype")
+    q_weight, k_weight = (None if w is None else _aligned(w.contiguous()) for w in (q_weight, k_weight))
+    q, k = _head_rows(q), None if k is None else _head_rows(k)
+    args = (q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, float(eps), bool(interleaved))
+    return _QkNormRope.apply(*args) if _needs_grad(q, k, q_weight, k_weight) else _qk_norm_rope_fwd(*args)
+
+
+@lru_cache(maxsize=64)
+def _relative_thresholds(side, exact, max_distance):
+    """Least distances of buckets 1 .. side - 1 of one direction (whole numbers,
+    no logarithm): i for i <= exact, then the least n with
+    ``(n / exact)^steps >= (max_distance / exact)^k``, steps = side - exact."""
+    steps, edges = side - exact, list(range(1, exact + 1))
+    for k in range(1, steps):
+        reach = exact ** (steps - k) * max_distance ** k
+        lo, hi = edges[-1], max_distance  # max_distance itself satisfies every k < steps
+        while lo < hi:
+            mid = (lo + hi) // 2
+            lo, hi = (lo, mid) if mid ** steps >= reach else (mid + 1, hi)
+        edges.append(lo)
+    return (ctypes.c_int32 * len(edges))(*edges)
+
+
+def _relative_args(data, buckets, heads, q_pos, k_pos, batch, thresholds, bidirectional):
+    (q_pos, q_sb), (k_pos, k_sb) = q_pos, k_pos
+    return (data.data_ptr(), _code(data.dtype), buckets, heads, q_pos.data_ptr(), k_pos.data_ptr(),
+            int(q_pos.dtype == torch.int64), 1 if batch is None else batch, q_pos.shape[-1], k_pos.shape[-1], q_sb, k_sb, thresholds,
+            len(thresholds), int(bidirectional))
+
+
+def _relative_bias_fwd(table, q_pos, k_pos, batch, thresholds, bidirectional):
+    buckets, heads = table.shape
+    shape = (heads, q_pos[0].shape[-1], k_pos[0].shape[-1])
+    out = torch.empty(shape if batch is None else (batch, *shape), device=table.device, dtype=table.dtype)
+    if out.numel():
+        with _at_device(table):
+            N.call("bmx_relative_bias_fwd", *_relative_args(table, buckets, heads, q_pos, k_pos, batch, thresholds,
+                                                            bidirectional), out.data_ptr(), _stream(table))
+    return out
+
+
+class _RelativeBias(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, table, q_pos, k_pos, batch, thresholds, bidirectional):
+        ctx.save_for_backward(q_pos[0], k_pos[0])
+        ctx.rest = table.shape, q_pos[1], k_pos[1], batch, thresholds, bidirectional
+        return _relative_bias_fwd(table, q_pos, k_pos, batch, thresholds, bidirectional)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dbias):
+        q_pos, k_pos = ctx.saved_tensors
+        (buckets, heads), q_sb, k_sb, batch, thresholds, bidirectional = ctx.rest
+        dbias = dbias.contiguous()
+        dtable = torch.empty(buckets, heads, device=dbias.device, dtype=dbias.dtype)
+        args = _relative_args(dbias, buckets, heads, (q_pos, q_sb), (k_pos, k_sb), batch, thresholds, bidirectional)
+        m, n = q_pos.shape[-1], k_pos.shape[-1]
+        ws = _workspace(N.lib().bmx_relative_bias_workspace_bytes(_code(dbias.dtype), buckets, heads, args[7], m, n),
+                        dbias.device)
+        with _at_device(dbias):
+            N.call("bmx_relative_bias_bwd", *args, dtable.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dbias))
+        return dtable, None, None, None, None, None
+
+
+MAX_BUCKETS = 256
+
+
+def relative_bias(table, q_pos, k_pos, exact=None, max_distance=128, bidirectional=True):
+    """Learned relative-position bias (``bmx_relative_bias_fwd``):
+    ``bias[h, i, j] = table[bucket(k_pos[j] - q_pos[i]), h]``, [H, M, N] (or
+    [B, H, M, N] where a position tensor has a batch axis), dense, in the type
+    of ``table`` [buckets, H] (fp32 or bf16): the additive bias of
+    ``cross_attention`` or ``seq_attention``.
+
+    Bidirectional, half of the buckets (``side``) hold d <= 0 and half d > 0,
+    by n = |d|; otherwise all hold n = max(-d, 0).  Distances below ``exact``
+    (default side // 2) have a bucket each; the others share the rest by
+    logarithm, ``exact + floor(log(n / exact) / log(max_distance / exact) *
+    (side - exact))``, the last from ``max_distance`` on.  ``exact = side - 1``
+    is the clipped form (every distance its own bucket up to side - 1).
+    Positions are int32 / int64, |pos| < 2^62, in any order.  The gradient
+    reaches the table (fp32 sums, the same bits on every run)."""
+    _check(table.dim() == 2 and table.shape[0] > 0 and table.shape[1] > 0, "expected a [buckets, heads] table")
+    _cuda(table)
+    _code(table.dtype)
+    buckets, heads = table.shape
+    _check(buckets <= MAX_BUCKETS and heads <= 65535, "at most 256 buckets and 65535 heads")
+    _check(not bidirectional or buckets % 2 == 0, "bidirectional buckets must be even in number")
+    side = buckets // 2 if bidirectional else buckets
+    _check(side >= 2, "expected at least two buckets a direction")
+    exact = side // 2 if exact is None else int(exact)
+    _check(1 <= exact < side, "exact must be in [1, buckets of a direction)")
+    if exact == side - 1:
+        max_distance = side - 1  # nothing is shared by logarithm
+    _check(exact == side - 1 or exact < max_distance <= 1 << 30, "max_distance must be above exact, at most 2^30")
+    _check(q_pos.dim() in (1, 2) and k_pos.dim() in (1, 2), "expected positions [tokens] or [batch, tokens]")
+    batch = next((p.shape[0] for p in (q_pos, k_pos) if p.dim() == 2), None)
+    q_pos = _positions(q_pos, q_pos.shape[-1], batch, table, "q_pos")
+    k_pos = _positions(k_pos, k_pos.shape[-1], batch, table, "k_pos")
+    _check(q_pos[0].dtype == k_pos[0].dtype, "the positions must share a dtype")
+    args = (table.contiguous(), q_pos, k_pos, batch, _relative_thresholds(side, exact, int(max_distance)),
+            bool(bidirectional))
+    return _RelativeBias.apply(*args) if _needs_grad(table) else _relative_bias_fwd(*args)

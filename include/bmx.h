@@ -401,6 +401,51 @@ int bmx_seq_attention_x3_batched_split_fwd(const float* q, const float* k, const
                                            void* out_op, void* workspace, size_t workspace_bytes,
                                            bmx_stream_t stream);
 
+/* ---- Sequence operators, with their gradients ----------------------------
+ * No reference kernel (the reference is inference only): what a sequence encoder / decoder beside
+ * the pair stack needs.  Strides are in elements.  A gradient pointer may be NULL: not computed.
+ * Results do not depend on atomics' order. */
+
+/* y = R(pos) (x / sqrt(mean(x^2) + eps) * weight) for every head vector x of q [batch, m, heads, dim]
+ * and k [batch, n, kv_heads, dim].  shape = {batch, m, n, heads, kv_heads, dim}; strides = {q's batch,
+ * token, head; k's; q_pos's and k_pos's batch stride (0: shared)}, the last axis dense; x strides
+ * multiples of 4.  R turns the channel pairs (i, half + i) (interleaved: (2 i, 2 i + 1)), i < half, by
+ * pos * inv_freq[i] (product in 64 bits); other channels pass.  dim a multiple of 8 in [8, 256],
+ * half of 4.  Weights [dim] in w_dtype or NULL (1); positions int32 / int64 [m] / [n] per batch element;
+ * inv_freq fp32 / fp64 [half].  Outputs and gradients dense.  Tensors aligned to 4 elements, weights
+ * to 16 bytes.  n or m may be 0.  No reference kernel. */
+int bmx_qk_norm_rope_fwd(const void* q, const void* k, int dtype, const int64_t* shape, const int64_t* strides,
+                         const void* q_weight, const void* k_weight, int w_dtype, const void* q_pos, const void* k_pos,
+                         int pos64, const void* inv_freq, int inv_freq64, int64_t half, int interleaved, float eps,
+                         void* q_out, void* k_out, bmx_stream_t stream);
+
+/* Gradients of bmx_qk_norm_rope_fwd from dq_out / dk_out (dense).  dq and dk are written whole;
+ * dq_weight / dk_weight [dim] in w_dtype or NULL; workspace (needed for a weight gradient):
+ * bmx_qk_norm_rope_workspace_bytes(dim).  No reference kernel. */
+size_t bmx_qk_norm_rope_workspace_bytes(int64_t dim);
+int bmx_qk_norm_rope_bwd(const void* q, const void* k, int dtype, const int64_t* shape, const int64_t* strides,
+                         const void* q_weight, const void* k_weight, int w_dtype, const void* q_pos, const void* k_pos,
+                         int pos64, const void* inv_freq, int inv_freq64, int64_t half, int interleaved, float eps,
+                         const void* dq_out, const void* dk_out, void* dq, void* dk, void* dq_weight, void* dk_weight,
+                         void* workspace, size_t workspace_bytes, bmx_stream_t stream);
+
+/* out[b][h][i][j] = table[c][h], c the bucket of d = k_pos[b][j] - q_pos[b][i]: the number of
+ * thresholds (host array, count of them, rising) that are <= n, where n = max(-d, 0), or, bidirectional,
+ * n = |d| with count + 1 added for d > 0.  table [buckets][heads] dense, buckets = count + 1 (twice that
+ * when bidirectional) <= 256; positions int32 / int64 at batch strides q_sb / k_sb (0: shared), |pos| <
+ * 2^62; out dense.  Element copies: exact.  No reference kernel. */
+int bmx_relative_bias_fwd(const void* table, int dtype, int64_t buckets, int64_t heads, const void* q_pos,
+                          const void* k_pos, int pos64, int64_t batch, int64_t m, int64_t n, int64_t q_sb, int64_t k_sb,
+                          const int32_t* thresholds, int count, int bidirectional, void* out, bmx_stream_t stream);
+
+/* dtable[c][h] = sum of dbias[b][h][i][j] (dense) over the (b, i, j) of bucket c, fp32 sums in a
+ * fixed order; workspace: bmx_relative_bias_workspace_bytes.  No reference kernel. */
+size_t bmx_relative_bias_workspace_bytes(int dtype, int64_t buckets, int64_t heads, int64_t batch, int64_t m, int64_t n);
+int bmx_relative_bias_bwd(const void* dbias, int dtype, int64_t buckets, int64_t heads, const void* q_pos,
+                          const void* k_pos, int pos64, int64_t batch, int64_t m, int64_t n, int64_t q_sb, int64_t k_sb,
+                          const int32_t* thresholds, int count, int bidirectional, void* dtable, void* workspace,
+                          size_t workspace_bytes, bmx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
