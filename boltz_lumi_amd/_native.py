@@ -24,6 +24,7 @@ _I64P = ctypes.POINTER(c_int64)
 
 _NORM_ROPE = [_P, _P, c_int, _I64P, _I64P, _P, _P, c_int, _P, _P, c_int, _P, c_int, c_int64, c_int, c_float]
 _RELATIVE = [_P, c_int, c_int64, c_int64, _P, _P, c_int] + [c_int64] * 5 + [_P, c_int, c_int]
+_CROSS = [_P, _P, _P, _P, _P, c_int, _I64P, _I64P, c_float]
 
 # name -> (restype, argtypes); mirrors include/bmx.h
 SIGNATURES = {
@@ -90,6 +91,10 @@ SIGNATURES = {
     "bmx_relative_bias_fwd": (c_int, _RELATIVE + [_P, _P]),
     "bmx_relative_bias_workspace_bytes": (c_size_t, [c_int] + [c_int64] * 5),
     "bmx_relative_bias_bwd": (c_int, _RELATIVE + [_P, _P, c_size_t, _P]),
+    "bmx_cross_attention_workspace_bytes": (c_size_t, [c_int] + [c_int64] * 6),
+    "bmx_cross_attention_fwd": (c_int, _CROSS + [_P, _P, _P, _P, c_size_t, _P]),
+    "bmx_cross_attention_bwd_workspace_bytes": (c_size_t, [c_int64] * 3),
+    "bmx_cross_attention_bwd": (c_int, _CROSS + [_P] * 8 + [_I64P, _P, c_size_t, _P]),
 }
 
 

@@ -1,0 +1,447 @@
+// Softmax attention of one sequence's queries over another's keys and values,
+// with a key mask, an additive bias and key / value heads shared by groups of
+// query heads (bf16 or fp32, head dims up to 128).
+//
+//   S = scale q k^T + bias, masked keys left out;  out = softmax(S) v
+//
+// One pass over the keys with a running maximum and sum (fp32).  A wave holds 32 query
+// rows: S^T = K Q^T puts a query in a lane, so maximum and sum are one lane's
+// registers plus one exchange between the halves, and the weights in registers are the next product's
+// operand as they stand (out^T += V^T P^T, V read transposed from LDS).  The
+// weights are rounded to the operand's type, and their sum is taken over the rounded values, so a row's
+// weights add up to one: the error is a rounding of each weight against the others.
+//
+// A row without keys (masked, or -inf bias throughout) gives zeros.
+#include "cross_attention.h"
+
+using namespace bmx;
+
+namespace {
+
+// State of a wave's 32 rows: lane l holds row l % 32, in both halves.
+template <typename T, int DP>
+struct Rows {
+  RowOperand<T, DP> q;
+  f32x16 o[DP / 32];
+  float top, sum;  // running maximum (of S, or of q k^T without a bias); this half's share of the sum
+  const T* bias;
+
+  __device__ __forceinline__ void init(const CrossArgs& a, int64_t b, int c, int row) {
+    const int r = min(row, a.rows - 1), g = r / (int)a.m, i = r - g * (int)a.m;
+    const int64_t head = (int64_t)c * a.group + g;
+    q.load((const T*)a.q + b * a.sq[0] + i * a.sq[1] + head * a.sq[2], a.dim, lane_id() >> 5);
+    bias = (const T*)a.bias + b * a.sb[0] + head * a.sb[1] + i * a.sb[2];
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();
+    top = -INFINITY, sum = 0.f;
+  }
+
+  // NB times 32 keys: rows row0 .. of the tiles, keys `key` .. of the sequence, presence bits.
+  template <int NB, bool kBias>
+  __device__ __forceinline__ void attend(const CrossArgs& a, const char* kt, const char* vt, int64_t key, uint64_t bits) {
+    f32x16 s[NB];
+#pragma unroll
+    for (int u = 0; u < NB; ++u) s[u] = product<T, DP>(kt, 32 * u, q, zero16());
+    if (kBias) {
+#pragma unroll
+      for (int u = 0; u < NB; ++u) {
+        // A tail sub-tile may lie past the last key altogether.
+        const f32x16 b = bias_tile(bias, min(key + 32 * u, a.n - 1), a.n);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[u][r] = s[u][r] * a.scale + b[r];
+      }
+    }
+    const uint64_t all = NB == 2 ? ~0ull : 0xffffffffull;
+    if (bits != all) {
+      const uint64_t mine = bits >> (4 * (lane_id() >> 5));
+#pragma unroll
+      for (int u = 0; u < NB; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!key_bit((uint32_t)(mine >> (32 * u)), r)) s[u][r] = -INFINITY;
+    }
+    float mx = s[0][0];
+#pragma unroll
+    for (int u = 0; u < NB; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
+    mx = fmaxf(halves_max(mx), top);
+    // Without a bias the logits stay unscaled; with one they are in natural units and the difference is taken
+    // before the change to base 2, so that biases of the type's lowest value do not overflow. fp32 takes
+    // the difference first too: the largest logit's weight is then exactly 1 (bf16 rounds it to 1).
+    constexpr bool kFirst = kBias || sizeof(T) == 4;
+    const float c = (kBias ? 1.f : a.scale) * kLog2E;
+    const float base = mx == -INFINITY ? 0.f : mx;
+    if (__any(mx > top)) {
+      const float f = __builtin_amdgcn_exp2f((top - base) * c);
+      sum *= f;
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt) o[dt] *= f;
+      top = mx;
+    }
+    const float shift = -base * c;
+#pragma unroll
+    for (int u = 0; u < NB; ++u) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[u][r] = __builtin_amdgcn_exp2f(kFirst ? (s[u][r] - base) * c : s[u][r] * c + shift);
+      Weights<T> w;
+      w.set(s[u]);
+      sum = w.sum(sum);
+      transposed_product<DP>(vt, 32 * u, w, o);
+    }
+  }
+};
+
+// Four channels of a row, rounded; and what the rounding left, for the gradient's row sums.
+template <typename T>
+__device__ __forceinline__ void store_out(const CrossArgs& a, int64_t at, f32x4 v);
+template <>
+__device__ __forceinline__ void store_out<bf16>(const CrossArgs& a, int64_t at, f32x4 v) {
+  bf16x4 hi, lo;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    hi[e] = (bf16)v[e];
+    lo[e] = (bf16)(v[e] - (float)hi[e]);
+  }
+  *(bf16x4*)((bf16*)a.out + at) = hi;
+  if (a.out_lo) *(bf16x4*)((bf16*)a.out_lo + at) = lo;
+}
+template <>
+__device__ __forceinline__ void store_out<float>(const CrossArgs& a, int64_t at, f32x4 v) {
+  *(f32x4*)((float*)a.out + at) = v;
+}
+
+// Row maximum in natural units and log2 of the sum; a row without keys gets weights exp2(-inf) = 0.
+__device__ __forceinline__ float2 row_stats(const CrossArgs& a, float top, float sum, bool bias) {
+  if (!(sum != 0.f) || top == -INFINITY) return make_float2(0.f, INFINITY);
+  return make_float2(bias ? top : top * a.scale, __builtin_amdgcn_logf(sum));
+}
+
+// The lane's row of a wave's result: to out (and stats), or as a partial sum of its split.
+template <typename T, int DP>
+__device__ __forceinline__ void write_rows(const CrossArgs& a, int64_t b, int c, int split, int row,
+                                           const f32x16 (&o)[DP / 32], float top, float sum, bool bias) {
+  if (row >= a.rows) return;
+  const int h = lane_id() >> 5;
+  if (a.splits > 1) {
+    const int64_t at = ((int64_t)split * a.batch * a.kv_heads + b * a.kv_heads + c) * a.rows + row;
+    if (h == 0) a.part_ml[at] = make_float2(top, sum);
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = 32 * dt + 8 * g + 4 * h;
+        if (d < a.dim)
+          *(f32x4*)(a.part_o + at * a.dim + d) = f32x4{o[dt][4 * g], o[dt][4 * g + 1], o[dt][4 * g + 2], o[dt][4 * g + 3]};
+      }
+    return;
+  }
+  const int g0 = row / (int)a.m, i = row - g0 * (int)a.m;
+  const int64_t head = (int64_t)c * a.group + g0;
+  const int64_t at = ((b * a.m + i) * a.heads + head) * a.dim;
+  const bool none = top == -INFINITY;
+  const float f = none ? 0.f : 1.f / sum;
+  if (a.stats && h == 0) a.stats[(b * a.heads + head) * a.m + i] = row_stats(a, top, sum, bias);
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = 32 * dt + 8 * g + 4 * h;
+      f32x4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = none ? 0.f : o[dt][4 * g + e] * f;
+      if (d < a.dim) store_out<T>(a, at + d, v);
+    }
+}
+
+// Position of a block: row block, split, key head, batch element.
+struct Place {
+  int row_block, split, c;
+  int64_t b, first, stop;  // keys of the split
+  __device__ __forceinline__ Place(const CrossArgs& a) {
+    int64_t at = xcd_position(blockIdx.x, gridDim.x);
+    row_block = (int)(at % a.row_blocks), at /= a.row_blocks;
+    split = (int)(at % a.splits), at /= a.splits;
+    c = (int)(at % a.kv_heads), b = at / a.kv_heads;
+    first = split * a.split_keys;
+    stop = min(first + a.split_keys, a.n);
+  }
+};
+
+template <typename T>
+constexpr int kWideKeys = sizeof(T) == 2 ? 64 : 32;
+
+// Many rows: four waves of 32 rows share a tile of keys, staged through registers into two LDS buffers: while a
+// tile is attended the next one's loads are in flight, one barrier per tile. Tiles without a present key are
+// passed over.
+template <typename T, int DP, bool kBias>
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_wide(CrossArgs a) {
+  constexpr int KT = kWideKeys<T>, kTile = KT * Tile<T, DP>::kRowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[4 * kTile + kMaskChunk / 8];
+  const Place p(a);
+  const int t = threadIdx.x, row = p.row_block * 128 + (t >> 6) * 32 + (t & 31);
+  Rows<T, DP> rows;
+  rows.init(a, p.b, p.c, row);
+  const T* k = (const T*)a.k + p.b * a.sk[0] + p.c * a.sk[2];
+  const T* v = (const T*)a.v + p.b * a.sv[0] + p.c * a.sv[2];
+  KeyWords words{(uint64_t*)(lds + 4 * kTile), a.mask ? a.mask + p.b * a.smask : nullptr};
+  Stage<T, DP, KT, 256> sk, sv;
+  int buf = 0;
+  for (int64_t c0 = p.first; c0 < p.stop; c0 += kMaskChunk) {
+    words.fill(c0, p.stop);
+    const int64_t end = min(c0 + kMaskChunk, p.stop);
+    auto next = [&](int64_t key) {
+      while (key < end && words.bits(key, KT) == 0) key += KT;
+      return key;
+    };
+    auto load = [&](int64_t key) {
+      sk.load(t, a.dim, [&](int r) { return k + min(key + r, a.n - 1) * a.sk[1]; });
+      sv.load(t, a.dim, [&](int r) { return v + min(key + r, a.n - 1) * a.sv[1]; });
+    };
+    int64_t key = next(c0);
+    if (key < end) load(key);
+    while (key < end) {
+      const uint64_t bits = words.bits(key, KT);
+      char* kt = lds + buf * 2 * kTile;
+      auto live = [&](int r) { return (bits >> r) & 1; };
+      sk.store(t, a.dim, kt, live);
+      sv.store(t, a.dim, kt + kTile, live);
+      const int64_t after = next(key + KT);
+      if (after < end) load(after);
+      __syncthreads();
+      rows.template attend<KT / 32, kBias>(a, kt, kt + kTile, key, bits);
+      buf ^= 1, key = after;
+    }
+  }
+  write_rows<T, DP>(a, p.b, p.c, p.split, row, rows.o, rows.top, halves_sum(rows.sum), kBias);
+}
+
+// Up to 32 rows (a decoding step): the four waves take 32 keys in turn, each through a tile of its own without
+// barriers, so every wave keeps its next 32 keys' loads in flight, and merge their sums at the end. The bound
+// is the read of the keys and values.
+template <typename T, int DP, bool kBias>
+__global__ __launch_bounds__(256) void cross_attention_few(CrossArgs a) {
+  constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[8 * kTile + kMaskChunk / 8 + 4 * 32 * 4];
+  const Place p(a);
+  const int t = threadIdx.x, w = t >> 6, l = t & 63, row = l & 31;
+  Rows<T, DP> rows;
+  rows.init(a, p.b, p.c, row);
+  const T* k = (const T*)a.k + p.b * a.sk[0] + p.c * a.sk[2];
+  const T* v = (const T*)a.v + p.b * a.sv[0] + p.c * a.sv[2];
+  char* kt = lds + w * 2 * kTile;
+  KeyWords words{(uint64_t*)(lds + 8 * kTile), a.mask ? a.mask + p.b * a.smask : nullptr};
+  Stage<T, DP, 32, 64> sk, sv;
+  for (int64_t c0 = p.first; c0 < p.stop; c0 += kMaskChunk) {
+    words.fill(c0, p.stop);
+    const int64_t end = min(c0 + kMaskChunk, p.stop);
+    auto next = [&](int64_t key) {
+      while (key < end && words.bits(key, 32) == 0) key += 128;
+      return key;
+    };
+    auto load = [&](int64_t key) {
+      sk.load(l, a.dim, [&](int r) { return k + min(key + r, a.n - 1) * a.sk[1]; });
+      sv.load(l, a.dim, [&](int r) { return v + min(key + r, a.n - 1) * a.sv[1]; });
+    };
+    int64_t key = next(c0 + 32 * w);
+    if (key < end) load(key);
+    while (key < end) {
+      const uint64_t bits = words.bits(key, 32);
+      auto live = [&](int r) { return (bits >> r) & 1; };
+      sk.store(l, a.dim, kt, live);
+      sv.store(l, a.dim, kt + kTile, live);
+      const int64_t after = next(key + 128);
+      if (after < end) load(after);
+      wave_order();
+      rows.template attend<1, kBias>(a, kt, kt + kTile, key, bits);
+      wave_order();
+      key = after;
+    }
+  }
+  // Merge: the common maximum, then the waves' sums and outputs added in order.
+  float* ml = (float*)(lds + 8 * kTile + kMaskChunk / 8);  // [4][32] maxima
+  float sum = halves_sum(rows.sum);
+  if (l < 32) ml[w * 32 + row] = rows.top;
+  __syncthreads();  // also: every wave is done with its tiles
+  float top = ml[row];
+#pragma unroll
+  for (int i = 1; i < 4; ++i) top = fmaxf(top, ml[i * 32 + row]);
+  const float c = (kBias ? 1.f : a.scale) * kLog2E, base = top == -INFINITY ? 0.f : top;
+  const float f = __builtin_amdgcn_exp2f((rows.top - base) * c);  // 0 for a wave without keys
+  sum *= f;
+#pragma unroll
+  for (int dt = 0; dt < DP / 32; ++dt) rows.o[dt] *= f;
+  // Waves 1 .. 3 leave [register][lane] values; wave 0 adds them.
+  float* part = (float*)lds;
+  constexpr int kPart = (DP / 2 + 1) * 64;
+  static_assert(3 * kPart * 4 <= 8 * kTile, "the merge fits the tiles");
+  if (w > 0) {
+    float* mine = part + (w - 1) * kPart;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mine[(16 * dt + r) * 64 + l] = rows.o[dt][r];
+    mine[(DP / 2) * 64 + l] = sum;
+  }
+  __syncthreads();
+  if (w > 0) return;
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const float* other = part + i * kPart;
+#pragma unroll
+    for (int dt = 0; dt < DP / 32; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) rows.o[dt][r] += other[(16 * dt + r) * 64 + l];
+    sum += other[(DP / 2) * 64 + l];
+  }
+  write_rows<T, DP>(a, p.b, p.c, p.split, row, rows.o, top, sum, kBias);
+}
+
+// Joins the splits: a thread per four channels of a row.
+template <typename T>
+__global__ __launch_bounds__(256) void cross_attention_join(CrossArgs a, int bias) {
+  const int quads = a.dim / 4;
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x, lists = a.batch * a.kv_heads;
+  const int64_t at = id / quads;  // (batch, key head, row)
+  if (at >= lists * a.rows) return;
+  const int d = (int)(id - at * quads) * 4;
+  const int64_t step = lists * a.rows;
+  float top = -INFINITY;
+  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[s * step + at].x);
+  const float c = (bias ? 1.f : a.scale) * kLog2E, base = top == -INFINITY ? 0.f : top;
+  float sum = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 ml = a.part_ml[s * step + at];
+    const float f = __builtin_amdgcn_exp2f((ml.x - base) * c);
+    sum += ml.y * f;
+    o += *(const f32x4*)(a.part_o + (s * step + at) * a.dim + d) * f;
+  }
+  const int64_t list = at / a.rows, b = list / a.kv_heads;
+  const int row = (int)(at - list * a.rows), g = row / (int)a.m, i = row - g * (int)a.m;
+  const int64_t head = (list - b * a.kv_heads) * a.group + g;
+  const bool none = top == -INFINITY;
+  if (a.stats && d == 0) a.stats[(b * a.heads + head) * a.m + i] = row_stats(a, top, sum, bias);
+  const float f = none ? 0.f : 1.f / sum;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = none ? 0.f : o[e] * f;
+  store_out<T>(a, ((b * a.m + i) * a.heads + head) * a.dim + d, o);
+}
+
+struct Split {
+  bool few;
+  int row_blocks, splits;
+  int64_t keys;  // per split, a multiple of 128
+};
+
+// Few rows run as many splits as give every compute unit two blocks, each of at least 128 keys (one tile a wave); many rows
+// split only where their blocks leave compute units idle.
+Split plan(int dtype, int64_t batch, int64_t kv_heads, int64_t rows, int64_t n) {
+  Split s;
+  s.few = rows <= 32;
+  s.row_blocks = s.few ? 1 : (int)((rows + 127) / 128);
+  const int64_t blocks = (int64_t)s.row_blocks * batch * kv_heads, least = s.few ? 128 : 256;
+  const int64_t want = s.few ? 512 : 256;
+  int64_t splits = blocks ? want / blocks : 1;
+  const int64_t most = (n + least - 1) / least;
+  splits = splits < 1 ? 1 : splits > most ? (most > 0 ? most : 1) : splits;
+  s.keys = ((n + splits - 1) / splits + 127) / 128 * 128;
+  if (s.keys == 0) s.keys = 128;
+  s.splits = (int)(n > 0 ? (n + s.keys - 1) / s.keys : 1);
+  return s;
+}
+
+template <typename T, int DP, bool kBias>
+void launch(const CrossArgs& a, bool few, hipStream_t stream) {
+  const dim3 grid((unsigned)((int64_t)a.row_blocks * a.splits * a.kv_heads * a.batch));
+  if (few)
+    cross_attention_few<T, DP, kBias><<<grid, 256, 0, stream>>>(a);
+  else
+    cross_attention_wide<T, DP, kBias><<<grid, 256, 0, stream>>>(a);
+}
+
+template <typename T>
+void launch_dim(const CrossArgs& a, bool few, hipStream_t stream) {
+  const int dp = (a.dim + 31) / 32;
+  if (a.bias) {
+    dp == 1 ? launch<T, 32, true>(a, few, stream) : dp == 2 ? launch<T, 64, true>(a, few, stream)
+    : dp == 3 ? launch<T, 96, true>(a, few, stream) : launch<T, 128, true>(a, few, stream);
+  } else {
+    dp == 1 ? launch<T, 32, false>(a, few, stream) : dp == 2 ? launch<T, 64, false>(a, few, stream)
+    : dp == 3 ? launch<T, 96, false>(a, few, stream) : launch<T, 128, false>(a, few, stream);
+  }
+}
+
+}  // namespace
+
+namespace bmx {
+
+int cross_setup(CrossArgs& a, int dtype, const int64_t* shape, const int64_t* strides, float scale, bool has_bias) {
+  BMX_REQUIRE(dtype == kF32 || dtype == kBF16, "cross_attention: dtype must be fp32 or bf16");
+  BMX_REQUIRE(shape && strides, "cross_attention: null shape or strides");
+  for (int i = 0; i < 6; ++i) BMX_REQUIRE(shape[i] >= 0, "cross_attention: negative size");
+  a.batch = shape[0], a.m = shape[1], a.n = shape[2];
+  const int64_t heads = shape[3], kv = shape[4], dim = shape[5];
+  BMX_REQUIRE(dim >= 8 && dim <= 128 && dim % 8 == 0, "cross_attention: head dim must be a multiple of 8 in [8, 128]");
+  BMX_REQUIRE(heads >= 1 && heads <= 65536 && kv >= 1 && heads % kv == 0,
+              "cross_attention: the query heads must be a multiple of the key heads");
+  const int64_t rows = heads / kv * a.m;
+  BMX_REQUIRE(a.batch < (1ll << 31) && a.m < (1ll << 31) && rows < (1ll << 30), "cross_attention: too many query rows");
+  BMX_REQUIRE(scale > 0.f && scale < INFINITY, "cross_attention: scale must be positive and finite");
+  const int vec = dtype == kF32 ? 4 : 8;
+  for (int i = 0; i < 3; ++i) {
+    a.sq[i] = strides[i], a.sk[i] = strides[3 + i], a.sv[i] = strides[6 + i], a.sb[i] = has_bias ? strides[10 + i] : 0;
+    BMX_REQUIRE(a.sq[i] % vec == 0 && a.sk[i] % vec == 0 && a.sv[i] % vec == 0,
+                "cross_attention: strides must be multiples of 16 bytes");
+  }
+  a.smask = strides[9];
+  a.heads = (int)heads, a.kv_heads = (int)kv, a.group = (int)(heads / kv), a.dim = (int)dim, a.rows = (int)rows;
+  a.scale = scale;
+  return BMX_OK;
+}
+
+}  // namespace bmx
+
+extern "C" size_t bmx_cross_attention_workspace_bytes(int dtype, int64_t batch, int64_t m, int64_t n, int64_t heads,
+                                                      int64_t kv_heads, int64_t dim) {
+  if (batch < 1 || m < 1 || n < 1 || heads < 1 || kv_heads < 1 || dim < 1) return 0;
+  const int64_t rows = heads / kv_heads * m;
+  const Split s = plan(dtype, batch, kv_heads, rows, n);
+  return s.splits < 2 ? 0 : (size_t)(s.splits * batch * kv_heads * rows) * (dim + 2) * sizeof(float);
+}
+
+extern "C" int bmx_cross_attention_fwd(const void* q, const void* k, const void* v, const void* mask, const void* bias,
+                                       int dtype, const int64_t* shape, const int64_t* strides, float scale, void* out,
+                                       void* out_lo, float* stats, void* workspace, size_t workspace_bytes,
+                                       void* stream) {
+  CrossArgs a = {};
+  if (int rc = cross_setup(a, dtype, shape, strides, scale, bias != nullptr)) return rc;
+  if (a.batch == 0 || a.rows == 0) return BMX_OK;
+  BMX_REQUIRE(q && out && (a.n == 0 || (k && v)), "cross_attention: null pointer");
+  BMX_REQUIRE(((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)out | (uintptr_t)out_lo) % 16 == 0,
+              "cross_attention: q, k, v and out must be 16-byte aligned");
+  BMX_REQUIRE(!stats || (uintptr_t)stats % 8 == 0, "cross_attention: stats must be 8-byte aligned");
+  const Split s = plan(dtype, a.batch, a.kv_heads, a.rows, a.n);
+  const size_t need = bmx_cross_attention_workspace_bytes(dtype, a.batch, a.m, a.n, a.heads, a.kv_heads, a.dim);
+  BMX_REQUIRE(need == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need),
+              "cross_attention: workspace too small or not 16-byte aligned");
+  a.q = q, a.k = k, a.v = v, a.mask = (const uint8_t*)mask, a.bias = bias;
+  a.out = out, a.out_lo = dtype == kBF16 ? out_lo : nullptr, a.stats = (float2*)stats;
+  a.row_blocks = s.row_blocks, a.splits = s.splits, a.split_keys = s.keys;
+  const int64_t lists = (int64_t)s.splits * a.batch * a.kv_heads;
+  BMX_REQUIRE(lists * s.row_blocks < (1ll << 31), "cross_attention: too many blocks");
+  a.part_o = (float*)workspace;
+  a.part_ml = (float2*)((float*)workspace + lists * a.rows * a.dim);
+  hipStream_t hs = (hipStream_t)stream;
+  dtype == kF32 ? launch_dim<float>(a, s.few, hs) : launch_dim<bf16>(a, s.few, hs);
+  if (s.splits > 1) {
+    const int64_t threads = a.batch * a.kv_heads * a.rows * (a.dim / 4);
+    const dim3 grid((unsigned)((threads + 255) / 256));
+    if (dtype == kF32)
+      cross_attention_join<float><<<grid, 256, 0, hs>>>(a, bias != nullptr);
+    else
+      cross_attention_join<bf16><<<grid, 256, 0, hs>>>(a, bias != nullptr);
+  }
+  return check_launch("cross_attention");
+}

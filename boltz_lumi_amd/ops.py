@@ -8,8 +8,8 @@ Three groups:
   ``RuntimeError`` on bad input like the reference's ``TORCH_CHECK``s;
 * the fused hot-path modules (``trimul``, ``triattn``, ``pair_transition``,
   ``adaln``) that take a module with Boltz's parameter names;
-* sequence operators with gradients (``qk_norm_rope``, ``relative_bias``) for
-  an encoder / decoder beside the pair stack.
+* sequence operators with gradients (``qk_norm_rope``, ``relative_bias``,
+  ``cross_attention``) for an encoder / decoder beside the pair stack.
 
 Every call launches on torch's current stream of the input's device, allocates
 outputs and workspaces through torch's caching allocator and never
@@ -1390,3 +1390,110 @@ def relative_bias(table, q_pos, k_pos, exact=None, max_distance=128, bidirection
     args = (table.contiguous(), q_pos, k_pos, batch, _relative_thresholds(side, exact, int(max_distance)),
             bool(bidirectional))
     return _RelativeBias.apply(*args) if _needs_grad(table) else _relative_bias_fwd(*args)
+
+
+def _head_tokens(x):
+    """``x`` [B, T, H, D] with a dense last axis, outer strides of multiples of
+    16 bytes and 16-byte alignment: itself, or a dense copy."""
+    vec = 16 // x.element_size()
+    ok = x.stride(3) == 1 and x.data_ptr() % 16 == 0
+    if not ok or any(x.stride(i) % vec for i in range(3) if x.shape[i] > 1):
+        return _aligned(x.contiguous())
+    return x
+
+
+def _cross_args(q, k, v, mask, bias, scale):
+    b, m, h, d = q.shape
+    n, hk = k.shape[1], k.shape[2]
+    strides = _strides(q, 3) + _strides(k, 3) + _strides(v, 3)
+    strides.append(0 if mask is None else _strides(mask, 1)[0])
+    strides += [0, 0, 0] if bias is None else _strides(bias, 3)
+    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), _ptr(bias), _code(q.dtype),
+            N.int64_array([b, m, n, h, hk, d]), N.int64_array(strides), scale)
+
+
+def _cross_attention_fwd(q, k, v, mask, bias, scale, for_backward=False):
+    """(out, what rounding out left or None, row statistics or None)."""
+    b, m, h, d = q.shape
+    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    lo = torch.empty_like(out) if for_backward and q.dtype == torch.bfloat16 else None
+    stats = torch.empty(b, h, m, 2, device=q.device, dtype=torch.float32) if for_backward else None
+    if out.numel():
+        nbytes = N.lib().bmx_cross_attention_workspace_bytes(_code(q.dtype), b, m, k.shape[1], h, k.shape[2], d)
+        ws = _workspace(nbytes, q.device) if nbytes else None
+        with _at_device(q):
+            N.call("bmx_cross_attention_fwd", *_cross_args(q, k, v, mask, bias, scale), out.data_ptr(), _ptr(lo),
+                   _ptr(stats), _ptr(ws), nbytes, _stream(q))
+    return out, lo, stats
+
+
+class _CrossAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, mask, bias, scale):
+        out, lo, stats = _cross_attention_fwd(q, k, v, mask, bias, scale, for_backward=True)
+        ctx.save_for_backward(q, k, v, mask, bias, out, lo, stats)
+        ctx.scale = scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        q, k, v, mask, bias, out, lo, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dq, dk, dv, dbias = (torch.empty(t.shape, device=q.device, dtype=q.dtype) if need[i] else None
+                             for i, t in ((0, q), (1, k), (2, v), (4, bias)))
+        b, m, h, _ = q.shape
+        if q.numel() and k.numel():
+            dout = _aligned(dout.contiguous())
+            nbytes = N.lib().bmx_cross_attention_bwd_workspace_bytes(b, m, h)
+            ws = _workspace(nbytes, q.device)
+            with _at_device(q):
+                N.call("bmx_cross_attention_bwd", *_cross_args(q, k, v, mask, bias, ctx.scale), out.data_ptr(), _ptr(lo),
+                       stats.data_ptr(), dout.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dbias),
+                       None if dbias is None else N.int64_array(_strides(dbias, 2) + [dbias.stride(2)]), ws.data_ptr(), nbytes,
+                       _stream(q))
+        else:  # no queries or no keys: nothing depends on anything
+            for t in (dq, dk, dv, dbias):
+                if t is not None:
+                    t.zero_()
+        return dq, dk, dv, None, dbias, None
+
+
+def cross_attention(q, k, v, mask=None, bias=None, scale=None):
+    """Softmax attention of q [B, M, H, D] over another sequence's k and v
+    [B, N, Hk, D] (``bmx_cross_attention_fwd``):
+    ``softmax(scale q k^T + bias) v``, dense [B, M, H, D].
+
+    fp32 or bf16, D a multiple of 8 up to 128, H a multiple of Hk (query head h
+    reads key head ``h // (H / Hk)``), any M and N down to 0 and 1; layouts that
+    the kernel cannot read in place (a strided last axis, rows off 16 bytes) are
+    copied.  mask: bool [B, N] (or [1, N], [N]), True for the keys that take
+    part; the others' values are never looked at, NaN or not.  bias: q's type,
+    [B or 1, H or 1, M, N], added to the logits; -inf leaves a pair out.  A
+    query without keys gives zeros, and zero gradients.  scale: positive,
+    1 / sqrt(D) by default.  Weights are rounded to q's type before the product
+    with v; sums are fp32.  Gradients reach q, k, v and bias (summed over its
+    shared axes in fp32) and are the same bits on every run."""
+    _check(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "expected q, k and v of shape [B, tokens, heads, D]")
+    _cuda(q, k, v, *(t for t in (mask, bias) if t is not None))
+    b, m, h, d = q.shape
+    n, hk = k.shape[1], k.shape[2]
+    _code(q.dtype)
+    _check(k.shape == v.shape and k.shape[0] == b and k.shape[3] == d and k.dtype == v.dtype == q.dtype,
+           "k and v must match q's batch, head dim and dtype")
+    _check(8 <= d <= 128 and d % 8 == 0, "head dim must be a multiple of 8 in [8, 128]")
+    _check(h > 0 and hk > 0 and h % hk == 0, "the query heads must be a multiple of the key heads")
+    scale = d ** -0.5 if scale is None else float(scale)
+    _check(0 < scale < float("inf"), "scale must be positive and finite")
+    if mask is not None:
+        _check(mask.dtype == torch.bool and mask.shape in ((b, n), (1, n), (n,)), "expected a bool mask [B, N]")
+        mask = mask if mask.dim() == 2 else mask[None]
+        mask = mask if mask.stride(1) == 1 or n <= 1 else mask.contiguous()
+    if bias is not None:
+        _check(bias.dim() == 4 and bias.dtype == q.dtype and bias.shape[0] in (1, b) and bias.shape[1] in (1, h)
+               and bias.shape[2:] == (m, n), "expected a bias [B or 1, H or 1, M, N] in q's dtype")
+        bias = bias if bias.stride(3) == 1 or n <= 1 else bias.contiguous()
+    q, k, v = _head_tokens(q), _head_tokens(k), _head_tokens(v)
+    if _needs_grad(q, k, v, bias):
+        return _CrossAttention.apply(q, k, v, mask, bias, scale)
+    return _cross_attention_fwd(q, k, v, mask, bias, scale)[0]

@@ -446,6 +446,33 @@ int bmx_relative_bias_bwd(const void* dbias, int dtype, int64_t buckets, int64_t
                           const int32_t* thresholds, int count, int bidirectional, void* dtable, void* workspace,
                           size_t workspace_bytes, bmx_stream_t stream);
 
+/* out = softmax(scale q k^T + bias over the present keys) v for q [batch, m, heads, dim] and k, v
+ * [batch, n, kv_heads, dim], query head h on key head h / (heads / kv_heads); shape = {batch, m, n, heads,
+ * kv_heads, dim}, dim a multiple of 8 in [8, 128].  strides: batch, token, head of q, of k and of v (multiples
+ * of 16 bytes, the last axis dense), the mask's batch stride (0: shared), the bias's batch, head and
+ * query strides (any; 0: shared; keys dense).  mask: bytes [n] per batch element, 0 = the key (whatever its
+ * values) is left out, or NULL; bias in dtype or NULL.  A row without keys gives zeros.  out dense [batch, m,
+ * heads, dim].  For the backward pass, or NULL: out_lo (bf16 only, out's shape: what rounding out left),
+ * stats fp32 [batch, heads, m, 2] (row maximum of the logits, log2 of the sum of exp(logit - maximum)).
+ * workspace: bmx_cross_attention_workspace_bytes, 16-byte aligned.  No reference kernel. */
+size_t bmx_cross_attention_workspace_bytes(int dtype, int64_t batch, int64_t m, int64_t n, int64_t heads,
+                                           int64_t kv_heads, int64_t dim);
+int bmx_cross_attention_fwd(const void* q, const void* k, const void* v, const void* mask, const void* bias, int dtype,
+                            const int64_t* shape, const int64_t* strides, float scale, void* out, void* out_lo,
+                            float* stats, void* workspace, size_t workspace_bytes, bmx_stream_t stream);
+
+/* Gradients of bmx_cross_attention_fwd from dout (dense, out's shape) and the forward pass's out,
+ * out_lo (bf16) and stats: dq, dk, dv dense (each may be NULL), dbias in dtype at dbias_strides = {batch
+ * (0: one for the batch), head (0: one for the heads), query}, keys dense, or NULL.  Left-out keys and rows
+ * without keys get zeros.  batch, m, n >= 1.  workspace: bmx_cross_attention_bwd_workspace_bytes, 16-byte aligned.
+ * No reference kernel. */
+size_t bmx_cross_attention_bwd_workspace_bytes(int64_t batch, int64_t m, int64_t heads);
+int bmx_cross_attention_bwd(const void* q, const void* k, const void* v, const void* mask, const void* bias, int dtype,
+                            const int64_t* shape, const int64_t* strides, float scale, const void* out,
+                            const void* out_lo, const float* stats, const void* dout, void* dq, void* dk, void* dv,
+                            void* dbias, const int64_t* dbias_strides, void* workspace, size_t workspace_bytes,
+                            bmx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -85,3 +85,47 @@ def test_thresholds(side, exact, top):
     for k, edge in enumerate(edges[exact:], 1):
         reach = exact ** (steps - k) * top ** k
         assert edge ** steps >= reach and (edge - 1) ** steps < reach
+
+
+def test_cross_attention_rejects_bad_arguments(lib):
+    b, m, n, h, hk, d = 2, 40, 50, 4, 2, 64
+    good_shape = (b, m, n, h, hk, d)
+    good_strides = (m * h * d, h * d, d, n * hk * d, hk * d, d, n * hk * d, hk * d, d, n, 0, m * n, n)
+    need = lib.bmx_cross_attention_workspace_bytes(1, *good_shape)
+    assert lib.bmx_cross_attention_workspace_bytes(1, b, 0, n, h, hk, d) == 0
+    assert lib.bmx_cross_attention_workspace_bytes(1, 1, 1, 4096, 8, 2, d) > 0  # one query: split over the keys
+
+    def fwd(q=FAKE, dtype=1, shape=good_shape, strides=good_strides, scale=0.1, out=FAKE, lo=FAKE, stats=FAKE, ws=FAKE,
+            size=need):
+        return lib.bmx_cross_attention_fwd(q, FAKE, FAKE, None, FAKE, dtype, N.int64_array(shape), N.int64_array(strides),
+                                           scale, out, lo, stats, ws, size, None)
+
+    assert refused(lib, fwd(dtype=2), b"dtype") and refused(lib, fwd(shape=(b, m, n, h, hk, 136)), b"[8, 128]")
+    assert refused(lib, fwd(shape=(b, m, n, h, hk, 60)), b"multiple of 8")
+    assert refused(lib, fwd(shape=(b, m, n, 5, hk, d)), b"multiple of the key heads")
+    assert refused(lib, fwd(shape=(b, -1, n, h, hk, d)), b"negative size")
+    assert refused(lib, fwd(scale=0.0), b"scale") and refused(lib, fwd(scale=float("nan")), b"scale")
+    assert refused(lib, fwd(strides=(4, *good_strides[1:])), b"16 bytes")
+    assert refused(lib, fwd(q=None), b"null pointer") and refused(lib, fwd(out=None), b"null pointer")
+    assert refused(lib, fwd(q=ODD), b"16-byte aligned") and refused(lib, fwd(lo=ODD), b"16-byte aligned")
+    assert refused(lib, fwd(stats=ODD), b"8-byte aligned")
+    assert fwd(shape=(0, m, n, h, hk, d), q=None) == N.BMX_OK and fwd(shape=(b, 0, n, h, hk, d), q=None) == N.BMX_OK
+    long = (1, 1, 4096, 8, 2, d)
+    need_long = lib.bmx_cross_attention_workspace_bytes(1, *long)
+    assert refused(lib, fwd(shape=long, size=need_long - 1), b"workspace")
+    assert refused(lib, fwd(shape=long, ws=None, size=need_long), b"workspace")
+
+    need_bwd = lib.bmx_cross_attention_bwd_workspace_bytes(b, m, h)
+    assert need_bwd == b * m * h * 4
+
+    def bwd(shape=good_shape, bias=FAKE, lo=FAKE, stats=FAKE, dout=FAKE, dq=FAKE, dbias=FAKE, steps=(0, m * n, n),
+            ws=FAKE, size=need_bwd):
+        return lib.bmx_cross_attention_bwd(FAKE, FAKE, FAKE, None, bias, 1, N.int64_array(shape),
+                                           N.int64_array(good_strides), 0.1, FAKE, lo, stats, dout, dq, FAKE, FAKE, dbias,
+                                           None if steps is None else N.int64_array(steps), ws, size, None)
+
+    assert refused(lib, bwd(shape=(b, m, 0, h, hk, d)), b"empty") and refused(lib, bwd(lo=None), b"out_lo")
+    assert refused(lib, bwd(bias=None), b"dbias needs") and refused(lib, bwd(steps=None), b"dbias needs")
+    assert refused(lib, bwd(stats=None), b"null pointer") and refused(lib, bwd(dout=None), b"null pointer")
+    assert refused(lib, bwd(dq=ODD), b"16-byte aligned") and refused(lib, bwd(stats=ODD), b"8-byte aligned")
+    assert refused(lib, bwd(size=need_bwd - 1), b"workspace") and refused(lib, bwd(ws=ODD), b"workspace")
