@@ -6,9 +6,11 @@
 // single query of a shared head still fills MFMA columns.
 //
 // Operand layout (v_mfma_f32_32x32x16_bf16, or v_mfma_f32_32x32x2f32 for fp32; lane l, half
-// h = l / 32): a product tile holds column l % 32 and, in register r, row 8 (r / 4) + 4 h + r % 4. A
-// logits tile S^T (keys x queries) is then itself the B operand of the next product over its keys:
-// registers 8 t .. 8 t + 7 are the 16 keys of bf16 step t, and register r the keys of fp32 step r.
+// h = l / 32): a product tile holds column l % 32 and, in register r, row 8 (r / 4) + 4 h + r % 4. The
+// A operand's rows are read in the order that makes this row 16 h + r of the LDS tile (tile_row), so a
+// lane's 16 values are 16 rows in a run: of keys, whose bias lies in a run too. A logits tile S^T
+// (keys x queries) is then itself the B operand of the next product over its keys: registers 8 t .. 8 t + 7 are
+// bf16 step t, register r is fp32 step r.
 #pragma once
 
 #include "bmx_common.h"
@@ -27,14 +29,14 @@ struct CrossArgs {
   const uint8_t* mask;
   int64_t sq[3], sk[3], sv[3];  // batch, token, head strides
   int64_t sb[3], smask;         // bias: batch, head, query strides; keys dense
-  int64_t batch, m, n;
-  int heads, kv_heads, group, dim, rows;  // rows = group * m
+  int64_t batch, m;
+  int n, heads, kv_heads, group, dim, rows;  // rows = group * m
   float scale;
   void *out, *out_lo;
   float2* stats;  // [batch][heads][m]: row maximum of the logits and log2 of the sum of exp(logit - maximum)
   // work split
   int row_blocks, splits;
-  int64_t split_keys;
+  int split_keys;
   float* part_o;   // [split][batch * kv_heads][rows][dim] sums before the division
   float2* part_ml;  // [split][batch * kv_heads][rows] maximum and sum
   // backward
@@ -96,13 +98,28 @@ __device__ __forceinline__ f32x16 mfma_step(const float*, u32x4 a, u32x4 b, f32x
   return acc;
 }
 
-// acc += tile rows row0 .. row0 + 31 (A) times the operand's columns (B), over the channels.
+// Tile row of A-operand row i.
+__device__ __forceinline__ int tile_row(int i) { return 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3); }
+
+// Where a lane reads its parts of a 32-row tile, worked out once: with the tile's position a constant of the unrolled
+// loops, a read is one register and an immediate.
 template <typename T, int DP>
-__device__ __forceinline__ f32x16 product(const char* tile, int row0, const RowOperand<T, DP>& b, f32x16 acc) {
-  const int r = row0 + (lane_id() & 31), h = lane_id() >> 5;
+struct RowReads {
+  int off[RowOperand<T, DP>::kSteps];
+  __device__ __forceinline__ void init() {
+    const int r = tile_row(lane_id() & 31), h = lane_id() >> 5;
+#pragma unroll
+    for (int s = 0; s < RowOperand<T, DP>::kSteps; ++s) off[s] = Tile<T, DP>::at(r, 2 * s + h);
+  }
+};
+
+// Tile rows (A) times the operand's columns (B), over the channels.
+template <typename T, int DP>
+__device__ __forceinline__ f32x16 product(const char* tile, const RowReads<T, DP>& at, const RowOperand<T, DP>& b) {
+  f32x16 acc = zero16();
 #pragma unroll
   for (int s = 0; s < RowOperand<T, DP>::kSteps; ++s)
-    acc = mfma_step((const T*)nullptr, *(const u32x4*)(tile + Tile<T, DP>::at(r, 2 * s + h)), b.c[s], acc);
+    acc = mfma_step((const T*)nullptr, *(const u32x4*)(tile + at.off[s]), b.c[s], acc);
   return acc;
 }
 
@@ -140,15 +157,26 @@ struct Weights<float> {
   }
 };
 
-// acc[dt] += (tile rows row0 .. row0 + 31)^T (channels 32 dt .. as rows) times the weights, over those rows.
+// acc[dt] += (tile rows)^T (channels 32 dt .. as rows) times the weights, over the rows.
+template <typename T, int DP>
+struct ColumnReads;
 template <int DP>
-__device__ __forceinline__ void transposed_product(const char* tile, int row0, const Weights<bf16>& w,
-                                                   f32x16 (&acc)[DP / 32]) {
-  const int l = lane_id(), h = l >> 5, i = l & 15;
-  const int chunk = 2 * ((l >> 4) & 1) + ((i & 3) >> 1), byte = 8 * (i & 1);
+struct ColumnReads<bf16, DP> {
+  int off[4][DP / 32];  // of four rows each
+  __device__ __forceinline__ void init() {
+    const int l = lane_id(), h = l >> 5, i = l & 15, chunk = 2 * ((l >> 4) & 1) + ((i & 3) >> 1);
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const int r = row0 + 16 * t + 4 * h + (i >> 2);
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int dt = 0; dt < DP / 32; ++dt)
+        off[u][dt] = Tile<bf16, DP>::at(16 * h + 4 * u + (i >> 2), 4 * dt + chunk) + 8 * (i & 1);
+  }
+};
+template <int DP>
+__device__ __forceinline__ void transposed_product(const char* tile, const ColumnReads<bf16, DP>& at,
+                                                   const Weights<bf16>& w, f32x16 (&acc)[DP / 32]) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) {
       union {
@@ -158,55 +186,139 @@ __device__ __forceinline__ void transposed_product(const char* tile, int row0, c
 #pragma unroll
       for (int u = 0; u < 2; ++u)
         a.half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)(tile + Tile<bf16, DP>::at(r + 8 * u, 4 * dt + chunk) + byte));
+            (__attribute__((address_space(3))) s16x4*)(tile + at.off[2 * t + u][dt]));
       acc[dt] = mfma32(a.all, w.v[t], acc[dt]);
     }
-  }
 }
 template <int DP>
-__device__ __forceinline__ void transposed_product(const char* tile, int row0, const Weights<float>& w,
-                                                   f32x16 (&acc)[DP / 32]) {
+struct ColumnReads<float, DP> {
+  __device__ __forceinline__ void init() {}
+};
+template <int DP>
+__device__ __forceinline__ void transposed_product(const char* tile, const ColumnReads<float, DP>&,
+                                                   const Weights<float>& w, f32x16 (&acc)[DP / 32]) {
   const int l = lane_id(), h = l >> 5, i = l & 31;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int row = row0 + 8 * (r >> 2) + 4 * h + (r & 3);
+  for (int r = 0; r < 16; ++r)
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) {
-      const float a = *(const float*)(tile + Tile<float, DP>::at(row, 8 * dt + (i >> 2)) + 4 * (i & 3));
+      const float a = *(const float*)(tile + Tile<float, DP>::at(16 * h + r, 8 * dt + (i >> 2)) + 4 * (i & 3));
       acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w.v[r], acc[dt], 0, 0, 0);
     }
-  }
 }
 
 // ---- staging -------------------------------------------------------------
-// ROWS rows of a [.., tokens, .., dim] tensor through registers into an LDS tile, by THREADS threads.
+// ROWS rows of a tensor through registers into an LDS tile, by THREADS threads. Every load is unconditional (a load in
+// a branch of its own would wait for all others): channels past dim read the row's first ones and are stored as zeros.
+// Offsets within a tile are 32 bits (a row stride is below kMaxStride elements), so a load is a scalar base and
+// one register.
+constexpr int64_t kMaxStride = 1 << 22;
+
 template <typename T, int DP, int ROWS, int THREADS>
 struct Stage {
   using L = Tile<T, DP>;
   static constexpr int kCount = (ROWS * L::kChunks + THREADS - 1) / THREADS;
+  static constexpr bool kEven = (ROWS * L::kChunks) % THREADS == 0;
   u32x4 v[kCount];
+  uint32_t off[kCount];
 
-  // row(r): pointer to row r, always readable; channels past dim read the row's first ones.
-  template <typename Row>
-  __device__ __forceinline__ void load(int t, int dim, Row row) {
+  static __device__ __forceinline__ int row(int t, int i) { return min((t + i * THREADS) / L::kChunks, ROWS - 1); }
+  static __device__ __forceinline__ int chunk(int t, int i) { return (t + i * THREADS) % L::kChunks; }
+
+  __device__ __forceinline__ uint32_t offset(int t, int i, int last, int dim, int64_t stride) const {
+    const int c = chunk(t, i);
+    return (uint32_t)(min(row(t, i), last) * (int)(stride * sizeof(T)) + (c * L::kElems < dim ? c : 0) * 16);
+  }
+  __device__ __forceinline__ void init(int t, int dim, int64_t stride) {
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-      const int at = t + i * THREADS, r = at / L::kChunks, d = (at % L::kChunks) * L::kElems;
-      if ((ROWS * L::kChunks) % THREADS == 0 || r < ROWS) v[i] = *(const u32x4*)(row(r) + (d < dim ? d : 0));
+    for (int i = 0; i < kCount; ++i) off[i] = offset(t, i, ROWS - 1, dim, stride);
+  }
+  // Rows 0 .. ROWS - 1 from `base` on; of a tile with `rows` < ROWS of them the last one again.
+  __device__ __forceinline__ void load(int t, const T* base, int rows, int dim, int64_t stride) {
+    const char* p = (const char*)base;
+    if (rows >= ROWS) {
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) v[i] = *(const u32x4*)(p + off[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) v[i] = *(const u32x4*)(p + offset(t, i, rows - 1, dim, stride));
     }
   }
-  // live(r): rows that hold data; the others, and channels past dim, are stored as zeros.
-  template <typename Live>
-  __device__ __forceinline__ void store(int t, int dim, char* tile, Live live) const {
+  // live: the tile's rows that hold data (bits); the others are stored as zeros.
+  __device__ __forceinline__ void store(int t, char* tile, uint64_t live, int dim) const {
+    constexpr uint64_t all = ROWS == 64 ? ~0ull : (1ull << (ROWS & 63)) - 1;
+    if (live == all && dim == DP) {
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-      const int at = t + i * THREADS, r = at / L::kChunks, c = at % L::kChunks;
-      if ((ROWS * L::kChunks) % THREADS != 0 && r >= ROWS) continue;
-      const bool ok = c * L::kElems < dim && live(r);
-      *(u32x4*)(tile + L::at(r, c)) = ok ? v[i] : u32x4{0, 0, 0, 0};
+      for (int i = 0; i < kCount; ++i)
+        if (kEven || t + i * THREADS < ROWS * L::kChunks) *(u32x4*)(tile + L::at(row(t, i), chunk(t, i))) = v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < kCount; ++i) {
+        const bool ok = ((live >> row(t, i)) & 1) && chunk(t, i) * L::kElems < dim;
+        if (kEven || t + i * THREADS < ROWS * L::kChunks)
+          *(u32x4*)(tile + L::at(row(t, i), chunk(t, i))) = ok ? v[i] : u32x4{0, 0, 0, 0};
+      }
     }
   }
 };
+
+// LDS DMA of 64 lanes x 16 bytes, each from base + its off, to lds_addr + 16 * lane (base and lds_addr uniform). It reads
+// M0 and the base's SGPRs: one wait state must lie between M0's write and the read, five after a vector write
+// of the SGPRs (s_nop 4). The compiler does not see into the asm, nor does it wait for the copy. Every
+// wave waits for its own copies of a tile (wait_copies) before the barrier that publishes the tile, and a tile is
+// overwritten only after a barrier that every wave reached with its reads of it done.
+__device__ __forceinline__ void lds_copy16(const void* base, uint32_t off, unsigned lds_addr) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds_addr) : "memory");
+}
+__device__ __forceinline__ void wait_copies() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
+}
+
+// ROWS rows of a tensor into an LDS tile by WAVES waves' DMA. A copy writes its lanes' 16 bytes in a run, so the twist is
+// in the addresses read. Chunks past dim are not copied: clear_tiles zeroes them once, before the first copy.
+template <typename T, int DP, int ROWS, int WAVES>
+struct Copy {
+  using L = Tile<T, DP>;
+  static constexpr int kTotal = ROWS * L::kRow / 64, kPer = (kTotal + WAVES - 1) / WAVES;
+  static_assert(ROWS * L::kRow % 64 == 0, "whole copies");
+  uint32_t off[kPer];  // ~0: past dim
+
+  static __device__ __forceinline__ uint32_t offset(int part, int last, int dim, int64_t stride) {
+    const int p = part * 64 + lane_id(), r = p / L::kRow, c = (p % L::kRow) ^ L::twist(r);
+    return c * L::kElems < dim ? (uint32_t)(min(r, last) * (int)(stride * sizeof(T)) + c * 16) : ~0u;
+  }
+  __device__ __forceinline__ void init(int wave, int dim, int64_t stride) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) off[j] = offset(wave + j * WAVES, ROWS - 1, dim, stride);
+  }
+  // Rows 0 .. ROWS - 1 from `base` on; of a tile with `rows` < ROWS of them the last one again. wave and tile are uniform.
+  __device__ __forceinline__ void issue(int wave, const T* base, int rows, int dim, int64_t stride, unsigned tile) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int part = wave + j * WAVES;
+      if (kTotal % WAVES != 0 && part >= kTotal) break;
+      const uint32_t o = rows >= ROWS ? off[j] : offset(part, rows - 1, dim, stride);
+      if (o != ~0u) lds_copy16(base, o, tile + part * 1024);
+    }
+  }
+};
+
+// Zeros in `bytes` of LDS by THREADS threads, where tiles have chunks past dim.
+template <typename T, int DP, int THREADS>
+__device__ __forceinline__ void clear_tiles(int t, char* lds, int bytes, int dim) {
+  if (dim == Tile<T, DP>::kRow * Tile<T, DP>::kElems) return;
+  for (int at = 16 * t; at < bytes; at += 16 * THREADS) *(u32x4*)(lds + at) = u32x4{0, 0, 0, 0};
+  __syncthreads();
+}
+
+// Zeros in the tile rows whose bit is not set, by THREADS threads.
+template <typename T, int DP, int ROWS, int THREADS>
+__device__ __forceinline__ void clear_rows(int t, char* tile, uint64_t live) {
+  constexpr int kRow = Tile<T, DP>::kRow;
+  for (int at = t; at < ROWS * kRow; at += THREADS)
+    if (!((live >> (at / kRow)) & 1)) *(u32x4*)(tile + at * 16) = u32x4{0, 0, 0, 0};
+}
 
 // Orders a wave's LDS writes and its other lanes' reads where no barrier does: the LDS serves a wave in order, so
 // only the compiler has to keep them.
@@ -216,39 +328,37 @@ __device__ __forceinline__ void wave_order() {
 }
 
 // ---- key mask ------------------------------------------------------------
-// Bit words of a chunk of keys: bit j of word w is key c0 + 64 w + j present (inside the mask and below end).
-// All threads call fill (two barriers); key c0 is a multiple of 64.
+// Bit words of a chunk of keys: bit j of word w is key c0 + 32 w + j present (inside the mask and below end).
+// All threads call fill (two barriers); key c0 is a multiple of 32.
 struct KeyWords {
-  uint64_t* words;  // LDS [kMaskChunk / 64]
+  uint32_t* words;  // LDS [kMaskChunk / 32]
   const uint8_t* mask;
-  int64_t c0, end;
+  int c0, end;
 
-  __device__ __forceinline__ void fill(int64_t first, int64_t stop) {
+  __device__ __forceinline__ void fill(int first, int stop) {
     c0 = first, end = stop;
     if (!mask) return;
     __syncthreads();
-    const int64_t left = min(stop - first, (int64_t)kMaskChunk);
+    const int left = min(stop - first, kMaskChunk);
     for (int w = threadIdx.x >> 6; 64 * w < left; w += blockDim.x >> 6) {
-      const int64_t key = first + 64 * w + lane_id();
+      const int key = first + 64 * w + lane_id();
       const bool on = key < stop && mask[key < stop ? key : stop - 1] != 0;
       const uint64_t bits = __ballot(on);
-      if (lane_id() == 0) words[w] = bits;
+      if (lane_id() < 2) words[2 * w + lane_id()] = (uint32_t)(bits >> (32 * lane_id()));
     }
     __syncthreads();
   }
-  // Presence of the `count` (32 or 64) keys from `key` on, the same in every lane; key - c0 a multiple of count.
-  __device__ __forceinline__ uint64_t bits(int64_t key, int count) const {
-    const uint64_t all = count == 64 ? ~0ull : 0xffffffffull;
-    const int64_t left = end - key;
-    if (left <= 0) return 0;
-    uint64_t b = left >= count ? all : (1ull << left) - 1;
-    if (mask) {
-      const int at = (int)(key - c0);
-      const uint64_t w = words[at >> 6] >> (at & 63);
-      b &= (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)w) |
-           (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(w >> 32)) << 32;
-    }
-    return b;
+  // Presence of the 32 keys from `key` on, the same in every lane; key - c0 a multiple of 32.
+  __device__ __forceinline__ uint32_t bits(int key) const {
+    if (key >= end) return 0;
+    if (mask) return (uint32_t)__builtin_amdgcn_readfirstlane((int)words[(key - c0) >> 5]);
+    return end - key >= 32 ? ~0u : (1u << (end - key)) - 1;
+  }
+  // The next 32 keys from `key` on that hold a present one, or the first past `last`.
+  __device__ __forceinline__ int next(int key, int last) const {
+    if (mask)
+      while (key < last && bits(key) == 0) key += 32;
+    return key;
   }
 };
 
@@ -266,25 +376,25 @@ __device__ __forceinline__ f32x4 bias4(const bf16* p) {
 // Bias of the lane's query at the 16 keys of a logits tile from key `key` on, in register order; keys from n on
 // read the last one (they are masked).
 template <typename T>
-__device__ __forceinline__ f32x16 bias_tile(const T* row, int64_t key, int64_t n) {
+__device__ __forceinline__ f32x16 bias_tile(const T* row, int key, int n) {
   f32x16 b;
-  const int64_t k = key + 4 * (lane_id() >> 5);
+  const int k = key + 16 * (lane_id() >> 5);
   if (key + 32 <= n) {
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const f32x4 v = bias4(row + k + 8 * g);
+      const f32x4 v = bias4(row + k + 4 * g);
 #pragma unroll
       for (int e = 0; e < 4; ++e) b[4 * g + e] = v[e];
     }
   } else {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) b[r] = (float)row[min(k + 8 * (r >> 2) + (r & 3), n - 1)];
+    for (int r = 0; r < 16; ++r) b[r] = (float)row[min(k + r, n - 1)];
   }
   return b;
 }
 
-// Bit of register r's key in a logits tile whose 32 keys are `bits`, already shifted by 4 h.
-__device__ __forceinline__ bool key_bit(uint32_t bits, int r) { return (bits >> (8 * (r >> 2) + (r & 3))) & 1; }
+// Bit of register r's key in a logits tile whose 32 keys are `bits`, already shifted by 16 h.
+__device__ __forceinline__ bool key_bit(uint32_t bits, int r) { return (bits >> r) & 1; }
 
 // Maximum / sum over the two halves of the wave, per column.
 __device__ __forceinline__ float halves_max(float v) {

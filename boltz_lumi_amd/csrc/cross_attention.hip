@@ -12,6 +12,8 @@
 // weights add up to one: the error is a rounding of each weight against the others.
 //
 // A row without keys (masked, or -inf bias throughout) gives zeros.
+#include <type_traits>
+
 #include "cross_attention.h"
 
 using namespace bmx;
@@ -19,77 +21,71 @@ using namespace bmx;
 namespace {
 
 // State of a wave's 32 rows: lane l holds row l % 32, in both halves.
-template <typename T, int DP>
+template <typename T, int DP, bool kBias>
 struct Rows {
+  // Without a bias the logits stay unscaled (q k^T); with one they are in natural units and the difference to the maximum is
+  // taken before the change to base 2, so that biases of the type's lowest value do not overflow. fp32 takes
+  // the difference first too: the largest logit's weight is then exactly 1 (bf16 rounds it to 1).
+  static constexpr bool kFirst = kBias || sizeof(T) == 4;
   RowOperand<T, DP> q;
+  RowReads<T, DP> kr;
+  ColumnReads<T, DP> vr;
   f32x16 o[DP / 32];
-  float top, sum;  // running maximum (of S, or of q k^T without a bias); this half's share of the sum
+  float top, sum;  // maximum that the weights refer to; this half's share of their sum
+  float limit;     // the maximum moves when a logit passes this
+  float shift;     // of the exponent: the maximum, or minus its product with c
+  float c;         // logits to base 2
   const T* bias;
 
-  __device__ __forceinline__ void init(const CrossArgs& a, int64_t b, int c, int row) {
+  __device__ __forceinline__ void init(const CrossArgs& a, int64_t b, int kv, int row) {
     const int r = min(row, a.rows - 1), g = r / (int)a.m, i = r - g * (int)a.m;
-    const int64_t head = (int64_t)c * a.group + g;
+    const int64_t head = (int64_t)kv * a.group + g;
     q.load((const T*)a.q + b * a.sq[0] + i * a.sq[1] + head * a.sq[2], a.dim, lane_id() >> 5);
     bias = (const T*)a.bias + b * a.sb[0] + head * a.sb[1] + i * a.sb[2];
+    kr.init();
+    vr.init();
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();
-    top = -INFINITY, sum = 0.f;
+    top = limit = -INFINITY, sum = shift = 0.f;
+    c = (kBias ? 1.f : a.scale) * kLog2E;
   }
 
-  // NB times 32 keys: rows row0 .. of the tiles, keys `key` .. of the sequence, presence bits.
-  template <int NB, bool kBias>
-  __device__ __forceinline__ void attend(const CrossArgs& a, const char* kt, const char* vt, int64_t key, uint64_t bits) {
-    f32x16 s[NB];
-#pragma unroll
-    for (int u = 0; u < NB; ++u) s[u] = product<T, DP>(kt, 32 * u, q, zero16());
+  // 32 keys: rows of the tiles, keys `key` .. of the sequence, presence bits.
+  __device__ __forceinline__ void attend(const CrossArgs& a, const char* kt, const char* vt, int key, uint32_t bits) {
+    f32x16 s = product<T, DP>(kt, kr, q);
     if (kBias) {
+      const f32x16 b = bias_tile(bias, key, a.n);
 #pragma unroll
-      for (int u = 0; u < NB; ++u) {
-        // A tail sub-tile may lie past the last key altogether.
-        const f32x16 b = bias_tile(bias, min(key + 32 * u, a.n - 1), a.n);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[u][r] = s[u][r] * a.scale + b[r];
-      }
+      for (int r = 0; r < 16; ++r) s[r] = s[r] * a.scale + b[r];
     }
-    const uint64_t all = NB == 2 ? ~0ull : 0xffffffffull;
-    if (bits != all) {
-      const uint64_t mine = bits >> (4 * (lane_id() >> 5));
+    if (bits != ~0u) {
+      const uint32_t mine = bits >> (16 * (lane_id() >> 5));
 #pragma unroll
-      for (int u = 0; u < NB; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!key_bit((uint32_t)(mine >> (32 * u)), r)) s[u][r] = -INFINITY;
+      for (int r = 0; r < 16; ++r)
+        if (!key_bit(mine, r)) s[r] = -INFINITY;
     }
-    float mx = s[0][0];
+    float mx = s[0];
 #pragma unroll
-    for (int u = 0; u < NB; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
-    mx = fmaxf(halves_max(mx), top);
-    // Without a bias the logits stay unscaled; with one they are in natural units and the difference is taken
-    // before the change to base 2, so that biases of the type's lowest value do not overflow. fp32 takes
-    // the difference first too: the largest logit's weight is then exactly 1 (bf16 rounds it to 1).
-    constexpr bool kFirst = kBias || sizeof(T) == 4;
-    const float c = (kBias ? 1.f : a.scale) * kLog2E;
-    const float base = mx == -INFINITY ? 0.f : mx;
-    if (__any(mx > top)) {
-      const float f = __builtin_amdgcn_exp2f((top - base) * c);
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    // bf16 moves the maximum (and scales the sums) only when a logit passes it by 2^6: the weights' rounding is relative, and
+    // their sums stay far inside fp32. After the first tiles that hardly happens, so the halves' exchange, the
+    // factor and the products with it are off the common path.
+    if (__any(mx > limit)) {
+      mx = fmaxf(halves_max(mx), top);
+      const float base = mx == -INFINITY ? 0.f : mx, f = __builtin_amdgcn_exp2f((top - base) * c);
       sum *= f;
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) o[dt] *= f;
       top = mx;
+      limit = sizeof(T) == 2 ? mx + 6.f / c : mx;
+      shift = kFirst ? base : -base * c;
     }
-    const float shift = -base * c;
 #pragma unroll
-    for (int u = 0; u < NB; ++u) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        s[u][r] = __builtin_amdgcn_exp2f(kFirst ? (s[u][r] - base) * c : s[u][r] * c + shift);
-      Weights<T> w;
-      w.set(s[u]);
-      sum = w.sum(sum);
-      transposed_product<DP>(vt, 32 * u, w, o);
-    }
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(kFirst ? (s[r] - shift) * c : s[r] * c + shift);
+    Weights<T> w;
+    w.set(s);
+    sum = w.sum(sum);
+    transposed_product<DP>(vt, vr, w, o);
   }
 };
 
@@ -157,8 +153,8 @@ __device__ __forceinline__ void write_rows(const CrossArgs& a, int64_t b, int c,
 
 // Position of a block: row block, split, key head, batch element.
 struct Place {
-  int row_block, split, c;
-  int64_t b, first, stop;  // keys of the split
+  int row_block, split, c, first, stop;  // keys of the split
+  int64_t b;
   __device__ __forceinline__ Place(const CrossArgs& a) {
     int64_t at = xcd_position(blockIdx.x, gridDim.x);
     row_block = (int)(at % a.row_blocks), at /= a.row_blocks;
@@ -169,49 +165,56 @@ struct Place {
   }
 };
 
-template <typename T>
-constexpr int kWideKeys = sizeof(T) == 2 ? 64 : 32;
-
-// Many rows: four waves of 32 rows share a tile of keys, staged through registers into two LDS buffers: while a
-// tile is attended the next one's loads are in flight, one barrier per tile. Tiles without a present key are
-// passed over.
+// Many rows: four waves of 32 rows share tiles of 32 keys in two LDS buffers, copied there by DMA: the next tile's
+// copies are in flight while a tile is attended, one barrier per tile. No staging registers and small tiles leave
+// room for three blocks on a compute unit, so one wave's exponentials run under another's
+// MFMA. Tiles without a present key are passed over.
 template <typename T, int DP, bool kBias>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_wide(CrossArgs a) {
-  constexpr int KT = kWideKeys<T>, kTile = KT * Tile<T, DP>::kRowBytes;
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : sizeof(T) == 4 || kBias || DP == 128 ? 2 : 3)
+void cross_attention_wide(CrossArgs a) {
+  constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[4 * kTile + kMaskChunk / 8];
   const Place p(a);
-  const int t = threadIdx.x, row = p.row_block * 128 + (t >> 6) * 32 + (t & 31);
-  Rows<T, DP> rows;
+  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), row = p.row_block * 128 + w * 32 + (t & 31);
+  Rows<T, DP, kBias> rows;
   rows.init(a, p.b, p.c, row);
   const T* k = (const T*)a.k + p.b * a.sk[0] + p.c * a.sk[2];
   const T* v = (const T*)a.v + p.b * a.sv[0] + p.c * a.sv[2];
-  KeyWords words{(uint64_t*)(lds + 4 * kTile), a.mask ? a.mask + p.b * a.smask : nullptr};
-  Stage<T, DP, KT, 256> sk, sv;
-  int buf = 0;
-  for (int64_t c0 = p.first; c0 < p.stop; c0 += kMaskChunk) {
-    words.fill(c0, p.stop);
-    const int64_t end = min(c0 + kMaskChunk, p.stop);
-    auto next = [&](int64_t key) {
-      while (key < end && words.bits(key, KT) == 0) key += KT;
-      return key;
+  KeyWords words{(uint32_t*)(lds + 4 * kTile), a.mask ? a.mask + p.b * a.smask : nullptr};
+  Copy<T, DP, 32, 4> ck, cv;
+  ck.init(w, a.dim, a.sk[1]);
+  cv.init(w, a.dim, a.sv[1]);
+  const unsigned lds0 = lds_address(lds);
+  clear_tiles<T, DP, 256>(t, lds, 4 * kTile, a.dim);
+  const int chunk = a.mask ? kMaskChunk : a.n;
+  for (int c0 = p.first; c0 < p.stop; c0 += chunk) {
+    words.fill(c0, p.stop);  // its barrier also ends the last chunk's reads of the tiles
+    const int end = min(c0 + chunk, p.stop);
+    auto copy = [&](int key, unsigned tile) {
+      ck.issue(w, k + key * a.sk[1], a.n - key, a.dim, a.sk[1], tile);
+      cv.issue(w, v + key * a.sv[1], a.n - key, a.dim, a.sv[1], tile + kTile);
     };
-    auto load = [&](int64_t key) {
-      sk.load(t, a.dim, [&](int r) { return k + min(key + r, a.n - 1) * a.sk[1]; });
-      sv.load(t, a.dim, [&](int r) { return v + min(key + r, a.n - 1) * a.sv[1]; });
-    };
-    int64_t key = next(c0);
-    if (key < end) load(key);
-    while (key < end) {
-      const uint64_t bits = words.bits(key, KT);
-      char* kt = lds + buf * 2 * kTile;
-      auto live = [&](int r) { return (bits >> r) & 1; };
-      sk.store(t, a.dim, kt, live);
-      sv.store(t, a.dim, kt + kTile, live);
-      const int64_t after = next(key + KT);
-      if (after < end) load(after);
+    int key = words.next(c0, end);
+    // One tile in the buffer at B; false after the last.
+    auto step = [&](auto B) {
+      constexpr int kAt = decltype(B)::value * 2 * kTile, kOther = 2 * kTile - kAt;
+      const uint32_t bits = words.bits(key);
+      const int after = words.next(key + 32, end);
+      wait_copies();
       __syncthreads();
-      rows.template attend<KT / 32, kBias>(a, kt, kt + kTile, key, bits);
-      buf ^= 1, key = after;
+      if (after < end) copy(after, lds0 + kOther);
+      if (bits != ~0u) {  // what a left-out value holds must not meet its weight of zero
+        clear_rows<T, DP, 32, 256>(t, lds + kAt + kTile, bits);
+        __syncthreads();
+      }
+      rows.attend(a, lds + kAt, lds + kAt + kTile, key, bits);
+      key = after;
+      return key < end;
+    };
+    if (key < end) {
+      copy(key, lds0);
+      while (step(std::integral_constant<int, 0>()) && step(std::integral_constant<int, 1>())) {
+      }
     }
   }
   write_rows<T, DP>(a, p.b, p.c, p.split, row, rows.o, rows.top, halves_sum(rows.sum), kBias);
@@ -226,35 +229,36 @@ __global__ __launch_bounds__(256) void cross_attention_few(CrossArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[8 * kTile + kMaskChunk / 8 + 4 * 32 * 4];
   const Place p(a);
   const int t = threadIdx.x, w = t >> 6, l = t & 63, row = l & 31;
-  Rows<T, DP> rows;
+  Rows<T, DP, kBias> rows;
   rows.init(a, p.b, p.c, row);
   const T* k = (const T*)a.k + p.b * a.sk[0] + p.c * a.sk[2];
   const T* v = (const T*)a.v + p.b * a.sv[0] + p.c * a.sv[2];
   char* kt = lds + w * 2 * kTile;
-  KeyWords words{(uint64_t*)(lds + 8 * kTile), a.mask ? a.mask + p.b * a.smask : nullptr};
+  KeyWords words{(uint32_t*)(lds + 8 * kTile), a.mask ? a.mask + p.b * a.smask : nullptr};
   Stage<T, DP, 32, 64> sk, sv;
-  for (int64_t c0 = p.first; c0 < p.stop; c0 += kMaskChunk) {
+  sk.init(l, a.dim, a.sk[1]);
+  sv.init(l, a.dim, a.sv[1]);
+  for (int c0 = p.first; c0 < p.stop; c0 += kMaskChunk) {
     words.fill(c0, p.stop);
-    const int64_t end = min(c0 + kMaskChunk, p.stop);
-    auto next = [&](int64_t key) {
-      while (key < end && words.bits(key, 32) == 0) key += 128;
+    const int end = min(c0 + kMaskChunk, p.stop);
+    auto next = [&](int key) {
+      while (key < end && words.bits(key) == 0) key += 128;
       return key;
     };
-    auto load = [&](int64_t key) {
-      sk.load(l, a.dim, [&](int r) { return k + min(key + r, a.n - 1) * a.sk[1]; });
-      sv.load(l, a.dim, [&](int r) { return v + min(key + r, a.n - 1) * a.sv[1]; });
+    auto load = [&](int key) {
+      sk.load(l, k + key * a.sk[1], a.n - key, a.dim, a.sk[1]);
+      sv.load(l, v + key * a.sv[1], a.n - key, a.dim, a.sv[1]);
     };
-    int64_t key = next(c0 + 32 * w);
+    int key = next(c0 + 32 * w);
     if (key < end) load(key);
     while (key < end) {
-      const uint64_t bits = words.bits(key, 32);
-      auto live = [&](int r) { return (bits >> r) & 1; };
-      sk.store(l, a.dim, kt, live);
-      sv.store(l, a.dim, kt + kTile, live);
-      const int64_t after = next(key + 128);
+      const uint32_t bits = words.bits(key);
+      sk.store(l, kt, bits, a.dim);
+      sv.store(l, kt + kTile, bits, a.dim);
+      const int after = next(key + 128);
       if (after < end) load(after);
       wave_order();
-      rows.template attend<1, kBias>(a, kt, kt + kTile, key, bits);
+      rows.attend(a, kt, kt + kTile, key, bits);
       wave_order();
       key = after;
     }
@@ -267,8 +271,8 @@ __global__ __launch_bounds__(256) void cross_attention_few(CrossArgs a) {
   float top = ml[row];
 #pragma unroll
   for (int i = 1; i < 4; ++i) top = fmaxf(top, ml[i * 32 + row]);
-  const float c = (kBias ? 1.f : a.scale) * kLog2E, base = top == -INFINITY ? 0.f : top;
-  const float f = __builtin_amdgcn_exp2f((rows.top - base) * c);  // 0 for a wave without keys
+  const float base = top == -INFINITY ? 0.f : top;
+  const float f = __builtin_amdgcn_exp2f((rows.top - base) * rows.c);  // 0 for a wave without keys
   sum *= f;
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) rows.o[dt] *= f;
@@ -332,7 +336,7 @@ __global__ __launch_bounds__(256) void cross_attention_join(CrossArgs a, int bia
 struct Split {
   bool few;
   int row_blocks, splits;
-  int64_t keys;  // per split, a multiple of 128
+  int keys;  // per split, a multiple of 128
 };
 
 // Few rows run as many splits as give every compute unit two blocks, each of at least 128 keys (one tile a wave); many rows
@@ -346,7 +350,7 @@ Split plan(int dtype, int64_t batch, int64_t kv_heads, int64_t rows, int64_t n) 
   int64_t splits = blocks ? want / blocks : 1;
   const int64_t most = (n + least - 1) / least;
   splits = splits < 1 ? 1 : splits > most ? (most > 0 ? most : 1) : splits;
-  s.keys = ((n + splits - 1) / splits + 127) / 128 * 128;
+  s.keys = (int)(((n + splits - 1) / splits + 127) / 128 * 128);
   if (s.keys == 0) s.keys = 128;
   s.splits = (int)(n > 0 ? (n + s.keys - 1) / s.keys : 1);
   return s;
@@ -381,7 +385,8 @@ int cross_setup(CrossArgs& a, int dtype, const int64_t* shape, const int64_t* st
   BMX_REQUIRE(dtype == kF32 || dtype == kBF16, "cross_attention: dtype must be fp32 or bf16");
   BMX_REQUIRE(shape && strides, "cross_attention: null shape or strides");
   for (int i = 0; i < 6; ++i) BMX_REQUIRE(shape[i] >= 0, "cross_attention: negative size");
-  a.batch = shape[0], a.m = shape[1], a.n = shape[2];
+  BMX_REQUIRE(shape[2] < (1ll << 31) - (1 << 20), "cross_attention: too many keys");
+  a.batch = shape[0], a.m = shape[1], a.n = (int)shape[2];
   const int64_t heads = shape[3], kv = shape[4], dim = shape[5];
   BMX_REQUIRE(dim >= 8 && dim <= 128 && dim % 8 == 0, "cross_attention: head dim must be a multiple of 8 in [8, 128]");
   BMX_REQUIRE(heads >= 1 && heads <= 65536 && kv >= 1 && heads % kv == 0,
@@ -395,6 +400,9 @@ int cross_setup(CrossArgs& a, int dtype, const int64_t* shape, const int64_t* st
     BMX_REQUIRE(a.sq[i] % vec == 0 && a.sk[i] % vec == 0 && a.sv[i] % vec == 0,
                 "cross_attention: strides must be multiples of 16 bytes");
   }
+  BMX_REQUIRE(a.sq[1] >= 0 && a.sk[1] >= 0 && a.sv[1] >= 0 && a.sq[1] < kMaxStride && a.sk[1] < kMaxStride &&
+                  a.sv[1] < kMaxStride && heads * dim < kMaxStride,
+              "cross_attention: token strides must be below 2^22 elements");
   a.smask = strides[9];
   a.heads = (int)heads, a.kv_heads = (int)kv, a.group = (int)(heads / kv), a.dim = (int)dim, a.rows = (int)rows;
   a.scale = scale;

@@ -9,6 +9,8 @@
 // registers: no atomics, and the same bits on every run.  P and dS are rounded to
 // the operand's type for the products over them; delta is taken from the output before its rounding
 // (out + out_lo), so that dP - delta cancels as it does in the formula.
+#include <type_traits>
+
 #include "cross_attention.h"
 
 using namespace bmx;
@@ -77,9 +79,9 @@ __device__ __forceinline__ void store_rows(T* row, int dim, const f32x16& acc, i
 
 // P of a logits tile whose column is a query: maximum and log2 of the sum are the lane's.
 template <typename T, bool kBias>
-__device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, const T* bias, int64_t key, float2 st) {
+__device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, const T* bias, int key, float2 st) {
   if (kBias) {
-    const f32x16 b = bias_tile(bias, min(key, a.n - 1), a.n);
+    const f32x16 b = bias_tile(bias, key, a.n);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + b[r] - st.x) * kLog2E - st.y);
   } else if (sizeof(T) == 4) {  // as the forward pass: the difference first
@@ -92,20 +94,18 @@ __device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, const 
   }
 }
 
-template <typename T>
-constexpr int kKeys = sizeof(T) == 2 ? 64 : 32;
-
 // dQ: four waves of 32 rows over all keys, as the forward pass runs.
 template <typename T, int DP, bool kBias>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dq(CrossArgs a) {
-  constexpr int KT = kKeys<T>, kTile = KT * Tile<T, DP>::kRowBytes;
+  constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[4 * kTile + kMaskChunk / 8];
   int64_t at = xcd_position(blockIdx.x, gridDim.x);
   const int row_block = (int)(at % a.row_blocks);
   at /= a.row_blocks;
   const int c = (int)(at % a.kv_heads);
   const int64_t b = at / a.kv_heads;
-  const int t = threadIdx.x, row = row_block * 128 + (t >> 6) * 32 + (t & 31), h = lane_id() >> 5;
+  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), h = lane_id() >> 5;
+  const int row = row_block * 128 + w * 32 + (t & 31);
   const RowAt ra(a, c, row);
   RowOperand<T, DP> q, g;
   q.load((const T*)a.q + ra.q(a, b), a.dim, h);
@@ -113,55 +113,63 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   const float2 st = a.stats[ra.stat(a, b)];
   const float delta = a.delta[ra.stat(a, b)];
   const T* bias = (const T*)a.bias + ra.bias(a, b);
+  RowReads<T, DP> rr;
+  ColumnReads<T, DP> cr;
+  rr.init();
+  cr.init();
   f32x16 dq[DP / 32];
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) dq[dt] = zero16();
   const T* k = (const T*)a.k + b * a.sk[0] + c * a.sk[2];
   const T* v = (const T*)a.v + b * a.sv[0] + c * a.sv[2];
-  KeyWords words{(uint64_t*)(lds + 4 * kTile), a.mask ? a.mask + b * a.smask : nullptr};
-  Stage<T, DP, KT, 256> sk, sv;
-  int buf = 0;
-  for (int64_t c0 = 0; c0 < a.n; c0 += kMaskChunk) {
-    words.fill(c0, a.n);
-    const int64_t end = min(c0 + kMaskChunk, a.n);
-    auto next = [&](int64_t key) {
-      while (key < end && words.bits(key, KT) == 0) key += KT;
-      return key;
+  KeyWords words{(uint32_t*)(lds + 4 * kTile), a.mask ? a.mask + b * a.smask : nullptr};
+  Copy<T, DP, 32, 4> ck, cv;
+  ck.init(w, a.dim, a.sk[1]);
+  cv.init(w, a.dim, a.sv[1]);
+  const unsigned lds0 = lds_address(lds);
+  clear_tiles<T, DP, 256>(t, lds, 4 * kTile, a.dim);
+  const int chunk = a.mask ? kMaskChunk : a.n;
+  for (int c0 = 0; c0 < a.n; c0 += chunk) {
+    words.fill(c0, a.n);  // its barrier also ends the last chunk's reads of the tiles
+    const int end = min(c0 + chunk, a.n);
+    auto copy = [&](int key, unsigned tile) {
+      ck.issue(w, k + key * a.sk[1], a.n - key, a.dim, a.sk[1], tile);
+      cv.issue(w, v + key * a.sv[1], a.n - key, a.dim, a.sv[1], tile + kTile);
     };
-    auto load = [&](int64_t key) {
-      sk.load(t, a.dim, [&](int r) { return k + min(key + r, a.n - 1) * a.sk[1]; });
-      sv.load(t, a.dim, [&](int r) { return v + min(key + r, a.n - 1) * a.sv[1]; });
-    };
-    int64_t key = next(c0);
-    if (key < end) load(key);
-    while (key < end) {
-      const uint64_t bits = words.bits(key, KT);
-      char* kt = lds + buf * 2 * kTile;
-      auto live = [&](int r) { return (bits >> r) & 1; };
-      sk.store(t, a.dim, kt, live);
-      sv.store(t, a.dim, kt + kTile, live);
-      const int64_t after = next(key + KT);
-      if (after < end) load(after);
+    int key = words.next(c0, end);
+    auto step = [&](auto B) {
+      constexpr int kAt = decltype(B)::value * 2 * kTile, kOther = 2 * kTile - kAt;
+      const char *kt = lds + kAt, *vt = lds + kAt + kTile;
+      const uint32_t bits = words.bits(key);
+      const int after = words.next(key + 32, end);
+      wait_copies();
       __syncthreads();
-#pragma unroll
-      for (int u = 0; u < KT / 32; ++u) {
-        const uint32_t sub = (uint32_t)(bits >> (32 * u));
-        f32x16 s = product<T, DP>(kt, 32 * u, q, zero16());
-        const f32x16 dp = product<T, DP>(kt + kTile, 32 * u, g, zero16());
-        weights_of<T, kBias>(a, s, bias, key + 32 * u, st);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
-        if (sub != 0xffffffffu) {
-          const uint32_t mine = sub >> (4 * h);
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (!key_bit(mine, r)) s[r] = 0.f;
-        }
-        Weights<T> w;
-        w.set(s);
-        transposed_product<DP>(kt, 32 * u, w, dq);
+      if (after < end) copy(after, lds0 + kOther);
+      if (bits != ~0u) {  // what a left-out key holds must not meet its zero dS
+        clear_rows<T, DP, 32, 256>(t, lds + kAt, bits);
+        __syncthreads();
       }
-      buf ^= 1, key = after;
+      f32x16 s = product<T, DP>(kt, rr, q);
+      const f32x16 dp = product<T, DP>(vt, rr, g);
+      weights_of<T, kBias>(a, s, bias, key, st);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
+      if (bits != ~0u) {
+        const uint32_t mine = bits >> (16 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!key_bit(mine, r)) s[r] = 0.f;
+      }
+      Weights<T> wt;
+      wt.set(s);
+      transposed_product<DP>(kt, cr, wt, dq);
+      key = after;
+      return key < end;
+    };
+    if (key < end) {
+      copy(key, lds0);
+      while (step(std::integral_constant<int, 0>()) && step(std::integral_constant<int, 1>())) {
+      }
     }
   }
   if (row >= a.rows) return;
@@ -171,91 +179,113 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
 }
 
 // dK and dV: four waves of 32 keys (in the lanes, their K and V in registers) over all rows of the group's
-// heads in tiles of 32, so a shared key head's gradient is one sum in row order.
+// heads in tiles of 32 queries of one head, so a shared key head's gradient is one sum in row order.
+// Queries past the last repeat it with weights of zero.
 template <typename T, int DP, bool kBias>
 __global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void cross_attention_dkv(CrossArgs a) {
   constexpr bool kFirst = kBias || sizeof(T) == 4;
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
-  constexpr int kStat = 32 * 3 * 4 + 32 * 8;  // maximum (or the whole shift), log2 of the sum, delta; bias offset
-  __shared__ __attribute__((aligned(16))) char lds[4 * kTile + 2 * kStat + kMaskChunk / 8];
-  const int key_blocks = (int)((a.n + 127) / 128);
+  constexpr int kStat = 32 * 3 * 4;  // of a row: maximum (or the whole shift), log2 of the sum, delta
+  __shared__ __attribute__((aligned(16))) char lds[4 * kTile + 2 * kStat + 16];
+  const int key_blocks = (a.n + 127) / 128;
   int64_t at = xcd_position(blockIdx.x, gridDim.x);
-  const int64_t first = (at % key_blocks) * 128;
+  const int first = (int)(at % key_blocks) * 128;
   at /= key_blocks;
   const int c = (int)(at % a.kv_heads);
   const int64_t b = at / a.kv_heads;
-  const int t = threadIdx.x, l = lane_id(), h = l >> 5;
-  const int64_t key = first + (t >> 6) * 32 + (l & 31), safe = min(key, a.n - 1);
-  KeyWords words{(uint64_t*)(lds + 4 * kTile + 2 * kStat), a.mask ? a.mask + b * a.smask : nullptr};
+  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = lane_id(), h = l >> 5;
+  const int key = first + w * 32 + (l & 31), safe = min(key, a.n - 1);
+  KeyWords words{(uint32_t*)(lds + 4 * kTile + 2 * kStat), a.mask ? a.mask + b * a.smask : nullptr};
   words.fill(first, min(first + 128, a.n));
-  const uint64_t lo = words.bits(first, 64), hi = words.bits(first + 64, 64);
-  const bool live = ((t >> 7 ? hi : lo) >> (t >> 6 & 1 ? 32 + (l & 31) : l & 31)) & 1;
-  RowOperand<T, DP> kf, vf;
+  const bool live = (words.bits(first + w * 32) >> (l & 31)) & 1;
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) any |= words.bits(first + 32 * i);
   f32x16 dk[DP / 32], dv[DP / 32];
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) dk[dt] = zero16(), dv[dt] = zero16();
-  if ((lo | hi) != 0) {
+  if (any) {
+    RowOperand<T, DP> kf, vf;
     kf.load((const T*)a.k + b * a.sk[0] + safe * a.sk[1] + c * a.sk[2], a.dim, h);
     vf.load((const T*)a.v + b * a.sv[0] + safe * a.sv[1] + c * a.sv[2], a.dim, h);
-    Stage<T, DP, 32, 256> sq, sg;
+    RowReads<T, DP> rr;
+    ColumnReads<T, DP> cr;
+    rr.init();
+    cr.init();
+    const int64_t row_step = (int64_t)a.heads * a.dim;
+    Copy<T, DP, 32, 4> cq, cg;
+    cq.init(w, a.dim, a.sq[1]);
+    cg.init(w, a.dim, row_step);
+    const unsigned lds0 = lds_address(lds);
+    clear_tiles<T, DP, 256>(t, lds, 4 * kTile, a.dim);
+    const int m = (int)a.m;
     float2 st;
     float delta;
-    int64_t bias_at;
-    auto load = [&](int row0) {
-      sq.load(t, a.dim, [&](int r) { return (const T*)a.q + RowAt(a, c, row0 + r).q(a, b); });
-      sg.load(t, a.dim, [&](int r) { return (const T*)a.dout + RowAt(a, c, row0 + r).dense(a, b); });
-      if (t < 32) {
-        const RowAt ra(a, c, row0 + t);
-        st = a.stats[ra.stat(a, b)], delta = a.delta[ra.stat(a, b)];
-        if (kBias) bias_at = ra.bias(a, b);
-        if (row0 + t >= a.rows) st = make_float2(0.f, INFINITY), delta = 0.f;
-      }
+    auto copy = [&](int g, int i, unsigned tile) {
+      const int64_t head = (int64_t)c * a.group + g;
+      cq.issue(w, (const T*)a.q + b * a.sq[0] + i * a.sq[1] + head * a.sq[2], m - i, a.dim, a.sq[1], tile);
+      cg.issue(w, (const T*)a.dout + ((b * a.m + i) * a.heads + head) * a.dim, m - i, a.dim, row_step, tile + kTile);
     };
-    load(0);
-    int buf = 0;
-    for (int row0 = 0; row0 < a.rows; row0 += 32, buf ^= 1) {
-      char* qt = lds + buf * 2 * kTile;
-      char* gt = qt + kTile;
-      float* stat = (float*)(lds + 4 * kTile + buf * kStat);
-      int64_t* offs = (int64_t*)(stat + 96);
-      auto in = [&](int r) { return row0 + r < a.rows; };
-      sq.store(t, a.dim, qt, in);
-      sg.store(t, a.dim, gt, in);
+    auto load_stats = [&](int g, int i) {
+      const int64_t stat = (b * a.heads + (int64_t)c * a.group + g) * a.m + min(i + (t & 31), m - 1);
+      st = a.stats[stat], delta = a.delta[stat];
+      if (i + (t & 31) >= m) st = make_float2(0.f, INFINITY), delta = 0.f;
+    };
+    int g = 0, i = 0;
+    auto step = [&](auto B) {
+      constexpr int kAt = decltype(B)::value * 2 * kTile, kOther = 2 * kTile - kAt;
+      const char *qt = lds + kAt, *gt = lds + kAt + kTile;
+      float* stat = (float*)(lds + 4 * kTile + decltype(B)::value * kStat);
       if (t < 32) {
         stat[t] = kFirst ? st.x : st.x * kLog2E + st.y;
         stat[32 + t] = st.y;
         stat[64 + t] = delta;
-        if (kBias) offs[t] = bias_at;
       }
-      if (row0 + 32 < a.rows) load(row0 + 32);
+      const T* bias = (const T*)a.bias + b * a.sb[0] + ((int64_t)c * a.group + g) * a.sb[1] + safe;
+      const int i0 = i;
+      i += 32;
+      if (i >= m) i = 0, ++g;
+      const bool more = g < a.group;
+      wait_copies();
       __syncthreads();
-      f32x16 s = product<T, DP>(qt, 0, kf, zero16());
-      const f32x16 dp = product<T, DP>(gt, 0, vf, zero16());
+      if (more) {
+        copy(g, i, lds0 + kOther);
+        load_stats(g, i);
+      }
+      f32x16 s = product<T, DP>(qt, rr, kf);
+      const f32x16 dp = product<T, DP>(gt, rr, vf);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 top = *(const f32x4*)(stat + 8 * g + 4 * h);
+      for (int g4 = 0; g4 < 4; ++g4) {
+        const f32x4 top = *(const f32x4*)(stat + 4 * g4 + 16 * h);
+        f32x4 log;
+        if (kFirst) log = *(const f32x4*)(stat + 32 + 4 * g4 + 16 * h);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int r = 4 * g + e;
+          const int r = 4 * g4 + e;
           if (kFirst) {
-            const float x = kBias ? (float)((const T*)a.bias)[offs[8 * g + 4 * h + e] + safe] : 0.f;
-            s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + x - top[e]) * kLog2E - stat[32 + 8 * g + 4 * h + e]);
+            const float x = kBias ? (float)bias[min(i0 + 16 * h + r, m - 1) * a.sb[2]] : 0.f;
+            s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + x - top[e]) * kLog2E - log[e]);
           } else {
             s[r] = __builtin_amdgcn_exp2f(s[r] * (a.scale * kLog2E) - top[e]);
           }
         }
       }
-      Weights<T> w;
-      w.set(s);
-      transposed_product<DP>(gt, 0, w, dv);
+      Weights<T> wt;
+      wt.set(s);
+      transposed_product<DP>(gt, cr, wt, dv);
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const f32x4 dl = *(const f32x4*)(stat + 64 + 8 * g + 4 * h);
+      for (int g4 = 0; g4 < 4; ++g4) {
+        const f32x4 dl = *(const f32x4*)(stat + 64 + 4 * g4 + 16 * h);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[4 * g + e] *= dp[4 * g + e] - dl[e];
+        for (int e = 0; e < 4; ++e) s[4 * g4 + e] *= dp[4 * g4 + e] - dl[e];
       }
-      w.set(s);
-      transposed_product<DP>(qt, 0, w, dk);
+      wt.set(s);
+      transposed_product<DP>(qt, cr, wt, dk);
+      return more;
+    };
+    copy(0, 0, lds0);
+    load_stats(0, 0);
+    while (step(std::integral_constant<int, 0>()) && step(std::integral_constant<int, 1>())) {
     }
   }
   if (key >= a.n) return;
@@ -267,15 +297,15 @@ __global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void cross_attention_dkv(Cros
   }
 }
 
-// dbias: a block holds 128 queries x 64 (fp32: 32) keys of one bias plane in registers and walks the batch elements and
-// heads that share the plane, in order.
+// dbias: a block holds 128 queries x 32 keys of one bias plane in registers and walks the batch elements and
+// heads that share the plane, in order. Keys and values go through one LDS buffer by DMA.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dbias(CrossArgs a) {
-  constexpr int KT = kKeys<T>, kTile = KT * Tile<T, DP>::kRowBytes;
-  __shared__ __attribute__((aligned(16))) char lds[4 * kTile + kMaskChunk / 8];
-  const int key_blocks = (int)((a.n + KT - 1) / KT), query_blocks = (int)((a.m + 127) / 128);
+  constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
+  __shared__ __attribute__((aligned(16))) char lds[4 * kTile + 16];
+  const int key_blocks = (a.n + 31) / 32, query_blocks = (int)((a.m + 127) / 128);
   int64_t at = xcd_position(blockIdx.x, gridDim.x);
-  const int64_t key = (at % key_blocks) * KT;
+  const int key = (int)(at % key_blocks) * 32;
   at /= key_blocks;
   const int q0 = (int)(at % query_blocks) * 128;
   at /= query_blocks;
@@ -283,25 +313,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   const int64_t ph = at % plane_heads, pb = at / plane_heads;
   const int64_t b0 = a.sdb[0] ? pb : 0, b1 = a.sdb[0] ? pb + 1 : a.batch;
   const int h0 = a.sdb[1] ? (int)ph : 0, h1 = a.sdb[1] ? (int)ph + 1 : a.heads;
-  const int t = threadIdx.x, h = lane_id() >> 5;
-  const int64_t i = q0 + (t >> 6) * 32 + (t & 31), safe = min(i, a.m - 1);
-  f32x16 sum[KT / 32];
-#pragma unroll
-  for (int u = 0; u < KT / 32; ++u) sum[u] = zero16();
-  KeyWords words{(uint64_t*)(lds + 4 * kTile), nullptr};
-  Stage<T, DP, KT, 256> sk, sv;
+  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), h = lane_id() >> 5;
+  const int64_t i = q0 + w * 32 + (t & 31), safe = min(i, a.m - 1);
+  f32x16 sum = zero16();
+  KeyWords words{(uint32_t*)(lds + 4 * kTile), nullptr};
+  RowReads<T, DP> rr;
+  rr.init();
+  Copy<T, DP, 32, 4> ck, cv;
+  ck.init(w, a.dim, a.sk[1]);
+  cv.init(w, a.dim, a.sv[1]);
+  const unsigned lds0 = lds_address(lds);
+  clear_tiles<T, DP, 256>(t, lds, 4 * kTile, a.dim);
   int buf = 0;
   for (int64_t b = b0; b < b1; ++b) {
     words.mask = a.mask ? a.mask + b * a.smask : nullptr;
-    words.fill(key, min(key + KT, a.n));
-    const uint64_t bits = words.bits(key, KT);
+    words.fill(key, min(key + 32, a.n));
+    const uint32_t bits = words.bits(key), mine = bits >> (16 * h);
     if (bits == 0) continue;
     for (int head = h0; head < h1; ++head) {
       const int c = head / a.group;
-      const T* k = (const T*)a.k + b * a.sk[0] + c * a.sk[2];
-      const T* v = (const T*)a.v + b * a.sv[0] + c * a.sv[2];
-      sk.load(t, a.dim, [&](int r) { return k + min(key + r, a.n - 1) * a.sk[1]; });
-      sv.load(t, a.dim, [&](int r) { return v + min(key + r, a.n - 1) * a.sv[1]; });
+      const unsigned tile = lds0 + buf * 2 * kTile;
+      ck.issue(w, (const T*)a.k + b * a.sk[0] + c * a.sk[2] + key * a.sk[1], a.n - key, a.dim, a.sk[1], tile);
+      cv.issue(w, (const T*)a.v + b * a.sv[0] + c * a.sv[2] + key * a.sv[1], a.n - key, a.dim, a.sv[1], tile + kTile);
       RowOperand<T, DP> q, g;
       q.load((const T*)a.q + b * a.sq[0] + safe * a.sq[1] + head * a.sq[2], a.dim, h);
       g.load((const T*)a.dout + ((b * a.m + safe) * a.heads + head) * a.dim, a.dim, h);
@@ -309,32 +342,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
       const float2 st = a.stats[stat];
       const float delta = a.delta[stat];
       const T* bias = (const T*)a.bias + b * a.sb[0] + head * a.sb[1] + safe * a.sb[2];
-      char* kt = lds + buf * 2 * kTile;
-      auto live = [&](int r) { return (bits >> r) & 1; };
-      sk.store(t, a.dim, kt, live);
-      sv.store(t, a.dim, kt + kTile, live);
+      wait_copies();
       __syncthreads();
+      f32x16 s = product<T, DP>(lds + buf * 2 * kTile, rr, q);
+      const f32x16 dp = product<T, DP>(lds + buf * 2 * kTile + kTile, rr, g);
+      weights_of<T, true>(a, s, bias, key, st);
 #pragma unroll
-      for (int u = 0; u < KT / 32; ++u) {
-        const uint32_t mine = (uint32_t)(bits >> (32 * u)) >> (4 * h);
-        f32x16 s = product<T, DP>(kt, 32 * u, q, zero16());
-        const f32x16 dp = product<T, DP>(kt + kTile, 32 * u, g, zero16());
-        weights_of<T, true>(a, s, bias, key + 32 * u, st);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sum[u][r] += key_bit(mine, r) ? s[r] * (dp[r] - delta) : 0.f;
-      }
+      for (int r = 0; r < 16; ++r) sum[r] += key_bit(mine, r) ? s[r] * (dp[r] - delta) : 0.f;
       buf ^= 1;
     }
   }
   if (i >= a.m) return;
   T* out = (T*)a.dbias + pb * a.sdb[0] + ph * a.sdb[1] + i * a.sdb[2];
 #pragma unroll
-  for (int u = 0; u < KT / 32; ++u)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int64_t at_key = key + 32 * u + 8 * (r >> 2) + 4 * h + (r & 3);
-      if (at_key < a.n) out[at_key] = (T)sum[u][r];
-    }
+  for (int r = 0; r < 16; ++r) {
+    const int at_key = key + 16 * h + r;
+    if (at_key < a.n) out[at_key] = (T)sum[r];
+  }
 }
 
 template <typename T, int DP>
@@ -342,7 +366,7 @@ int launch(CrossArgs& a, hipStream_t stream) {
   const int64_t lists = a.batch * a.kv_heads, key_blocks = (a.n + 127) / 128;
   a.row_blocks = (a.rows + 127) / 128;
   const int64_t planes = (a.sdb[0] ? a.batch : 1) * (a.sdb[1] ? a.heads : 1);
-  const int64_t bias_blocks = planes * ((a.m + 127) / 128) * ((a.n + kKeys<T> - 1) / kKeys<T>);
+  const int64_t bias_blocks = planes * ((a.m + 127) / 128) * ((a.n + 31) / 32);
   const int64_t delta_blocks = (a.batch * a.m * a.heads + 15) / 16;
   BMX_REQUIRE(lists * a.row_blocks < (1ll << 31) && lists * key_blocks < (1ll << 31) && bias_blocks < (1ll << 31) &&
                   delta_blocks < (1ll << 31),

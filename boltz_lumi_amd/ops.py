@@ -1394,9 +1394,9 @@ def relative_bias(table, q_pos, k_pos, exact=None, max_distance=128, bidirection
 
 def _head_tokens(x):
     """``x`` [B, T, H, D] with a dense last axis, outer strides of multiples of
-    16 bytes and 16-byte alignment: itself, or a dense copy."""
+    16 bytes (a token's below 2^22 elements) and 16-byte alignment: itself, or a dense copy."""
     vec = 16 // x.element_size()
-    ok = x.stride(3) == 1 and x.data_ptr() % 16 == 0
+    ok = x.stride(3) == 1 and x.data_ptr() % 16 == 0 and x.stride(1) < 1 << 22
     if not ok or any(x.stride(i) % vec for i in range(3) if x.shape[i] > 1):
         return _aligned(x.contiguous())
     return x
@@ -1483,6 +1483,7 @@ def cross_attention(q, k, v, mask=None, bias=None, scale=None):
            "k and v must match q's batch, head dim and dtype")
     _check(8 <= d <= 128 and d % 8 == 0, "head dim must be a multiple of 8 in [8, 128]")
     _check(h > 0 and hk > 0 and h % hk == 0, "the query heads must be a multiple of the key heads")
+    _check(h * d < 1 << 22, "expected fewer than 2^22 channels")
     scale = d ** -0.5 if scale is None else float(scale)
     _check(0 < scale < float("inf"), "scale must be positive and finite")
     if mask is not None:
