@@ -101,25 +101,31 @@ __device__ __forceinline__ f32x16 mfma_step(const float*, u32x4 a, u32x4 b, f32x
 // Tile row of A-operand row i.
 __device__ __forceinline__ int tile_row(int i) { return 16 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3); }
 
-// Where a lane reads its parts of a 32-row tile, worked out once: with the tile's position a constant of the unrolled
-// loops, a read is one register and an immediate.
-template <typename T, int DP>
+// Where a lane reads its parts of a 32-row tile. kKeep: every offset in a register, worked out once; with the tile's
+// position a constant of an unrolled loop a read is then that register and an immediate. Else the first
+// one, from which the others differ by an exclusive or with a constant (one instruction with the tile's position added):
+// for kernels that are short of registers.
+template <typename T, int DP, bool kKeep = true>
 struct RowReads {
-  int off[RowOperand<T, DP>::kSteps];
+  int off[kKeep ? RowOperand<T, DP>::kSteps : 1];
   __device__ __forceinline__ void init() {
     const int r = tile_row(lane_id() & 31), h = lane_id() >> 5;
 #pragma unroll
-    for (int s = 0; s < RowOperand<T, DP>::kSteps; ++s) off[s] = Tile<T, DP>::at(r, 2 * s + h);
+    for (int s = 0; s < (kKeep ? RowOperand<T, DP>::kSteps : 1); ++s) off[s] = Tile<T, DP>::at(r, 2 * s + h);
   }
+  __device__ __forceinline__ int at(int s) const { return kKeep ? off[s] : off[0] ^ (s << 5); }
+  // In a loop: keeps the compiler from working the others out before it.
+  __device__ __forceinline__ void renew() { asm volatile("" : "+v"(off[0])); }
 };
 
 // Tile rows (A) times the operand's columns (B), over the channels.
-template <typename T, int DP>
-__device__ __forceinline__ f32x16 product(const char* tile, const RowReads<T, DP>& at, const RowOperand<T, DP>& b) {
+template <typename T, int DP, bool kKeep>
+__device__ __forceinline__ f32x16 product(const char* tile, const RowReads<T, DP, kKeep>& reads,
+                                          const RowOperand<T, DP>& b) {
   f32x16 acc = zero16();
 #pragma unroll
   for (int s = 0; s < RowOperand<T, DP>::kSteps; ++s)
-    acc = mfma_step((const T*)nullptr, *(const u32x4*)(tile + at.off[s]), b.c[s], acc);
+    acc = mfma_step((const T*)nullptr, *(const u32x4*)(tile + reads.at(s)), b.c[s], acc);
   return acc;
 }
 
@@ -158,22 +164,27 @@ struct Weights<float> {
 };
 
 // acc[dt] += (tile rows)^T (channels 32 dt .. as rows) times the weights, over the rows.
-template <typename T, int DP>
+template <typename T, int DP, bool kKeep = true>
 struct ColumnReads;
-template <int DP>
-struct ColumnReads<bf16, DP> {
-  int off[4][DP / 32];  // of four rows each
+template <int DP, bool kKeep>
+struct ColumnReads<bf16, DP, kKeep> {
+  int off[4][kKeep ? DP / 32 : 1];  // of four rows each
   __device__ __forceinline__ void init() {
     const int l = lane_id(), h = l >> 5, i = l & 15, chunk = 2 * ((l >> 4) & 1) + ((i & 3) >> 1);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
-      for (int dt = 0; dt < DP / 32; ++dt)
+      for (int dt = 0; dt < (kKeep ? DP / 32 : 1); ++dt)
         off[u][dt] = Tile<bf16, DP>::at(16 * h + 4 * u + (i >> 2), 4 * dt + chunk) + 8 * (i & 1);
   }
+  __device__ __forceinline__ int at(int u, int dt) const { return kKeep ? off[u][dt] : off[u][0] ^ (dt << 6); }
+  __device__ __forceinline__ void renew() {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) asm volatile("" : "+v"(off[u][0]));
+  }
 };
-template <int DP>
-__device__ __forceinline__ void transposed_product(const char* tile, const ColumnReads<bf16, DP>& at,
+template <int DP, bool kKeep>
+__device__ __forceinline__ void transposed_product(const char* tile, const ColumnReads<bf16, DP, kKeep>& reads,
                                                    const Weights<bf16>& w, f32x16 (&acc)[DP / 32]) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
@@ -186,16 +197,17 @@ __device__ __forceinline__ void transposed_product(const char* tile, const Colum
 #pragma unroll
       for (int u = 0; u < 2; ++u)
         a.half[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-            (__attribute__((address_space(3))) s16x4*)(tile + at.off[2 * t + u][dt]));
+            (__attribute__((address_space(3))) s16x4*)(tile + reads.at(2 * t + u, dt)));
       acc[dt] = mfma32(a.all, w.v[t], acc[dt]);
     }
 }
-template <int DP>
-struct ColumnReads<float, DP> {
+template <int DP, bool kKeep>
+struct ColumnReads<float, DP, kKeep> {
   __device__ __forceinline__ void init() {}
+  __device__ __forceinline__ void renew() {}
 };
-template <int DP>
-__device__ __forceinline__ void transposed_product(const char* tile, const ColumnReads<float, DP>&,
+template <int DP, bool kKeep>
+__device__ __forceinline__ void transposed_product(const char* tile, const ColumnReads<float, DP, kKeep>&,
                                                    const Weights<float>& w, f32x16 (&acc)[DP / 32]) {
   const int l = lane_id(), h = l >> 5, i = l & 31;
 #pragma unroll
@@ -307,7 +319,7 @@ struct Copy {
 // Zeros in `bytes` of LDS by THREADS threads, where tiles have chunks past dim.
 template <typename T, int DP, int THREADS>
 __device__ __forceinline__ void clear_tiles(int t, char* lds, int bytes, int dim) {
-  if (dim == Tile<T, DP>::kRow * Tile<T, DP>::kElems) return;
+  if (dim == DP) return;  // chunks past DP are never read
   for (int at = 16 * t; at < bytes; at += 16 * THREADS) *(u32x4*)(lds + at) = u32x4{0, 0, 0, 0};
   __syncthreads();
 }

@@ -178,15 +178,18 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   for (int dt = 0; dt < DP / 32; ++dt) store_rows(out, a.dim, dq[dt], dt, a.scale, true);
 }
 
-// dK and dV: four waves of 32 keys (in the lanes, their K and V in registers) over all rows of the group's
-// heads in tiles of 32 queries of one head, so a shared key head's gradient is one sum in row order.
-// Queries past the last repeat it with weights of zero.
+// dK and dV: four waves of 32 keys (in the lanes, in tile_row order) over all rows of the group's heads in
+// tiles of 32 queries of one head, so a shared key head's gradient is one sum in row order.
+// Queries past the last repeat it with weights of zero. A wave's K, and V for narrow heads, are in registers;
+// bf16 heads past 64 channels keep V in LDS, which makes room for two waves on a SIMD.
 template <typename T, int DP, bool kBias>
-__global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void cross_attention_dkv(CrossArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dkv(CrossArgs a) {
+  constexpr bool kValuesInLds = sizeof(T) == 2 && DP > 64;
   constexpr bool kFirst = kBias || sizeof(T) == 4;
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   constexpr int kStat = 32 * 3 * 4;  // of a row: maximum (or the whole shift), log2 of the sum, delta
-  __shared__ __attribute__((aligned(16))) char lds[4 * kTile + 2 * kStat + 16];
+  constexpr int kValues = 4 * kTile + 2 * kStat + 16;  // V of the block's 128 keys
+  __shared__ __attribute__((aligned(16))) char lds[kValues + (kValuesInLds ? 4 * kTile : 0)];
   const int key_blocks = (a.n + 127) / 128;
   int64_t at = xcd_position(blockIdx.x, gridDim.x);
   const int first = (int)(at % key_blocks) * 128;
@@ -194,10 +197,10 @@ __global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void cross_attention_dkv(Cros
   const int c = (int)(at % a.kv_heads);
   const int64_t b = at / a.kv_heads;
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = lane_id(), h = l >> 5;
-  const int key = first + w * 32 + (l & 31), safe = min(key, a.n - 1);
+  const int lane_key = tile_row(l & 31), key = first + w * 32 + lane_key, safe = min(key, a.n - 1);
   KeyWords words{(uint32_t*)(lds + 4 * kTile + 2 * kStat), a.mask ? a.mask + b * a.smask : nullptr};
   words.fill(first, min(first + 128, a.n));
-  const bool live = (words.bits(first + w * 32) >> (l & 31)) & 1;
+  const bool live = (words.bits(first + w * 32) >> lane_key) & 1;
   uint32_t any = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) any |= words.bits(first + 32 * i);
@@ -207,9 +210,9 @@ __global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void cross_attention_dkv(Cros
   if (any) {
     RowOperand<T, DP> kf, vf;
     kf.load((const T*)a.k + b * a.sk[0] + safe * a.sk[1] + c * a.sk[2], a.dim, h);
-    vf.load((const T*)a.v + b * a.sv[0] + safe * a.sv[1] + c * a.sv[2], a.dim, h);
-    RowReads<T, DP> rr;
-    ColumnReads<T, DP> cr;
+    if (!kValuesInLds) vf.load((const T*)a.v + b * a.sv[0] + safe * a.sv[1] + c * a.sv[2], a.dim, h);
+    RowReads<T, DP, !kValuesInLds> rr;
+    ColumnReads<T, DP, !kValuesInLds> cr;
     rr.init();
     cr.init();
     const int64_t row_step = (int64_t)a.heads * a.dim;
@@ -218,6 +221,16 @@ __global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void cross_attention_dkv(Cros
     cg.init(w, a.dim, row_step);
     const unsigned lds0 = lds_address(lds);
     clear_tiles<T, DP, 256>(t, lds, 4 * kTile, a.dim);
+    if (kValuesInLds) {  // waited for with the first tile; each wave reads the 32 rows of its keys
+      Copy<T, DP, 128, 4> values;
+      values.init(w, a.dim, a.sv[1]);
+      if (a.dim != DP) {
+        for (int z = 16 * t; z < 4 * kTile; z += 16 * 256) *(u32x4*)(lds + kValues + z) = u32x4{0, 0, 0, 0};
+        __syncthreads();
+      }
+      values.issue(w, (const T*)a.v + b * a.sv[0] + first * a.sv[1] + c * a.sv[2], a.n - first, a.dim, a.sv[1],
+                   lds0 + kValues);
+    }
     const int m = (int)a.m;
     float2 st;
     float delta;
@@ -232,10 +245,11 @@ __global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void cross_attention_dkv(Cros
       if (i + (t & 31) >= m) st = make_float2(0.f, INFINITY), delta = 0.f;
     };
     int g = 0, i = 0;
-    auto step = [&](auto B) {
-      constexpr int kAt = decltype(B)::value * 2 * kTile, kOther = 2 * kTile - kAt;
-      const char *qt = lds + kAt, *gt = lds + kAt + kTile;
-      float* stat = (float*)(lds + 4 * kTile + decltype(B)::value * kStat);
+    auto step = [&](auto buffer) {  // one tile; false after the last
+      const int buf = buffer;
+      if (kValuesInLds) rr.renew(), cr.renew();
+      const char *qt = lds + buf * 2 * kTile, *gt = qt + kTile;
+      float* stat = (float*)(lds + 4 * kTile + buf * kStat);
       if (t < 32) {
         stat[t] = kFirst ? st.x : st.x * kLog2E + st.y;
         stat[32 + t] = st.y;
@@ -249,11 +263,10 @@ __global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void cross_attention_dkv(Cros
       wait_copies();
       __syncthreads();
       if (more) {
-        copy(g, i, lds0 + kOther);
+        copy(g, i, lds0 + (buf ^ 1) * 2 * kTile);
         load_stats(g, i);
       }
       f32x16 s = product<T, DP>(qt, rr, kf);
-      const f32x16 dp = product<T, DP>(gt, rr, vf);
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4) {
         const f32x4 top = *(const f32x4*)(stat + 4 * g4 + 16 * h);
@@ -270,22 +283,45 @@ __global__ __launch_bounds__(256, DP > 64 ? 1 : 2) void cross_attention_dkv(Cros
           }
         }
       }
-      Weights<T> wt;
-      wt.set(s);
-      transposed_product<DP>(gt, cr, wt, dv);
+      if (kValuesInLds) __builtin_amdgcn_sched_barrier(0);
+      {
+        Weights<T> wt;
+        wt.set(s);
+        transposed_product<DP>(gt, cr, wt, dv);
+      }
+      if (kValuesInLds) __builtin_amdgcn_sched_barrier(0);
+      f32x16 dp;
+      if (kValuesInLds) {
+        dp = zero16();
+#pragma unroll
+        for (int u = 0; u < RowOperand<T, DP>::kSteps; ++u) {
+          dp = mfma_step((const T*)nullptr, *(const u32x4*)(gt + rr.at(u)),
+                         *(const u32x4*)(lds + kValues + w * kTile + rr.at(u)), dp);
+          if (u % 2) __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {
+        dp = product<T, DP>(gt, rr, vf);
+      }
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4) {
         const f32x4 dl = *(const f32x4*)(stat + 64 + 4 * g4 + 16 * h);
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[4 * g4 + e] *= dp[4 * g4 + e] - dl[e];
       }
+      if (kValuesInLds) __builtin_amdgcn_sched_barrier(0);
+      Weights<T> wt;
       wt.set(s);
       transposed_product<DP>(qt, cr, wt, dk);
       return more;
     };
     copy(0, 0, lds0);
     load_stats(0, 0);
-    while (step(std::integral_constant<int, 0>()) && step(std::integral_constant<int, 1>())) {
+    if (kValuesInLds) {
+      for (int buf = 0; step(buf); buf ^= 1) {
+      }
+    } else {
+      while (step(std::integral_constant<int, 0>()) && step(std::integral_constant<int, 1>())) {
+      }
     }
   }
   if (key >= a.n) return;
