@@ -93,7 +93,7 @@ SIGNATURES = {
     "bmx_relative_bias_bwd": (c_int, _RELATIVE + [_P, _P, c_size_t, _P]),
     "bmx_cross_attention_workspace_bytes": (c_size_t, [c_int] + [c_int64] * 6),
     "bmx_cross_attention_fwd": (c_int, _CROSS + [_P, _P, _P, _P, c_size_t, _P]),
-    "bmx_cross_attention_bwd_workspace_bytes": (c_size_t, [c_int64] * 3),
+    "bmx_cross_attention_bwd_workspace_bytes": (c_size_t, [c_int64] * 6),
     "bmx_cross_attention_bwd": (c_int, _CROSS + [_P] * 8 + [_I64P, _P, c_size_t, _P]),
 }
 

@@ -36,8 +36,8 @@ struct CrossArgs {
   float2* stats;  // [batch][heads][m]: row maximum of the logits and log2 of the sum of exp(logit - maximum)
   // work split
   int row_blocks, splits;
-  int split_keys;
-  float* part_o;   // [split][batch * kv_heads][rows][dim] sums before the division
+  int split_keys;  // or, of dK and dV, tiles of 32 queries
+  float* part_o;   // [split][batch * kv_heads][rows][dim] sums before the division; backward: [split] gradients
   float2* part_ml;  // [split][batch * kv_heads][rows] maximum and sum
   // backward
   const void* dout;
@@ -280,7 +280,10 @@ struct Stage {
 // wave waits for its own copies of a tile (wait_copies) before the barrier that publishes the tile, and a tile is
 // overwritten only after a barrier that every wave reached with its reads of it done.
 __device__ __forceinline__ void lds_copy16(const void* base, uint32_t off, unsigned lds_addr) {
-  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(lds_addr) : "memory");
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uintptr_t)base);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)((uintptr_t)base >> 32));
+  const void* at = (const void*)((uintptr_t)hi << 32 | lo);
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(at), "{m0}"(lds_addr) : "memory");
 }
 __device__ __forceinline__ void wait_copies() { __builtin_amdgcn_s_waitcnt(0x0F70); }  // vmcnt(0)
 __device__ __forceinline__ unsigned lds_address(const void* p) {
@@ -375,35 +378,65 @@ struct KeyWords {
 };
 
 // ---- bias ----------------------------------------------------------------
-// Four consecutive bias values at any element alignment.
-typedef uint32_t u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
-typedef uint32_t u32x2_at2 __attribute__((ext_vector_type(2), aligned(2)));
-__device__ __forceinline__ f32x4 bias4(const float* p) { return __builtin_bit_cast(f32x4, (u32x4) * (const u32x4_at4*)p); }
-__device__ __forceinline__ f32x4 bias4(const bf16* p) {
-  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-  const bf16x4 v = __builtin_bit_cast(bf16x4, (u32x2) * (const u32x2_at2*)p);
-  return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
-}
-
-// Bias of the lane's query at the 16 keys of a logits tile from key `key` on, in register order; keys from n on
-// read the last one (they are masked).
+// Bias of a lane's query at the 16 keys of a logits tile, in register order, as it lies in memory: loaded a tile ahead,
+// together with the tile's copies, whose wait is then its own. bf16 rows at an odd element (an odd number of keys) are read
+// from the dword before and shifted: 16-byte loads at 2-byte alignment took 109 us against 74 at 1531 keys.
 template <typename T>
-__device__ __forceinline__ f32x16 bias_tile(const T* row, int key, int n) {
-  f32x16 b;
-  const int k = key + 16 * (lane_id() >> 5);
-  if (key + 32 <= n) {
+struct BiasTile;
+template <>
+struct BiasTile<float> {
+  typedef uint32_t u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+  u32x4 v[4];
+
+  // Keys from `key` on; those from n on repeat the last one (they are masked).
+  __device__ __forceinline__ void load(const float* row, int key, int n) {
+    const int k = key + 16 * (lane_id() >> 5);
+    if (key + 32 <= n) {
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const f32x4 v = bias4(row + k + 4 * g);
+      for (int i = 0; i < 4; ++i) v[i] = *(const u32x4_at4*)(row + k + 4 * i);
+    } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) b[4 * g + e] = v[e];
+      for (int r = 0; r < 16; ++r) v[r >> 2][r & 3] = __float_as_uint(row[min(k + r, n - 1)]);
     }
-  } else {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) b[r] = (float)row[min(k + r, n - 1)];
   }
-  return b;
-}
+  __device__ __forceinline__ void ready() {}
+  __device__ __forceinline__ float at(int r) const { return __uint_as_float(v[r >> 2][r & 3]); }
+};
+template <>
+struct BiasTile<bf16> {
+  typedef uint32_t u32x4_at4 __attribute__((ext_vector_type(4), aligned(4)));
+  u32x4 v[2];
+  uint32_t last, shift;
+
+  __device__ __forceinline__ void load(const bf16* row, int key, int n) {
+    const int k = key + 16 * (lane_id() >> 5);
+    if (key + 32 <= n) {
+      const uintptr_t at = (uintptr_t)(row + k), odd = at & 2;
+      const uint32_t* p = (const uint32_t*)(at - odd);  // every dword read holds one of the keys' values
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[i] = *(const u32x4_at4*)(p + 4 * i);
+      last = p[odd ? 8 : 7];
+      shift = (uint32_t)odd * 8;
+    } else {
+      uint16_t x[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x[r] = __builtin_bit_cast(uint16_t, row[min(k + r, n - 1)]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = x[2 * i] | (uint32_t)x[2 * i + 1] << 16;
+      last = shift = 0;
+    }
+  }
+  // Shifts the words into place: before the first at().
+  __device__ __forceinline__ void ready() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      v[i >> 2][i & 3] = __builtin_amdgcn_alignbit(i < 7 ? v[(i + 1) >> 2][(i + 1) & 3] : last, v[i >> 2][i & 3], shift);
+  }
+  __device__ __forceinline__ float at(int r) const {
+    const uint32_t w = v[r >> 3][(r >> 1) & 3];
+    return __uint_as_float(r & 1 ? w & 0xffff0000u : w << 16);
+  }
+};
 
 // Bit of register r's key in a logits tile whose 32 keys are `bits`, already shifted by 16 h.
 __device__ __forceinline__ bool key_bit(uint32_t bits, int r) { return (bits >> r) & 1; }

@@ -50,13 +50,14 @@ struct Rows {
     c = (kBias ? 1.f : a.scale) * kLog2E;
   }
 
-  // 32 keys: rows of the tiles, keys `key` .. of the sequence, presence bits.
-  __device__ __forceinline__ void attend(const CrossArgs& a, const char* kt, const char* vt, int key, uint32_t bits) {
+  // 32 keys: rows of the tiles, presence bits, bias.
+  __device__ __forceinline__ void attend(const CrossArgs& a, const char* kt, const char* vt, uint32_t bits,
+                                         BiasTile<T>& b) {
     f32x16 s = product<T, DP>(kt, kr, q);
     if (kBias) {
-      const f32x16 b = bias_tile(bias, key, a.n);
+      b.ready();
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = s[r] * a.scale + b[r];
+      for (int r = 0; r < 16; ++r) s[r] = s[r] * a.scale + b.at(r);
     }
     if (bits != ~0u) {
       const uint32_t mine = bits >> (16 * (lane_id() >> 5));
@@ -195,6 +196,7 @@ void cross_attention_wide(CrossArgs a) {
       cv.issue(w, v + key * a.sv[1], a.n - key, a.dim, a.sv[1], tile + kTile);
     };
     int key = words.next(c0, end);
+    BiasTile<T> bias[2];
     // One tile in the buffer at B; false after the last.
     auto step = [&](auto B) {
       constexpr int kAt = decltype(B)::value * 2 * kTile, kOther = 2 * kTile - kAt;
@@ -202,17 +204,21 @@ void cross_attention_wide(CrossArgs a) {
       const int after = words.next(key + 32, end);
       wait_copies();
       __syncthreads();
-      if (after < end) copy(after, lds0 + kOther);
+      if (after < end) {
+        copy(after, lds0 + kOther);
+        if (kBias) bias[1 - decltype(B)::value].load(rows.bias, after, a.n);
+      }
       if (bits != ~0u) {  // what a left-out value holds must not meet its weight of zero
         clear_rows<T, DP, 32, 256>(t, lds + kAt + kTile, bits);
         __syncthreads();
       }
-      rows.attend(a, lds + kAt, lds + kAt + kTile, key, bits);
+      rows.attend(a, lds + kAt, lds + kAt + kTile, bits, bias[decltype(B)::value]);
       key = after;
       return key < end;
     };
     if (key < end) {
       copy(key, lds0);
+      if (kBias) bias[0].load(rows.bias, key, a.n);
       while (step(std::integral_constant<int, 0>()) && step(std::integral_constant<int, 1>())) {
       }
     }
@@ -250,15 +256,23 @@ __global__ __launch_bounds__(256) void cross_attention_few(CrossArgs a) {
       sv.load(l, v + key * a.sv[1], a.n - key, a.dim, a.sv[1]);
     };
     int key = next(c0 + 32 * w);
-    if (key < end) load(key);
+    BiasTile<T> bias, ahead;
+    if (key < end) {
+      load(key);
+      if (kBias) ahead.load(rows.bias, key, a.n);
+    }
     while (key < end) {
       const uint32_t bits = words.bits(key);
       sk.store(l, kt, bits, a.dim);
       sv.store(l, kt + kTile, bits, a.dim);
+      bias = ahead;
       const int after = next(key + 128);
-      if (after < end) load(after);
+      if (after < end) {
+        load(after);
+        if (kBias) ahead.load(rows.bias, after, a.n);
+      }
       wave_order();
-      rows.attend(a, kt, kt + kTile, key, bits);
+      rows.attend(a, kt, kt + kTile, bits, bias);
       wave_order();
       key = after;
     }
@@ -403,6 +417,7 @@ int cross_setup(CrossArgs& a, int dtype, const int64_t* shape, const int64_t* st
   BMX_REQUIRE(a.sq[1] >= 0 && a.sk[1] >= 0 && a.sv[1] >= 0 && a.sq[1] < kMaxStride && a.sk[1] < kMaxStride &&
                   a.sv[1] < kMaxStride && heads * dim < kMaxStride,
               "cross_attention: token strides must be below 2^22 elements");
+  BMX_REQUIRE(a.sb[2] >= 0 && a.sb[2] < (1ll << 26), "cross_attention: the bias's query stride must be below 2^26 elements");
   a.smask = strides[9];
   a.heads = (int)heads, a.kv_heads = (int)kv, a.group = (int)(heads / kv), a.dim = (int)dim, a.rows = (int)rows;
   a.scale = scale;

@@ -79,11 +79,11 @@ __device__ __forceinline__ void store_rows(T* row, int dim, const f32x16& acc, i
 
 // P of a logits tile whose column is a query: maximum and log2 of the sum are the lane's.
 template <typename T, bool kBias>
-__device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, const T* bias, int key, float2 st) {
+__device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, BiasTile<T>& b, float2 st) {
   if (kBias) {
-    const f32x16 b = bias_tile(bias, key, a.n);
+    b.ready();
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + b[r] - st.x) * kLog2E - st.y);
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + b.at(r) - st.x) * kLog2E - st.y);
   } else if (sizeof(T) == 4) {  // as the forward pass: the difference first
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale - st.x) * kLog2E - st.y);
@@ -102,6 +102,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   int64_t at = xcd_position(blockIdx.x, gridDim.x);
   const int row_block = (int)(at % a.row_blocks);
   at /= a.row_blocks;
+  const int split = (int)(at % a.splits), first = split * a.split_keys, stop = min(first + a.split_keys, a.n);
+  at /= a.splits;
   const int c = (int)(at % a.kv_heads);
   const int64_t b = at / a.kv_heads;
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), h = lane_id() >> 5;
@@ -112,7 +114,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   g.load((const T*)a.dout + ra.dense(a, b), a.dim, h);
   const float2 st = a.stats[ra.stat(a, b)];
   const float delta = a.delta[ra.stat(a, b)];
-  const T* bias = (const T*)a.bias + ra.bias(a, b);
+  const T* bias_row = (const T*)a.bias + ra.bias(a, b);
   RowReads<T, DP> rr;
   ColumnReads<T, DP> cr;
   rr.init();
@@ -129,14 +131,15 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   const unsigned lds0 = lds_address(lds);
   clear_tiles<T, DP, 256>(t, lds, 4 * kTile, a.dim);
   const int chunk = a.mask ? kMaskChunk : a.n;
-  for (int c0 = 0; c0 < a.n; c0 += chunk) {
-    words.fill(c0, a.n);  // its barrier also ends the last chunk's reads of the tiles
-    const int end = min(c0 + chunk, a.n);
+  for (int c0 = first; c0 < stop; c0 += chunk) {
+    words.fill(c0, stop);  // its barrier also ends the last chunk's reads of the tiles
+    const int end = min(c0 + chunk, stop);
     auto copy = [&](int key, unsigned tile) {
       ck.issue(w, k + key * a.sk[1], a.n - key, a.dim, a.sk[1], tile);
       cv.issue(w, v + key * a.sv[1], a.n - key, a.dim, a.sv[1], tile + kTile);
     };
     int key = words.next(c0, end);
+    BiasTile<T> bias[2];
     auto step = [&](auto B) {
       constexpr int kAt = decltype(B)::value * 2 * kTile, kOther = 2 * kTile - kAt;
       const char *kt = lds + kAt, *vt = lds + kAt + kTile;
@@ -144,14 +147,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
       const int after = words.next(key + 32, end);
       wait_copies();
       __syncthreads();
-      if (after < end) copy(after, lds0 + kOther);
+      if (after < end) {
+        copy(after, lds0 + kOther);
+        if (kBias) bias[1 - decltype(B)::value].load(bias_row, after, a.n);
+      }
       if (bits != ~0u) {  // what a left-out key holds must not meet its zero dS
         clear_rows<T, DP, 32, 256>(t, lds + kAt, bits);
         __syncthreads();
       }
       f32x16 s = product<T, DP>(kt, rr, q);
       const f32x16 dp = product<T, DP>(vt, rr, g);
-      weights_of<T, kBias>(a, s, bias, key, st);
+      weights_of<T, kBias>(a, s, bias[decltype(B)::value], st);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
       if (bits != ~0u) {
@@ -168,21 +174,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
     };
     if (key < end) {
       copy(key, lds0);
+      if (kBias) bias[0].load(bias_row, key, a.n);
       while (step(std::integral_constant<int, 0>()) && step(std::integral_constant<int, 1>())) {
       }
     }
   }
   if (row >= a.rows) return;
-  T* out = (T*)a.dq + ra.dense(a, b);
+  float* part = a.part_o + split * a.batch * a.m * a.heads * a.dim + ra.dense(a, b);
 #pragma unroll
-  for (int dt = 0; dt < DP / 32; ++dt) store_rows(out, a.dim, dq[dt], dt, a.scale, true);
+  for (int dt = 0; dt < DP / 32; ++dt) {
+    if (a.splits > 1)
+      store_rows(part, a.dim, dq[dt], dt, a.scale, true);
+    else
+      store_rows((T*)a.dq + ra.dense(a, b), a.dim, dq[dt], dt, a.scale, true);
+  }
 }
 
 // dK and dV: four waves of 32 keys (in the lanes, in tile_row order) over all rows of the group's heads in
 // tiles of 32 queries of one head, so a shared key head's gradient is one sum in row order.
 // Queries past the last repeat it with weights of zero. A wave's K, and V for narrow heads, are in registers;
 // bf16 heads past 64 channels keep V in LDS, which makes room for two waves on a SIMD.
-template <typename T, int DP, bool kBias>
+// A bias of its own for every head and batch element has its gradient written here, as dS is at hand (kGrad).
+template <typename T, int DP, bool kBias, bool kGrad>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dkv(CrossArgs a) {
   constexpr bool kValuesInLds = sizeof(T) == 2 && DP > 64;
   constexpr bool kFirst = kBias || sizeof(T) == 4;
@@ -194,6 +207,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   int64_t at = xcd_position(blockIdx.x, gridDim.x);
   const int first = (int)(at % key_blocks) * 128;
   at /= key_blocks;
+  const int split = (int)(at % a.splits);
+  at /= a.splits;
   const int c = (int)(at % a.kv_heads);
   const int64_t b = at / a.kv_heads;
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = lane_id(), h = l >> 5;
@@ -201,7 +216,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   KeyWords words{(uint32_t*)(lds + 4 * kTile + 2 * kStat), a.mask ? a.mask + b * a.smask : nullptr};
   words.fill(first, min(first + 128, a.n));
   const bool live = (words.bits(first + w * 32) >> lane_key) & 1;
-  uint32_t any = 0;
+  uint32_t any = kGrad;  // left-out keys have a gradient of zero to write
 #pragma unroll
   for (int i = 0; i < 4; ++i) any |= words.bits(first + 32 * i);
   f32x16 dk[DP / 32], dv[DP / 32];
@@ -231,7 +246,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
       values.issue(w, (const T*)a.v + b * a.sv[0] + first * a.sv[1] + c * a.sv[2], a.n - first, a.dim, a.sv[1],
                    lds0 + kValues);
     }
-    const int m = (int)a.m;
+    const int m = (int)a.m, head_tiles = (m + 31) / 32;
+    int tile_at = split * a.split_keys;
+    const int tile_end = min(tile_at + a.split_keys, a.group * head_tiles);
     float2 st;
     float delta;
     auto copy = [&](int g, int i, unsigned tile) {
@@ -244,7 +261,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
       st = a.stats[stat], delta = a.delta[stat];
       if (i + (t & 31) >= m) st = make_float2(0.f, INFINITY), delta = 0.f;
     };
-    int g = 0, i = 0;
+    T bias[16];  // of the lane's key and 16 queries, a tile ahead
+    const uint32_t bias_lane = (uint32_t)(16 * h * a.sb[2]) + safe;
+    auto load_bias = [&](int g, int i) {
+      const T* at = (const T*)a.bias + b * a.sb[0] + ((int64_t)c * a.group + g) * a.sb[1];
+      if (i + 32 <= m) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bias[r] = (at + (i + r) * a.sb[2])[bias_lane];
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) bias[r] = at[min(i + 16 * h + r, m - 1) * a.sb[2] + safe];
+      }
+    };
+    int g = __builtin_amdgcn_readfirstlane(tile_at / head_tiles), i = (tile_at - g * head_tiles) * 32;
     auto step = [&](auto buffer) {  // one tile; false after the last
       const int buf = buffer;
       if (kValuesInLds) rr.renew(), cr.renew();
@@ -255,18 +284,29 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
         stat[32 + t] = st.y;
         stat[64 + t] = delta;
       }
-      const T* bias = (const T*)a.bias + b * a.sb[0] + ((int64_t)c * a.group + g) * a.sb[1] + safe;
-      const int i0 = i;
+      T* dbias = nullptr;
+      int left = 0;  // of the lane's 16 queries
+      if (kGrad) {
+        dbias = (T*)a.dbias + b * a.sdb[0] + ((int64_t)c * a.group + g) * a.sdb[1] + (i + 16 * h) * a.sdb[2] + key;
+        left = key < a.n ? m - i - 16 * h : 0;
+      }
       i += 32;
       if (i >= m) i = 0, ++g;
-      const bool more = g < a.group;
+      const bool more = ++tile_at < tile_end;
       wait_copies();
       __syncthreads();
+      float x[16];
+      if (kBias) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = (float)bias[r];
+      }
       if (more) {
         copy(g, i, lds0 + (buf ^ 1) * 2 * kTile);
         load_stats(g, i);
+        if (kBias) load_bias(g, i);
       }
-      f32x16 s = product<T, DP>(qt, rr, kf);
+      f32x16 s = product<T, DP>(qt, rr, kf), dp;
+      if (!kValuesInLds) dp = product<T, DP>(gt, rr, vf);
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4) {
         const f32x4 top = *(const f32x4*)(stat + 4 * g4 + 16 * h);
@@ -276,8 +316,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
         for (int e = 0; e < 4; ++e) {
           const int r = 4 * g4 + e;
           if (kFirst) {
-            const float x = kBias ? (float)bias[min(i0 + 16 * h + r, m - 1) * a.sb[2]] : 0.f;
-            s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + x - top[e]) * kLog2E - log[e]);
+            s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + (kBias ? x[r] : 0.f) - top[e]) * kLog2E - log[e]);
           } else {
             s[r] = __builtin_amdgcn_exp2f(s[r] * (a.scale * kLog2E) - top[e]);
           }
@@ -290,7 +329,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
         transposed_product<DP>(gt, cr, wt, dv);
       }
       if (kValuesInLds) __builtin_amdgcn_sched_barrier(0);
-      f32x16 dp;
       if (kValuesInLds) {
         dp = zero16();
 #pragma unroll
@@ -299,8 +337,6 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
                          *(const u32x4*)(lds + kValues + w * kTile + rr.at(u)), dp);
           if (u % 2) __builtin_amdgcn_sched_barrier(0);
         }
-      } else {
-        dp = product<T, DP>(gt, rr, vf);
       }
 #pragma unroll
       for (int g4 = 0; g4 < 4; ++g4) {
@@ -308,14 +344,20 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[4 * g4 + e] *= dp[4 * g4 + e] - dl[e];
       }
+      if (kGrad) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (r < left) dbias[r * a.sdb[2]] = live ? (T)s[r] : (T)0.f;
+      }
       if (kValuesInLds) __builtin_amdgcn_sched_barrier(0);
       Weights<T> wt;
       wt.set(s);
       transposed_product<DP>(qt, cr, wt, dk);
       return more;
     };
-    copy(0, 0, lds0);
-    load_stats(0, 0);
+    copy(g, i, lds0);
+    load_stats(g, i);
+    if (kBias) load_bias(g, i);
     if (kValuesInLds) {
       for (int buf = 0; step(buf); buf ^= 1) {
       }
@@ -325,23 +367,32 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
     }
   }
   if (key >= a.n) return;
-  const int64_t out = ((b * a.n + key) * a.kv_heads + c) * a.dim;
+  const int64_t out = ((b * a.n + key) * a.kv_heads + c) * a.dim, whole = a.batch * a.n * a.kv_heads * a.dim;
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) {
-    if (a.dk) store_rows((T*)a.dk + out, a.dim, dk[dt], dt, a.scale, live);
-    if (a.dv) store_rows((T*)a.dv + out, a.dim, dv[dt], dt, 1.f, live);
+    if (a.splits > 1) {
+      if (a.dk) store_rows(a.part_o + split * whole + out, a.dim, dk[dt], dt, a.scale, live);
+      if (a.dv) store_rows(a.part_o + (a.splits + split) * whole + out, a.dim, dv[dt], dt, 1.f, live);
+    } else {
+      if (a.dk) store_rows((T*)a.dk + out, a.dim, dk[dt], dt, a.scale, live);
+      if (a.dv) store_rows((T*)a.dv + out, a.dim, dv[dt], dt, 1.f, live);
+    }
   }
 }
 
-// dbias: a block holds 128 queries x 32 keys of one bias plane in registers and walks the batch elements and
-// heads that share the plane, in order. Keys and values go through one LDS buffer by DMA.
+// dbias of a bias that batch elements or heads share: a block holds 128 queries x 32 kParts keys of one bias plane in
+// registers and walks the batch elements and heads that share the plane, in order. bf16 heads up to 64 channels have
+// all four operands in LDS, copied there by DMA; wider ones read the queries' straight into registers.
 template <typename T, int DP>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dbias(CrossArgs a) {
-  constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
-  __shared__ __attribute__((aligned(16))) char lds[4 * kTile + 16];
-  const int key_blocks = (a.n + 31) / 32, query_blocks = (int)((a.m + 127) / 128);
+  constexpr bool kRowsInLds = sizeof(T) == 2 && DP <= 64;
+  constexpr int kParts = sizeof(T) == 2 ? 2 : 1, KT = 32 * kParts;
+  constexpr int kTile = KT * Tile<T, DP>::kRowBytes, kRowTile = kRowsInLds ? 128 * Tile<T, DP>::kRowBytes : 0;
+  constexpr int kWords = 2 * kTile + 2 * kRowTile;
+  __shared__ __attribute__((aligned(16))) char lds[kWords + 16];
+  const int key_blocks = (a.n + KT - 1) / KT, query_blocks = (int)((a.m + 127) / 128);
   int64_t at = xcd_position(blockIdx.x, gridDim.x);
-  const int key = (int)(at % key_blocks) * 32;
+  const int key = (int)(at % key_blocks) * KT;
   at /= key_blocks;
   const int q0 = (int)(at % query_blocks) * 128;
   at /= query_blocks;
@@ -349,76 +400,170 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   const int64_t ph = at % plane_heads, pb = at / plane_heads;
   const int64_t b0 = a.sdb[0] ? pb : 0, b1 = a.sdb[0] ? pb + 1 : a.batch;
   const int h0 = a.sdb[1] ? (int)ph : 0, h1 = a.sdb[1] ? (int)ph + 1 : a.heads;
-  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), h = lane_id() >> 5;
-  const int64_t i = q0 + w * 32 + (t & 31), safe = min(i, a.m - 1);
-  f32x16 sum = zero16();
-  KeyWords words{(uint32_t*)(lds + 4 * kTile), nullptr};
+  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = lane_id(), h = l >> 5;
+  const int m = (int)a.m, i = q0 + w * 32 + tile_row(l & 31), safe = min(i, m - 1);
+  f32x16 sum[kParts];
+#pragma unroll
+  for (int u = 0; u < kParts; ++u) sum[u] = zero16();
+  KeyWords words{(uint32_t*)(lds + kWords), nullptr};
   RowReads<T, DP> rr;
   rr.init();
-  Copy<T, DP, 32, 4> ck, cv;
+  const int64_t row_step = (int64_t)a.heads * a.dim;
+  Copy<T, DP, KT, 4> ck, cv;
+  Copy<T, DP, 128, 4> cq, cg;
   ck.init(w, a.dim, a.sk[1]);
   cv.init(w, a.dim, a.sv[1]);
+  if (kRowsInLds) {
+    cq.init(w, a.dim, a.sq[1]);
+    cg.init(w, a.dim, row_step);
+  }
   const unsigned lds0 = lds_address(lds);
-  clear_tiles<T, DP, 256>(t, lds, 4 * kTile, a.dim);
-  int buf = 0;
+  clear_tiles<T, DP, 256>(t, lds, kWords, a.dim);
   for (int64_t b = b0; b < b1; ++b) {
     words.mask = a.mask ? a.mask + b * a.smask : nullptr;
-    words.fill(key, min(key + 32, a.n));
-    const uint32_t bits = words.bits(key), mine = bits >> (16 * h);
-    if (bits == 0) continue;
+    words.fill(key, min(key + KT, a.n));
+    uint32_t any = 0;
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) any |= words.bits(key + 32 * u);
+    if (any == 0) continue;
     for (int head = h0; head < h1; ++head) {
       const int c = head / a.group;
-      const unsigned tile = lds0 + buf * 2 * kTile;
-      ck.issue(w, (const T*)a.k + b * a.sk[0] + c * a.sk[2] + key * a.sk[1], a.n - key, a.dim, a.sk[1], tile);
-      cv.issue(w, (const T*)a.v + b * a.sv[0] + c * a.sv[2] + key * a.sv[1], a.n - key, a.dim, a.sv[1], tile + kTile);
+      __syncthreads();  // every wave is done with the last step's tiles
+      ck.issue(w, (const T*)a.k + b * a.sk[0] + c * a.sk[2] + key * a.sk[1], a.n - key, a.dim, a.sk[1], lds0);
+      cv.issue(w, (const T*)a.v + b * a.sv[0] + c * a.sv[2] + key * a.sv[1], a.n - key, a.dim, a.sv[1], lds0 + kTile);
       RowOperand<T, DP> q, g;
-      q.load((const T*)a.q + b * a.sq[0] + safe * a.sq[1] + head * a.sq[2], a.dim, h);
-      g.load((const T*)a.dout + ((b * a.m + safe) * a.heads + head) * a.dim, a.dim, h);
+      const T* q_row = (const T*)a.q + b * a.sq[0] + head * a.sq[2];
+      const T* g_row = (const T*)a.dout + (b * a.m * a.heads + head) * a.dim;
+      if (kRowsInLds) {
+        cq.issue(w, q_row + q0 * a.sq[1], m - q0, a.dim, a.sq[1], lds0 + 2 * kTile);
+        cg.issue(w, g_row + q0 * row_step, m - q0, a.dim, row_step, lds0 + 2 * kTile + kRowTile);
+      } else {
+        q.load(q_row + safe * a.sq[1], a.dim, h);
+        g.load(g_row + safe * row_step, a.dim, h);
+      }
       const int64_t stat = (b * a.heads + head) * a.m + safe;
       const float2 st = a.stats[stat];
       const float delta = a.delta[stat];
-      const T* bias = (const T*)a.bias + b * a.sb[0] + head * a.sb[1] + safe * a.sb[2];
+      const T* bias_row = (const T*)a.bias + b * a.sb[0] + head * a.sb[1] + safe * a.sb[2];
+      BiasTile<T> bias[kParts];
+#pragma unroll
+      for (int u = 0; u < kParts; ++u) bias[u].load(bias_row, min(key + 32 * u, a.n - 1), a.n);
       wait_copies();
       __syncthreads();
-      f32x16 s = product<T, DP>(lds + buf * 2 * kTile, rr, q);
-      const f32x16 dp = product<T, DP>(lds + buf * 2 * kTile + kTile, rr, g);
-      weights_of<T, true>(a, s, bias, key, st);
+      if (kRowsInLds) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sum[r] += key_bit(mine, r) ? s[r] * (dp[r] - delta) : 0.f;
-      buf ^= 1;
+        for (int s = 0; s < RowOperand<T, DP>::kSteps; ++s) {
+          q.c[s] = *(const u32x4*)(lds + 2 * kTile + w * 32 * Tile<T, DP>::kRowBytes + rr.at(s));
+          g.c[s] = *(const u32x4*)(lds + 2 * kTile + kRowTile + w * 32 * Tile<T, DP>::kRowBytes + rr.at(s));
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kParts; ++u) {
+        const char* kt = lds + u * 32 * Tile<T, DP>::kRowBytes;
+        f32x16 s = product<T, DP>(kt, rr, q);
+        const f32x16 dp = product<T, DP>(kt + kTile, rr, g);
+        weights_of<T, true>(a, s, bias[u], st);
+        const uint32_t mine = words.bits(key + 32 * u) >> (16 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum[u][r] += key_bit(mine, r) ? s[r] * (dp[r] - delta) : 0.f;
+        __builtin_amdgcn_sched_barrier(0);  // one part's operands at a time: both spill
+      }
     }
   }
-  if (i >= a.m) return;
+  if (i >= m) return;
   T* out = (T*)a.dbias + pb * a.sdb[0] + ph * a.sdb[1] + i * a.sdb[2];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int at_key = key + 16 * h + r;
-    if (at_key < a.n) out[at_key] = (T)sum[r];
-  }
+  for (int u = 0; u < kParts; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int at_key = key + 32 * u + 16 * h + r;
+      if (at_key < a.n) out[at_key] = (T)sum[u][r];
+    }
+}
+
+// out = the splits' parts added in order.
+template <typename T>
+__global__ __launch_bounds__(256) void cross_attention_sum(const float* part, int splits, int64_t quads, T* out) {
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (at >= quads) return;
+  f32x4 v = *(const f32x4*)(part + 4 * at);
+  for (int s = 1; s < splits; ++s) v += *(const f32x4*)(part + 4 * (s * quads + at));
+  store4(out + 4 * at, v);
+}
+
+struct Split {
+  int splits, size;
+};
+
+// Splits of `units` (keys, or query tiles) for `blocks` blocks: so many that every SIMD gets two waves (two blocks a compute unit),
+// each of at least `least` units, since the parts are written and read once more in fp32.
+Split plan(int64_t blocks, int64_t units, int64_t least, int64_t round) {
+  int64_t splits = 512 / blocks;
+  const int64_t most = units / least;
+  splits = splits > most ? most : splits;
+  if (splits < 1) splits = 1;
+  const int64_t size = ((units + splits - 1) / splits + round - 1) / round * round;
+  return {(int)((units + size - 1) / size), (int)size};
+}
+Split plan_dq(int64_t batch, int64_t kv_heads, int64_t rows, int64_t n) {
+  return plan((rows + 127) / 128 * batch * kv_heads, n, 256, 128);
+}
+Split plan_dkv(int64_t batch, int64_t kv_heads, int64_t group, int64_t m, int64_t n) {
+  return plan((n + 127) / 128 * batch * kv_heads, group * ((m + 31) / 32), 4, 1);
+}
+
+// Floats of the workspace: delta, then the parts of dQ or of dK and dV, whichever is more.
+int64_t workspace_floats(int64_t batch, int64_t m, int64_t n, int64_t heads, int64_t kv_heads, int64_t dim,
+                         int64_t* parts) {
+  const int64_t group = heads / kv_heads, delta = (batch * m * heads + 3) / 4 * 4;
+  const Split q = plan_dq(batch, kv_heads, group * m, n), kv = plan_dkv(batch, kv_heads, group, m, n);
+  const int64_t pq = q.splits > 1 ? q.splits * batch * m * heads * dim : 0;
+  const int64_t pkv = kv.splits > 1 ? 2 * kv.splits * batch * n * kv_heads * dim : 0;
+  if (parts) *parts = delta;
+  return delta + (pq > pkv ? pq : pkv);
 }
 
 template <typename T, int DP>
 int launch(CrossArgs& a, hipStream_t stream) {
   const int64_t lists = a.batch * a.kv_heads, key_blocks = (a.n + 127) / 128;
   a.row_blocks = (a.rows + 127) / 128;
+  const Split q = plan_dq(a.batch, a.kv_heads, a.rows, a.n), kv = plan_dkv(a.batch, a.kv_heads, a.group, a.m, a.n);
   const int64_t planes = (a.sdb[0] ? a.batch : 1) * (a.sdb[1] ? a.heads : 1);
-  const int64_t bias_blocks = planes * ((a.m + 127) / 128) * ((a.n + 31) / 32);
+  // Shared by batch elements or heads: a kernel of its own; otherwise dK and dV's writes it.
+  const bool shared = a.dbias && ((!a.sdb[0] && a.batch > 1) || (!a.sdb[1] && a.heads > 1));
+  constexpr int KT = sizeof(T) == 4 ? 32 : 64;  // cross_attention_dbias's keys
+  const int64_t bias_blocks = planes * ((a.m + 127) / 128) * ((a.n + KT - 1) / KT);
   const int64_t delta_blocks = (a.batch * a.m * a.heads + 15) / 16;
-  BMX_REQUIRE(lists * a.row_blocks < (1ll << 31) && lists * key_blocks < (1ll << 31) && bias_blocks < (1ll << 31) &&
-                  delta_blocks < (1ll << 31),
+  const int64_t q_quads = a.batch * a.m * a.heads * a.dim / 4, k_quads = a.batch * a.n * a.kv_heads * a.dim / 4;
+  constexpr int64_t most = 1ll << 31;
+  BMX_REQUIRE(lists * a.row_blocks * q.splits < most && lists * key_blocks * kv.splits < most && bias_blocks < most &&
+                  delta_blocks < most && q_quads / 256 < most - 1 && k_quads / 256 < most - 1,
               "cross_attention_bwd: too many blocks");
   cross_attention_delta<T><<<dim3((unsigned)delta_blocks), 256, 0, stream>>>(a);
+  auto sum = [&](const Split& s, int64_t part, int64_t quads, void* out) {
+    cross_attention_sum<<<dim3((unsigned)((quads + 255) / 256)), 256, 0, stream>>>(a.part_o + part * s.splits * quads * 4,
+                                                                                  s.splits, quads, (T*)out);
+  };
   if (a.dq) {
-    const dim3 grid((unsigned)(lists * a.row_blocks));
+    a.splits = q.splits, a.split_keys = q.size;
+    const dim3 grid((unsigned)(lists * a.row_blocks * q.splits));
     a.bias ? cross_attention_dq<T, DP, true><<<grid, 256, 0, stream>>>(a)
            : cross_attention_dq<T, DP, false><<<grid, 256, 0, stream>>>(a);
+    if (q.splits > 1) sum(q, 0, q_quads, a.dq);
   }
-  if (a.dk || a.dv) {
-    const dim3 grid((unsigned)(lists * key_blocks));
-    a.bias ? cross_attention_dkv<T, DP, true><<<grid, 256, 0, stream>>>(a)
-           : cross_attention_dkv<T, DP, false><<<grid, 256, 0, stream>>>(a);
+  if (a.dk || a.dv || (a.dbias && !shared)) {
+    a.splits = kv.splits, a.split_keys = kv.size;
+    const dim3 grid((unsigned)(lists * key_blocks * kv.splits));
+    if (a.dbias && !shared)
+      cross_attention_dkv<T, DP, true, true><<<grid, 256, 0, stream>>>(a);
+    else if (a.bias)
+      cross_attention_dkv<T, DP, true, false><<<grid, 256, 0, stream>>>(a);
+    else
+      cross_attention_dkv<T, DP, false, false><<<grid, 256, 0, stream>>>(a);
+    if (kv.splits > 1 && a.dk) sum(kv, 0, k_quads, a.dk);
+    if (kv.splits > 1 && a.dv) sum(kv, 1, k_quads, a.dv);
   }
-  if (a.dbias) cross_attention_dbias<T, DP><<<dim3((unsigned)bias_blocks), 256, 0, stream>>>(a);
+  if (shared) cross_attention_dbias<T, DP><<<dim3((unsigned)bias_blocks), 256, 0, stream>>>(a);
   return check_launch("cross_attention_bwd");
 }
 
@@ -431,8 +576,10 @@ int launch_dim(CrossArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-extern "C" size_t bmx_cross_attention_bwd_workspace_bytes(int64_t batch, int64_t m, int64_t heads) {
-  return batch < 1 || m < 1 || heads < 1 ? 0 : (size_t)(batch * m * heads) * sizeof(float);
+extern "C" size_t bmx_cross_attention_bwd_workspace_bytes(int64_t batch, int64_t m, int64_t n, int64_t heads,
+                                                          int64_t kv_heads, int64_t dim) {
+  if (batch < 1 || m < 1 || n < 1 || heads < 1 || kv_heads < 1 || dim < 1) return 0;
+  return (size_t)workspace_floats(batch, m, n, heads, kv_heads, dim, nullptr) * sizeof(float);
 }
 
 extern "C" int bmx_cross_attention_bwd(const void* q, const void* k, const void* v, const void* mask, const void* bias,
@@ -451,10 +598,13 @@ extern "C" int bmx_cross_attention_bwd(const void* q, const void* k, const void*
               "cross_attention_bwd: tensors must be 16-byte aligned");
   BMX_REQUIRE((uintptr_t)stats % 8 == 0, "cross_attention_bwd: stats must be 8-byte aligned");
   BMX_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
-                  workspace_bytes >= bmx_cross_attention_bwd_workspace_bytes(a.batch, a.m, a.heads),
+                  workspace_bytes >= bmx_cross_attention_bwd_workspace_bytes(a.batch, a.m, a.n, a.heads, a.kv_heads, a.dim),
               "cross_attention_bwd: workspace too small or not 16-byte aligned");
   a.q = q, a.k = k, a.v = v, a.mask = (const uint8_t*)mask, a.bias = bias;
   a.out = (void*)out, a.out_lo = dtype == kBF16 ? (void*)out_lo : nullptr, a.stats = (float2*)stats, a.dout = dout;
+  int64_t parts = 0;
+  workspace_floats(a.batch, a.m, a.n, a.heads, a.kv_heads, a.dim, &parts);
+  a.part_o = (float*)workspace + parts;
   a.delta = (float*)workspace, a.dq = dq, a.dk = dk, a.dv = dv, a.dbias = dbias;
   for (int i = 0; i < 3; ++i) a.sdb[i] = dbias ? dbias_strides[i] : 0;
   hipStream_t hs = (hipStream_t)stream;

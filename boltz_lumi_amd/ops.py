@@ -1442,10 +1442,10 @@ class _CrossAttention(torch.autograd.Function):
         need = ctx.needs_input_grad
         dq, dk, dv, dbias = (torch.empty(t.shape, device=q.device, dtype=q.dtype) if need[i] else None
                              for i, t in ((0, q), (1, k), (2, v), (4, bias)))
-        b, m, h, _ = q.shape
+        b, m, h, d = q.shape
         if q.numel() and k.numel():
             dout = _aligned(dout.contiguous())
-            nbytes = N.lib().bmx_cross_attention_bwd_workspace_bytes(b, m, h)
+            nbytes = N.lib().bmx_cross_attention_bwd_workspace_bytes(b, m, k.shape[1], h, k.shape[2], d)
             ws = _workspace(nbytes, q.device)
             with _at_device(q):
                 N.call("bmx_cross_attention_bwd", *_cross_args(q, k, v, mask, bias, ctx.scale), out.data_ptr(), _ptr(lo),
@@ -1493,7 +1493,8 @@ def cross_attention(q, k, v, mask=None, bias=None, scale=None):
     if bias is not None:
         _check(bias.dim() == 4 and bias.dtype == q.dtype and bias.shape[0] in (1, b) and bias.shape[1] in (1, h)
                and bias.shape[2:] == (m, n), "expected a bias [B or 1, H or 1, M, N] in q's dtype")
-        bias = bias if bias.stride(3) == 1 or n <= 1 else bias.contiguous()
+        _check(n < 1 << 26, "a bias takes at most 2^26 - 1 keys")
+        bias = bias if (bias.stride(3) == 1 or n <= 1) and bias.stride(2) < 1 << 26 else bias.contiguous()
     q, k, v = _head_tokens(q), _head_tokens(k), _head_tokens(v)
     if _needs_grad(q, k, v, bias):
         return _CrossAttention.apply(q, k, v, mask, bias, scale)

@@ -466,7 +466,8 @@ int bmx_cross_attention_fwd(const void* q, const void* k, const void* v, const v
  * (0: one for the batch), head (0: one for the heads), query}, keys dense, or NULL.  Left-out keys and rows
  * without keys get zeros.  batch, m, n >= 1.  workspace: bmx_cross_attention_bwd_workspace_bytes, 16-byte aligned.
  * No reference kernel. */
-size_t bmx_cross_attention_bwd_workspace_bytes(int64_t batch, int64_t m, int64_t heads);
+size_t bmx_cross_attention_bwd_workspace_bytes(int64_t batch, int64_t m, int64_t n, int64_t heads, int64_t kv_heads,
+                                               int64_t dim);
 int bmx_cross_attention_bwd(const void* q, const void* k, const void* v, const void* mask, const void* bias, int dtype,
                             const int64_t* shape, const int64_t* strides, float scale, const void* out,
                             const void* out_lo, const float* stats, const void* dout, void* dq, void* dk, void* dv,

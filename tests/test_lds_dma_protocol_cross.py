@@ -20,4 +20,4 @@ def test_cross_attention_lds_dmas_follow_the_protocol(stem, tmp_path):
 def test_cross_attention_copies_wait_five_states():
     text = (CSRC / "cross_attention.h").read_text()
     asm = re.findall(r'asm\s+volatile\s*\(\s*"([^"]*)"', text)
-    assert asm == [r"s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"]
+    assert [a for a in asm if a] == [r"s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1"]

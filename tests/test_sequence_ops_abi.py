@@ -115,8 +115,10 @@ def test_cross_attention_rejects_bad_arguments(lib):
     assert refused(lib, fwd(shape=long, size=need_long - 1), b"workspace")
     assert refused(lib, fwd(shape=long, ws=None, size=need_long), b"workspace")
 
-    need_bwd = lib.bmx_cross_attention_bwd_workspace_bytes(b, m, h)
-    assert need_bwd == b * m * h * 4
+    need_bwd = lib.bmx_cross_attention_bwd_workspace_bytes(b, m, n, h, hk, d)
+    assert need_bwd == b * m * h * 4  # too few keys and queries to split
+    assert lib.bmx_cross_attention_bwd_workspace_bytes(b, m, 0, h, hk, d) == 0
+    assert lib.bmx_cross_attention_bwd_workspace_bytes(1, 128, 2048, 8, 8, d) >= 128 * 8 * 4 + 2 * 128 * 8 * d * 4
 
     def bwd(shape=good_shape, bias=FAKE, lo=FAKE, stats=FAKE, dout=FAKE, dq=FAKE, dbias=FAKE, steps=(0, m * n, n),
             ws=FAKE, size=need_bwd):
