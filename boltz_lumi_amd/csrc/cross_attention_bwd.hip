@@ -77,6 +77,28 @@ __device__ __forceinline__ void store_rows(T* row, int dim, const f32x16& acc, i
   }
 }
 
+// The 16 values of a run of keys of one row, at any element alignment.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+template <typename T>
+__device__ __forceinline__ void store_keys(T* row, int key, int n, const f32x16& v) {
+  if (key + 16 <= n) {
+    constexpr int kElems = 16 / sizeof(T);
+#pragma unroll
+    for (int i = 0; i < 16 / kElems; ++i) {
+      T x[kElems];
+#pragma unroll
+      for (int e = 0; e < kElems; ++e) x[e] = (T)v[i * kElems + e];
+      u32x4 word;
+      __builtin_memcpy(&word, x, 16);
+      *(u32x4_any*)(row + key + i * kElems) = word;
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      if (key + r < n) row[key + r] = (T)v[r];
+  }
+}
+
 // P of a logits tile whose column is a query: maximum and log2 of the sum are the lane's.
 template <typename T, bool kBias>
 __device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, BiasTile<T>& b, float2 st) {
@@ -473,12 +495,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   if (i >= m) return;
   T* out = (T*)a.dbias + pb * a.sdb[0] + ph * a.sdb[1] + i * a.sdb[2];
 #pragma unroll
-  for (int u = 0; u < kParts; ++u)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int at_key = key + 32 * u + 16 * h + r;
-      if (at_key < a.n) out[at_key] = (T)sum[u][r];
-    }
+  for (int u = 0; u < kParts; ++u) store_keys(out, key + 32 * u + 16 * h, a.n, sum[u]);
 }
 
 // out = the splits' parts added in order.
