@@ -22,6 +22,8 @@ using namespace bmx;
 
 namespace {
 
+constexpr int kBwdBlocks = 1024;  // of a tensor's gradient at most: four per compute unit
+
 // One of the two tensors: x [batch, tokens, heads, D] at element strides, y dense.
 struct HeadRows {
   const void *x, *w, *dy;
@@ -217,24 +219,38 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(NormRope s) {
   }
 }
 
-// Weight gradient: 16 channels per block, 16 slices of the partial rows each.
-template <typename T>
-__global__ __launch_bounds__(256) void norm_weight_grad_kernel(const float* partial, int blocks, int dim, T* out) {
-  __shared__ float sums[256];
-  const int channel = blockIdx.x * 16 + (threadIdx.x & 15), slice = threadIdx.x >> 4;
-  float v = 0.f;
-  if (channel < dim)
-    for (int b = slice; b < blocks; b += 16) v += partial[(int64_t)b * dim + channel];
-  sums[threadIdx.x] = v;
-  __syncthreads();
-  if (slice == 0 && channel < dim) {
+// Weight gradients of both tensors in one launch: a block per four channels, its 256 threads' partial rows
+// in flight together, added over the lanes and then the waves.
+struct WeightGrads {
+  const float* partial[2];
+  void* out[2];
+  int blocks[2];  // partial rows
+  int dim, out_bf16;
+};
+__global__ __launch_bounds__(256) void norm_weight_grad_kernel(WeightGrads s) {
+  __shared__ float sums[4][4];
+  const int quads = s.dim / 4, which = (int)blockIdx.x / quads, d = 4 * ((int)blockIdx.x % quads);
+  if (!s.out[which]) return;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 1; i < 16; ++i) v += sums[threadIdx.x + 16 * i];
-    out[channel] = (T)v;
+  for (int u = 0; u < kBwdBlocks / 256; ++u) {
+    const int row = threadIdx.x + 256 * u;
+    if (row < s.blocks[which]) v += *(const f32x4*)(s.partial[which] + (int64_t)row * s.dim + d);
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const float x = wave_sum_full(v[e]);
+    if (lane_id() == 0) sums[threadIdx.x >> 6][e] = x;
+  }
+  __syncthreads();
+  if (threadIdx.x >= 4) return;
+  const float x = sums[0][threadIdx.x] + sums[1][threadIdx.x] + sums[2][threadIdx.x] + sums[3][threadIdx.x];
+  if (s.out_bf16)
+    ((bf16*)s.out[which])[d + threadIdx.x] = (bf16)x;
+  else
+    ((float*)s.out[which])[d + threadIdx.x] = x;
 }
 
-constexpr int kBwdBlocks = 1024;  // four per compute unit
 
 // Items of a tensor at `rows` heads per item, and its blocks (at most `most`).
 int64_t plan(HeadRows& t, int64_t batch, int rows, int groups, int64_t most) {
@@ -372,15 +388,10 @@ extern "C" int bmx_qk_norm_rope_bwd(const void* q, const void* k, int dtype, con
     else
       few ? launch<bf16, 1>(true, lanes, s, hs) : launch<bf16, 4>(true, lanes, s, hs);
   }
-  const HeadRows* rows_of[2] = {&s.q, &s.k};
-  void* dws[2] = {dq_weight, dk_weight};
-  for (int i = 0; i < 2; ++i) {
-    if (!dws[i]) continue;  // no rows: zero partial rows, a gradient of zeros
-    const int grid = (s.dim + 15) / 16;
-    if (w_dtype == kF32)
-      norm_weight_grad_kernel<<<grid, 256, 0, hs>>>(rows_of[i]->partial, rows_of[i]->blocks, s.dim, (float*)dws[i]);
-    else
-      norm_weight_grad_kernel<<<grid, 256, 0, hs>>>(rows_of[i]->partial, rows_of[i]->blocks, s.dim, (bf16*)dws[i]);
+  if (dq_weight || dk_weight) {  // without rows: no partial rows, a gradient of zeros
+    const WeightGrads w = {{s.q.partial, s.k.partial}, {dq_weight, dk_weight}, {s.q.blocks, s.k.blocks}, s.dim,
+                           w_dtype == kBF16};
+    norm_weight_grad_kernel<<<dim3(s.dim / 4 * 2), 256, 0, hs>>>(w);
   }
   return check_launch("qk_norm_rope_bwd");
 }

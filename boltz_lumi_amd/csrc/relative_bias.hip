@@ -102,15 +102,26 @@ __global__ __launch_bounds__(256) void relative_bias_kernel(Relative s, const U*
   }
 }
 
-// Gradient.  A block sums a strip of columns over a run of rows of one (b, h)
-// plane.  Every thread has its own bin per bucket in LDS (bins[bucket][thread]: consecutive
-// threads in consecutive banks), so there is no atomic and the order of every sum is
-// fixed; a thread keeps its columns' positions in registers and walks down the rows.
-// A distance's bucket comes from a byte table where the last threshold is below kLut.
-constexpr int kLut = 2048;
+// Gradient.  A block sums a strip of columns over every row_blocks-th row of one (b, h)
+// plane: a wave reads 64 x 16 bytes of a row, four rows in flight. Where a wave's columns all lie past the last
+// threshold on one side of the row's position, which is most of a plane of running positions, the row is added
+// to one sum in registers. Otherwise every thread adds to its own bin per bucket in LDS (bins[bucket][thread],
+// consecutive threads in consecutive banks). Nothing is shared, so there is no atomic and the order of every
+// sum is fixed. A distance's bucket comes from a byte table where the last threshold is below kLut.
+constexpr int kLut = 2048, kAhead = 4;
+
+__device__ __forceinline__ int64_t wave_extreme(int64_t v, bool largest) {
+#pragma unroll
+  for (int m = 32; m >= 1; m >>= 1) {
+    const int64_t o = __shfl_xor((long long)v, m, kWave);
+    v = (o > v) == largest ? o : v;
+  }
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)v), hi = __builtin_amdgcn_readfirstlane((int)(v >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
 
 template <typename T>
-__global__ __launch_bounds__(256) void relative_bias_bwd_kernel(Relative s, const T* dbias, int width, int64_t rows,
+__global__ __launch_bounds__(256) void relative_bias_bwd_kernel(Relative s, const T* dbias, int waves_across,
                                                                 int64_t row_blocks, int64_t col_blocks,
                                                                 float* partial) {
   constexpr int V = 16 / sizeof(T);
@@ -122,51 +133,73 @@ __global__ __launch_bounds__(256) void relative_bias_bwd_kernel(Relative s, cons
   for (int i = t; i < s.count; i += threads) edges[i] = s.t[i];
   for (int i = t; i < s.buckets * threads; i += threads) bins[i] = 0.f;
   __syncthreads();
-  const int last = s.count ? edges[s.count - 1] : 0;  // every distance from here on is in one bucket
+  const int last = s.count ? s.t[s.count - 1] : 1;  // every distance from here on is in one bucket
   const bool small = last < kLut;
   if (small)
     for (int i = t; i <= last; i += threads) lut[i] = (uint8_t)bucket_of(s, edges, -i);
   __syncthreads();
   const int64_t cb = blockIdx.x % col_blocks, rest = blockIdx.x / col_blocks;
   const int64_t rb = rest % row_blocks, plane = rest / row_blocks, b = plane / s.heads;
-  const int tx = t % width, ty = t / width, step = threads / width;
-  const int64_t j0 = (cb * width + tx) * V;
-  const int64_t r1 = min((rb + 1) * rows, s.m);
-  if (j0 < s.n) {
-    int64_t kp[V];
+  // The row blocks take rows in turn, so that rows near the diagonal, which cost more, are dealt to all of them.
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6), down = threads / 64 / waves_across;
+  const int64_t step = down * row_blocks;
+  const int64_t j0 = ((cb * waves_across + wave % waves_across) * 64 + lane_id()) * V;
+  const int held = (int)max(min(s.n - j0, (int64_t)V), (int64_t)0);  // the lane's columns
+  const bool whole = __all(held == V);
+  int64_t kp[V], least = INT64_MAX, most = INT64_MIN;
 #pragma unroll
-    for (int e = 0; e < V; ++e) kp[e] = position(s.k_pos, s.pos64, b * s.k_sb + min(j0 + e, s.n - 1));
-    const bool whole = j0 + V <= s.n;
-    const T* src = dbias + (plane * s.m + rb * rows + ty) * s.n + j0;
-    for (int64_t i = rb * rows + ty; i < r1; i += step, src += step * s.n) {
-      float v[V];
-      if (whole) {
-        union {
-          T e[V];
-          u32x4_u v;
-        } w;
-        w.v = *(const u32x4_u*)src;
+  for (int e = 0; e < V; ++e) {
+    kp[e] = position(s.k_pos, s.pos64, b * s.k_sb + min(j0 + e, s.n - 1));
+    least = min(least, kp[e]), most = max(most, kp[e]);
+  }
+  // Rows up to `ahead` have every column past the thresholds ahead of them, rows from `behind` on behind them.
+  const int64_t ahead = wave_extreme(least, false) - (s.bidirectional ? last : 1), behind = wave_extreme(most, true) + last;
+  float far_ahead = 0.f, far_behind = 0.f;
+  auto add = [&](int64_t qp, const float (&v)[V]) {
+    if (qp <= ahead || qp >= behind) {
+      float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = (float)w.e[e];
-      } else {
+      for (int e = 0; e < V; ++e) sum += v[e];
+      qp <= ahead ? far_ahead += sum : far_behind += sum;
+      return;
+    }
 #pragma unroll
-        for (int e = 0; e < V; ++e) v[e] = j0 + e < s.n ? (float)src[e] : 0.f;
-      }
-      const int64_t qp = position(s.q_pos, s.pos64, b * s.q_sb + i);
+    for (int e = 0; e < V; ++e) {
+      const int d = distance(kp[e], qp);
+      const int n = d < 0 ? -d : (s.bidirectional ? d : 0);
+      const int c = small ? lut[min(n, last)] + (s.bidirectional && d > 0 ? s.count + 1 : 0) : bucket_of(s, edges, d);
+      bins[c * threads + t] += v[e];
+    }
+  };
+  const T* src = dbias + plane * s.m * s.n;
+  int64_t i = rb * down + wave / waves_across;
+  if (whole) {
+    for (; i < s.m; i += kAhead * step) {  // rows past the plane read its last one and add nothing
+      union {
+        T e[V];
+        u32x4_u v;
+      } w[kAhead];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const int d = distance(kp[e], qp);
-        int c;
-        if (small) {
-          const int n = d < 0 ? -d : (s.bidirectional ? d : 0);
-          c = lut[min(n, last)] + (s.bidirectional && d > 0 ? s.count + 1 : 0);
-        } else {
-          c = bucket_of(s, edges, d);
-        }
-        if (whole || j0 + e < s.n) bins[c * threads + t] += v[e];
+      for (int u = 0; u < kAhead; ++u) w[u].v = *(const u32x4_u*)(src + min(i + u * step, s.m - 1) * s.n + j0);
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        if (i + u * step >= s.m) break;
+        float v[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = (float)w[u].e[e];
+        add(position(s.q_pos, s.pos64, b * s.q_sb + i + u * step), v);
       }
     }
+  } else {
+    for (; i < s.m; i += step) {
+      float v[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = e < held ? (float)src[i * s.n + j0 + e] : 0.f;
+      add(position(s.q_pos, s.pos64, b * s.q_sb + i), v);
+    }
   }
+  bins[s.count * threads + t] += far_behind;
+  bins[(s.bidirectional ? 2 * s.count + 1 : 0) * threads + t] += far_ahead;
   __syncthreads();
   // one wave per bucket in turn
   const int lane = t & 63, waves = threads / 64;
@@ -193,25 +226,23 @@ __global__ __launch_bounds__(64) void relative_table_grad_kernel(const float* pa
 }
 
 struct BwdPlan {
-  int threads, width;
-  int64_t rows, row_blocks, col_blocks, blocks;
+  int threads, across;  // waves of a block side by side
+  int64_t row_blocks, col_blocks, blocks;
 };
 
-// Threads by the bins' LDS (64 KB at most); columns of a block as wide as the plane allows,
-// rows so that a thread adds about 32 vectors, fewer where that leaves under four blocks a compute unit.
+// Threads by the bins' LDS (64 KB at most); waves of a block side by side as the plane is wide,
+// rows so that a wave reads about 64, fewer where that leaves under four blocks a compute unit.
 BwdPlan bwd_plan(int dtype, int64_t buckets, int64_t planes, int64_t m, int64_t n) {
   BwdPlan p;
-  const int vec = dtype == kF32 ? 4 : 8;
+  const int64_t wide = 64 * (dtype == kF32 ? 4 : 8);
   p.threads = buckets <= 64 ? 256 : buckets <= 128 ? 128 : 64;
-  p.width = p.threads;
-  while (p.width > 1 && (int64_t)p.width / 2 * vec >= n) p.width /= 2;
-  const int64_t wide = (int64_t)p.width * vec;
-  p.col_blocks = (n + wide - 1) / wide;
-  const int64_t step = p.threads / p.width;
-  int64_t turns = 32;
+  p.across = p.threads / 64;
+  while (p.across > 1 && p.across / 2 * wide >= n) p.across /= 2;
+  p.col_blocks = (n + p.across * wide - 1) / (p.across * wide);
+  const int64_t step = p.threads / 64 / p.across;
+  int64_t turns = 64;
   while (turns > 4 && planes * p.col_blocks * ((m + step * turns - 1) / (step * turns)) < 1024) turns /= 2;
-  p.rows = step * turns;
-  p.row_blocks = (m + p.rows - 1) / p.rows;
+  p.row_blocks = (m + step * turns - 1) / (step * turns);
   p.blocks = p.row_blocks * p.col_blocks;
   return p;
 }
@@ -295,10 +326,10 @@ extern "C" int bmx_relative_bias_bwd(const void* dbias, int dtype, int64_t bucke
     const size_t lds = kMaxSide * 4 + kLut + (size_t)buckets * p.threads * 4;
     const dim3 grid((unsigned)(p.blocks * batch * heads));
     if (dtype == kF32)
-      relative_bias_bwd_kernel<float><<<grid, p.threads, lds, hs>>>(s, (const float*)dbias, p.width, p.rows, p.row_blocks,
+      relative_bias_bwd_kernel<float><<<grid, p.threads, lds, hs>>>(s, (const float*)dbias, p.across, p.row_blocks,
                                                                     p.col_blocks, (float*)workspace);
     else
-      relative_bias_bwd_kernel<bf16><<<grid, p.threads, lds, hs>>>(s, (const bf16*)dbias, p.width, p.rows, p.row_blocks,
+      relative_bias_bwd_kernel<bf16><<<grid, p.threads, lds, hs>>>(s, (const bf16*)dbias, p.across, p.row_blocks,
                                                                    p.col_blocks, (float*)workspace);
   }
   const dim3 grid((unsigned)(heads * buckets));
