@@ -21,7 +21,6 @@ from __future__ import annotations
 
 import ctypes
 import os
-from contextlib import nullcontext
 from functools import lru_cache
 
 import torch
@@ -1155,11 +1154,6 @@ def adaln_modulate(a, scale, shift, eps):
 # with torch.autograd.grad, as for torch's own operators.
 
 
-def _at_device(t):
-    """The context a launch on ``t``'s device needs: none on the current device."""
-    return nullcontext() if t.get_device() == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
 def _needs_grad(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
@@ -1168,86 +1162,135 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _head_rows(x):
-    """``x`` [B, T, H, D] with a dense last axis, outer strides of multiples of
-    four elements and four-element alignment: itself, or a dense copy."""
-    ok = x.stride(3) == 1 and x.data_ptr() % (4 * x.element_size()) == 0
-    if not ok or any(x.stride(i) % 4 for i in range(3) if x.shape[i] > 1):
-        x = x.contiguous()
-        return x if x.data_ptr() % (4 * x.element_size()) == 0 else x.clone()
-    return x
+def _layout(t):
+    """What a plan needs to know of a tensor."""
+    return None if t is None else (t.shape, t.stride(), t.dtype)
 
 
-def _strides(x, axes):
-    """Strides of the leading ``axes`` axes; those of single elements, which nothing steps, as 0."""
-    return [x.stride(i) if x.shape[i] > 1 else 0 for i in range(axes)]
+def _same_device(first, *tensors) -> int:
+    """The device index that the tensors share; raises as ``_cuda`` does."""
+    dev = first.get_device()
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            _cuda(first, t)
+    if dev < 0:
+        _cuda(first)
+    return dev
 
 
-def _positions(pos, tokens, batch, like, what):
-    """Checked positions: int32 / int64 [tokens] or [batch, tokens], dense; their batch stride."""
-    _check(isinstance(pos, torch.Tensor) and pos.dtype in (torch.int32, torch.int64),
-           f"expected int32 or int64 {what}")
-    _check(pos.shape in ((tokens,), (batch, tokens)), f"expected {what} of shape [tokens] or [batch, tokens]")
-    _cuda(like, pos)
-    pos = pos.contiguous()
-    return pos, tokens if pos.dim() == 2 else 0
+def _launch(dev, name, *args):
+    """One native call on the current stream of device ``dev``."""
+    if dev == torch.cuda.current_device():
+        N.call(name, *args, _raw_stream(dev) if _raw_stream is not None else torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            N.call(name, *args, torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _qk_norm_rope_args(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved):
-    b, m, h, d = q.shape
-    n, hk = (k.shape[1], k.shape[2]) if k is not None else (0, 0)
-    q_pos, q_sb = q_pos
-    k_pos, k_sb = k_pos
-    shape = N.int64_array([b, m, n, h, hk, d])
-    strides = N.int64_array(_strides(q, 3) + (_strides(k, 3) if k is not None else [0, 0, 0]) + [q_sb, k_sb])
-    w = q_weight if q_weight is not None else k_weight
-    return (q.data_ptr(), _ptr(k), _code(q.dtype), shape, strides, _ptr(q_weight), _ptr(k_weight),
-            _code(w.dtype if w is not None else q.dtype), _ptr(q_pos), _ptr(k_pos),
-            int(q_pos is not None and q_pos.dtype == torch.int64), _ptr(inv_freq),
-            int(inv_freq is not None and inv_freq.dtype == torch.float64),
-            inv_freq.numel() if inv_freq is not None else 0, int(interleaved), eps)
+def _rows_ok(shape, stride, unit, most=1 << 62) -> bool:
+    """[B, T, H, D] strides that a kernel reads in place: a dense last axis, the others multiples of ``unit``
+    elements (a token's below ``most``); axes of one element are never stepped."""
+    return stride[3] == 1 and all(n <= 1 or st % unit == 0 for n, st in zip(shape, stride[:3])) and (
+        shape[1] <= 1 or stride[1] < most)
 
 
-def _qk_norm_rope_fwd(q, k, *args):
+def _steps(shape, stride, axes):
+    """Strides of the leading axes, 0 for those of one element."""
+    return [st if n > 1 else 0 for n, st in zip(shape[:axes], stride)]
+
+
+class _Plan:
+    """What one layout of operands needs of a native call: checked once, kept by sizes, strides and types (never by a
+    tensor's identity or address)."""
+
+
+def _check_positions(pos, tokens, batch, what):
+    """The batch stride of positions [tokens] or [batch, tokens]."""
+    shape, _, dtype = pos
+    _check(dtype in (torch.int32, torch.int64), f"expected int32 or int64 {what}")
+    _check(shape in ((tokens,), (batch, tokens)), f"expected {what} of shape [tokens] or [batch, tokens]")
+    return tokens if len(shape) == 2 else 0
+
+
+@lru_cache(maxsize=512)
+def _norm_rope_plan(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq):
+    _check(len(q[0]) == 4 and (k is None or len(k[0]) == 4), "expected q and k of shape [B, tokens, heads, D]")
+    (b, m, h, d), dtype = q[0], q[2]
+    code = _code(dtype)
+    _check(8 <= d <= 256 and d % 8 == 0, "head dim must be a multiple of 8 in [8, 256]")
+    _check(k is None or (k[0][0] == b and k[0][3] == d and k[2] == dtype), "k must match q's batch, head dim and dtype")
+    _check(k is not None or k_weight is None, "k_weight needs k")
+    for w in (q_weight, k_weight):
+        _check(w is None or (w[0] == (d,) and w[2] in (torch.float32, dtype)), "expected weights of [D] in fp32 or q's dtype")
+    _check(q_weight is None or k_weight is None or q_weight[2] == k_weight[2], "the weights must share a dtype")
+    n, hk = k[0][1:3] if k is not None else (0, 0)
+    half, freq64, pos64, sbs = 0, 0, 0, [0, 0]
+    if inv_freq is not None:
+        (half,), freq64 = inv_freq[0] if len(inv_freq[0]) == 1 else (0,), int(inv_freq[2] == torch.float64)
+        _check(inv_freq[2] in (torch.float32, torch.float64) and half > 0 and half % 4 == 0 and 2 * half <= d,
+               "expected fp32 or fp64 inv_freq, a multiple of 4 of at most D / 2 values")
+        _check(q_pos is not None and (k is None or k_pos is not None), "expected int32 or int64 positions")
+        sbs[0] = _check_positions(q_pos, m, b, "q_pos")
+        if k is not None:
+            sbs[1] = _check_positions(k_pos, n, b, "k_pos")
+            _check(q_pos[2] == k_pos[2], "the positions must share a dtype")
+        pos64 = int(q_pos[2] == torch.int64)
+    plan = _Plan()
+    plan.q_ok, plan.k_ok = _rows_ok(q[0], q[1], 4), k is None or _rows_ok(k[0], k[1], 4)
+    plan.unit = 4 * (4 if code == N.F32 else 2)  # bytes
+    strides = _steps(q[0], q[1], 3) + (_steps(k[0], k[1], 3) if k is not None else [0, 0, 0]) + sbs
+    weight = q_weight or k_weight
+    plan.code, plan.w_code = code, _code(weight[2]) if weight else code
+    plan.shape, plan.strides = N.int64_array([b, m, n, h, hk, d]), N.int64_array(strides)
+    plan.no_q, plan.no_k = N.int64_array([b, 0, n, h, hk, d]), N.int64_array([b, m, 0, h, 0, d])
+    plan.tail = (pos64, freq64, half)
+    plan.ws = N.lib().bmx_qk_norm_rope_workspace_bytes(d)
+    return plan
+
+
+def _norm_rope_args(plan, shape, q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved):
+    pos64, freq64, half = plan.tail
+    return (q.data_ptr(), _ptr(k), plan.code, shape, plan.strides, _ptr(q_weight), _ptr(k_weight), plan.w_code, _ptr(q_pos),
+            _ptr(k_pos), pos64, _ptr(inv_freq), freq64, half, interleaved, eps)
+
+
+def _norm_rope_fwd(plan, dev, q, k, *rest):
     q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     k_out = torch.empty(k.shape, device=k.device, dtype=k.dtype) if k is not None else None
-    with _at_device(q):
-        N.call("bmx_qk_norm_rope_fwd", *_qk_norm_rope_args(q, k, *args), q_out.data_ptr(), _ptr(k_out), _stream(q))
+    _launch(dev, "bmx_qk_norm_rope_fwd", *_norm_rope_args(plan, plan.shape, q, k, *rest), q_out.data_ptr(), _ptr(k_out))
     return q_out, k_out
 
 
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved):
-        ctx.save_for_backward(q, k, q_weight, k_weight, q_pos[0], k_pos[0], inv_freq)
-        ctx.rest = q_pos[1], k_pos[1], eps, interleaved
+    def forward(ctx, plan, dev, q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved):
+        ctx.save_for_backward(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq)
+        ctx.rest = plan, dev, eps, interleaved
         ctx.set_materialize_grads(False)
-        return _qk_norm_rope_fwd(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved)
+        return _norm_rope_fwd(plan, dev, q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dq_out, dk_out):
+        plan, dev, eps, interleaved = ctx.rest
         q, k, q_weight, k_weight, q_pos, k_pos, inv_freq = ctx.saved_tensors
-        q_sb, k_sb, eps, interleaved = ctx.rest
+        dq = dk = dqw = dkw = ws = None
         # A tensor whose result got no gradient takes no part: no tokens of it.
-        q_in, k_in = dq_out is not None, dk_out is not None
-        dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if q_in else None
-        dk = torch.empty(k.shape, device=k.device, dtype=k.dtype) if k_in else None
-        dqw = torch.empty_like(q_weight) if q_in and ctx.needs_input_grad[2] else None
-        dkw = torch.empty_like(k_weight) if k_in and ctx.needs_input_grad[3] else None
-        if q_in or k_in:
-            d = q.shape[3]
-            ws = None
-            if dqw is not None or dkw is not None:
-                ws = _workspace(N.lib().bmx_qk_norm_rope_workspace_bytes(d), q.device)
-            args = _qk_norm_rope_args(q if q_in else q[:, :0], k if k_in else None, q_weight, k_weight, (q_pos, q_sb),
-                                      (k_pos, k_sb), inv_freq, eps, interleaved)
-            dq_out = _aligned(dq_out.contiguous()) if q_in else None
-            dk_out = _aligned(dk_out.contiguous()) if k_in else None
-            with _at_device(q):
-                N.call("bmx_qk_norm_rope_bwd", *args, _ptr(dq_out), _ptr(dk_out), _ptr(dq), _ptr(dk), _ptr(dqw),
-                       _ptr(dkw), _ptr(ws), 0 if ws is None else ws.numel(), _stream(q))
-        return dq, dk, dqw, dkw, None, None, None, None, None
+        shape = plan.shape if dk_out is not None and dq_out is not None else plan.no_q if dq_out is None else plan.no_k
+        if dq_out is not None:
+            dq_out, dq = _aligned(dq_out.contiguous()), torch.empty(q.shape, device=q.device, dtype=q.dtype)
+            dqw = torch.empty_like(q_weight) if ctx.needs_input_grad[4] else None
+        if dk_out is not None:
+            dk_out, dk = _aligned(dk_out.contiguous()), torch.empty(k.shape, device=k.device, dtype=k.dtype)
+            dkw = torch.empty_like(k_weight) if ctx.needs_input_grad[5] else None
+        if dqw is not None or dkw is not None:
+            ws = _workspace(plan.ws, q.device)
+        if dq is not None or dk is not None:
+            _launch(dev, "bmx_qk_norm_rope_bwd",
+                    *_norm_rope_args(plan, shape, q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved),
+                    _ptr(dq_out), _ptr(dk_out), _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(ws),
+                    plan.ws if ws is not None else 0)
+        return None, None, dq, dk, dqw, dkw, None, None, None, None, None
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps=1e-6, interleaved=False):
@@ -1264,34 +1307,29 @@ def qk_norm_rope(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps=1e-6, int
     (2 i, 2 i + 1)); channels past 2 R are only normalised.  With inv_freq None
     nothing turns and the positions may be None.  Returns dense (q', k');
     gradients reach q, k and the weights."""
-    _check(q.dim() == 4 and (k is None or k.dim() == 4), "expected q and k of shape [B, tokens, heads, D]")
-    _cuda(q, *(t for t in (k, q_weight, k_weight, inv_freq) if t is not None))
-    b, m, _, d = q.shape
-    _code(q.dtype)
-    _check(8 <= d <= 256 and d % 8 == 0, "head dim must be a multiple of 8 in [8, 256]")
-    _check(k is None or (k.shape[0] == b and k.shape[3] == d and k.dtype == q.dtype),
-           "k must match q's batch, head dim and dtype")
-    _check(k is not None or k_weight is None, "k_weight needs k")
-    for w in (q_weight, k_weight):
-        _check(w is None or (w.shape == (d,) and w.dtype in (torch.float32, q.dtype)),
-               "expected weights of [D] in fp32 or q's dtype")
-    _check(q_weight is None or k_weight is None or q_weight.dtype == k_weight.dtype, "the weights must share a dtype")
-    _check(eps > 0, "eps must be positive")
     if inv_freq is None:
-        q_pos, k_pos = (None, 0), (None, 0)
+        q_pos = k_pos = None
     else:
-        _check(inv_freq.dim() == 1 and inv_freq.dtype in (torch.float32, torch.float64) and inv_freq.numel() > 0
-               and inv_freq.numel() % 4 == 0 and 2 * inv_freq.numel() <= d,
-               "expected fp32 or fp64 inv_freq, a multiple of 4 of at most D / 2 values")
+        _check(isinstance(q_pos, torch.Tensor) and (k is None or isinstance(k_pos, torch.Tensor)),
+               "expected int32 or int64 positions")
         _check(not inv_freq.requires_grad, "inv_freq takes no gradient")
+        k_pos = None if k is None else k_pos
+        q_pos, k_pos = q_pos.contiguous(), None if k_pos is None else k_pos.contiguous()
         inv_freq = inv_freq.contiguous()
-        q_pos = _positions(q_pos, m, b, q, "q_pos")
-        k_pos = _positions(k_pos, k.shape[1], b, q, "k_pos") if k is not None else (None, 0)
-        _check(k is None or q_pos[0].dtype == k_pos[0].dtype, "the positions must share a dtype")
-    q_weight, k_weight = (None if w is None else _aligned(w.contiguous()) for w in (q_weight, k_weight))
-    q, k = _head_rows(q), None if k is None else _head_rows(k)
-    args = (q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, float(eps), bool(interleaved))
-    return _QkNormRope.apply(*args) if _needs_grad(q, k, q_weight, k_weight) else _qk_norm_rope_fwd(*args)
+    dev = _same_device(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq)
+    _check(eps > 0, "eps must be positive")
+    plan = _norm_rope_plan(_layout(q), _layout(k), _layout(q_weight), _layout(k_weight), _layout(q_pos), _layout(k_pos),
+                           _layout(inv_freq))
+    if not plan.q_ok or q.data_ptr() % plan.unit or not plan.k_ok or (k is not None and k.data_ptr() % plan.unit):
+        q, k = _aligned(q.contiguous()), None if k is None else _aligned(k.contiguous())
+        plan = _norm_rope_plan(_layout(q), _layout(k), _layout(q_weight), _layout(k_weight), _layout(q_pos),
+                               _layout(k_pos), _layout(inv_freq))
+    if q_weight is not None:
+        q_weight = _aligned(q_weight.contiguous())
+    if k_weight is not None:
+        k_weight = _aligned(k_weight.contiguous())
+    args = (plan, dev, q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, float(eps), int(interleaved))
+    return _QkNormRope.apply(*args) if _needs_grad(q, k, q_weight, k_weight) else _norm_rope_fwd(*args)
 
 
 @lru_cache(maxsize=64)
@@ -1310,45 +1348,60 @@ def _relative_thresholds(side, exact, max_distance):
     return (ctypes.c_int32 * len(edges))(*edges)
 
 
-def _relative_args(data, buckets, heads, q_pos, k_pos, batch, thresholds, bidirectional):
-    (q_pos, q_sb), (k_pos, k_sb) = q_pos, k_pos
-    return (data.data_ptr(), _code(data.dtype), buckets, heads, q_pos.data_ptr(), k_pos.data_ptr(),
-            int(q_pos.dtype == torch.int64), 1 if batch is None else batch, q_pos.shape[-1], k_pos.shape[-1], q_sb, k_sb, thresholds,
-            len(thresholds), int(bidirectional))
+@lru_cache(maxsize=512)
+def _relative_plan(table, q_pos, k_pos, exact, max_distance, bidirectional):
+    _check(len(table[0]) == 2 and table[0][0] > 0 and table[0][1] > 0, "expected a [buckets, heads] table")
+    (buckets, heads), code = table[0], _code(table[2])
+    _check(buckets <= MAX_BUCKETS and heads <= 65535, "at most 256 buckets and 65535 heads")
+    _check(not bidirectional or buckets % 2 == 0, "bidirectional buckets must be even in number")
+    side = buckets // 2 if bidirectional else buckets
+    _check(side >= 2, "expected at least two buckets a direction")
+    exact = side // 2 if exact is None else exact
+    _check(1 <= exact < side, "exact must be in [1, buckets of a direction)")
+    if exact == side - 1:
+        max_distance = side - 1  # nothing is shared by logarithm
+    _check(exact == side - 1 or exact < max_distance <= 1 << 30, "max_distance must be above exact, at most 2^30")
+    _check(len(q_pos[0]) in (1, 2) and len(k_pos[0]) in (1, 2), "expected positions [tokens] or [batch, tokens]")
+    batch = next((p[0][0] for p in (q_pos, k_pos) if len(p[0]) == 2), None)
+    m, n = q_pos[0][-1], k_pos[0][-1]
+    steps = _check_positions(q_pos, m, batch, "q_pos"), _check_positions(k_pos, n, batch, "k_pos")
+    _check(q_pos[2] == k_pos[2], "the positions must share a dtype")
+    plan = _Plan()
+    thresholds = _relative_thresholds(side, exact, max_distance)
+    plan.head = code, buckets, heads
+    plan.tail = (int(q_pos[2] == torch.int64), 1 if batch is None else batch, m, n, *steps, thresholds, len(thresholds),
+                 int(bidirectional))
+    plan.shape = (heads, m, n) if batch is None else (batch, heads, m, n)
+    plan.ws = N.lib().bmx_relative_bias_workspace_bytes(code, buckets, heads, plan.tail[1], m, n)
+    return plan
 
 
-def _relative_bias_fwd(table, q_pos, k_pos, batch, thresholds, bidirectional):
-    buckets, heads = table.shape
-    shape = (heads, q_pos[0].shape[-1], k_pos[0].shape[-1])
-    out = torch.empty(shape if batch is None else (batch, *shape), device=table.device, dtype=table.dtype)
+def _relative_bias_fwd(plan, dev, table, q_pos, k_pos):
+    out = torch.empty(plan.shape, device=table.device, dtype=table.dtype)
     if out.numel():
-        with _at_device(table):
-            N.call("bmx_relative_bias_fwd", *_relative_args(table, buckets, heads, q_pos, k_pos, batch, thresholds,
-                                                            bidirectional), out.data_ptr(), _stream(table))
+        _launch(dev, "bmx_relative_bias_fwd", table.data_ptr(), *plan.head, q_pos.data_ptr(), k_pos.data_ptr(), *plan.tail,
+                out.data_ptr())
     return out
 
 
 class _RelativeBias(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, table, q_pos, k_pos, batch, thresholds, bidirectional):
-        ctx.save_for_backward(q_pos[0], k_pos[0])
-        ctx.rest = table.shape, q_pos[1], k_pos[1], batch, thresholds, bidirectional
-        return _relative_bias_fwd(table, q_pos, k_pos, batch, thresholds, bidirectional)
+    def forward(ctx, plan, dev, table, q_pos, k_pos):
+        ctx.save_for_backward(q_pos, k_pos)
+        ctx.rest = plan, dev
+        return _relative_bias_fwd(plan, dev, table, q_pos, k_pos)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dbias):
         q_pos, k_pos = ctx.saved_tensors
-        (buckets, heads), q_sb, k_sb, batch, thresholds, bidirectional = ctx.rest
+        plan, dev = ctx.rest
         dbias = dbias.contiguous()
-        dtable = torch.empty(buckets, heads, device=dbias.device, dtype=dbias.dtype)
-        args = _relative_args(dbias, buckets, heads, (q_pos, q_sb), (k_pos, k_sb), batch, thresholds, bidirectional)
-        m, n = q_pos.shape[-1], k_pos.shape[-1]
-        ws = _workspace(N.lib().bmx_relative_bias_workspace_bytes(_code(dbias.dtype), buckets, heads, args[7], m, n),
-                        dbias.device)
-        with _at_device(dbias):
-            N.call("bmx_relative_bias_bwd", *args, dtable.data_ptr(), ws.data_ptr(), ws.numel(), _stream(dbias))
-        return dtable, None, None, None, None, None
+        dtable = torch.empty(plan.head[1:], device=dbias.device, dtype=dbias.dtype)
+        ws = _workspace(plan.ws, dbias.device)
+        _launch(dev, "bmx_relative_bias_bwd", dbias.data_ptr(), *plan.head, q_pos.data_ptr(), k_pos.data_ptr(), *plan.tail,
+                dtable.data_ptr(), ws.data_ptr(), plan.ws)
+        return None, None, dtable, None, None
 
 
 MAX_BUCKETS = 256
@@ -1369,94 +1422,89 @@ def relative_bias(table, q_pos, k_pos, exact=None, max_distance=128, bidirection
     is the clipped form (every distance its own bucket up to side - 1).
     Positions are int32 / int64, |pos| < 2^62, in any order.  The gradient
     reaches the table (fp32 sums, the same bits on every run)."""
-    _check(table.dim() == 2 and table.shape[0] > 0 and table.shape[1] > 0, "expected a [buckets, heads] table")
-    _cuda(table)
-    _code(table.dtype)
-    buckets, heads = table.shape
-    _check(buckets <= MAX_BUCKETS and heads <= 65535, "at most 256 buckets and 65535 heads")
-    _check(not bidirectional or buckets % 2 == 0, "bidirectional buckets must be even in number")
-    side = buckets // 2 if bidirectional else buckets
-    _check(side >= 2, "expected at least two buckets a direction")
-    exact = side // 2 if exact is None else int(exact)
-    _check(1 <= exact < side, "exact must be in [1, buckets of a direction)")
-    if exact == side - 1:
-        max_distance = side - 1  # nothing is shared by logarithm
-    _check(exact == side - 1 or exact < max_distance <= 1 << 30, "max_distance must be above exact, at most 2^30")
-    _check(q_pos.dim() in (1, 2) and k_pos.dim() in (1, 2), "expected positions [tokens] or [batch, tokens]")
-    batch = next((p.shape[0] for p in (q_pos, k_pos) if p.dim() == 2), None)
-    q_pos = _positions(q_pos, q_pos.shape[-1], batch, table, "q_pos")
-    k_pos = _positions(k_pos, k_pos.shape[-1], batch, table, "k_pos")
-    _check(q_pos[0].dtype == k_pos[0].dtype, "the positions must share a dtype")
-    args = (table.contiguous(), q_pos, k_pos, batch, _relative_thresholds(side, exact, int(max_distance)),
-            bool(bidirectional))
+    q_pos, k_pos, table = q_pos.contiguous(), k_pos.contiguous(), table.contiguous()
+    dev = _same_device(table, q_pos, k_pos)
+    plan = _relative_plan(_layout(table), _layout(q_pos), _layout(k_pos), None if exact is None else int(exact),
+                          int(max_distance), bool(bidirectional))
+    args = plan, dev, table, q_pos, k_pos
     return _RelativeBias.apply(*args) if _needs_grad(table) else _relative_bias_fwd(*args)
 
 
-def _head_tokens(x):
-    """``x`` [B, T, H, D] with a dense last axis, outer strides of multiples of
-    16 bytes (a token's below 2^22 elements) and 16-byte alignment: itself, or a dense copy."""
-    vec = 16 // x.element_size()
-    ok = x.stride(3) == 1 and x.data_ptr() % 16 == 0 and x.stride(1) < 1 << 22
-    if not ok or any(x.stride(i) % vec for i in range(3) if x.shape[i] > 1):
-        return _aligned(x.contiguous())
-    return x
+MAX_TOKEN_STRIDE = 1 << 22  # elements, of cross_attention's operands
+MAX_BIAS_STRIDE = 1 << 26
 
 
-def _cross_args(q, k, v, mask, bias, scale):
-    b, m, h, d = q.shape
-    n, hk = k.shape[1], k.shape[2]
-    strides = _strides(q, 3) + _strides(k, 3) + _strides(v, 3)
-    strides.append(0 if mask is None else _strides(mask, 1)[0])
-    strides += [0, 0, 0] if bias is None else _strides(bias, 3)
-    return (q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), _ptr(bias), _code(q.dtype),
-            N.int64_array([b, m, n, h, hk, d]), N.int64_array(strides), scale)
+@lru_cache(maxsize=512)
+def _cross_plan(q, k, v, mask, bias):
+    _check(len(q[0]) == 4 and len(k[0]) == 4 and len(v[0]) == 4, "expected q, k and v of shape [B, tokens, heads, D]")
+    (b, m, h, d), (n, hk), dtype = q[0], k[0][1:3], q[2]
+    code = _code(dtype)
+    _check(k[0] == v[0] and k[0][0] == b and k[0][3] == d and k[2] == v[2] == dtype,
+           "k and v must match q's batch, head dim and dtype")
+    _check(8 <= d <= 128 and d % 8 == 0, "head dim must be a multiple of 8 in [8, 128]")
+    _check(h > 0 and hk > 0 and h % hk == 0, "the query heads must be a multiple of the key heads")
+    _check(h * d < MAX_TOKEN_STRIDE, "expected fewer than 2^22 channels")
+    plan, unit = _Plan(), 16 // (4 if code == N.F32 else 2)
+    plan.ok = tuple(_rows_ok(*t[:2], unit, MAX_TOKEN_STRIDE) for t in (q, k, v))
+    strides = [st for t in (q, k, v) for st in _steps(t[0], t[1], 3)] + [0, 0, 0, 0]
+    plan.mask_ok = plan.bias_ok = True
+    if mask is not None:
+        shape, stride, kind = mask
+        _check(kind == torch.bool and shape in ((b, n), (1, n), (n,)), "expected a bool mask [B, N]")
+        plan.mask_ok = stride[-1] == 1 or n <= 1
+        strides[9] = stride[0] if len(shape) == 2 and shape[0] > 1 else 0
+    if bias is not None:
+        shape, stride, kind = bias
+        _check(len(shape) == 4 and kind == dtype and shape[0] in (1, b) and shape[1] in (1, h) and shape[2:] == (m, n),
+               "expected a bias [B or 1, H or 1, M, N] in q's dtype")
+        _check(n < MAX_BIAS_STRIDE, "a bias takes at most 2^26 - 1 keys")
+        plan.bias_ok = (stride[3] == 1 or n <= 1) and (m <= 1 or stride[2] < MAX_BIAS_STRIDE)
+        strides[10:] = _steps(shape, stride, 3)
+        dense = [shape[1] * m * n if shape[0] > 1 else 0, m * n if shape[1] > 1 else 0, n]
+        plan.dbias_strides = N.int64_array(dense)
+    plan.code, plan.scale = code, d ** -0.5
+    plan.shape, plan.strides = N.int64_array([b, m, n, h, hk, d]), N.int64_array(strides)
+    plan.out, plan.stats, plan.empty = (b, m, h, d), (b, h, m, 2), not (b and m and n)
+    plan.ws = N.lib().bmx_cross_attention_workspace_bytes(code, b, m, n, h, hk, d)
+    plan.ws_bwd = N.lib().bmx_cross_attention_bwd_workspace_bytes(b, m, n, h, hk, d)
+    return plan
 
 
-def _cross_attention_fwd(q, k, v, mask, bias, scale, for_backward=False):
+def _cross_attention_fwd(plan, dev, q, k, v, mask, bias, scale, for_backward=False):
     """(out, what rounding out left or None, row statistics or None)."""
-    b, m, h, d = q.shape
-    out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    lo = torch.empty_like(out) if for_backward and q.dtype == torch.bfloat16 else None
-    stats = torch.empty(b, h, m, 2, device=q.device, dtype=torch.float32) if for_backward else None
-    if out.numel():
-        nbytes = N.lib().bmx_cross_attention_workspace_bytes(_code(q.dtype), b, m, k.shape[1], h, k.shape[2], d)
-        ws = _workspace(nbytes, q.device) if nbytes else None
-        with _at_device(q):
-            N.call("bmx_cross_attention_fwd", *_cross_args(q, k, v, mask, bias, scale), out.data_ptr(), _ptr(lo),
-                   _ptr(stats), _ptr(ws), nbytes, _stream(q))
+    out = torch.empty(plan.out, device=q.device, dtype=q.dtype)
+    lo = torch.empty_like(out) if for_backward and plan.code == N.BF16 else None
+    stats = torch.empty(plan.stats, device=q.device, dtype=torch.float32) if for_backward else None
+    ws = _workspace(plan.ws, q.device) if plan.ws else None
+    _launch(dev, "bmx_cross_attention_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), _ptr(bias), plan.code,
+            plan.shape, plan.strides, scale, out.data_ptr(), _ptr(lo), _ptr(stats), _ptr(ws), plan.ws)
     return out, lo, stats
 
 
 class _CrossAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, mask, bias, scale):
-        out, lo, stats = _cross_attention_fwd(q, k, v, mask, bias, scale, for_backward=True)
+    def forward(ctx, plan, dev, q, k, v, mask, bias, scale):
+        out, lo, stats = _cross_attention_fwd(plan, dev, q, k, v, mask, bias, scale, for_backward=True)
         ctx.save_for_backward(q, k, v, mask, bias, out, lo, stats)
-        ctx.scale = scale
+        ctx.rest = plan, dev, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
         q, k, v, mask, bias, out, lo, stats = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dq, dk, dv, dbias = (torch.empty(t.shape, device=q.device, dtype=q.dtype) if need[i] else None
-                             for i, t in ((0, q), (1, k), (2, v), (4, bias)))
-        b, m, h, d = q.shape
-        if q.numel() and k.numel():
+        plan, dev, scale = ctx.rest
+        make = torch.zeros if plan.empty else torch.empty  # without queries or keys nothing depends on anything
+        dq, dk, dv, dbias = (make(t.shape, device=q.device, dtype=q.dtype) if need else None
+                             for need, t in zip((*ctx.needs_input_grad[2:5], ctx.needs_input_grad[6]), (q, k, v, bias)))
+        if not plan.empty:
             dout = _aligned(dout.contiguous())
-            nbytes = N.lib().bmx_cross_attention_bwd_workspace_bytes(b, m, k.shape[1], h, k.shape[2], d)
-            ws = _workspace(nbytes, q.device)
-            with _at_device(q):
-                N.call("bmx_cross_attention_bwd", *_cross_args(q, k, v, mask, bias, ctx.scale), out.data_ptr(), _ptr(lo),
-                       stats.data_ptr(), dout.data_ptr(), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dbias),
-                       None if dbias is None else N.int64_array(_strides(dbias, 2) + [dbias.stride(2)]), ws.data_ptr(), nbytes,
-                       _stream(q))
-        else:  # no queries or no keys: nothing depends on anything
-            for t in (dq, dk, dv, dbias):
-                if t is not None:
-                    t.zero_()
-        return dq, dk, dv, None, dbias, None
+            ws = _workspace(plan.ws_bwd, q.device)
+            _launch(dev, "bmx_cross_attention_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(mask), _ptr(bias),
+                    plan.code, plan.shape, plan.strides, scale, out.data_ptr(), _ptr(lo), stats.data_ptr(), dout.data_ptr(),
+                    _ptr(dq), _ptr(dk), _ptr(dv), _ptr(dbias), None if dbias is None else plan.dbias_strides,
+                    ws.data_ptr(), plan.ws_bwd)
+        return None, None, dq, dk, dv, None, dbias, None
 
 
 def cross_attention(q, k, v, mask=None, bias=None, scale=None):
@@ -1474,28 +1522,15 @@ def cross_attention(q, k, v, mask=None, bias=None, scale=None):
     1 / sqrt(D) by default.  Weights are rounded to q's type before the product
     with v; sums are fp32.  Gradients reach q, k, v and bias (summed over its
     shared axes in fp32) and are the same bits on every run."""
-    _check(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "expected q, k and v of shape [B, tokens, heads, D]")
-    _cuda(q, k, v, *(t for t in (mask, bias) if t is not None))
-    b, m, h, d = q.shape
-    n, hk = k.shape[1], k.shape[2]
-    _code(q.dtype)
-    _check(k.shape == v.shape and k.shape[0] == b and k.shape[3] == d and k.dtype == v.dtype == q.dtype,
-           "k and v must match q's batch, head dim and dtype")
-    _check(8 <= d <= 128 and d % 8 == 0, "head dim must be a multiple of 8 in [8, 128]")
-    _check(h > 0 and hk > 0 and h % hk == 0, "the query heads must be a multiple of the key heads")
-    _check(h * d < 1 << 22, "expected fewer than 2^22 channels")
-    scale = d ** -0.5 if scale is None else float(scale)
+    dev = _same_device(q, k, v, mask, bias)
+    plan = _cross_plan(_layout(q), _layout(k), _layout(v), _layout(mask), _layout(bias))
+    scale = plan.scale if scale is None else float(scale)
     _check(0 < scale < float("inf"), "scale must be positive and finite")
-    if mask is not None:
-        _check(mask.dtype == torch.bool and mask.shape in ((b, n), (1, n), (n,)), "expected a bool mask [B, N]")
-        mask = mask if mask.dim() == 2 else mask[None]
-        mask = mask if mask.stride(1) == 1 or n <= 1 else mask.contiguous()
-    if bias is not None:
-        _check(bias.dim() == 4 and bias.dtype == q.dtype and bias.shape[0] in (1, b) and bias.shape[1] in (1, h)
-               and bias.shape[2:] == (m, n), "expected a bias [B or 1, H or 1, M, N] in q's dtype")
-        _check(n < 1 << 26, "a bias takes at most 2^26 - 1 keys")
-        bias = bias if (bias.stride(3) == 1 or n <= 1) and bias.stride(2) < 1 << 26 else bias.contiguous()
-    q, k, v = _head_tokens(q), _head_tokens(k), _head_tokens(v)
+    if not (all(plan.ok) and plan.mask_ok and plan.bias_ok) or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        q, k, v = (t if ok and t.data_ptr() % 16 == 0 else _aligned(t.contiguous()) for t, ok in zip((q, k, v), plan.ok))
+        mask = mask if plan.mask_ok else mask.contiguous()
+        bias = bias if plan.bias_ok else bias.contiguous()
+        plan = _cross_plan(_layout(q), _layout(k), _layout(v), _layout(mask), _layout(bias))
     if _needs_grad(q, k, v, bias):
-        return _CrossAttention.apply(q, k, v, mask, bias, scale)
-    return _cross_attention_fwd(q, k, v, mask, bias, scale)[0]
+        return _CrossAttention.apply(plan, dev, q, k, v, mask, bias, scale)
+    return _cross_attention_fwd(plan, dev, q, k, v, mask, bias, scale)[0]
