@@ -48,9 +48,15 @@ struct CrossArgs {
 
 // Blocks go round the XCDs in turn: block b of `total` becomes a position such that each XCD
 // works through consecutive ones, whose keys then stay in its own L2.
-__device__ __forceinline__ int64_t xcd_position(int64_t b, int64_t total) {
-  const int64_t per = total / 8, whole = per * 8;
+__device__ __forceinline__ uint32_t xcd_position(uint32_t b, uint32_t total) {
+  const uint32_t per = total / 8, whole = per * 8;
   return b < whole ? (b % 8) * per + b / 8 : b;
+}
+// at % n, with at / n left in at: one axis of a block's position.
+__device__ __forceinline__ int take(uint32_t& at, uint32_t n) {
+  const uint32_t q = at / n, r = at - q * n;
+  at = q;
+  return (int)r;
 }
 
 // ---- LDS tiles -----------------------------------------------------------

@@ -12,6 +12,7 @@
 // weights add up to one: the error is a rounding of each weight against the others.
 //
 // A row without keys (masked, or -inf bias throughout) gives zeros.
+#include <algorithm>
 #include <type_traits>
 
 #include "cross_attention.h"
@@ -157,10 +158,8 @@ struct Place {
   int row_block, split, c, first, stop;  // keys of the split
   int64_t b;
   __device__ __forceinline__ Place(const CrossArgs& a) {
-    int64_t at = xcd_position(blockIdx.x, gridDim.x);
-    row_block = (int)(at % a.row_blocks), at /= a.row_blocks;
-    split = (int)(at % a.splits), at /= a.splits;
-    c = (int)(at % a.kv_heads), b = at / a.kv_heads;
+    uint32_t at = xcd_position(blockIdx.x, gridDim.x);
+    row_block = take(at, a.row_blocks), split = take(at, a.splits), c = take(at, a.kv_heads), b = at;
     first = split * a.split_keys;
     stop = min(first + a.split_keys, a.n);
   }
@@ -176,7 +175,7 @@ void cross_attention_wide(CrossArgs a) {
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[4 * kTile + kMaskChunk / 8];
   const Place p(a);
-  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), row = p.row_block * 128 + w * 32 + (t & 31);
+  const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), row = (p.row_block * 4 + w) * 32 + (t & 31);
   Rows<T, DP, kBias> rows;
   rows.init(a, p.b, p.c, row);
   const T* k = (const T*)a.k + p.b * a.sk[0] + p.c * a.sk[2];
@@ -353,17 +352,18 @@ struct Split {
   int keys;  // per split, a multiple of 128
 };
 
-// Few rows run as many splits as give every compute unit two blocks, each of at least 128 keys (one tile a wave); many rows
-// split only where their blocks leave compute units idle.
+// Few rows run as many splits as give every compute unit two blocks, each of at least 128 keys (one tile a wave).
+// Many rows split where their blocks leave compute units idle, or, for a second wave on every SIMD, where the keys
+// are many enough to pay for writing and joining the parts (bf16, 256 blocks, D = 64: 1024 keys 26 us whole and
+// 30 in two, 4096 keys 77 and 57; fp32's keys cost several times as much: 96 blocks of 1134 keys 63 in two, 50 in five).
 Split plan(int dtype, int64_t batch, int64_t kv_heads, int64_t rows, int64_t n) {
   Split s;
   s.few = rows <= 32;
   s.row_blocks = s.few ? 1 : (int)((rows + 127) / 128);
-  const int64_t blocks = (int64_t)s.row_blocks * batch * kv_heads, least = s.few ? 128 : 256;
-  const int64_t want = s.few ? 512 : 256;
-  int64_t splits = blocks ? want / blocks : 1;
-  const int64_t most = (n + least - 1) / least;
-  splits = splits < 1 ? 1 : splits > most ? (most > 0 ? most : 1) : splits;
+  const int64_t blocks = (int64_t)s.row_blocks * batch * kv_heads;
+  auto fill = [&](int64_t want, int64_t least) { return blocks ? std::min(want / blocks, (n + least - 1) / least) : 1; };
+  int64_t splits = s.few ? fill(512, 128) : dtype == kF32 ? fill(512, 256) : std::max(fill(256, 256), fill(512, 1024));
+  if (splits < 1) splits = 1;
   s.keys = (int)(((n + splits - 1) / splits + 127) / 128 * 128);
   if (s.keys == 0) s.keys = 128;
   s.splits = (int)(n > 0 ? (n + s.keys - 1) / s.keys : 1);

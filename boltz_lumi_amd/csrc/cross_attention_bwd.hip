@@ -121,13 +121,10 @@ template <typename T, int DP, bool kBias>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dq(CrossArgs a) {
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[4 * kTile + kMaskChunk / 8];
-  int64_t at = xcd_position(blockIdx.x, gridDim.x);
-  const int row_block = (int)(at % a.row_blocks);
-  at /= a.row_blocks;
-  const int split = (int)(at % a.splits), first = split * a.split_keys, stop = min(first + a.split_keys, a.n);
-  at /= a.splits;
-  const int c = (int)(at % a.kv_heads);
-  const int64_t b = at / a.kv_heads;
+  uint32_t at = xcd_position(blockIdx.x, gridDim.x);
+  const int row_block = take(at, a.row_blocks), split = take(at, a.splits), c = take(at, a.kv_heads);
+  const int64_t b = at;
+  const int first = split * a.split_keys, stop = min(first + a.split_keys, a.n);
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), h = lane_id() >> 5;
   const int row = row_block * 128 + w * 32 + (t & 31);
   const RowAt ra(a, c, row);
@@ -226,13 +223,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   constexpr int kValues = 4 * kTile + 2 * kStat + 16;  // V of the block's 128 keys
   __shared__ __attribute__((aligned(16))) char lds[kValues + (kValuesInLds ? 4 * kTile : 0)];
   const int key_blocks = (a.n + 127) / 128;
-  int64_t at = xcd_position(blockIdx.x, gridDim.x);
-  const int first = (int)(at % key_blocks) * 128;
-  at /= key_blocks;
-  const int split = (int)(at % a.splits);
-  at /= a.splits;
-  const int c = (int)(at % a.kv_heads);
-  const int64_t b = at / a.kv_heads;
+  uint32_t at = xcd_position(blockIdx.x, gridDim.x);
+  const int first = take(at, key_blocks) * 128, split = take(at, a.splits), c = take(at, a.kv_heads);
+  const int64_t b = at;
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = lane_id(), h = l >> 5;
   const int lane_key = tile_row(l & 31), key = first + w * 32 + lane_key, safe = min(key, a.n - 1);
   KeyWords words{(uint32_t*)(lds + 4 * kTile + 2 * kStat), a.mask ? a.mask + b * a.smask : nullptr};
@@ -413,13 +406,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   constexpr int kWords = 2 * kTile + 2 * kRowTile;
   __shared__ __attribute__((aligned(16))) char lds[kWords + 16];
   const int key_blocks = (a.n + KT - 1) / KT, query_blocks = (int)((a.m + 127) / 128);
-  int64_t at = xcd_position(blockIdx.x, gridDim.x);
-  const int key = (int)(at % key_blocks) * KT;
-  at /= key_blocks;
-  const int q0 = (int)(at % query_blocks) * 128;
-  at /= query_blocks;
-  const int plane_heads = a.sdb[1] ? a.heads : 1;
-  const int64_t ph = at % plane_heads, pb = at / plane_heads;
+  uint32_t at = xcd_position(blockIdx.x, gridDim.x);
+  const int key = take(at, key_blocks) * KT, q0 = take(at, query_blocks) * 128;
+  const int64_t ph = take(at, a.sdb[1] ? a.heads : 1), pb = at;
   const int64_t b0 = a.sdb[0] ? pb : 0, b1 = a.sdb[0] ? pb + 1 : a.batch;
   const int h0 = a.sdb[1] ? (int)ph : 0, h1 = a.sdb[1] ? (int)ph + 1 : a.heads;
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = lane_id(), h = l >> 5;
