@@ -114,7 +114,9 @@ __device__ __forceinline__ int tile_row(int i) { return 16 * ((i >> 2) & 1) + 4 
 template <typename T, int DP, bool kKeep = true>
 struct RowReads {
   int off[kKeep ? RowOperand<T, DP>::kSteps : 1];
-  __device__ __forceinline__ void init() {
+  int steps;  // fp32: with channels below dim, the others are passed over (four MFMA a step)
+  __device__ __forceinline__ void init(int dim) {
+    steps = (dim + 2 * Tile<T, DP>::kElems - 1) / (2 * Tile<T, DP>::kElems);
     const int r = tile_row(lane_id() & 31), h = lane_id() >> 5;
 #pragma unroll
     for (int s = 0; s < (kKeep ? RowOperand<T, DP>::kSteps : 1); ++s) off[s] = Tile<T, DP>::at(r, 2 * s + h);
@@ -129,9 +131,15 @@ template <typename T, int DP, bool kKeep>
 __device__ __forceinline__ f32x16 product(const char* tile, const RowReads<T, DP, kKeep>& reads,
                                           const RowOperand<T, DP>& b) {
   f32x16 acc = zero16();
+  auto step = [&](int s) { acc = mfma_step((const T*)nullptr, *(const u32x4*)(tile + reads.at(s)), b.c[s], acc); };
+  if (sizeof(T) == 2 || reads.steps == RowOperand<T, DP>::kSteps) {
 #pragma unroll
-  for (int s = 0; s < RowOperand<T, DP>::kSteps; ++s)
-    acc = mfma_step((const T*)nullptr, *(const u32x4*)(tile + reads.at(s)), b.c[s], acc);
+    for (int s = 0; s < RowOperand<T, DP>::kSteps; ++s) step(s);
+  } else {
+#pragma unroll
+    for (int s = 0; s < RowOperand<T, DP>::kSteps; ++s)
+      if (s < reads.steps) step(s);
+  }
   return acc;
 }
 

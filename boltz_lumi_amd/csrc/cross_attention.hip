@@ -43,7 +43,7 @@ struct Rows {
     const int64_t head = (int64_t)kv * a.group + g;
     q.load((const T*)a.q + b * a.sq[0] + i * a.sq[1] + head * a.sq[2], a.dim, lane_id() >> 5);
     bias = (const T*)a.bias + b * a.sb[0] + head * a.sb[1] + i * a.sb[2];
-    kr.init();
+    kr.init(a.dim);
     vr.init();
 #pragma unroll
     for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();

@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   const T* bias_row = (const T*)a.bias + ra.bias(a, b);
   RowReads<T, DP> rr;
   ColumnReads<T, DP> cr;
-  rr.init();
+  rr.init(a.dim);
   cr.init();
   f32x16 dq[DP / 32];
 #pragma unroll
@@ -243,7 +243,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
     if (!kValuesInLds) vf.load((const T*)a.v + b * a.sv[0] + safe * a.sv[1] + c * a.sv[2], a.dim, h);
     RowReads<T, DP, !kValuesInLds> rr;
     ColumnReads<T, DP, !kValuesInLds> cr;
-    rr.init();
+    rr.init(a.dim);
     cr.init();
     const int64_t row_step = (int64_t)a.heads * a.dim;
     Copy<T, DP, 32, 4> cq, cg;
@@ -418,7 +418,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   for (int u = 0; u < kParts; ++u) sum[u] = zero16();
   KeyWords words{(uint32_t*)(lds + kWords), nullptr};
   RowReads<T, DP> rr;
-  rr.init();
+  rr.init(a.dim);
   const int64_t row_step = (int64_t)a.heads * a.dim;
   Copy<T, DP, KT, 4> ck, cv;
   Copy<T, DP, 128, 4> cq, cg;
