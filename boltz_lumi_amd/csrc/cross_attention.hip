@@ -110,9 +110,12 @@ __device__ __forceinline__ void store_out<float>(const CrossArgs& a, int64_t at,
   *(f32x4*)((float*)a.out + at) = v;
 }
 
+// A row without keys. A row whose logits are all NaN has no maximum either, but a sum that is NaN, and stays NaN.
+__device__ __forceinline__ bool no_keys(float top, float sum) { return top == -INFINITY && sum == sum; }
+
 // Row maximum in natural units and log2 of the sum; a row without keys gets weights exp2(-inf) = 0.
 __device__ __forceinline__ float2 row_stats(const CrossArgs& a, float top, float sum, bool bias) {
-  if (!(sum != 0.f) || top == -INFINITY) return make_float2(0.f, INFINITY);
+  if (no_keys(top, sum)) return make_float2(0.f, INFINITY);
   return make_float2(bias ? top : top * a.scale, __builtin_amdgcn_logf(sum));
 }
 
@@ -138,7 +141,7 @@ __device__ __forceinline__ void write_rows(const CrossArgs& a, int64_t b, int c,
   const int g0 = row / (int)a.m, i = row - g0 * (int)a.m;
   const int64_t head = (int64_t)c * a.group + g0;
   const int64_t at = ((b * a.m + i) * a.heads + head) * a.dim;
-  const bool none = top == -INFINITY;
+  const bool none = no_keys(top, sum);
   const float f = none ? 0.f : 1.f / sum;
   if (a.stats && h == 0) a.stats[(b * a.heads + head) * a.m + i] = row_stats(a, top, sum, bias);
 #pragma unroll
@@ -338,7 +341,7 @@ __global__ __launch_bounds__(256) void cross_attention_join(CrossArgs a, int bia
   const int64_t list = at / a.rows, b = list / a.kv_heads;
   const int row = (int)(at - list * a.rows), g = row / (int)a.m, i = row - g * (int)a.m;
   const int64_t head = (list - b * a.kv_heads) * a.group + g;
-  const bool none = top == -INFINITY;
+  const bool none = no_keys(top, sum);
   if (a.stats && d == 0) a.stats[(b * a.heads + head) * a.m + i] = row_stats(a, top, sum, bias);
   const float f = none ? 0.f : 1.f / sum;
 #pragma unroll

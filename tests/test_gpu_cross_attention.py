@@ -190,6 +190,29 @@ def test_masks_hide_anything(gpu, dtype, m):
         check(out[i, 0, 0], weights @ x, weights @ x.abs(), "lowest")
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n", [(1, 40), (1, 3000), (50, 40), (200, 700)])
+def test_nan_is_kept(gpu, dtype, m, n):
+    """NaN in a query or in a present key shows in every result it belongs to, and in no other row."""
+    g = torch.Generator(device=gpu).manual_seed(9)
+    q, k, v = (randn(g, 2, t, 2, 32, dtype=dtype) for t in (m, n, n))
+    dout = torch.ones_like(q)
+    q[0, m - 1, 1, 3] = math.nan
+    k[1, n // 2, 0, 5] = math.nan
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    out = ops.cross_attention(*leaves)
+    dq, dk, dv = torch.autograd.grad(out, leaves, dout)
+    want = torch.zeros(2, m, 2, dtype=torch.bool, device=gpu)
+    want[0, m - 1, 1] = True
+    want[1, :, 0] = True
+    for t in (out, dq):
+        bad = torch.isnan(t)
+        assert torch.equal(bad.all(-1), want) and torch.equal(bad.any(-1), want)
+    heads = torch.tensor([[False, True], [True, False]], device=gpu)[:, None].expand(2, n, 2)
+    for t in (dk, dv):
+        assert torch.equal(torch.isnan(t).any(-1), heads)
+
+
 def test_layouts(gpu):
     """Column slices of joint projections, head-major tensors, odd storage offsets, a bias and a mask by strides: the
     same bits as dense operands."""
