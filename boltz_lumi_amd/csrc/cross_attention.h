@@ -35,6 +35,7 @@ struct CrossArgs {
   void *out, *out_lo;
   float2* stats;  // [batch][heads][m]: row maximum of the logits and log2 of the sum of exp(logit - maximum)
   // work split
+  int batch_first;  // a bias shared by the batch: its elements' blocks follow each other, so that it stays in L2
   int row_blocks, splits;
   int split_keys;  // or, of dK and dV, tiles of 32 queries
   float* part_o;   // [split][batch * kv_heads][rows][dim] sums before the division; backward: [split] gradients
@@ -395,6 +396,10 @@ struct KeyWords {
 // Bias of a lane's query at the 16 keys of a logits tile, in register order, as it lies in memory: loaded a tile ahead,
 // together with the tile's copies, whose wait is then its own. bf16 rows at an odd element (an odd number of keys) are read
 // from the dword before and shifted: 16-byte loads at 2-byte alignment took 109 us against 74 at 1531 keys.
+__device__ __forceinline__ bool bias_odd(const CrossArgs& a) {
+  return (((int)((uintptr_t)a.bias >> 1) | (int)a.sb[0] | (int)a.sb[1] | (int)a.sb[2]) & 1) != 0;
+}
+
 template <typename T>
 struct BiasTile;
 template <>
@@ -413,7 +418,7 @@ struct BiasTile<float> {
       for (int r = 0; r < 16; ++r) v[r >> 2][r & 3] = __float_as_uint(row[min(k + r, n - 1)]);
     }
   }
-  __device__ __forceinline__ void ready() {}
+  __device__ __forceinline__ void ready(bool) {}
   __device__ __forceinline__ float at(int r) const { return __uint_as_float(v[r >> 2][r & 3]); }
 };
 template <>
@@ -440,8 +445,9 @@ struct BiasTile<bf16> {
       last = shift = 0;
     }
   }
-  // Shifts the words into place: before the first at().
-  __device__ __forceinline__ void ready() {
+  // Shifts the words into place, before the first at(); odd: some row of the bias may need it (uniform).
+  __device__ __forceinline__ void ready(bool odd) {
+    if (!odd) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
       v[i >> 2][i & 3] = __builtin_amdgcn_alignbit(i < 7 ? v[(i + 1) >> 2][(i + 1) & 3] : last, v[i >> 2][i & 3], shift);

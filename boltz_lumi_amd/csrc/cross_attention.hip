@@ -24,19 +24,20 @@ namespace {
 // State of a wave's 32 rows: lane l holds row l % 32, in both halves.
 template <typename T, int DP, bool kBias>
 struct Rows {
-  // Without a bias the logits stay unscaled (q k^T); with one they are in natural units and the difference to the maximum is
-  // taken before the change to base 2, so that biases of the type's lowest value do not overflow. fp32 takes
-  // the difference first too: the largest logit's weight is then exactly 1 (bf16 rounds it to 1).
-  static constexpr bool kFirst = kBias || sizeof(T) == 4;
+  // The weight of a logit x is exp2(x c + shift), shift = -top c: without a bias x is q k^T, with one the logit in natural
+  // units. fp32 takes the difference first, exp2((x - top) c): the largest logit's weight is then exactly 1 (bf16
+  // rounds it to 1).
+  static constexpr bool kFirst = sizeof(T) == 4;
   RowOperand<T, DP> q;
   RowReads<T, DP> kr;
   ColumnReads<T, DP> vr;
   f32x16 o[DP / 32];
   float top, sum;  // maximum that the weights refer to; this half's share of their sum
   float limit;     // the maximum moves when a logit passes this
-  float shift;     // of the exponent: the maximum, or minus its product with c
+  float shift;     // of the exponent: -top c, or (fp32) top
   float c;         // logits to base 2
   const T* bias;
+  bool odd;  // some bias rows start at an odd element
 
   __device__ __forceinline__ void init(const CrossArgs& a, int64_t b, int kv, int row) {
     const int r = min(row, a.rows - 1), g = r / (int)a.m, i = r - g * (int)a.m;
@@ -49,6 +50,7 @@ struct Rows {
     for (int dt = 0; dt < DP / 32; ++dt) o[dt] = zero16();
     top = limit = -INFINITY, sum = shift = 0.f;
     c = (kBias ? 1.f : a.scale) * kLog2E;
+    odd = bias_odd(a);
   }
 
   // 32 keys: rows of the tiles, presence bits, bias.
@@ -56,7 +58,7 @@ struct Rows {
                                          BiasTile<T>& b) {
     f32x16 s = product<T, DP>(kt, kr, q);
     if (kBias) {
-      b.ready();
+      b.ready(odd);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = s[r] * a.scale + b.at(r);
     }
@@ -79,7 +81,10 @@ struct Rows {
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) o[dt] *= f;
       top = mx;
-      limit = sizeof(T) == 2 ? mx + 6.f / c : mx;
+      // A maximum near the type's lowest (or largest) value would overflow in base 2. Logits that size differ by 0
+      // or by more than any exponent, so half of them tells the same weights. (fp32's difference is taken first.)
+      if (kBias && !kFirst) c = fabsf(base) > 1e38f ? 0.5f : kLog2E;
+      limit = kFirst ? mx : mx + 6.f / c;
       shift = kFirst ? base : -base * c;
     }
 #pragma unroll
@@ -162,7 +167,9 @@ struct Place {
   int64_t b;
   __device__ __forceinline__ Place(const CrossArgs& a) {
     uint32_t at = xcd_position(blockIdx.x, gridDim.x);
-    row_block = take(at, a.row_blocks), split = take(at, a.splits), c = take(at, a.kv_heads), b = at;
+    b = a.batch_first ? take(at, a.batch) : 0;
+    row_block = take(at, a.row_blocks), split = take(at, a.splits), c = take(at, a.kv_heads);
+    if (!a.batch_first) b = at;
     first = split * a.split_keys;
     stop = min(first + a.split_keys, a.n);
   }
@@ -424,6 +431,7 @@ int cross_setup(CrossArgs& a, int dtype, const int64_t* shape, const int64_t* st
   a.smask = strides[9];
   a.heads = (int)heads, a.kv_heads = (int)kv, a.group = (int)(heads / kv), a.dim = (int)dim, a.rows = (int)rows;
   a.scale = scale;
+  a.batch_first = has_bias && a.batch > 1 && a.sb[0] == 0;
   return BMX_OK;
 }
 

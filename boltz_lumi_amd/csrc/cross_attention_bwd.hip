@@ -103,7 +103,7 @@ __device__ __forceinline__ void store_keys(T* row, int key, int n, const f32x16&
 template <typename T, bool kBias>
 __device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, BiasTile<T>& b, float2 st) {
   if (kBias) {
-    b.ready();
+    b.ready(true);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + b.at(r) - st.x) * kLog2E - st.y);
   } else if (sizeof(T) == 4) {  // as the forward pass: the difference first
@@ -122,8 +122,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[4 * kTile + kMaskChunk / 8];
   uint32_t at = xcd_position(blockIdx.x, gridDim.x);
+  int64_t b = a.batch_first ? take(at, a.batch) : 0;
   const int row_block = take(at, a.row_blocks), split = take(at, a.splits), c = take(at, a.kv_heads);
-  const int64_t b = at;
+  if (!a.batch_first) b = at;
   const int first = split * a.split_keys, stop = min(first + a.split_keys, a.n);
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), h = lane_id() >> 5;
   const int row = row_block * 128 + w * 32 + (t & 31);
@@ -224,8 +225,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   __shared__ __attribute__((aligned(16))) char lds[kValues + (kValuesInLds ? 4 * kTile : 0)];
   const int key_blocks = (a.n + 127) / 128;
   uint32_t at = xcd_position(blockIdx.x, gridDim.x);
+  int64_t b = a.batch_first ? take(at, a.batch) : 0;
   const int first = take(at, key_blocks) * 128, split = take(at, a.splits), c = take(at, a.kv_heads);
-  const int64_t b = at;
+  if (!a.batch_first) b = at;
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = lane_id(), h = l >> 5;
   const int lane_key = tile_row(l & 31), key = first + w * 32 + lane_key, safe = min(key, a.n - 1);
   KeyWords words{(uint32_t*)(lds + 4 * kTile + 2 * kStat), a.mask ? a.mask + b * a.smask : nullptr};
