@@ -18,7 +18,6 @@
 namespace bmx {
 
 constexpr float kLog2E = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kMaskChunk = 4096;  // keys whose mask words are in LDS at a time
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -414,6 +413,7 @@ struct BiasTile<float> {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = *(const u32x4_at4*)(row + k + 4 * i);
     } else {
+      asm volatile("" : "+s"(n));  // keeps a loop's compiler from holding all these addresses over it
 #pragma unroll
       for (int r = 0; r < 16; ++r) v[r >> 2][r & 3] = __float_as_uint(row[min(k + r, n - 1)]);
     }
@@ -437,6 +437,7 @@ struct BiasTile<bf16> {
       last = p[odd ? 8 : 7];
       shift = (uint32_t)odd * 8;
     } else {
+      asm volatile("" : "+s"(n));
       uint16_t x[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r] = __builtin_bit_cast(uint16_t, row[min(k + r, n - 1)]);

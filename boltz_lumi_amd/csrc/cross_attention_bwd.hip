@@ -397,14 +397,25 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   }
 }
 
-// dbias of a bias that batch elements or heads share: a block holds 128 queries x 32 kParts keys of one bias plane in
-// registers and walks the batch elements and heads that share the plane, in order. bf16 heads up to 64 channels have
-// all four operands in LDS, copied there by DMA; wider ones read the queries' straight into registers.
+// dbias of a bias that batch elements or heads share: a block holds 128 queries x kBiasKeys keys of one bias plane in
+// registers and walks the batch elements and heads that share the plane, in order. bf16 has all four operands in LDS
+// by DMA. Up to 64 channels four waves and 64 keys take 48 KB, so that other blocks of the compute unit run under
+// one's copies (batch 5, 16 heads, 1024 x 1531, D = 64: 127 us; eight waves and 128 keys 155, four and 128 spill: 250).
+// Past 64 channels eight waves, four by the queries and two by the keys, and 128 keys take 128 KB (batch 2, 16 heads,
+// 1024 x 2048, D = 128: 125 us; four waves and 64 keys with the queries read into registers 154). fp32: four waves
+// and 32 keys, the queries' operands read straight into registers.
 template <typename T, int DP>
-__global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dbias(CrossArgs a) {
-  constexpr bool kRowsInLds = sizeof(T) == 2 && DP <= 64;
-  constexpr int kParts = sizeof(T) == 2 ? 2 : 1, KT = 32 * kParts;
-  constexpr int kTile = KT * Tile<T, DP>::kRowBytes, kRowTile = kRowsInLds ? 128 * Tile<T, DP>::kRowBytes : 0;
+constexpr int kBiasWaves = sizeof(T) == 2 && DP > 64 ? 8 : 4;
+template <typename T, int DP>
+constexpr int kBiasKeys = sizeof(T) == 4 ? 32 : DP > 64 ? 128 : 64;
+
+template <typename T, int DP>
+__global__ __launch_bounds__((64 * kBiasWaves<T, DP>), sizeof(T) == 4 && DP > 64 ? 1 : 2)
+void cross_attention_dbias(CrossArgs a) {
+  constexpr bool kRowsInLds = sizeof(T) == 2;
+  constexpr int kWaves = kBiasWaves<T, DP>, kThreads = 64 * kWaves, KT = kBiasKeys<T, DP>;
+  constexpr int kParts = KT / 32 / (kWaves / 4);  // of 32 keys, of a wave
+  constexpr int kRowBytes = Tile<T, DP>::kRowBytes, kTile = KT * kRowBytes, kRowTile = kRowsInLds ? 128 * kRowBytes : 0;
   constexpr int kWords = 2 * kTile + 2 * kRowTile;
   __shared__ __attribute__((aligned(16))) char lds[kWords + 16];
   const int key_blocks = (a.n + KT - 1) / KT, query_blocks = (int)((a.m + 127) / 128);
@@ -414,7 +425,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   const int64_t b0 = a.sdb[0] ? pb : 0, b1 = a.sdb[0] ? pb + 1 : a.batch;
   const int h0 = a.sdb[1] ? (int)ph : 0, h1 = a.sdb[1] ? (int)ph + 1 : a.heads;
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = lane_id(), h = l >> 5;
-  const int m = (int)a.m, i = q0 + w * 32 + tile_row(l & 31), safe = min(i, m - 1);
+  const int rows_at = (w & 3) * 32, keys_at = (w >> 2) * 32 * kParts;  // of the wave, in the block's
+  const int m = (int)a.m, i = q0 + rows_at + tile_row(l & 31), safe = min(i, m - 1);
   f32x16 sum[kParts];
 #pragma unroll
   for (int u = 0; u < kParts; ++u) sum[u] = zero16();
@@ -422,8 +434,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   RowReads<T, DP> rr;
   rr.init(a.dim);
   const int64_t row_step = (int64_t)a.heads * a.dim;
-  Copy<T, DP, KT, 4> ck, cv;
-  Copy<T, DP, 128, 4> cq, cg;
+  Copy<T, DP, KT, kWaves> ck, cv;
+  Copy<T, DP, 128, kWaves> cq, cg;
   ck.init(w, a.dim, a.sk[1]);
   cv.init(w, a.dim, a.sv[1]);
   if (kRowsInLds) {
@@ -431,13 +443,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
     cg.init(w, a.dim, row_step);
   }
   const unsigned lds0 = lds_address(lds);
-  clear_tiles<T, DP, 256>(t, lds, kWords, a.dim);
+  clear_tiles<T, DP, kThreads>(t, lds, kWords, a.dim);
   for (int64_t b = b0; b < b1; ++b) {
     words.mask = a.mask ? a.mask + b * a.smask : nullptr;
     words.fill(key, min(key + KT, a.n));
     uint32_t any = 0;
 #pragma unroll
-    for (int u = 0; u < kParts; ++u) any |= words.bits(key + 32 * u);
+    for (int u = 0; u < KT / 32; ++u) any |= words.bits(key + 32 * u);
     if (any == 0) continue;
     for (int head = h0; head < h1; ++head) {
       const int c = head / a.group;
@@ -460,33 +472,33 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
       const T* bias_row = (const T*)a.bias + b * a.sb[0] + head * a.sb[1] + safe * a.sb[2];
       BiasTile<T> bias[kParts];
 #pragma unroll
-      for (int u = 0; u < kParts; ++u) bias[u].load(bias_row, min(key + 32 * u, a.n - 1), a.n);
+      for (int u = 0; u < kParts; ++u) bias[u].load(bias_row, min(key + keys_at + 32 * u, a.n - 1), a.n);
       wait_copies();
       __syncthreads();
       if (kRowsInLds) {
 #pragma unroll
         for (int s = 0; s < RowOperand<T, DP>::kSteps; ++s) {
-          q.c[s] = *(const u32x4*)(lds + 2 * kTile + w * 32 * Tile<T, DP>::kRowBytes + rr.at(s));
-          g.c[s] = *(const u32x4*)(lds + 2 * kTile + kRowTile + w * 32 * Tile<T, DP>::kRowBytes + rr.at(s));
+          q.c[s] = *(const u32x4*)(lds + 2 * kTile + rows_at * kRowBytes + rr.at(s));
+          g.c[s] = *(const u32x4*)(lds + 2 * kTile + kRowTile + rows_at * kRowBytes + rr.at(s));
         }
       }
 #pragma unroll
       for (int u = 0; u < kParts; ++u) {
-        const char* kt = lds + u * 32 * Tile<T, DP>::kRowBytes;
+        const char* kt = lds + (keys_at + 32 * u) * kRowBytes;
         f32x16 s = product<T, DP>(kt, rr, q);
         const f32x16 dp = product<T, DP>(kt + kTile, rr, g);
         weights_of<T, true>(a, s, bias[u], st);
-        const uint32_t mine = words.bits(key + 32 * u) >> (16 * h);
+        const uint32_t mine = words.bits(key + keys_at + 32 * u) >> (16 * h);
 #pragma unroll
         for (int r = 0; r < 16; ++r) sum[u][r] += key_bit(mine, r) ? s[r] * (dp[r] - delta) : 0.f;
-        __builtin_amdgcn_sched_barrier(0);  // one part's operands at a time: both spill
+        __builtin_amdgcn_sched_barrier(0);  // one part's operands at a time: all of them spill
       }
     }
   }
   if (i >= m) return;
   T* out = (T*)a.dbias + pb * a.sdb[0] + ph * a.sdb[1] + i * a.sdb[2];
 #pragma unroll
-  for (int u = 0; u < kParts; ++u) store_keys(out, key + 32 * u + 16 * h, a.n, sum[u]);
+  for (int u = 0; u < kParts; ++u) store_keys(out, key + keys_at + 32 * u + 16 * h, a.n, sum[u]);
 }
 
 // out = the splits' parts added in order.
@@ -539,7 +551,7 @@ int launch(CrossArgs& a, hipStream_t stream) {
   const int64_t planes = (a.sdb[0] ? a.batch : 1) * (a.sdb[1] ? a.heads : 1);
   // Shared by batch elements or heads: a kernel of its own; otherwise dK and dV's writes it.
   const bool shared = a.dbias && ((!a.sdb[0] && a.batch > 1) || (!a.sdb[1] && a.heads > 1));
-  constexpr int KT = sizeof(T) == 4 ? 32 : 64;  // cross_attention_dbias's keys
+  constexpr int KT = kBiasKeys<T, DP>;
   const int64_t bias_blocks = planes * ((a.m + 127) / 128) * ((a.n + KT - 1) / KT);
   const int64_t delta_blocks = (a.batch * a.m * a.heads + 15) / 16;
   const int64_t q_quads = a.batch * a.m * a.heads * a.dim / 4, k_quads = a.batch * a.n * a.kv_heads * a.dim / 4;
@@ -571,7 +583,7 @@ int launch(CrossArgs& a, hipStream_t stream) {
     if (kv.splits > 1 && a.dk) sum(kv, 0, k_quads, a.dk);
     if (kv.splits > 1 && a.dv) sum(kv, 1, k_quads, a.dv);
   }
-  if (shared) cross_attention_dbias<T, DP><<<dim3((unsigned)bias_blocks), 256, 0, stream>>>(a);
+  if (shared) cross_attention_dbias<T, DP><<<dim3((unsigned)bias_blocks), 64 * kBiasWaves<T, DP>, 0, stream>>>(a);
   return check_launch("cross_attention_bwd");
 }
 

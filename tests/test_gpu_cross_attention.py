@@ -108,6 +108,7 @@ CASES = [  # batch, m, n, heads, kv_heads, dim, mask, bias (per batch element, p
     (5, 64, 64, 2, 2, 40, "some", (0, 1), torch.bfloat16),
     (1, 17, 8300, 1, 1, 64, "some", None, torch.bfloat16),
     (1, 200, 4161, 2, 1, 64, "tail", None, torch.float32),
+    (2, 140, 300, 4, 2, 128, "empty", (1, 0), torch.bfloat16),
 ]
 
 
