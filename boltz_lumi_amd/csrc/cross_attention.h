@@ -13,11 +13,14 @@
 // bf16 step t, register r is fp32 step r.
 #pragma once
 
+#include <type_traits>
+
 #include "bmx_common.h"
 
 namespace bmx {
 
 constexpr float kLog2E = 1.4426950408889634f;
+constexpr int kFewRows = 32;      // a decoding step's rows of one key head, at most
 constexpr int kMaskChunk = 4096;  // keys whose mask words are in LDS at a time
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -34,6 +37,7 @@ struct CrossArgs {
   void *out, *out_lo;
   float2* stats;  // [batch][heads][m]: row maximum of the logits and log2 of the sum of exp(logit - maximum)
   // work split
+  bool exact;       // bf16: weights of 16 bits instead of 8 in the products over them
   int batch_first;  // a bias shared by the batch: its elements' blocks follow each other, so that it stays in L2
   int row_blocks, splits;
   int split_keys;  // or, of dK and dV, tiles of 32 queries
@@ -155,6 +159,18 @@ struct Weights<bf16> {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[t][e] = (bf16)p[8 * t + e];
   }
+  // p cut off to its upper half, and into rest what that left.
+  __device__ __forceinline__ void cut(const f32x16& p, Weights& rest) {
+    uint32_t word[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      word[i] = __builtin_amdgcn_perm(__float_as_uint(p[2 * i + 1]), __float_as_uint(p[2 * i]), 0x07060302);
+    __builtin_memcpy(v, word, 32);
+    f32x16 left;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) left[r] = p[r] - __uint_as_float(__float_as_uint(p[r]) & 0xffff0000u);
+    rest.set(left);
+  }
   // Sum of the rounded values: what the product over them adds up.
   __device__ __forceinline__ float sum(float acc) const {
     const bf16x2 one = {(bf16)1.f, (bf16)1.f};
@@ -231,6 +247,35 @@ __device__ __forceinline__ void transposed_product(const char* tile, const Colum
       const float a = *(const float*)(tile + Tile<float, DP>::at(16 * h + r, 8 * dt + (i >> 2)) + 4 * (i & 3));
       acc[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, w.v[r], acc[dt], 0, 0, 0);
     }
+}
+
+// transposed_product over the weights p, with kExact to 16 bits (two products); their sum to *sum.
+template <typename T, int DP, bool kExact, bool kKeep>
+__device__ __forceinline__ void weighted_sum(const char* tile, const ColumnReads<T, DP, kKeep>& reads, const f32x16& p,
+                                             f32x16 (&acc)[DP / 32], float* sum = nullptr) {
+  Weights<T> w;
+  if constexpr (kExact) {
+    Weights<T> rest;
+    w.cut(p, rest);
+    if (sum) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) *sum += p[r];
+    }
+    transposed_product<DP>(tile, reads, rest, acc);
+  } else {
+    w.set(p);
+    if (sum) *sum = w.sum(*sum);
+  }
+  transposed_product<DP>(tile, reads, w, acc);
+}
+
+// f(std::bool_constant): kernels with kExact are their own, as a branch in their loops would cost the others 4%.
+template <typename T, typename F>
+void with_exact(const CrossArgs& a, F f) {
+  if constexpr (sizeof(T) == 2) {
+    if (a.exact) return f(std::true_type());
+  }
+  f(std::false_type());
 }
 
 // ---- staging -------------------------------------------------------------

@@ -8,8 +8,8 @@
 // rows: S^T = K Q^T puts a query in a lane, so maximum and sum are one lane's
 // registers plus one exchange between the halves, and the weights in registers are the next product's
 // operand as they stand (out^T += V^T P^T, V read transposed from LDS).  The
-// weights are rounded to the operand's type, and their sum is taken over the rounded values, so a row's
-// weights add up to one: the error is a rounding of each weight against the others.
+// weights are rounded to the operand's type (small calls: to two of them), and their sum is taken over the rounded
+// values, so a row's weights add up to one: the error is a rounding of each weight against the others.
 //
 // A row without keys (masked, or -inf bias throughout) gives zeros.
 #include <algorithm>
@@ -22,7 +22,7 @@ using namespace bmx;
 namespace {
 
 // State of a wave's 32 rows: lane l holds row l % 32, in both halves.
-template <typename T, int DP, bool kBias>
+template <typename T, int DP, bool kBias, bool kExact>
 struct Rows {
   // The weight of a logit x is exp2(x c + shift), shift = -top c: without a bias x is q k^T, with one the logit in natural
   // units. fp32 takes the difference first, exp2((x - top) c): the largest logit's weight is then exactly 1 (bf16
@@ -89,10 +89,7 @@ struct Rows {
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(kFirst ? (s[r] - shift) * c : s[r] * c + shift);
-    Weights<T> w;
-    w.set(s);
-    sum = w.sum(sum);
-    transposed_product<DP>(vt, vr, w, o);
+    weighted_sum<T, DP, kExact>(vt, vr, s, o, &sum);
   }
 };
 
@@ -176,17 +173,19 @@ struct Place {
 };
 
 // Many rows: four waves of 32 rows share tiles of 32 keys in two LDS buffers, copied there by DMA: the next tile's
-// copies are in flight while a tile is attended, one barrier per tile. No staging registers and small tiles leave
-// room for three blocks on a compute unit, so one wave's exponentials run under another's
-// MFMA. Tiles without a present key are passed over.
-template <typename T, int DP, bool kBias>
+// copies are in flight while a tile is attended, one barrier per tile. No staging registers and small tiles leave room
+// for two to four blocks on a compute unit, so one wave's exponentials run under another's MFMA. Tiles without a
+// present key are passed over. Bound: D = 128 by the MFMA (batch 2, 32 / 8 heads, 2048 x 4096: 300 us, 920 TF/s;
+// blocks of two waves, three waves a SIMD, or a wave of its own for the copies took 377 to 440), narrower heads by the
+// exponentials and conversions between the products (D = 64 up to 800 TF/s), with a bias by those and the bias's reads.
+template <typename T, int DP, bool kBias, bool kExact>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : sizeof(T) == 4 || kBias || DP == 128 ? 2 : 3)
 void cross_attention_wide(CrossArgs a) {
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[4 * kTile + kMaskChunk / 8];
   const Place p(a);
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), row = (p.row_block * 4 + w) * 32 + (t & 31);
-  Rows<T, DP, kBias> rows;
+  Rows<T, DP, kBias, kExact> rows;
   rows.init(a, p.b, p.c, row);
   const T* k = (const T*)a.k + p.b * a.sk[0] + p.c * a.sk[2];
   const T* v = (const T*)a.v + p.b * a.sv[0] + p.c * a.sv[2];
@@ -235,16 +234,17 @@ void cross_attention_wide(CrossArgs a) {
   write_rows<T, DP>(a, p.b, p.c, p.split, row, rows.o, rows.top, halves_sum(rows.sum), kBias);
 }
 
-// Up to 32 rows (a decoding step): the four waves take 32 keys in turn, each through a tile of its own without
+// Up to kFewRows rows (a decoding step): the four waves take 32 keys in turn, each through a tile of its own without
 // barriers, so every wave keeps its next 32 keys' loads in flight, and merge their sums at the end. The bound
-// is the read of the keys and values.
+// is the read of the keys and values (batch 32, 32 / 8 heads, 4096 keys of 128 channels, 537 MB: 106 us, 5.1 TB/s).
 template <typename T, int DP, bool kBias>
-__global__ __launch_bounds__(256) void cross_attention_few(CrossArgs a) {
+__global__ __launch_bounds__(256, sizeof(T) == 4 || DP == 128 ? 1 : DP == 96 ? 2 : DP == 64 ? 3 - kBias : 4)
+void cross_attention_few(CrossArgs a) {
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[8 * kTile + kMaskChunk / 8 + 4 * 32 * 4];
   const Place p(a);
   const int t = threadIdx.x, w = t >> 6, l = t & 63, row = l & 31;
-  Rows<T, DP, kBias> rows;
+  Rows<T, DP, kBias, sizeof(T) == 2> rows;
   rows.init(a, p.b, p.c, row);
   const T* k = (const T*)a.k + p.b * a.sk[0] + p.c * a.sk[2];
   const T* v = (const T*)a.v + p.b * a.sv[0] + p.c * a.sv[2];
@@ -368,7 +368,7 @@ struct Split {
 // 30 in two, 4096 keys 77 and 57; fp32's keys cost several times as much: 96 blocks of 1134 keys 63 in two, 50 in five).
 Split plan(int dtype, int64_t batch, int64_t kv_heads, int64_t rows, int64_t n) {
   Split s;
-  s.few = rows <= 32;
+  s.few = rows <= kFewRows;
   s.row_blocks = s.few ? 1 : (int)((rows + 127) / 128);
   const int64_t blocks = (int64_t)s.row_blocks * batch * kv_heads;
   auto fill = [&](int64_t want, int64_t least) { return blocks ? std::min(want / blocks, (n + least - 1) / least) : 1; };
@@ -383,10 +383,13 @@ Split plan(int dtype, int64_t batch, int64_t kv_heads, int64_t rows, int64_t n) 
 template <typename T, int DP, bool kBias>
 void launch(const CrossArgs& a, bool few, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.row_blocks * a.splits * a.kv_heads * a.batch));
-  if (few)
+  if (few) {
     cross_attention_few<T, DP, kBias><<<grid, 256, 0, stream>>>(a);
-  else
-    cross_attention_wide<T, DP, kBias><<<grid, 256, 0, stream>>>(a);
+  } else {
+    with_exact<T>(a, [&](auto exact) {
+      cross_attention_wide<T, DP, kBias, decltype(exact)::value><<<grid, 256, 0, stream>>>(a);
+    });
+  }
 }
 
 template <typename T>
@@ -431,6 +434,13 @@ int cross_setup(CrossArgs& a, int dtype, const int64_t* shape, const int64_t* st
   a.smask = strides[9];
   a.heads = (int)heads, a.kv_heads = (int)kv, a.group = (int)(heads / kv), a.dim = (int)dim, a.rows = (int)rows;
   a.scale = scale;
+  // The weights' rounding moves a result by as much as its own rounding does, and over few keys the output's error does not
+  // average out before the gradients' differences dP - delta meet it. Weights of 16 bits leave the result's rounding alone:
+  // in decoding steps, which are bound by reading the keys (batch 32, 32 / 8 heads, 4096 keys, D = 128: 95.7 us with 8
+  // bits, 96.6 with 16; 16 heads, 2048 keys, D = 64: 45.7 and 47.3, D = 32 with a bias, the worst, 26.6 and 31.8), and
+  // where a call is mostly latency (300 queries, 500 keys, 16 heads, D = 64: forward 15.4 and 16.1 us, dQ, dK and dV 23.5
+  // and 26.5). Large calls would pay for the added products (2048 queries, 256 keys, D = 128: dK and dV 46 and 55).
+  a.exact = dtype == kBF16 && (rows <= kFewRows || a.n <= 256 || (double)a.batch * heads * a.m * a.n * dim <= 1ll << 28);
   a.batch_first = has_bias && a.batch > 1 && a.sb[0] == 0;
   return BMX_OK;
 }

@@ -7,7 +7,7 @@
 // No logits are kept: each kernel recomputes S and dP for its tiles.  Three
 // kernels instead of one, because each sums over another axis and keeps its sum in
 // registers: no atomics, and the same bits on every run.  P and dS are rounded to
-// the operand's type for the products over them; delta is taken from the output before its rounding
+// the operand's type for the products over them (small calls: to two of them); delta is taken from the output before its rounding
 // (out + out_lo), so that dP - delta cancels as it does in the formula.
 #include <type_traits>
 
@@ -116,8 +116,9 @@ __device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, BiasTi
   }
 }
 
-// dQ: four waves of 32 rows over all keys, as the forward pass runs.
-template <typename T, int DP, bool kBias>
+// dQ: four waves of 32 rows over all keys, as the forward pass runs (batch 2, 32 / 8 heads, 2048 x 4096, D = 128: 370 us,
+// 1110 TF/s).
+template <typename T, int DP, bool kBias, bool kExact>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dq(CrossArgs a) {
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[4 * kTile + kMaskChunk / 8];
@@ -186,9 +187,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
         for (int r = 0; r < 16; ++r)
           if (!key_bit(mine, r)) s[r] = 0.f;
       }
-      Weights<T> wt;
-      wt.set(s);
-      transposed_product<DP>(kt, cr, wt, dq);
+      weighted_sum<T, DP, kExact>(kt, cr, s, dq);
       key = after;
       return key < end;
     };
@@ -215,7 +214,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
 // Queries past the last repeat it with weights of zero. A wave's K, and V for narrow heads, are in registers;
 // bf16 heads past 64 channels keep V in LDS, which makes room for two waves on a SIMD.
 // A bias of its own for every head and batch element has its gradient written here, as dS is at hand (kGrad).
-template <typename T, int DP, bool kBias, bool kGrad>
+// Bound by the MFMA (batch 2, 32 / 8 heads, 2048 x 4096, D = 128: 512 us, 1070 TF/s), with a bias by its reads, whose
+// neighbours in a lane are rows apart (batch 5, 16 heads, 1024 x 1531, D = 64: 115 us, 560 TF/s).
+template <typename T, int DP, bool kBias, bool kGrad, bool kExact>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dkv(CrossArgs a) {
   constexpr bool kValuesInLds = sizeof(T) == 2 && DP > 64;
   constexpr bool kFirst = kBias || sizeof(T) == 4;
@@ -340,11 +341,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
         }
       }
       if (kValuesInLds) __builtin_amdgcn_sched_barrier(0);
-      {
-        Weights<T> wt;
-        wt.set(s);
-        transposed_product<DP>(gt, cr, wt, dv);
-      }
+      weighted_sum<T, DP, kExact>(gt, cr, s, dv);
       if (kValuesInLds) __builtin_amdgcn_sched_barrier(0);
       if (kValuesInLds) {
         dp = zero16();
@@ -367,9 +364,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
           if (r < left) dbias[r * a.sdb[2]] = live ? (T)s[r] : (T)0.f;
       }
       if (kValuesInLds) __builtin_amdgcn_sched_barrier(0);
-      Weights<T> wt;
-      wt.set(s);
-      transposed_product<DP>(qt, cr, wt, dk);
+      weighted_sum<T, DP, kExact>(qt, cr, s, dk);
       return more;
     };
     copy(g, i, lds0);
@@ -567,19 +562,25 @@ int launch(CrossArgs& a, hipStream_t stream) {
   if (a.dq) {
     a.splits = q.splits, a.split_keys = q.size;
     const dim3 grid((unsigned)(lists * a.row_blocks * q.splits));
-    a.bias ? cross_attention_dq<T, DP, true><<<grid, 256, 0, stream>>>(a)
-           : cross_attention_dq<T, DP, false><<<grid, 256, 0, stream>>>(a);
+    with_exact<T>(a, [&](auto exact) {
+      constexpr bool kExact = decltype(exact)::value;
+      a.bias ? cross_attention_dq<T, DP, true, kExact><<<grid, 256, 0, stream>>>(a)
+             : cross_attention_dq<T, DP, false, kExact><<<grid, 256, 0, stream>>>(a);
+    });
     if (q.splits > 1) sum(q, 0, q_quads, a.dq);
   }
   if (a.dk || a.dv || (a.dbias && !shared)) {
     a.splits = kv.splits, a.split_keys = kv.size;
     const dim3 grid((unsigned)(lists * key_blocks * kv.splits));
-    if (a.dbias && !shared)
-      cross_attention_dkv<T, DP, true, true><<<grid, 256, 0, stream>>>(a);
-    else if (a.bias)
-      cross_attention_dkv<T, DP, true, false><<<grid, 256, 0, stream>>>(a);
-    else
-      cross_attention_dkv<T, DP, false, false><<<grid, 256, 0, stream>>>(a);
+    with_exact<T>(a, [&](auto exact) {
+      constexpr bool kExact = decltype(exact)::value;
+      if (a.dbias && !shared)
+        cross_attention_dkv<T, DP, true, true, kExact><<<grid, 256, 0, stream>>>(a);
+      else if (a.bias)
+        cross_attention_dkv<T, DP, true, false, kExact><<<grid, 256, 0, stream>>>(a);
+      else
+        cross_attention_dkv<T, DP, false, false, kExact><<<grid, 256, 0, stream>>>(a);
+    });
     if (kv.splits > 1 && a.dk) sum(kv, 0, k_quads, a.dk);
     if (kv.splits > 1 && a.dv) sum(kv, 1, k_quads, a.dv);
   }

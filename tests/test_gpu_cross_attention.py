@@ -6,7 +6,9 @@ relative error is that of its logits plus the exponential's 2 u and the change o
 range), sums over N keys add at most N / 8 in a chain: with these inputs under 2^-14 of the sum of magnitudes.
 bf16: weights (and their gradients) are rounded once before the product over them, half a
 step (2^-8) of each, and the result once more; the output and dV, dQ, dK are compared with 2^-8 of the sum
-of the magnitudes of their terms plus 2^-8 of themselves, on top of the fp32 part."""
+of the magnitudes of their terms plus 2^-8 of themselves, on top of the fp32 part. Up to 256 keys, and in small calls,
+weights have 16 bits: what that leaves, 2^-16 of each, is inside the fp32 part's 2^-14 (whose own share with
+D = 128 and logits of a few units stays below 2^-15)."""
 
 import math
 
@@ -64,10 +66,11 @@ def formula(q, k, v, mask, bias, scale, dout=None):
     return back, dq, dk, dv, dbias
 
 
-def check(got, want, size, what):
+def check(got, want, size, what, weights=True):
+    """weights: bf16 weights are rounded to its 8 bits."""
     assert got.shape == want.shape, what
     step = half_step(got.dtype)
-    near = 2.0 ** -14 if got.dtype == torch.float32 else 2.0 ** -14 + step
+    near = 2.0 ** -14 + (step if weights and got.dtype == torch.bfloat16 else 0)
     err = (got.double() - want).abs() - near * size - step * want.abs()
     assert bool((err <= 1e-30).all()), f"{what}: {err.max().item()} past the bound"
 
@@ -144,6 +147,27 @@ def test_one_key_has_no_logit_gradient(gpu):
         size = (dout.double().abs() * v.detach().double().abs()).sum(-1, keepdim=True) * 64 * U
         assert bool((dq.double().abs() <= size * k.detach().double().abs() + 1e-30).all())
         assert bool((dk.double().abs() <= (size * q.detach().double().abs()).sum(1, keepdim=True) + 1e-30).all())
+
+
+@pytest.mark.parametrize("case", [  # few keys; then small calls over many
+    (2, 300, 2, 4, 2, 48, None, (0, 1), torch.bfloat16),
+    (5, 30, 23, 2, 2, 32, "some", (1, 1), torch.bfloat16),
+    (1, 200, 256, 2, 1, 128, "tail", None, torch.bfloat16),
+    (2, 1, 97, 4, 1, 96, None, None, torch.bfloat16),
+    (1, 40, 900, 2, 2, 64, "some", None, torch.bfloat16),
+    (1, 5, 2500, 2, 1, 24, None, (1, 0), torch.bfloat16),
+])
+def test_small_calls_round_the_result_alone(gpu, case):
+    q, k, v, mask, bias, g = inputs(case, gpu)
+    scale = case[5] ** -0.5
+    leaves = [t.requires_grad_() for t in (q, k, v, bias) if t is not None]
+    out = ops.cross_attention(q, k, v, mask, bias, scale)
+    dout = randn(g, *out.shape, dtype=out.dtype)
+    grads = torch.autograd.grad(out, leaves, dout)
+    with torch.no_grad():
+        want = formula(q, k, v, mask, bias, scale, dout)
+    for name, have, (ref, size) in zip(("out", "dq", "dk", "dv", "dbias"), (out.detach(), *grads), want):
+        check(have, ref, size, name, weights=False)
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
