@@ -101,9 +101,8 @@ __device__ __forceinline__ void store_keys(T* row, int key, int n, const f32x16&
 
 // P of a logits tile whose column is a query: maximum and log2 of the sum are the lane's.
 template <typename T, bool kBias>
-__device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, BiasTile<T>& b, float2 st) {
+__device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, const BiasTile<T>& b, float2 st) {
   if (kBias) {
-    b.ready(true);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + b.at(r) - st.x) * kLog2E - st.y);
   } else if (sizeof(T) == 4) {  // as the forward pass: the difference first
@@ -178,6 +177,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
       }
       f32x16 s = product<T, DP>(kt, rr, q);
       const f32x16 dp = product<T, DP>(vt, rr, g);
+      if (kBias) bias[decltype(B)::value].ready(true);
       weights_of<T, kBias>(a, s, bias[decltype(B)::value], st);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
@@ -393,11 +393,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
 }
 
 // dbias of a bias that batch elements or heads share: a block holds 128 queries x kBiasKeys keys of one bias plane in
-// registers and walks the batch elements and heads that share the plane, in order. bf16 has all four operands in LDS
-// by DMA. Up to 64 channels four waves and 64 keys take 48 KB, so that other blocks of the compute unit run under
-// one's copies (batch 5, 16 heads, 1024 x 1531, D = 64: 127 us; eight waves and 128 keys 155, four and 128 spill: 250).
+// registers and walks the batch elements and heads that share the plane, in order. A step is short, so what bounds it is
+// the chain of its loads: the next step's operands are copied while one is computed, its mask an element earlier, and
+// the bias is loaded once if it is the same in all steps (batch 5, 16 heads, 1024 x 1531, D = 64: 127 -> 102 us).
+// bf16 has all four operands in LDS by DMA. Up to 64 channels four waves and 64 keys take 64 KB, K and V in two buffers:
+// two blocks on a compute unit (before the copies ran ahead: eight waves and 128 keys 155 us, four and 128 spill: 250).
 // Past 64 channels eight waves, four by the queries and two by the keys, and 128 keys take 128 KB (batch 2, 16 heads,
-// 1024 x 2048, D = 128: 125 us; four waves and 64 keys with the queries read into registers 154). fp32: four waves
+// 1024 x 2048, D = 128: 105 us; four waves and 64 keys with the queries read into registers 154). fp32: four waves
 // and 32 keys, the queries' operands read straight into registers.
 template <typename T, int DP>
 constexpr int kBiasWaves = sizeof(T) == 2 && DP > 64 ? 8 : 4;
@@ -411,8 +413,9 @@ void cross_attention_dbias(CrossArgs a) {
   constexpr int kWaves = kBiasWaves<T, DP>, kThreads = 64 * kWaves, KT = kBiasKeys<T, DP>;
   constexpr int kParts = KT / 32 / (kWaves / 4);  // of 32 keys, of a wave
   constexpr int kRowBytes = Tile<T, DP>::kRowBytes, kTile = KT * kRowBytes, kRowTile = kRowsInLds ? 128 * kRowBytes : 0;
-  constexpr int kWords = 2 * kTile + 2 * kRowTile;
-  __shared__ __attribute__((aligned(16))) char lds[kWords + 16];
+  constexpr bool kDouble = !kRowsInLds || DP <= 64;  // K and V in two buffers
+  constexpr int kKeyTiles = kDouble ? 4 * kTile : 2 * kTile, kAll = kKeyTiles + 2 * kRowTile, kMasks = (KT + 63) / 64;
+  __shared__ __attribute__((aligned(16))) char lds[kAll];
   const int key_blocks = (a.n + KT - 1) / KT, query_blocks = (int)((a.m + 127) / 128);
   uint32_t at = xcd_position(blockIdx.x, gridDim.x);
   const int key = take(at, key_blocks) * KT, q0 = take(at, query_blocks) * 128;
@@ -425,7 +428,6 @@ void cross_attention_dbias(CrossArgs a) {
   f32x16 sum[kParts];
 #pragma unroll
   for (int u = 0; u < kParts; ++u) sum[u] = zero16();
-  KeyWords words{(uint32_t*)(lds + kWords), nullptr};
   RowReads<T, DP> rr;
   rr.init(a.dim);
   const int64_t row_step = (int64_t)a.heads * a.dim;
@@ -438,57 +440,107 @@ void cross_attention_dbias(CrossArgs a) {
     cg.init(w, a.dim, row_step);
   }
   const unsigned lds0 = lds_address(lds);
-  clear_tiles<T, DP, kThreads>(t, lds, kWords, a.dim);
-  for (int64_t b = b0; b < b1; ++b) {
-    words.mask = a.mask ? a.mask + b * a.smask : nullptr;
-    words.fill(key, min(key + KT, a.n));
-    uint32_t any = 0;
+  clear_tiles<T, DP, kThreads>(t, lds, kAll, a.dim);
+
+  // Presence of the keys in a batch element, whose mask is loaded an element ahead.
+  uint8_t ahead[kMasks];
+  uint64_t bits[kMasks];
+  auto load_mask = [&](int64_t b) {
 #pragma unroll
-    for (int u = 0; u < KT / 32; ++u) any |= words.bits(key + 32 * u);
-    if (any == 0) continue;
-    for (int head = h0; head < h1; ++head) {
-      const int c = head / a.group;
-      __syncthreads();  // every wave is done with the last step's tiles
-      ck.issue(w, (const T*)a.k + b * a.sk[0] + c * a.sk[2] + key * a.sk[1], a.n - key, a.dim, a.sk[1], lds0);
-      cv.issue(w, (const T*)a.v + b * a.sv[0] + c * a.sv[2] + key * a.sv[1], a.n - key, a.dim, a.sv[1], lds0 + kTile);
-      RowOperand<T, DP> q, g;
-      const T* q_row = (const T*)a.q + b * a.sq[0] + head * a.sq[2];
-      const T* g_row = (const T*)a.dout + (b * a.m * a.heads + head) * a.dim;
-      if (kRowsInLds) {
-        cq.issue(w, q_row + q0 * a.sq[1], m - q0, a.dim, a.sq[1], lds0 + 2 * kTile);
-        cg.issue(w, g_row + q0 * row_step, m - q0, a.dim, row_step, lds0 + 2 * kTile + kRowTile);
-      } else {
-        q.load(q_row + safe * a.sq[1], a.dim, h);
-        g.load(g_row + safe * row_step, a.dim, h);
+    for (int u = 0; u < kMasks; ++u)
+      ahead[u] = a.mask ? a.mask[min(b, b1 - 1) * a.smask + min(key + 64 * u + l, a.n - 1)] : 1;
+  };
+  auto find = [&](int64_t b) {  // the first element from b on (whose mask is in `ahead`) with a present key
+    for (; b < b1; ++b) {
+      uint64_t any = 0;
+#pragma unroll
+      for (int u = 0; u < kMasks; ++u) {
+        const int k = 64 * u + l;
+        any |= bits[u] = __ballot(ahead[u] != 0 && k < KT && key + k < a.n);
       }
-      const int64_t stat = (b * a.heads + head) * a.m + safe;
-      const float2 st = a.stats[stat];
-      const float delta = a.delta[stat];
-      const T* bias_row = (const T*)a.bias + b * a.sb[0] + head * a.sb[1] + safe * a.sb[2];
-      BiasTile<T> bias[kParts];
-#pragma unroll
-      for (int u = 0; u < kParts; ++u) bias[u].load(bias_row, min(key + keys_at + 32 * u, a.n - 1), a.n);
-      wait_copies();
-      __syncthreads();
-      if (kRowsInLds) {
-#pragma unroll
-        for (int s = 0; s < RowOperand<T, DP>::kSteps; ++s) {
-          q.c[s] = *(const u32x4*)(lds + 2 * kTile + rows_at * kRowBytes + rr.at(s));
-          g.c[s] = *(const u32x4*)(lds + 2 * kTile + kRowTile + rows_at * kRowBytes + rr.at(s));
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < kParts; ++u) {
-        const char* kt = lds + (keys_at + 32 * u) * kRowBytes;
-        f32x16 s = product<T, DP>(kt, rr, q);
-        const f32x16 dp = product<T, DP>(kt + kTile, rr, g);
-        weights_of<T, true>(a, s, bias[u], st);
-        const uint32_t mine = words.bits(key + keys_at + 32 * u) >> (16 * h);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sum[u][r] += key_bit(mine, r) ? s[r] * (dp[r] - delta) : 0.f;
-        __builtin_amdgcn_sched_barrier(0);  // one part's operands at a time: all of them spill
-      }
+      load_mask(b + 1);
+      if (any) break;
     }
+    return b;
+  };
+  // A step's operands: one batch element and head. The next step's are on their way while a step is computed.
+  float2 next_st;
+  float next_delta;
+  BiasTile<T> bias[kParts];
+  auto issue_keys = [&](int64_t b, int head, unsigned tile) {
+    const int c = head / a.group;
+    ck.issue(w, (const T*)a.k + b * a.sk[0] + c * a.sk[2] + key * a.sk[1], a.n - key, a.dim, a.sk[1], tile);
+    cv.issue(w, (const T*)a.v + b * a.sv[0] + c * a.sv[2] + key * a.sv[1], a.n - key, a.dim, a.sv[1], tile + kTile);
+  };
+  auto issue_rows = [&](int64_t b, int head) {
+    const int64_t stat = (b * a.heads + head) * a.m + safe;
+    next_st = a.stats[stat], next_delta = a.delta[stat];
+    if (!kRowsInLds) return;
+    cq.issue(w, (const T*)a.q + b * a.sq[0] + head * a.sq[2] + q0 * a.sq[1], m - q0, a.dim, a.sq[1], lds0 + kKeyTiles);
+    cg.issue(w, (const T*)a.dout + (b * a.m * a.heads + head) * a.dim + q0 * row_step, m - q0, a.dim, row_step,
+             lds0 + kKeyTiles + kRowTile);
+  };
+  auto load_bias = [&](int64_t b, int head) {
+    const T* row = (const T*)a.bias + b * a.sb[0] + head * a.sb[1] + safe * a.sb[2];
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) {
+      bias[u].load(row, min(key + keys_at + 32 * u, a.n - 1), a.n);
+      bias[u].ready(true);
+    }
+  };
+  load_mask(b0);
+  int64_t b = find(b0);
+  int head = h0, buf = 0;
+  if (b < b1) {
+    load_bias(b, head);
+    issue_rows(b, head);
+    issue_keys(b, head, lds0);
+  }
+  while (b < b1) {
+    uint64_t mine[kMasks];
+#pragma unroll
+    for (int u = 0; u < kMasks; ++u) mine[u] = bits[u];
+    wait_copies();
+    __syncthreads();
+    const float2 st = next_st;
+    const float delta = next_delta;
+    RowOperand<T, DP> q, g;
+    if (kRowsInLds) {
+#pragma unroll
+      for (int s = 0; s < RowOperand<T, DP>::kSteps; ++s) {
+        q.c[s] = *(const u32x4*)(lds + kKeyTiles + rows_at * kRowBytes + rr.at(s));
+        g.c[s] = *(const u32x4*)(lds + kKeyTiles + kRowTile + rows_at * kRowBytes + rr.at(s));
+      }
+      __syncthreads();  // every wave has its rows: the next step's may come
+    } else {
+      q.load((const T*)a.q + b * a.sq[0] + head * a.sq[2] + safe * a.sq[1], a.dim, h);
+      g.load((const T*)a.dout + (b * a.m * a.heads + head) * a.dim + safe * row_step, a.dim, h);
+    }
+    const int64_t this_b = b;
+    if (++head == h1) head = h0, b = find(b + 1);
+    if (b < b1) {
+      issue_rows(b, head);
+      if (kDouble) issue_keys(b, head, lds0 + (buf ^ 1) * 2 * kTile);
+    }
+#pragma unroll
+    for (int u = 0; u < kParts; ++u) {
+      const char* kt = lds + buf * 2 * kTile + (keys_at + 32 * u) * kRowBytes;
+      f32x16 s = product<T, DP>(kt, rr, q);
+      const f32x16 dp = product<T, DP>(kt + kTile, rr, g);
+      weights_of<T, true>(a, s, bias[u], st);
+      const uint32_t keys = (uint32_t)(mine[(keys_at + 32 * u) / 64] >> ((keys_at + 32 * u) % 64)) >> (16 * h);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum[u][r] += key_bit(keys, r) ? s[r] * (dp[r] - delta) : 0.f;
+      __builtin_amdgcn_sched_barrier(0);  // one part's operands at a time: all of them spill
+    }
+    if (b >= b1) break;
+    if (kDouble) {
+      buf ^= 1;
+    } else {
+      __syncthreads();  // every wave is done with the keys
+      issue_keys(b, head, lds0);
+    }
+    if ((a.sb[0] != 0 && b != this_b) || (a.sb[1] != 0 && h1 - h0 > 1)) load_bias(b, head);
   }
   if (i >= m) return;
   T* out = (T*)a.dbias + pb * a.sdb[0] + ph * a.sdb[1] + i * a.sdb[2];
