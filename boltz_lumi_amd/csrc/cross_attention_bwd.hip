@@ -214,8 +214,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
 // Queries past the last repeat it with weights of zero. A wave's K, and V for narrow heads, are in registers;
 // bf16 heads past 64 channels keep V in LDS, which makes room for two waves on a SIMD.
 // A bias of its own for every head and batch element has its gradient written here, as dS is at hand (kGrad).
-// Bound by the MFMA (batch 2, 32 / 8 heads, 2048 x 4096, D = 128: 512 us, 1070 TF/s), with a bias by its reads, whose
-// neighbours in a lane are rows apart (batch 5, 16 heads, 1024 x 1531, D = 64: 115 us, 560 TF/s).
+// Bound by the MFMA (batch 2, 32 / 8 heads, 2048 x 4096, D = 128: 512 us, 1070 TF/s), with a bias by
+// the work between the products at two waves a SIMD (batch 5, 16 heads, 1024 x 1531, D = 64: 116 us, 550 TF/s; its 16
+// two-byte loads a lane are not it: whole runs of keys turned through LDS took 124).
 template <typename T, int DP, bool kBias, bool kGrad, bool kExact>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dkv(CrossArgs a) {
   constexpr bool kValuesInLds = sizeof(T) == 2 && DP > 64;
