@@ -9,6 +9,7 @@
 // registers: no atomics, and the same bits on every run.  P and dS are rounded to
 // the operand's type for the products over them (small calls: to two of them); delta is taken from the output before its rounding
 // (out + out_lo), so that dP - delta cancels as it does in the formula.
+#include <algorithm>
 #include <type_traits>
 
 #include "cross_attention.h"
@@ -563,28 +564,41 @@ struct Split {
   int splits, size;
 };
 
-// Splits of `units` (keys, or query tiles) for `blocks` blocks: so many that every SIMD gets two waves (two blocks a compute unit),
-// each of at least `least` units, since the parts are written and read once more in fp32.
-Split plan(int64_t blocks, int64_t units, int64_t least, int64_t round) {
-  int64_t splits = 512 / blocks;
-  const int64_t most = units / least;
-  splits = splits > most ? most : splits;
-  if (splits < 1) splits = 1;
-  const int64_t size = ((units + splits - 1) / splits + round - 1) / round * round;
-  return {(int)((units + size - 1) / size), (int)size};
+// Splits of a block's `units` (keys, or query tiles) by what they cost: rounds of blocks over the 256 compute units, where
+// a lone block (one wave a SIMD) takes 1.4 times its share of a pair's time, against writing and adding the parts.
+// whole: us of an unsplit block; part_bytes: of one split's parts. fp32, D = 48, 96 blocks of dQ over 1134 keys: 3 splits
+// 74 us, 5 splits 53; D = 128, 32 blocks of dK and dV: 107 and 69; bf16, D = 64, 16 blocks of dK and dV: 37 and 30.
+Split plan(int64_t blocks, int64_t units, int64_t least, int64_t round, double whole, double part_bytes) {
+  Split best = {1, (int)std::max<int64_t>(units, 1)};
+  double best_us = 0;
+  for (int64_t want = 1; want == 1 || (want <= 512 / blocks + 3 && want * least <= units); ++want) {
+    const int64_t size = std::max<int64_t>((units + want - 1) / want + round - 1, round) / round * round;
+    const int64_t splits = std::max<int64_t>((units + size - 1) / size, 1), all = blocks * splits;
+    const double rounds = all <= 256 ? 1.4 : (double)((all + 255) / 256);
+    const double us = rounds * whole * std::min<double>(size, units) / (double)std::max<int64_t>(units, 1) +
+                      (splits > 1 ? 4 + 2 * part_bytes * splits / 3e6 : 0);
+    if (want == 1 || us < best_us) best = {(int)splits, (int)size}, best_us = us;
+  }
+  return best;
 }
-Split plan_dq(int64_t batch, int64_t kv_heads, int64_t rows, int64_t n) {
-  return plan((rows + 127) / 128 * batch * kv_heads, n, 256, 128);
+// A block's products over `flops` at what a compute unit reaches (fp32 110 TF/s of the whole card, bf16 700).
+double block_us(int dtype, double flops) { return flops / (dtype == kF32 ? 110e6 : 700e6) * 256; }
+Split plan_dq(int dtype, int64_t batch, int64_t kv_heads, int64_t rows, int64_t n, int64_t dim) {
+  return plan((rows + 127) / 128 * batch * kv_heads, n, 128, 32, block_us(dtype, 6. * 128 * n * dim),
+              4. * batch * kv_heads * rows * dim);
 }
-Split plan_dkv(int64_t batch, int64_t kv_heads, int64_t group, int64_t m, int64_t n) {
-  return plan((n + 127) / 128 * batch * kv_heads, group * ((m + 31) / 32), 4, 1);
+Split plan_dkv(int dtype, int64_t batch, int64_t kv_heads, int64_t group, int64_t m, int64_t n, int64_t dim) {
+  const int64_t tiles = group * ((m + 31) / 32);
+  return plan((n + 127) / 128 * batch * kv_heads, tiles, 3, 1, block_us(dtype, 8. * 128 * 32 * tiles * dim),
+              8. * batch * kv_heads * n * dim);
 }
 
 // Floats of the workspace: delta, then the parts of dQ or of dK and dV, whichever is more.
-int64_t workspace_floats(int64_t batch, int64_t m, int64_t n, int64_t heads, int64_t kv_heads, int64_t dim,
+int64_t workspace_floats(int dtype, int64_t batch, int64_t m, int64_t n, int64_t heads, int64_t kv_heads, int64_t dim,
                          int64_t* parts) {
   const int64_t group = heads / kv_heads, delta = (batch * m * heads + 3) / 4 * 4;
-  const Split q = plan_dq(batch, kv_heads, group * m, n), kv = plan_dkv(batch, kv_heads, group, m, n);
+  const Split q = plan_dq(dtype, batch, kv_heads, group * m, n, dim);
+  const Split kv = plan_dkv(dtype, batch, kv_heads, group, m, n, dim);
   const int64_t pq = q.splits > 1 ? q.splits * batch * m * heads * dim : 0;
   const int64_t pkv = kv.splits > 1 ? 2 * kv.splits * batch * n * kv_heads * dim : 0;
   if (parts) *parts = delta;
@@ -595,7 +609,9 @@ template <typename T, int DP>
 int launch(CrossArgs& a, hipStream_t stream) {
   const int64_t lists = a.batch * a.kv_heads, key_blocks = (a.n + 127) / 128;
   a.row_blocks = (a.rows + 127) / 128;
-  const Split q = plan_dq(a.batch, a.kv_heads, a.rows, a.n), kv = plan_dkv(a.batch, a.kv_heads, a.group, a.m, a.n);
+  constexpr int dtype = sizeof(T) == 4 ? kF32 : kBF16;
+  const Split q = plan_dq(dtype, a.batch, a.kv_heads, a.rows, a.n, a.dim);
+  const Split kv = plan_dkv(dtype, a.batch, a.kv_heads, a.group, a.m, a.n, a.dim);
   const int64_t planes = (a.sdb[0] ? a.batch : 1) * (a.sdb[1] ? a.heads : 1);
   // Shared by batch elements or heads: a kernel of its own; otherwise dK and dV's writes it.
   const bool shared = a.dbias && ((!a.sdb[0] && a.batch > 1) || (!a.sdb[1] && a.heads > 1));
@@ -653,7 +669,9 @@ int launch_dim(CrossArgs& a, hipStream_t stream) {
 extern "C" size_t bmx_cross_attention_bwd_workspace_bytes(int64_t batch, int64_t m, int64_t n, int64_t heads,
                                                           int64_t kv_heads, int64_t dim) {
   if (batch < 1 || m < 1 || n < 1 || heads < 1 || kv_heads < 1 || dim < 1) return 0;
-  return (size_t)workspace_floats(batch, m, n, heads, kv_heads, dim, nullptr) * sizeof(float);
+  return (size_t)std::max(workspace_floats(kF32, batch, m, n, heads, kv_heads, dim, nullptr),
+                          workspace_floats(kBF16, batch, m, n, heads, kv_heads, dim, nullptr)) *
+         sizeof(float);
 }
 
 extern "C" int bmx_cross_attention_bwd(const void* q, const void* k, const void* v, const void* mask, const void* bias,
@@ -677,7 +695,7 @@ extern "C" int bmx_cross_attention_bwd(const void* q, const void* k, const void*
   a.q = q, a.k = k, a.v = v, a.mask = (const uint8_t*)mask, a.bias = bias;
   a.out = (void*)out, a.out_lo = dtype == kBF16 ? (void*)out_lo : nullptr, a.stats = (float2*)stats, a.dout = dout;
   int64_t parts = 0;
-  workspace_floats(a.batch, a.m, a.n, a.heads, a.kv_heads, a.dim, &parts);
+  workspace_floats(dtype, a.batch, a.m, a.n, a.heads, a.kv_heads, a.dim, &parts);
   a.part_o = (float*)workspace + parts;
   a.delta = (float*)workspace, a.dq = dq, a.dk = dk, a.dv = dv, a.dbias = dbias;
   for (int i = 0; i < 3; ++i) a.sdb[i] = dbias ? dbias_strides[i] : 0;
