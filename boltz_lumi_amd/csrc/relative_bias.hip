@@ -60,7 +60,7 @@ typedef uint32_t u32x4_u __attribute__((ext_vector_type(4), aligned(2)));
 
 // A thread holds the buckets of 16 bytes' worth of consecutive keys of one query row
 // and writes them for `per` heads from the table in LDS: the positions are looked at once,
-// a store is 16 bytes, and the floor is the write of the result.
+// a store is 16 bytes, and the floor is the write of the result (16 heads, 2048 x 2048, fp32, 268 MB: 46 us, 5.8 TB/s).
 template <typename U>  // the element's bits: uint32_t (fp32) or uint16_t (bf16); values are copied, not rounded
 __global__ __launch_bounds__(256) void relative_bias_kernel(Relative s, const U* table, int64_t batch, int per, U* out) {
   constexpr int V = 16 / sizeof(U);
@@ -107,7 +107,9 @@ __global__ __launch_bounds__(256) void relative_bias_kernel(Relative s, const U*
 // threshold on one side of the row's position, which is most of a plane of running positions, the row is added
 // to one sum in registers. Otherwise every thread adds to its own bin per bucket in LDS (bins[bucket][thread],
 // consecutive threads in consecutive banks). Nothing is shared, so there is no atomic and the order of every
-// sum is fixed. A distance's bucket comes from a byte table where the last threshold is below kLut.
+// sum is fixed. A distance's bucket comes from a byte table where the last threshold is below kLut. The bound is the
+// read of dbias (16 heads, 2048 x 2048, fp32, 268 MB: 72 us, 3.7 TB/s, as a plain sum over it; right behind the forward
+// pass, whose result is then still on its way to HBM, 105; LDS atomics instead of own bins 350).
 constexpr int kLut = 2048, kAhead = 4;
 
 __device__ __forceinline__ int64_t wave_extreme(int64_t v, bool largest) {

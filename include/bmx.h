@@ -449,10 +449,11 @@ int bmx_relative_bias_bwd(const void* dbias, int dtype, int64_t buckets, int64_t
 /* out = softmax(scale q k^T + bias over the present keys) v for q [batch, m, heads, dim] and k, v
  * [batch, n, kv_heads, dim], query head h on key head h / (heads / kv_heads); shape = {batch, m, n, heads,
  * kv_heads, dim}, dim a multiple of 8 in [8, 128].  strides: batch, token, head of q, of k and of v (multiples
- * of 16 bytes, the last axis dense), the mask's batch stride (0: shared), the bias's batch, head and
- * query strides (any; 0: shared; keys dense).  mask: bytes [n] per batch element, 0 = the key (whatever its
- * values) is left out, or NULL; bias in dtype or NULL.  A row without keys gives zeros.  out dense [batch, m,
- * heads, dim].  For the backward pass, or NULL: out_lo (bf16 only, out's shape: what rounding out left),
+ * of 16 bytes, the last axis dense; a token's in [0, 2^22), as heads * dim), the mask's batch stride (0: shared), the bias's batch, head and
+ * query strides (any, the query's in [0, 2^26); 0: shared; keys dense).  mask: bytes [n] per batch element, 0 = the key (whatever its
+ * values) is left out, or NULL; bias in dtype or NULL.  A row without keys gives zeros.  batch, m or n may be 0.
+ * out dense [batch, m, heads, dim].  scale positive.  bf16 weights have 16 bits in decoding steps (at most 32 rows
+ * m * heads / kv_heads), up to 256 keys and in small calls (batch * heads * m * n * dim <= 2^28), otherwise 8.  For the backward pass, or NULL: out_lo (bf16 only, out's shape: what rounding out left),
  * stats fp32 [batch, heads, m, 2] (row maximum of the logits, log2 of the sum of exp(logit - maximum)).
  * workspace: bmx_cross_attention_workspace_bytes, 16-byte aligned.  No reference kernel. */
 size_t bmx_cross_attention_workspace_bytes(int dtype, int64_t batch, int64_t m, int64_t n, int64_t heads,
