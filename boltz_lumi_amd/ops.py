@@ -1521,8 +1521,9 @@ def cross_attention(q, k, v, mask=None, bias=None, scale=None):
     query without keys gives zeros, and zero gradients.  scale: positive,
     1 / sqrt(D) by default.  Sums are fp32; bf16 weights enter the products with
     16 bits in decoding steps (M H / Hk <= 32) and small calls, else with 8, so
-    a large call's error is about 1.4 times that of rounding its result.  Gradients reach q, k, v and bias (summed over its
-    shared axes in fp32) and are the same bits on every run."""
+    a large call's error is about 1.4 times that of rounding its result.
+    Gradients reach q, k, v and bias (summed over its shared axes in fp32) and
+    are the same bits on every run."""
     dev = _same_device(q, k, v, mask, bias)
     plan = _cross_plan(_layout(q), _layout(k), _layout(v), _layout(mask), _layout(bias))
     scale = plan.scale if scale is None else float(scale)
