@@ -334,16 +334,36 @@ __global__ __launch_bounds__(256) void cross_attention_join(CrossArgs a, int bia
   if (at >= lists * a.rows) return;
   const int d = (int)(id - at * quads) * 4;
   const int64_t step = lists * a.rows;
+  // Loads go out kAhead splits at a time (those past the last repeat it, unused): one after another, 32
+  // splits of a few rows took longer than the attention itself.
+  constexpr int kAhead = 8;
   float top = -INFINITY;
-  for (int s = 0; s < a.splits; ++s) top = fmaxf(top, a.part_ml[s * step + at].x);
+  for (int s0 = 0; s0 < a.splits; s0 += kAhead) {
+    float x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) x[u] = a.part_ml[min(s0 + u, a.splits - 1) * step + at].x;
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) top = fmaxf(top, x[u]);
+  }
   const float c = (bias ? 1.f : a.scale) * kLog2E, base = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 ml = a.part_ml[s * step + at];
-    const float f = __builtin_amdgcn_exp2f((ml.x - base) * c);
-    sum += ml.y * f;
-    o += *(const f32x4*)(a.part_o + (s * step + at) * a.dim + d) * f;
+  for (int s0 = 0; s0 < a.splits; s0 += kAhead) {
+    float2 ml[kAhead];
+    f32x4 part[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t i = min(s0 + u, a.splits - 1) * step + at;
+      ml[u] = a.part_ml[i];
+      part[u] = *(const f32x4*)(a.part_o + i * a.dim + d);
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (s0 + u >= a.splits) break;
+      const float f = __builtin_amdgcn_exp2f((ml[u].x - base) * c);
+      sum += ml[u].y * f;
+      o += part[u] * f;
+    }
   }
   const int64_t list = at / a.rows, b = list / a.kv_heads;
   const int row = (int)(at - list * a.rows), g = row / (int)a.m, i = row - g * (int)a.m;
@@ -362,7 +382,9 @@ struct Split {
   int keys;  // per split, a multiple of 128
 };
 
-// Few rows run as many splits as give every compute unit two blocks, each of at least 128 keys (one tile a wave).
+// Few rows run as many splits as give every compute unit a block, each of at least 128 keys (one tile a wave), past 16
+// splits 512, since a short split costs less than joining another (one query, 32 / 8 heads, D = 128, 4096 keys: 32 splits
+// 23.8 us, 16 splits 18.6; batch 8: two blocks a compute unit 36 us, one 30).
 // Many rows split where their blocks leave compute units idle, or, for a second wave on every SIMD, where the keys
 // are many enough to pay for writing and joining the parts (bf16, 256 blocks, D = 64: 1024 keys 26 us whole and
 // 30 in two, 4096 keys 77 and 57; fp32's keys cost several times as much: 96 blocks of 1134 keys 63 in two, 50 in five).
@@ -372,7 +394,8 @@ Split plan(int dtype, int64_t batch, int64_t kv_heads, int64_t rows, int64_t n) 
   s.row_blocks = s.few ? 1 : (int)((rows + 127) / 128);
   const int64_t blocks = (int64_t)s.row_blocks * batch * kv_heads;
   auto fill = [&](int64_t want, int64_t least) { return blocks ? std::min(want / blocks, (n + least - 1) / least) : 1; };
-  int64_t splits = s.few ? fill(512, 128) : dtype == kF32 ? fill(512, 256) : std::max(fill(256, 256), fill(512, 1024));
+  int64_t splits = s.few ? std::min<int64_t>(fill(256, 128), std::max<int64_t>(16, fill(256, 512)))
+                   : dtype == kF32 ? fill(512, 256) : std::max(fill(256, 256), fill(512, 1024));
   if (splits < 1) splits = 1;
   s.keys = (int)(((n + splits - 1) / splits + 127) / 128 * 128);
   if (s.keys == 0) s.keys = 128;
