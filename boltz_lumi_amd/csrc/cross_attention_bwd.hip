@@ -550,13 +550,25 @@ void cross_attention_dbias(CrossArgs a) {
   for (int u = 0; u < kParts; ++u) store_keys(out, key + keys_at + 32 * u + 16 * h, a.n, sum[u]);
 }
 
-// out = the splits' parts added in order.
+// out = the splits' parts added in order, loaded kAhead at a time: of dQ, or (blockIdx.y) of dK and dV.
 template <typename T>
-__global__ __launch_bounds__(256) void cross_attention_sum(const float* part, int splits, int64_t quads, T* out) {
+__global__ __launch_bounds__(256) void cross_attention_sum(const float* part, int splits, int64_t quads, T* out0, T* out1) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (at >= quads) return;
-  f32x4 v = *(const f32x4*)(part + 4 * at);
-  for (int s = 1; s < splits; ++s) v += *(const f32x4*)(part + 4 * (s * quads + at));
+  T* out = blockIdx.y ? out1 : out0;
+  if (at >= quads || !out) return;
+  part += blockIdx.y * splits * quads * 4;
+  constexpr int kAhead = 4;
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < splits; s0 += kAhead) {
+    f32x4 x[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) x[u] = *(const f32x4*)(part + 4 * (min(s0 + u, splits - 1) * quads + at));
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (s0 + u >= splits) break;
+      v += x[u];
+    }
+  }
   store4(out + 4 * at, v);
 }
 
@@ -624,9 +636,9 @@ int launch(CrossArgs& a, hipStream_t stream) {
                   delta_blocks < most && q_quads / 256 < most - 1 && k_quads / 256 < most - 1,
               "cross_attention_bwd: too many blocks");
   cross_attention_delta<T><<<dim3((unsigned)delta_blocks), 256, 0, stream>>>(a);
-  auto sum = [&](const Split& s, int64_t part, int64_t quads, void* out) {
-    cross_attention_sum<<<dim3((unsigned)((quads + 255) / 256)), 256, 0, stream>>>(a.part_o + part * s.splits * quads * 4,
-                                                                                  s.splits, quads, (T*)out);
+  auto sum = [&](const Split& s, int64_t quads, void* out0, void* out1) {
+    const dim3 grid((unsigned)((quads + 255) / 256), out1 ? 2 : 1);
+    if (s.splits > 1) cross_attention_sum<<<grid, 256, 0, stream>>>(a.part_o, s.splits, quads, (T*)out0, (T*)out1);
   };
   if (a.dq) {
     a.splits = q.splits, a.split_keys = q.size;
@@ -636,7 +648,7 @@ int launch(CrossArgs& a, hipStream_t stream) {
       a.bias ? cross_attention_dq<T, DP, true, kExact><<<grid, 256, 0, stream>>>(a)
              : cross_attention_dq<T, DP, false, kExact><<<grid, 256, 0, stream>>>(a);
     });
-    if (q.splits > 1) sum(q, 0, q_quads, a.dq);
+    sum(q, q_quads, a.dq, nullptr);
   }
   if (a.dk || a.dv || (a.dbias && !shared)) {
     a.splits = kv.splits, a.split_keys = kv.size;
@@ -650,8 +662,7 @@ int launch(CrossArgs& a, hipStream_t stream) {
       else
         cross_attention_dkv<T, DP, false, false, kExact><<<grid, 256, 0, stream>>>(a);
     });
-    if (kv.splits > 1 && a.dk) sum(kv, 0, k_quads, a.dk);
-    if (kv.splits > 1 && a.dv) sum(kv, 1, k_quads, a.dv);
+    sum(kv, k_quads, a.dk, a.dv);
   }
   if (shared) cross_attention_dbias<T, DP><<<dim3((unsigned)bias_blocks), 64 * kBiasWaves<T, DP>, 0, stream>>>(a);
   return check_launch("cross_attention_bwd");
