@@ -15,6 +15,7 @@ import math
 import pytest
 import torch
 
+from boltz_lumi_amd import _native as N
 from boltz_lumi_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -325,6 +326,32 @@ def test_same_bits_streams_and_graph(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(want, held)) and torch.equal(single, one)
+
+
+@pytest.mark.parametrize("dtype,dim", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 32)])
+@pytest.mark.parametrize("axes", [(0,), (1,), (0, 1)])
+def test_native_dbias_shared_by_own_biases(gpu, dtype, dim, axes):
+    """The C entry sums dbias over axes along which the bias itself differs."""
+    b, m, n, h, hk = 3, 70, 150, 4, 2
+    q, k, v, mask, bias, g = inputs((b, m, n, h, hk, dim, "tail", (1, 1), dtype), gpu)
+    mask[1] = False
+    scale, dout = dim ** -0.5, randn(g, b, m, h, dim, dtype=dtype)
+    lo, out, stats = torch.empty_like(q), torch.empty_like(q), torch.empty(b, h, m, 2, device=gpu)
+    dbias = torch.full([1 if i in axes else s for i, s in enumerate((b, h))] + [m, n], math.nan, device=gpu, dtype=dtype)
+    code = N.F32 if dtype == torch.float32 else N.BF16
+    shape = N.int64_array([b, m, n, h, hk, dim])
+    strides = N.int64_array([*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], n, *bias.stride()[:3]])
+    steps = N.int64_array([0 if i in axes else st for i, st in enumerate(dbias.stride()[:3])])
+    size = max(N.lib().bmx_cross_attention_workspace_bytes(code, b, m, n, h, hk, dim),
+               N.lib().bmx_cross_attention_bwd_workspace_bytes(b, m, n, h, hk, dim))
+    ws, stream = torch.empty(size, device=gpu, dtype=torch.uint8), torch.cuda.current_stream().cuda_stream
+    head = (*(t.data_ptr() for t in (q, k, v, mask, bias)), code, shape, strides, scale, out.data_ptr(), lo.data_ptr(),
+            stats.data_ptr())
+    N.call("bmx_cross_attention_fwd", *head, ws.data_ptr(), size, stream)
+    N.call("bmx_cross_attention_bwd", *head, dout.data_ptr(), None, None, None, dbias.data_ptr(), steps, ws.data_ptr(), size,
+           stream)
+    ref, sizes = (t.sum(axes, keepdim=True) for t in formula(q, k, v, mask, bias, scale, dout)[4])
+    check(dbias, ref, sizes, "dbias", weights=False)
 
 
 def test_long_cache_offsets(gpu):
