@@ -35,7 +35,7 @@ struct CrossArgs {
   int n, heads, kv_heads, group, dim, rows;  // rows = group * m
   float scale;
   void *out, *out_lo;
-  float2* stats;  // [batch][heads][m]: row maximum of the logits and log2 of the sum of exp(logit - maximum)
+  float2* stats;  // [batch][heads][m]: reference point (without a bias before the scale) and log2 of the sum against it
   // work split
   bool exact;       // bf16: weights of 16 bits instead of 8 in the products over them
   int batch_first;  // a bias shared by the batch: its elements' blocks follow each other, so that it stays in L2
@@ -515,6 +515,33 @@ __device__ __forceinline__ float halves_max(float v) {
 __device__ __forceinline__ float halves_sum(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- reference point -----------------------------------------------------
+// A row's weights are taken against one of its logits, `top` (with a bias in natural units, without one before the scale;
+// c0 takes either to base 2). fp32: exp2((x - top) c0). bf16 saves the subtraction, exp2(x c - S) in one multiply-add with
+// S = top c rounded once: whatever that rounding is, all weights of the row share it, so sums
+// against another reference point are moved by the difference of the two S, and what is kept for the gradients is
+// corrected to top itself. From 2^29 on two logits differ by nothing or by at least 2^5, the weights are zeros and
+// ones in any unit, and one in which S is exact keeps the shared factor from leaving fp32's range (below it is 2^32 at most).
+__device__ __forceinline__ float logit_unit(float top, float c0) {
+  const float t = fabsf(top);
+  if (t * c0 <= 0x1p29f) return c0;
+  const float p = __uint_as_float(__float_as_uint(c0) & 0x7f800000u);  // the power of two below
+  return t > 0x1p64f ? fminf(p, 1.f) : p;
+}
+// S: the product on its own, not a part of a multiply-add.
+__device__ __forceinline__ float reference_shift(float top, float c) {
+  float s = top * c;
+  asm("" : "+v"(s));
+  return s;
+}
+// What sums taken against `from` (-inf: none yet) are multiplied by to be against `to` (finite).
+template <typename T>
+__device__ __forceinline__ float rescale(float from, float to, float c0) {
+  if (sizeof(T) == 4) return __builtin_amdgcn_exp2f((from - to) * c0);
+  const float c = logit_unit(from, c0), d = logit_unit(to, c0);
+  return __builtin_amdgcn_exp2f(c == d ? reference_shift(from, c) - reference_shift(to, d) : (from - to) * fminf(c, d));
 }
 
 int cross_setup(CrossArgs& a, int dtype, const int64_t* shape, const int64_t* strides, float scale, bool has_bias);

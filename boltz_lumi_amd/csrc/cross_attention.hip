@@ -24,9 +24,7 @@ namespace {
 // State of a wave's 32 rows: lane l holds row l % 32, in both halves.
 template <typename T, int DP, bool kBias, bool kExact>
 struct Rows {
-  // The weight of a logit x is exp2(x c + shift), shift = -top c: without a bias x is q k^T, with one the logit in natural
-  // units. fp32 takes the difference first, exp2((x - top) c): the largest logit's weight is then exactly 1 (bf16
-  // rounds it to 1).
+  // The weight of a logit x (without a bias q k^T, with one the logit in natural units): see the reference point.
   static constexpr bool kFirst = sizeof(T) == 4;
   RowOperand<T, DP> q;
   RowReads<T, DP> kr;
@@ -34,8 +32,8 @@ struct Rows {
   f32x16 o[DP / 32];
   float top, sum;  // maximum that the weights refer to; this half's share of their sum
   float limit;     // the maximum moves when a logit passes this
-  float shift;     // of the exponent: -top c, or (fp32) top
-  float c;         // logits to base 2
+  float shift;     // of the exponent: -S, or (fp32) top
+  float c;         // logits to base 2, or the unit of rows far from zero
   const T* bias;
   bool odd;  // some bias rows start at an odd element
 
@@ -76,16 +74,15 @@ struct Rows {
     // factor and the products with it are off the common path.
     if (__any(mx > limit)) {
       mx = fmaxf(halves_max(mx), top);
-      const float base = mx == -INFINITY ? 0.f : mx, f = __builtin_amdgcn_exp2f((top - base) * c);
+      const float base = mx == -INFINITY ? 0.f : mx, c0 = (kBias ? 1.f : a.scale) * kLog2E;
+      const float f = rescale<T>(top, base, c0);
       sum *= f;
 #pragma unroll
       for (int dt = 0; dt < DP / 32; ++dt) o[dt] *= f;
       top = mx;
-      // A maximum near the type's lowest (or largest) value would overflow in base 2. Logits that size differ by 0
-      // or by more than any exponent, so half of them tells the same weights. (fp32's difference is taken first.)
-      if (kBias && !kFirst) c = fabsf(base) > 1e38f ? 0.5f : kLog2E;
+      if (!kFirst) c = logit_unit(base, c0);
       limit = kFirst ? mx : mx + 6.f / c;
-      shift = kFirst ? base : -base * c;
+      shift = kFirst ? base : -reference_shift(base, c);
     }
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(kFirst ? (s[r] - shift) * c : s[r] * c + shift);
@@ -115,16 +112,22 @@ __device__ __forceinline__ void store_out<float>(const CrossArgs& a, int64_t at,
 // A row without keys. A row whose logits are all NaN has no maximum either, but a sum that is NaN, and stays NaN.
 __device__ __forceinline__ bool no_keys(float top, float sum) { return top == -INFINITY && sum == sum; }
 
-// Row maximum in natural units and log2 of the sum; a row without keys gets weights exp2(-inf) = 0.
-__device__ __forceinline__ float2 row_stats(const CrossArgs& a, float top, float sum, bool bias) {
+// Reference point and log2 of the sum against it; a row without keys gets weights exp2(-inf) = 0.
+template <typename T>
+__device__ __forceinline__ float2 row_stats(float top, float sum, float c0) {
   if (no_keys(top, sum)) return make_float2(0.f, INFINITY);
-  return make_float2(bias ? top : top * a.scale, __builtin_amdgcn_logf(sum));
+  float log = __builtin_amdgcn_logf(sum);
+  if (sizeof(T) == 2) {  // bf16's sum is against S, which is off top c by what its rounding left
+    const float c = logit_unit(top, c0);
+    log += fmaf(-top, c, reference_shift(top, c));
+  }
+  return make_float2(top, log);
 }
 
 // The lane's row of a wave's result: to out (and stats), or as a partial sum of its split.
 template <typename T, int DP>
 __device__ __forceinline__ void write_rows(const CrossArgs& a, int64_t b, int c, int split, int row,
-                                           const f32x16 (&o)[DP / 32], float top, float sum, bool bias) {
+                                           const f32x16 (&o)[DP / 32], float top, float sum, float c0) {
   if (row >= a.rows) return;
   const int h = lane_id() >> 5;
   if (a.splits > 1) {
@@ -145,7 +148,7 @@ __device__ __forceinline__ void write_rows(const CrossArgs& a, int64_t b, int c,
   const int64_t at = ((b * a.m + i) * a.heads + head) * a.dim;
   const bool none = no_keys(top, sum);
   const float f = none ? 0.f : 1.f / sum;
-  if (a.stats && h == 0) a.stats[(b * a.heads + head) * a.m + i] = row_stats(a, top, sum, bias);
+  if (a.stats && h == 0) a.stats[(b * a.heads + head) * a.m + i] = row_stats<T>(top, sum, c0);
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt)
 #pragma unroll
@@ -231,7 +234,8 @@ void cross_attention_wide(CrossArgs a) {
       }
     }
   }
-  write_rows<T, DP>(a, p.b, p.c, p.split, row, rows.o, rows.top, halves_sum(rows.sum), kBias);
+  write_rows<T, DP>(a, p.b, p.c, p.split, row, rows.o, rows.top, halves_sum(rows.sum),
+                    (kBias ? 1.f : a.scale) * kLog2E);
 }
 
 // Up to kFewRows rows (a decoding step): the four waves take 32 keys in turn, each through a tile of its own without
@@ -295,7 +299,7 @@ void cross_attention_few(CrossArgs a) {
 #pragma unroll
   for (int i = 1; i < 4; ++i) top = fmaxf(top, ml[i * 32 + row]);
   const float base = top == -INFINITY ? 0.f : top;
-  const float f = __builtin_amdgcn_exp2f((rows.top - base) * rows.c);  // 0 for a wave without keys
+  const float c0 = (kBias ? 1.f : a.scale) * kLog2E, f = rescale<T>(rows.top, base, c0);  // 0 for a wave without keys
   sum *= f;
 #pragma unroll
   for (int dt = 0; dt < DP / 32; ++dt) rows.o[dt] *= f;
@@ -322,7 +326,7 @@ void cross_attention_few(CrossArgs a) {
       for (int r = 0; r < 16; ++r) rows.o[dt][r] += other[(16 * dt + r) * 64 + l];
     sum += other[(DP / 2) * 64 + l];
   }
-  write_rows<T, DP>(a, p.b, p.c, p.split, row, rows.o, top, sum, kBias);
+  write_rows<T, DP>(a, p.b, p.c, p.split, row, rows.o, top, sum, c0);
 }
 
 // Joins the splits: a thread per four channels of a row.
@@ -345,7 +349,7 @@ __global__ __launch_bounds__(256) void cross_attention_join(CrossArgs a, int bia
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) top = fmaxf(top, x[u]);
   }
-  const float c = (bias ? 1.f : a.scale) * kLog2E, base = top == -INFINITY ? 0.f : top;
+  const float c0 = (bias ? 1.f : a.scale) * kLog2E, base = top == -INFINITY ? 0.f : top;
   float sum = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   for (int s0 = 0; s0 < a.splits; s0 += kAhead) {
@@ -360,7 +364,7 @@ __global__ __launch_bounds__(256) void cross_attention_join(CrossArgs a, int bia
 #pragma unroll
     for (int u = 0; u < kAhead; ++u) {
       if (s0 + u >= a.splits) break;
-      const float f = __builtin_amdgcn_exp2f((ml[u].x - base) * c);
+      const float f = rescale<T>(ml[u].x, base, c0);
       sum += ml[u].y * f;
       o += part[u] * f;
     }
@@ -369,7 +373,7 @@ __global__ __launch_bounds__(256) void cross_attention_join(CrossArgs a, int bia
   const int row = (int)(at - list * a.rows), g = row / (int)a.m, i = row - g * (int)a.m;
   const int64_t head = (list - b * a.kv_heads) * a.group + g;
   const bool none = no_keys(top, sum);
-  if (a.stats && d == 0) a.stats[(b * a.heads + head) * a.m + i] = row_stats(a, top, sum, bias);
+  if (a.stats && d == 0) a.stats[(b * a.heads + head) * a.m + i] = row_stats<T>(top, sum, c0);
   const float f = none ? 0.f : 1.f / sum;
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] = none ? 0.f : o[e] * f;

@@ -100,17 +100,24 @@ __device__ __forceinline__ void store_keys(T* row, int key, int n, const f32x16&
   }
 }
 
-// P of a logits tile whose column is a query: maximum and log2 of the sum are the lane's.
+// Without a bias bf16 weights are one multiply-add and an exponential, exp2(x c - (top c + log)), where that sum's rounding
+// stays below 2^-16. A row further from zero takes the difference x - top first, as rows with a bias and fp32 do.
+__device__ __forceinline__ bool far_row(const CrossArgs& a, float2 st) {
+  return fabsf(st.x) * (a.scale * kLog2E) > 256.f;
+}
+
+// P of a logits tile whose column is a query: reference point and log2 of the sum are the lane's. far: of some row.
 template <typename T, bool kBias>
-__device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, const BiasTile<T>& b, float2 st) {
+__device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, const BiasTile<T>& b, float2 st, bool far) {
+  const float c = a.scale * kLog2E;
   if (kBias) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + b.at(r) - st.x) * kLog2E - st.y);
-  } else if (sizeof(T) == 4) {  // as the forward pass: the difference first
+  } else if (sizeof(T) == 4 || far) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale - st.x) * kLog2E - st.y);
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f((s[r] - st.x) * c - st.y);
   } else {
-    const float c = a.scale * kLog2E, shift = -(st.x * kLog2E + st.y);
+    const float shift = -(st.x * c + st.y);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = __builtin_amdgcn_exp2f(s[r] * c + shift);
   }
@@ -135,6 +142,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   g.load((const T*)a.dout + ra.dense(a, b), a.dim, h);
   const float2 st = a.stats[ra.stat(a, b)];
   const float delta = a.delta[ra.stat(a, b)];
+  const bool far = !kBias && sizeof(T) == 2 && __any(far_row(a, st));
   const T* bias_row = (const T*)a.bias + ra.bias(a, b);
   RowReads<T, DP> rr;
   ColumnReads<T, DP> cr;
@@ -179,7 +187,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
       f32x16 s = product<T, DP>(kt, rr, q);
       const f32x16 dp = product<T, DP>(vt, rr, g);
       if (kBias) bias[decltype(B)::value].ready(true);
-      weights_of<T, kBias>(a, s, bias[decltype(B)::value], st);
+      weights_of<T, kBias>(a, s, bias[decltype(B)::value], st, far);
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] *= dp[r] - delta;
       if (bits != ~0u) {
@@ -223,7 +231,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   constexpr bool kValuesInLds = sizeof(T) == 2 && DP > 64;
   constexpr bool kFirst = kBias || sizeof(T) == 4;
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
-  constexpr int kStat = 32 * 3 * 4;  // of a row: maximum (or the whole shift), log2 of the sum, delta
+  constexpr int kStat = 32 * 3 * 4;  // of a row: reference point (or the whole shift), log2 of the sum, delta
   constexpr int kValues = 4 * kTile + 2 * kStat + 16;  // V of the block's 128 keys
   __shared__ __attribute__((aligned(16))) char lds[kValues + (kValuesInLds ? 4 * kTile : 0)];
   const int key_blocks = (a.n + 127) / 128;
@@ -299,8 +307,9 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
       if (kValuesInLds) rr.renew(), cr.renew();
       const char *qt = lds + buf * 2 * kTile, *gt = qt + kTile;
       float* stat = (float*)(lds + 4 * kTile + buf * kStat);
+      const bool far = !kFirst && __any(far_row(a, st));  // the same in all waves
       if (t < 32) {
-        stat[t] = kFirst ? st.x : st.x * kLog2E + st.y;
+        stat[t] = kFirst || far ? st.x : st.x * (a.scale * kLog2E) + st.y;
         stat[32 + t] = st.y;
         stat[64 + t] = delta;
       }
@@ -327,21 +336,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
       }
       f32x16 s = product<T, DP>(qt, rr, kf), dp;
       if (!kValuesInLds) dp = product<T, DP>(gt, rr, vf);
+      auto weigh = [&](auto first) {
 #pragma unroll
-      for (int g4 = 0; g4 < 4; ++g4) {
-        const f32x4 top = *(const f32x4*)(stat + 4 * g4 + 16 * h);
-        f32x4 log;
-        if (kFirst) log = *(const f32x4*)(stat + 32 + 4 * g4 + 16 * h);
+        for (int g4 = 0; g4 < 4; ++g4) {
+          const f32x4 top = *(const f32x4*)(stat + 4 * g4 + 16 * h);
+          f32x4 log;
+          if (first) log = *(const f32x4*)(stat + 32 + 4 * g4 + 16 * h);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int r = 4 * g4 + e;
-          if (kFirst) {
-            s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + (kBias ? x[r] : 0.f) - top[e]) * kLog2E - log[e]);
-          } else {
-            s[r] = __builtin_amdgcn_exp2f(s[r] * (a.scale * kLog2E) - top[e]);
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g4 + e;
+            if (kBias)
+              s[r] = __builtin_amdgcn_exp2f((s[r] * a.scale + x[r] - top[e]) * kLog2E - log[e]);
+            else if (first)
+              s[r] = __builtin_amdgcn_exp2f((s[r] - top[e]) * (a.scale * kLog2E) - log[e]);
+            else
+              s[r] = __builtin_amdgcn_exp2f(s[r] * (a.scale * kLog2E) - top[e]);
           }
         }
-      }
+      };
+      if (kFirst || far)
+        weigh(std::true_type());
+      else
+        weigh(std::bool_constant<kFirst>());
       if (kValuesInLds) __builtin_amdgcn_sched_barrier(0);
       weighted_sum<T, DP, kExact>(gt, cr, s, dv);
       if (kValuesInLds) __builtin_amdgcn_sched_barrier(0);
@@ -529,7 +545,7 @@ void cross_attention_dbias(CrossArgs a) {
       const char* kt = lds + buf * 2 * kTile + (keys_at + 32 * u) * kRowBytes;
       f32x16 s = product<T, DP>(kt, rr, q);
       const f32x16 dp = product<T, DP>(kt + kTile, rr, g);
-      weights_of<T, true>(a, s, bias[u], st);
+      weights_of<T, true>(a, s, bias[u], st, false);
       const uint32_t keys = (uint32_t)(mine[(keys_at + 32 * u) / 64] >> ((keys_at + 32 * u) % 64)) >> (16 * h);
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum[u][r] += key_bit(keys, r) ? s[r] * (dp[r] - delta) : 0.f;

@@ -454,7 +454,9 @@ int bmx_relative_bias_bwd(const void* dbias, int dtype, int64_t buckets, int64_t
  * values) is left out, or NULL; bias in dtype or NULL.  A row without keys gives zeros.  batch, m or n may be 0.
  * out dense [batch, m, heads, dim].  scale positive.  bf16 weights have 16 bits in decoding steps (at most 32 rows
  * m * heads / kv_heads), up to 256 keys and in small calls (batch * heads * m * n * dim <= 2^28), otherwise 8.  For the backward pass, or NULL: out_lo (bf16 only, out's shape: what rounding out left),
- * stats fp32 [batch, heads, m, 2] (row maximum of the logits, log2 of the sum of exp(logit - maximum)).
+ * stats fp32 [batch, heads, m, 2], for bmx_cross_attention_bwd alone: a reference point r of the row (a logit at or, in
+ * bf16, up to 6 ln 2 below the largest; without a bias before the scale) and log2 of the sum of exp(logit - r). Only the
+ * two together are defined. Where |logits| pass 2^29 that exponential is any that tells zero from one.
  * workspace: bmx_cross_attention_workspace_bytes, 16-byte aligned.  No reference kernel. */
 size_t bmx_cross_attention_workspace_bytes(int dtype, int64_t batch, int64_t m, int64_t n, int64_t heads,
                                            int64_t kv_heads, int64_t dim);
