@@ -8,7 +8,7 @@
 // rows: S^T = K Q^T puts a query in a lane, so maximum and sum are one lane's
 // registers plus one exchange between the halves, and the weights in registers are the next product's
 // operand as they stand (out^T += V^T P^T, V read transposed from LDS).  The
-// weights are rounded to the operand's type (small calls: to two of them), and their sum is taken over the rounded
+// weights are rounded to the operand's type (small elements: to two of them), and their sum is taken over the rounded
 // values, so a row's weights add up to one: the error is a rounding of each weight against the others.
 //
 // A row without keys (masked, or -inf bias throughout) gives zeros.
@@ -464,10 +464,14 @@ int cross_setup(CrossArgs& a, int dtype, const int64_t* shape, const int64_t* st
   // The weights' rounding moves a result by as much as its own rounding does, and over few keys the output's error does not
   // average out before the gradients' differences dP - delta meet it. Weights of 16 bits leave the result's rounding alone:
   // in decoding steps, which are bound by reading the keys (batch 32, 32 / 8 heads, 4096 keys, D = 128: 95.7 us with 8
-  // bits, 96.6 with 16; 16 heads, 2048 keys, D = 64: 45.7 and 47.3, D = 32 with a bias, the worst, 26.6 and 31.8), and
-  // where a call is mostly latency (300 queries, 500 keys, 16 heads, D = 64: forward 15.4 and 16.1 us, dQ, dK and dV 23.5
-  // and 26.5). Large calls would pay for the added products (2048 queries, 256 keys, D = 128: dK and dV 46 and 55).
-  a.exact = dtype == kBF16 && (rows <= kFewRows || a.n <= 256 || (double)a.batch * heads * a.m * a.n * dim <= 1ll << 28);
+  // bits, 96.6 with 16; 16 heads, 2048 keys, D = 64: 45.7 and 47.3, D = 32 with a bias, the worst, 26.6 and 31.8),
+  // and where an element's products are few, whatever the batch: its neighbours must not decide its error, and one such
+  // element alone is mostly latency (300 queries, 500 keys, 16 heads, D = 64: forward 15.4 and 16.1 us, dQ, dK and dV 23.5
+  // and 26.5). Large batches of them pay for the added products (32 of that size: forward 42 and 51 us, dQ 50 and 60, dK
+  // and dV 75 and 91; 16 x 250 queries, 500 keys, 16 / 4 heads, D = 128: 31 and 36, 37 and 42, 57 and 92), as calls over up
+  // to 256 keys do (2048 queries, D = 128: dK and dV 46 and 55), where the few weights' errors average out least. Large
+  // elements would pay as much on top of more work, and their rows have the most keys to average over.
+  a.exact = dtype == kBF16 && (rows <= kFewRows || a.n <= 256 || (double)heads * a.m * a.n * dim <= 1ll << 28);
   a.batch_first = has_bias && a.batch > 1 && a.sb[0] == 0;
   return BMX_OK;
 }

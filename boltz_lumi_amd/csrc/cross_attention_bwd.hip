@@ -7,8 +7,10 @@
 // No logits are kept: each kernel recomputes S and dP for its tiles.  Three
 // kernels instead of one, because each sums over another axis and keeps its sum in
 // registers: no atomics, and the same bits on every run.  P and dS are rounded to
-// the operand's type for the products over them (small calls: to two of them); delta is taken from the output before its rounding
-// (out + out_lo), so that dP - delta cancels as it does in the formula.
+// the operand's type for the products over them (small elements: to two of them),
+// and where the forward pass summed rounded weights, P is divided by that sum: half a step
+// more at most, of a row that one weight dominates.  delta is taken from the output
+// before its rounding (out + out_lo), so that dP - delta cancels as it does in the formula.
 #include <algorithm>
 #include <type_traits>
 

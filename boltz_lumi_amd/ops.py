@@ -1520,8 +1520,9 @@ def cross_attention(q, k, v, mask=None, bias=None, scale=None):
     [B or 1, H or 1, M, N], added to the logits; -inf leaves a pair out.  A
     query without keys gives zeros, and zero gradients.  scale: positive,
     1 / sqrt(D) by default.  Sums are fp32; bf16 weights enter the products with
-    16 bits in decoding steps (M H / Hk <= 32) and small calls, else with 8, so
-    a large call's error is about 1.4 times that of rounding its result.
+    16 bits in decoding steps (M H / Hk <= 32), over up to 256 keys and where a
+    batch element is small (H M N D <= 2^28), else with 8, whose error is about
+    1.4 times that of rounding the result.
     Gradients reach q, k, v and bias (summed over its shared axes in fp32) and
     are the same bits on every run."""
     dev = _same_device(q, k, v, mask, bias)
