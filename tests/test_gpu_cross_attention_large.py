@@ -12,6 +12,7 @@ import pytest
 import torch
 from test_gpu_cross_attention import check, formula, inputs, randn
 
+from boltz_lumi_amd import _native as N
 from boltz_lumi_amd import ops
 
 pytestmark = pytest.mark.gpu
@@ -45,3 +46,29 @@ def test_a_batch_of_small_elements_rounds_the_result_alone(gpu, case):
     assert not eight_bits(case) and b * h * m * n * d > 1 << 28
     for name, got, (ref, size) in run((*case, torch.bfloat16), gpu, 2 * case[5] ** -0.5):
         check(got, ref, size, name, weights=False)
+
+
+LARGE = [  # batch, m, n, heads, kv_heads, dim, mask, bias (per batch element, per head), whether the keys are split
+    (1, 910, 1031, 12, 3, 24, None, None, True),
+    (4, 700, 1031, 16, 16, 24, "empty", (1, 1), False),
+    (1, 700, 801, 10, 10, 48, "some", (1, 1), True),
+    (2, 520, 1031, 8, 2, 64, "empty", (0, 1), True),
+    (2, 520, 1031, 8, 8, 64, None, (1, 0), True),
+    (1, 3000, 1401, 1, 1, 64, "some", None, True),
+    (1, 400, 1777, 4, 4, 96, "tail", (0, 0), True),
+    (2, 700, 1031, 4, 2, 96, "empty", None, True),
+    (2, 300, 901, 8, 4, 128, None, None, True),
+    (2, 270, 1000, 8, 1, 128, "empty", (0, 1), True),
+    (2, 300, 901, 8, 8, 128, "some", (1, 1), True),
+    (1, 65, 5400, 6, 2, 128, "some", None, True),
+]
+
+
+@pytest.mark.parametrize("case", LARGE)
+def test_large_elements(gpu, case):
+    print(f"large element {case}", flush=True)
+    b, m, n, h, hk, d = case[:6]
+    assert eight_bits(case)
+    assert (N.lib().bmx_cross_attention_workspace_bytes(N.BF16, b, m, n, h, hk, d) > 0) == case[8]
+    for name, got, (ref, size) in run((*case[:8], torch.bfloat16), gpu, 0.9 * d ** -0.5):
+        check(got, ref, size if name == "out" else size * 2, name)
