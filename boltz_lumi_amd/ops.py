@@ -24,6 +24,7 @@ import os
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -1149,7 +1150,9 @@ def adaln_modulate(a, scale, shift, eps):
 # ------------------------------------------------------ sequence operators
 #
 # Differentiable (torch.autograd; one backward pass, no double backward).  A
-# call that needs no gradient does not go through autograd.  In a captured
+# call that needs no gradient does not go through autograd.  Forward-mode
+# derivatives and tracing are refused: neither sees a native launch, so the
+# result would have no tangent, or be an empty tensor in the trace.  In a captured
 # graph make the leaves inside or before the capture and take the gradients
 # with torch.autograd.grad, as for torch's own operators.
 
@@ -1167,8 +1170,18 @@ def _layout(t):
     return None if t is None else (t.shape, t.stride(), t.dtype)
 
 
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+
+
 def _same_device(first, *tensors) -> int:
-    """The device index that the tensors share; raises as ``_cuda`` does."""
+    """The device index that the tensors share; raises as ``_cuda`` does, and
+    where the call would be traced or carries forward-mode tangents."""
+    if forward_ad._current_level >= 0:
+        _check(all(t is None or forward_ad.unpack_dual(t).tangent is None for t in (first, *tensors)),
+               "forward-mode derivatives are not supported")
+    _check(torch._C._get_tracing_state() is None
+           and (not torch._C._len_torch_dispatch_stack() or torch._C._get_dispatch_mode(_PROXY) is None),
+           "tracing is not supported")
     dev = first.get_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
