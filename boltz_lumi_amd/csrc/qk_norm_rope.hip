@@ -28,7 +28,7 @@ constexpr int kBwdBlocks = 1024;  // of a tensor's gradient at most: four per co
 // One of the two tensors: x [batch, tokens, heads, D] at element strides, y dense.
 struct HeadRows {
   const void *x, *w, *dy;
-  void* y;          // forward: the result; backward: dx
+  void* y;          // forward: the result; backward: dx, or null
   float* partial;   // backward: [blocks][D] sums of g x r, or null
   const void* pos;
   int64_t sb, st, sh, pos_sb;
@@ -180,7 +180,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(NormRope s) {
     const int h0 = (int)(item % t.chunks) * kRows, last = t.heads - 1;
     const T* x = (const T*)t.x + batch * t.sb + token * t.st;
     const T* dy = (const T*)t.dy + row * t.heads * s.dim;
-    T* dx = (T*)t.y + row * t.heads * s.dim;
+    T* dx = t.y ? (T*)t.y + row * t.heads * s.dim : nullptr;
     Eight v[kRows], g[kRows];
 #pragma unroll
     for (int u = 0; u < kRows; ++u) {
@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_bwd_kernel(NormRope s) {
       dw.a += g[u].a * n.a, dw.b += g[u].b * n.b;
       const Eight gw = {g[u].a * c.w.a, g[u].b * c.w.b};
       const float mean = group_sum<L>(dot(gw, n)) / (float)s.dim;
-      store8(dx + (h0 + u) * s.dim, c, Eight{r * (gw.a - n.a * mean), r * (gw.b - n.b * mean)});
+      if (dx) store8(dx + (h0 + u) * s.dim, c, Eight{r * (gw.a - n.a * mean), r * (gw.b - n.b * mean)});
     }
   }
   if (!t.partial) return;
@@ -314,7 +314,7 @@ int setup(NormRope& s, int dtype, const int64_t* shape, const int64_t* strides, 
 
 int check_tensor(const HeadRows& t, int64_t batch, int64_t half, int elem, bool backward) {
   if (batch * t.tokens * t.heads == 0) return BMX_OK;
-  BMX_REQUIRE(t.x && t.y && (!backward || t.dy) && (half == 0 || t.pos), "qk_norm_rope: null pointer");
+  BMX_REQUIRE(t.x && (backward ? t.dy : t.y) && (half == 0 || t.pos), "qk_norm_rope: null pointer");
   const uintptr_t bits = (uintptr_t)t.x | (uintptr_t)t.y | (uintptr_t)t.dy | (uintptr_t)t.w;
   BMX_REQUIRE(bits % (4 * elem) == 0 && (uintptr_t)t.w % 16 == 0,
               "qk_norm_rope: tensors must be aligned to four elements, weights to 16 bytes");
@@ -366,6 +366,8 @@ extern "C" int bmx_qk_norm_rope_bwd(const void* q, const void* k, int dtype, con
   if (int rc = setup(s, dtype, shape, strides, w_dtype, pos64, inv_freq, inv_freq64, half, interleaved, eps)) return rc;
   s.q.x = q, s.q.w = q_weight, s.q.pos = q_pos, s.q.dy = dq_out, s.q.y = dq;
   s.k.x = k, s.k.w = k_weight, s.k.pos = k_pos, s.k.dy = dk_out, s.k.y = dk;
+  if (!dq && !dq_weight) s.q.tokens = 0;  // a tensor without a gradient to write takes no part
+  if (!dk && !dk_weight) s.k.tokens = 0;
   const int64_t batch = shape[0];
   const int elem = dtype == kF32 ? 4 : 2;
   if (int rc = check_tensor(s.q, batch, half, elem, true)) return rc;

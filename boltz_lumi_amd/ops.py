@@ -1255,22 +1255,21 @@ def _norm_rope_plan(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq):
     weight = q_weight or k_weight
     plan.code, plan.w_code = code, _code(weight[2]) if weight else code
     plan.shape, plan.strides = N.int64_array([b, m, n, h, hk, d]), N.int64_array(strides)
-    plan.no_q, plan.no_k = N.int64_array([b, 0, n, h, hk, d]), N.int64_array([b, m, 0, h, 0, d])
     plan.tail = (pos64, freq64, half)
     plan.ws = N.lib().bmx_qk_norm_rope_workspace_bytes(d)
     return plan
 
 
-def _norm_rope_args(plan, shape, q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved):
+def _norm_rope_args(plan, q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved):
     pos64, freq64, half = plan.tail
-    return (q.data_ptr(), _ptr(k), plan.code, shape, plan.strides, _ptr(q_weight), _ptr(k_weight), plan.w_code, _ptr(q_pos),
+    return (q.data_ptr(), _ptr(k), plan.code, plan.shape, plan.strides, _ptr(q_weight), _ptr(k_weight), plan.w_code, _ptr(q_pos),
             _ptr(k_pos), pos64, _ptr(inv_freq), freq64, half, interleaved, eps)
 
 
 def _norm_rope_fwd(plan, dev, q, k, *rest):
     q_out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
     k_out = torch.empty(k.shape, device=k.device, dtype=k.dtype) if k is not None else None
-    _launch(dev, "bmx_qk_norm_rope_fwd", *_norm_rope_args(plan, plan.shape, q, k, *rest), q_out.data_ptr(), _ptr(k_out))
+    _launch(dev, "bmx_qk_norm_rope_fwd", *_norm_rope_args(plan, q, k, *rest), q_out.data_ptr(), _ptr(k_out))
     return q_out, k_out
 
 
@@ -1287,20 +1286,21 @@ class _QkNormRope(torch.autograd.Function):
     def backward(ctx, dq_out, dk_out):
         plan, dev, eps, interleaved = ctx.rest
         q, k, q_weight, k_weight, q_pos, k_pos, inv_freq = ctx.saved_tensors
-        dq = dk = dqw = dkw = ws = None
-        # A tensor whose result got no gradient takes no part: no tokens of it.
-        shape = plan.shape if dk_out is not None and dq_out is not None else plan.no_q if dq_out is None else plan.no_k
+        need, ws = ctx.needs_input_grad, None
+        dq = dk = dqw = dkw = None  # a tensor whose result got no gradient takes no part
         if dq_out is not None:
-            dq_out, dq = _aligned(dq_out.contiguous()), torch.empty(q.shape, device=q.device, dtype=q.dtype)
-            dqw = torch.empty_like(q_weight) if ctx.needs_input_grad[4] else None
+            dq_out = _aligned(dq_out.contiguous())
+            dq = torch.empty(q.shape, device=q.device, dtype=q.dtype) if need[2] else None
+            dqw = torch.empty_like(q_weight) if need[4] else None
         if dk_out is not None:
-            dk_out, dk = _aligned(dk_out.contiguous()), torch.empty(k.shape, device=k.device, dtype=k.dtype)
-            dkw = torch.empty_like(k_weight) if ctx.needs_input_grad[5] else None
+            dk_out = _aligned(dk_out.contiguous())
+            dk = torch.empty(k.shape, device=k.device, dtype=k.dtype) if need[3] else None
+            dkw = torch.empty_like(k_weight) if need[5] else None
         if dqw is not None or dkw is not None:
             ws = _workspace(plan.ws, q.device)
-        if dq is not None or dk is not None:
+        if ws is not None or dq is not None or dk is not None:
             _launch(dev, "bmx_qk_norm_rope_bwd",
-                    *_norm_rope_args(plan, shape, q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved),
+                    *_norm_rope_args(plan, q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps, interleaved),
                     _ptr(dq_out), _ptr(dk_out), _ptr(dq), _ptr(dk), _ptr(dqw), _ptr(dkw), _ptr(ws),
                     plan.ws if ws is not None else 0)
         return None, None, dq, dk, dqw, dkw, None, None, None, None, None

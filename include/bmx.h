@@ -403,7 +403,8 @@ int bmx_seq_attention_x3_batched_split_fwd(const float* q, const float* k, const
 
 /* ---- Sequence operators, with their gradients ----------------------------
  * No reference kernel (the reference is inference only): what a sequence encoder / decoder beside
- * the pair stack needs.  Strides are in elements.  A gradient pointer may be NULL: not computed.
+ * the pair stack needs.  Strides are in elements.  Where a call has several gradients, each pointer
+ * may be NULL: not computed.
  * Results do not depend on atomics' order. */
 
 /* y = R(pos) (x / sqrt(mean(x^2) + eps) * weight) for every head vector x of q [batch, m, heads, dim]
@@ -419,8 +420,8 @@ int bmx_qk_norm_rope_fwd(const void* q, const void* k, int dtype, const int64_t*
                          int pos64, const void* inv_freq, int inv_freq64, int64_t half, int interleaved, float eps,
                          void* q_out, void* k_out, bmx_stream_t stream);
 
-/* Gradients of bmx_qk_norm_rope_fwd from dq_out / dk_out (dense).  dq and dk are written whole;
- * dq_weight / dk_weight [dim] in w_dtype or NULL; workspace (needed for a weight gradient):
+/* Gradients of bmx_qk_norm_rope_fwd from dq_out / dk_out (dense): dq and dk dense, dq_weight / dk_weight [dim] in
+ * w_dtype, each or NULL; of a tensor with neither nothing is read; workspace (needed for a weight gradient):
  * bmx_qk_norm_rope_workspace_bytes(dim).  No reference kernel. */
 size_t bmx_qk_norm_rope_workspace_bytes(int64_t dim);
 int bmx_qk_norm_rope_bwd(const void* q, const void* k, int dtype, const int64_t* shape, const int64_t* strides,
