@@ -98,6 +98,17 @@ __device__ __forceinline__ f32x16 zero16() {
   return z;
 }
 
+// A grid of `blocks` < 2^31 blocks. A launch takes fewer than 2^32 threads along an axis: more blocks are folded
+// into y (x a multiple of the 8 XCDs, so that neighbours stay on the XCD they would be on). Kernels take
+// their place from block_index() and leave where it is not below their number of blocks.
+inline dim3 fold_grid(int64_t blocks, int threads) {
+  const int64_t most = 0xffffffffll / threads / 8 * 8;
+  if (blocks <= most) return dim3((unsigned)blocks);
+  const int64_t y = (blocks + most - 1) / most;
+  return dim3((unsigned)(((blocks + y - 1) / y + 7) / 8 * 8), (unsigned)y);
+}
+__device__ __forceinline__ uint32_t block_index() { return blockIdx.y * gridDim.x + blockIdx.x; }
+
 __device__ __forceinline__ int lane_id() { return threadIdx.x & (kWave - 1); }
 
 // D-fragment row of register r for this lane (see header comment).

@@ -39,6 +39,7 @@ struct CrossArgs {
   // work split
   bool exact;       // bf16: weights of 16 bits instead of 8 in the products over them
   int batch_first;  // a bias shared by the batch: its elements' blocks follow each other, so that it stays in L2
+  uint32_t blocks;  // of the launch
   int row_blocks, splits;
   int split_keys;  // or, of dK and dV, tiles of 32 queries
   float* part_o;   // [split][batch * kv_heads][rows][dim] sums before the division; backward: [split] gradients

@@ -166,7 +166,7 @@ struct Place {
   int row_block, split, c, first, stop;  // keys of the split
   int64_t b;
   __device__ __forceinline__ Place(const CrossArgs& a) {
-    uint32_t at = xcd_position(blockIdx.x, gridDim.x);
+    uint32_t at = xcd_position(block_index(), a.blocks);
     b = a.batch_first ? take(at, a.batch) : 0;
     row_block = take(at, a.row_blocks), split = take(at, a.splits), c = take(at, a.kv_heads);
     if (!a.batch_first) b = at;
@@ -186,6 +186,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : sizeof(T) == 4
 void cross_attention_wide(CrossArgs a) {
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[4 * kTile + kMaskChunk / 8];
+  if (block_index() >= a.blocks) return;
   const Place p(a);
   const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), row = (p.row_block * 4 + w) * 32 + (t & 31);
   Rows<T, DP, kBias, kExact> rows;
@@ -246,6 +247,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 || DP == 128 ? 1 : DP == 96 ? 2
 void cross_attention_few(CrossArgs a) {
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[8 * kTile + kMaskChunk / 8 + 4 * 32 * 4];
+  if (block_index() >= a.blocks) return;
   const Place p(a);
   const int t = threadIdx.x, w = t >> 6, l = t & 63, row = l & 31;
   Rows<T, DP, kBias, sizeof(T) == 2> rows;
@@ -409,7 +411,7 @@ Split plan(int dtype, int64_t batch, int64_t kv_heads, int64_t rows, int64_t n) 
 
 template <typename T, int DP, bool kBias>
 void launch(const CrossArgs& a, bool few, hipStream_t stream) {
-  const dim3 grid((unsigned)((int64_t)a.row_blocks * a.splits * a.kv_heads * a.batch));
+  const dim3 grid = fold_grid(a.blocks, 256);
   if (few) {
     cross_attention_few<T, DP, kBias><<<grid, 256, 0, stream>>>(a);
   } else {
@@ -505,13 +507,15 @@ extern "C" int bmx_cross_attention_fwd(const void* q, const void* k, const void*
   a.out = out, a.out_lo = dtype == kBF16 ? out_lo : nullptr, a.stats = (float2*)stats;
   a.row_blocks = s.row_blocks, a.splits = s.splits, a.split_keys = s.keys;
   const int64_t lists = (int64_t)s.splits * a.batch * a.kv_heads;
-  BMX_REQUIRE(lists * s.row_blocks < (1ll << 31), "cross_attention: too many blocks");
+  const int64_t threads = a.batch * a.kv_heads * a.rows * (a.dim / 4);  // of the join
+  BMX_REQUIRE(lists * s.row_blocks < (1ll << 31) && (s.splits < 2 || threads < 0xffffff00ll),
+              "cross_attention: too many blocks");
+  a.blocks = (uint32_t)(lists * s.row_blocks);
   a.part_o = (float*)workspace;
   a.part_ml = (float2*)((float*)workspace + lists * a.rows * a.dim);
   hipStream_t hs = (hipStream_t)stream;
   dtype == kF32 ? launch_dim<float>(a, s.few, hs) : launch_dim<bf16>(a, s.few, hs);
   if (s.splits > 1) {
-    const int64_t threads = a.batch * a.kv_heads * a.rows * (a.dim / 4);
     const dim3 grid((unsigned)((threads + 255) / 256));
     if (dtype == kF32)
       cross_attention_join<float><<<grid, 256, 0, hs>>>(a, bias != nullptr);

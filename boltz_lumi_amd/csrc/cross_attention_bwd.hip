@@ -44,7 +44,7 @@ struct RowAt {
 // delta: 16 lanes per row of [batch, m, heads], written as [batch][heads][m].
 template <typename T>
 __global__ __launch_bounds__(256) void cross_attention_delta(CrossArgs a) {
-  const int64_t at = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4), total = a.batch * a.m * a.heads;
+  const int64_t at = (int64_t)block_index() * 16 + (threadIdx.x >> 4), total = a.batch * a.m * a.heads;
   const int l = threadIdx.x & 15;
   float sum = 0.f;
   if (at < total) {
@@ -131,7 +131,8 @@ template <typename T, int DP, bool kBias, bool kExact>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dq(CrossArgs a) {
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
   __shared__ __attribute__((aligned(16))) char lds[4 * kTile + kMaskChunk / 8];
-  uint32_t at = xcd_position(blockIdx.x, gridDim.x);
+  if (block_index() >= a.blocks) return;
+  uint32_t at = xcd_position(block_index(), a.blocks);
   int64_t b = a.batch_first ? take(at, a.batch) : 0;
   const int row_block = take(at, a.row_blocks), split = take(at, a.splits), c = take(at, a.kv_heads);
   if (!a.batch_first) b = at;
@@ -237,7 +238,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   constexpr int kValues = 4 * kTile + 2 * kStat + 16;  // V of the block's 128 keys
   __shared__ __attribute__((aligned(16))) char lds[kValues + (kValuesInLds ? 4 * kTile : 0)];
   const int key_blocks = (a.n + 127) / 128;
-  uint32_t at = xcd_position(blockIdx.x, gridDim.x);
+  if (block_index() >= a.blocks) return;
+  uint32_t at = xcd_position(block_index(), a.blocks);
   int64_t b = a.batch_first ? take(at, a.batch) : 0;
   const int first = take(at, key_blocks) * 128, split = take(at, a.splits), c = take(at, a.kv_heads);
   if (!a.batch_first) b = at;
@@ -437,7 +439,8 @@ void cross_attention_dbias(CrossArgs a) {
   constexpr int kKeyTiles = kDouble ? 4 * kTile : 2 * kTile, kAll = kKeyTiles + 2 * kRowTile, kMasks = (KT + 63) / 64;
   __shared__ __attribute__((aligned(16))) char lds[kAll];
   const int key_blocks = (a.n + KT - 1) / KT, query_blocks = (int)((a.m + 127) / 128);
-  uint32_t at = xcd_position(blockIdx.x, gridDim.x);
+  if (block_index() >= a.blocks) return;
+  uint32_t at = xcd_position(block_index(), a.blocks);
   const int key = take(at, key_blocks) * KT, q0 = take(at, query_blocks) * 128;
   const int64_t ph = take(at, a.sdb[1] ? a.heads : 1), pb = at;
   const int64_t b0 = a.sdb[0] ? pb : 0, b1 = a.sdb[0] ? pb + 1 : a.batch;
@@ -649,18 +652,19 @@ int launch(CrossArgs& a, hipStream_t stream) {
   const int64_t bias_blocks = planes * ((a.m + 127) / 128) * ((a.n + KT - 1) / KT);
   const int64_t delta_blocks = (a.batch * a.m * a.heads + 15) / 16;
   const int64_t q_quads = a.batch * a.m * a.heads * a.dim / 4, k_quads = a.batch * a.n * a.kv_heads * a.dim / 4;
-  constexpr int64_t most = 1ll << 31;
+  constexpr int64_t most = 1ll << 31, threads = 0xffffff00ll;
   BMX_REQUIRE(lists * a.row_blocks * q.splits < most && lists * key_blocks * kv.splits < most && bias_blocks < most &&
-                  delta_blocks < most && q_quads / 256 < most - 1 && k_quads / 256 < most - 1,
+                  delta_blocks < most && (q.splits < 2 || q_quads < threads) && (kv.splits < 2 || k_quads < threads),
               "cross_attention_bwd: too many blocks");
-  cross_attention_delta<T><<<dim3((unsigned)delta_blocks), 256, 0, stream>>>(a);
+  cross_attention_delta<T><<<fold_grid(delta_blocks, 256), 256, 0, stream>>>(a);
   auto sum = [&](const Split& s, int64_t quads, void* out0, void* out1) {
     const dim3 grid((unsigned)((quads + 255) / 256), out1 ? 2 : 1);
     if (s.splits > 1) cross_attention_sum<<<grid, 256, 0, stream>>>(a.part_o, s.splits, quads, (T*)out0, (T*)out1);
   };
   if (a.dq) {
     a.splits = q.splits, a.split_keys = q.size;
-    const dim3 grid((unsigned)(lists * a.row_blocks * q.splits));
+    a.blocks = (uint32_t)(lists * a.row_blocks * q.splits);
+    const dim3 grid = fold_grid(a.blocks, 256);
     with_exact<T>(a, [&](auto exact) {
       constexpr bool kExact = decltype(exact)::value;
       a.bias ? cross_attention_dq<T, DP, true, kExact><<<grid, 256, 0, stream>>>(a)
@@ -670,7 +674,8 @@ int launch(CrossArgs& a, hipStream_t stream) {
   }
   if (a.dk || a.dv || (a.dbias && !shared)) {
     a.splits = kv.splits, a.split_keys = kv.size;
-    const dim3 grid((unsigned)(lists * key_blocks * kv.splits));
+    a.blocks = (uint32_t)(lists * key_blocks * kv.splits);
+    const dim3 grid = fold_grid(a.blocks, 256);
     with_exact<T>(a, [&](auto exact) {
       constexpr bool kExact = decltype(exact)::value;
       if (a.dbias && !shared)
@@ -682,7 +687,11 @@ int launch(CrossArgs& a, hipStream_t stream) {
     });
     sum(kv, k_quads, a.dk, a.dv);
   }
-  if (shared) cross_attention_dbias<T, DP><<<dim3((unsigned)bias_blocks), 64 * kBiasWaves<T, DP>, 0, stream>>>(a);
+  if (shared) {
+    constexpr int threads = 64 * kBiasWaves<T, DP>;
+    a.blocks = (uint32_t)bias_blocks;
+    cross_attention_dbias<T, DP><<<fold_grid(bias_blocks, threads), threads, 0, stream>>>(a);
+  }
   return check_launch("cross_attention_bwd");
 }
 

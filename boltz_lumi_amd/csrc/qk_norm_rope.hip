@@ -340,9 +340,9 @@ extern "C" int bmx_qk_norm_rope_fwd(const void* q, const void* k, int dtype, con
   // Four heads share a token's angles; a few tokens take one head a group, for the latency of one.
   const int64_t rows = batch * (s.q.tokens * s.q.heads + s.k.tokens * s.k.heads);
   const bool few = rows * lanes < 256 * 1024;
-  const int64_t most = 1 << 30;
+  const int64_t most = (1 << 24) - 1;  // a launch takes fewer than 2^32 threads
   const int64_t total = plan(s.q, batch, few ? 1 : 4, groups, most) + plan(s.k, batch, few ? 1 : 4, groups, most);
-  BMX_REQUIRE(total < most, "qk_norm_rope: too many rows");
+  BMX_REQUIRE(total <= most, "qk_norm_rope: too many rows");
   if (total == 0) return BMX_OK;
   hipStream_t hs = (hipStream_t)stream;
   if (dtype == kF32)

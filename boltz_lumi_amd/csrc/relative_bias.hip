@@ -125,10 +125,12 @@ __device__ __forceinline__ int64_t wave_extreme(int64_t v, bool largest) {
 template <typename T>
 __global__ __launch_bounds__(256) void relative_bias_bwd_kernel(Relative s, const T* dbias, int waves_across,
                                                                 int64_t row_blocks, int64_t col_blocks,
-                                                                float* partial) {
+                                                                uint32_t blocks, float* partial) {
   constexpr int V = 16 / sizeof(T);
   extern __shared__ int lds[];
   const int threads = blockDim.x, t = threadIdx.x;
+  const uint32_t block = block_index();
+  if (block >= blocks) return;
   int* edges = lds;
   uint8_t* lut = (uint8_t*)(lds + kMaxSide);
   float* bins = (float*)(lds + kMaxSide + kLut / 4);
@@ -140,7 +142,7 @@ __global__ __launch_bounds__(256) void relative_bias_bwd_kernel(Relative s, cons
   if (small)
     for (int i = t; i <= last; i += threads) lut[i] = (uint8_t)bucket_of(s, edges, -i);
   __syncthreads();
-  const int64_t cb = blockIdx.x % col_blocks, rest = blockIdx.x / col_blocks;
+  const int64_t cb = block % col_blocks, rest = block / col_blocks;
   const int64_t rb = rest % row_blocks, plane = rest / row_blocks, b = plane / s.heads;
   // The row blocks take rows in turn, so that rows near the diagonal, which cost more, are dealt to all of them.
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6), down = threads / 64 / waves_across;
@@ -209,7 +211,7 @@ __global__ __launch_bounds__(256) void relative_bias_bwd_kernel(Relative s, cons
     float v = 0.f;
     for (int i = lane; i < threads; i += 64) v += bins[c * threads + i];
     v = wave_sum_full(v);
-    if (lane == 0) partial[(int64_t)blockIdx.x * s.buckets + c] = v;
+    if (lane == 0) partial[(int64_t)block * s.buckets + c] = v;
   }
 }
 
@@ -324,15 +326,16 @@ extern "C" int bmx_relative_bias_bwd(const void* dbias, int dtype, int64_t bucke
                     workspace_bytes >= bmx_relative_bias_workspace_bytes(dtype, buckets, heads, batch, m, n),
                 "relative_bias_bwd: workspace too small or not 16-byte aligned");
     p = bwd_plan(dtype, buckets, batch * heads, m, n);
-    BMX_REQUIRE(p.blocks * batch * heads < (1ll << 31), "relative_bias_bwd: too many elements");
+    const int64_t blocks = p.blocks * batch * heads;
+    BMX_REQUIRE(blocks < (1ll << 31), "relative_bias_bwd: too many elements");
     const size_t lds = kMaxSide * 4 + kLut + (size_t)buckets * p.threads * 4;
-    const dim3 grid((unsigned)(p.blocks * batch * heads));
+    const dim3 grid = fold_grid(blocks, p.threads);
     if (dtype == kF32)
       relative_bias_bwd_kernel<float><<<grid, p.threads, lds, hs>>>(s, (const float*)dbias, p.across, p.row_blocks,
-                                                                    p.col_blocks, (float*)workspace);
+                                                                    p.col_blocks, (uint32_t)blocks, (float*)workspace);
     else
       relative_bias_bwd_kernel<bf16><<<grid, p.threads, lds, hs>>>(s, (const bf16*)dbias, p.across, p.row_blocks,
-                                                                   p.col_blocks, (float*)workspace);
+                                                                   p.col_blocks, (uint32_t)blocks, (float*)workspace);
   }
   const dim3 grid((unsigned)(heads * buckets));
   const int64_t rows = any ? batch : 0;  // nothing to sum: a gradient of zeros
