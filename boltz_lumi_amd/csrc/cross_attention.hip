@@ -449,7 +449,8 @@ int cross_setup(CrossArgs& a, int dtype, const int64_t* shape, const int64_t* st
               "cross_attention: the query heads must be a multiple of the key heads");
   const int64_t rows = heads / kv * a.m;
   BMX_REQUIRE(a.batch < (1ll << 31) && a.m < (1ll << 31) && rows < (1ll << 30), "cross_attention: too many query rows");
-  BMX_REQUIRE(scale > 0.f && scale < INFINITY, "cross_attention: scale must be positive and finite");
+  // Its product with log2(e) is a number that fp32 holds to all its bits (denormals are flushed).
+  BMX_REQUIRE(scale >= 0x1p-126f && scale <= 0x1p127f, "cross_attention: scale must be in [2^-126, 2^127]");
   const int vec = dtype == kF32 ? 4 : 8;
   for (int i = 0; i < 3; ++i) {
     a.sq[i] = strides[i], a.sk[i] = strides[3 + i], a.sv[i] = strides[6 + i], a.sb[i] = has_bias ? strides[10 + i] : 0;

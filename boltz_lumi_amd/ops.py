@@ -1531,17 +1531,17 @@ def cross_attention(q, k, v, mask=None, bias=None, scale=None):
     copied.  mask: bool [B, N] (or [1, N], [N]), True for the keys that take
     part; the others' values are never looked at, NaN or not.  bias: q's type,
     [B or 1, H or 1, M, N], added to the logits; -inf leaves a pair out.  A
-    query without keys gives zeros, and zero gradients.  scale: positive,
-    1 / sqrt(D) by default.  Sums are fp32; bf16 weights enter the products with
-    16 bits in decoding steps (M H / Hk <= 32), over up to 256 keys and where a
-    batch element is small (H M N D <= 2^28), else with 8, whose error is about
-    1.4 times that of rounding the result.
-    Gradients reach q, k, v and bias (summed over its shared axes in fp32) and
-    are the same bits on every run."""
+    query without keys gives zeros, and zero gradients.  scale: positive
+    (2^-126 to 2^127), 1 / sqrt(D) by default.  Sums are fp32; bf16 weights
+    enter the products with 16 bits in decoding steps (M H / Hk <= 32), over up
+    to 256 keys and where a batch element is small (H M N D <= 2^28), else with
+    8, whose error is about 1.4 times that of rounding the result.  Gradients
+    reach q, k, v and bias (summed over its shared axes in fp32) and are the
+    same bits on every run."""
     dev = _same_device(q, k, v, mask, bias)
     plan = _cross_plan(_layout(q), _layout(k), _layout(v), _layout(mask), _layout(bias))
     scale = plan.scale if scale is None else float(scale)
-    _check(0 < scale < float("inf"), "scale must be positive and finite")
+    _check(2.0 ** -126 <= scale <= 2.0 ** 127, "scale must be positive and finite, in [2^-126, 2^127]")
     if not (all(plan.ok) and plan.mask_ok and plan.bias_ok) or (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
         q, k, v = (t if ok and t.data_ptr() % 16 == 0 else _aligned(t.contiguous()) for t, ok in zip((q, k, v), plan.ok))
         mask = mask if plan.mask_ok else mask.contiguous()

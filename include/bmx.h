@@ -453,7 +453,7 @@ int bmx_relative_bias_bwd(const void* dbias, int dtype, int64_t buckets, int64_t
  * of 16 bytes, the last axis dense; a token's in [0, 2^22), as heads * dim), the mask's batch stride (0: shared), the bias's batch, head and
  * query strides (any, the query's in [0, 2^26); 0: shared; keys dense).  mask: bytes [n] per batch element, 0 = the key (whatever its
  * values) is left out, or NULL; bias in dtype or NULL.  A row without keys gives zeros.  batch, m or n may be 0.
- * out dense [batch, m, heads, dim].  scale positive.  bf16 weights have 16 bits in decoding steps (at most 32 rows
+ * out dense [batch, m, heads, dim].  scale in [2^-126, 2^127].  bf16 weights have 16 bits in decoding steps (at most 32 rows
  * m * heads / kv_heads), up to 256 keys and for small elements (heads * m * n * dim <= 2^28), otherwise 8.
  * For the backward pass, or NULL: out_lo (bf16 only, out's shape: what rounding out left),
  * stats fp32 [batch, heads, m, 2], for bmx_cross_attention_bwd alone: a reference point r of the row (a logit at or, in

@@ -49,3 +49,16 @@ def test_table_gradient_blocks(lib):
     size = lib.bmx_relative_bias_workspace_bytes(N.F32, 4, heads, batch, 1, 1)
     rc = lib.bmx_relative_bias_bwd(FAKE, N.F32, 4, heads, FAKE, FAKE, 1, batch, 1, 1, 1, 1, edges, 1, 1, FAKE, FAKE, size, None)
     assert refused(lib, rc, b"too many elements")
+
+
+def test_attention_scale(lib):
+    """A scale that fp32 flushes to zero, or whose product with log2(e) it cannot hold, made every result NaN."""
+    def fwd(scale):
+        return lib.bmx_cross_attention_fwd(FAKE, FAKE, FAKE, None, None, N.BF16, N.int64_array((1, 0, 2, 1, 1, 8)),
+                                           N.int64_array((8, 8, 8, 16, 8, 8, 16, 8, 8, 0, 0, 0, 0)), scale, FAKE, None, None,
+                                           None, 0, None)
+
+    for scale in (1e-40, 2.0 ** -127, 3e38, -1.0):
+        assert refused(lib, fwd(scale), b"scale")
+    for scale in (2.0 ** -126, 2.0 ** 127, 0.125):
+        assert fwd(scale) == N.BMX_OK  # without queries nothing is launched
