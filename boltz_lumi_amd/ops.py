@@ -1152,9 +1152,12 @@ def adaln_modulate(a, scale, shift, eps):
 # Differentiable (torch.autograd; one backward pass, no double backward).  A
 # call that needs no gradient does not go through autograd.  Forward-mode
 # derivatives and tracing are refused: neither sees a native launch, so the
-# result would have no tangent, or be an empty tensor in the trace.  In a captured
-# graph make the leaves inside or before the capture and take the gradients
-# with torch.autograd.grad, as for torch's own operators.
+# result would have no tangent, or be an empty tensor in the trace.  To capture
+# a backward pass in a graph, make its leaves inside the capture
+# (``t.detach().requires_grad_()``) and take the gradients with
+# torch.autograd.grad.  A leaf from before it must not belong to an eager graph
+# that is still alive: that graph's stream enters the capture and ends the
+# process, as with torch's own operators.
 
 
 def _needs_grad(*tensors) -> bool:
