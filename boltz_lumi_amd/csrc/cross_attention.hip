@@ -199,7 +199,7 @@ void cross_attention_wide(CrossArgs a) {
   cv.init(w, a.dim, a.sv[1]);
   const unsigned lds0 = lds_address(lds);
   clear_tiles<T, DP, 256>(t, lds, 4 * kTile, a.dim);
-  const int chunk = a.mask ? kMaskChunk : a.n;
+  const int chunk = a.mask ? kMaskChunk : p.stop - p.first;  // c0 + chunk stays below 2^31, as the keys do
   for (int c0 = p.first; c0 < p.stop; c0 += chunk) {
     words.fill(c0, p.stop);  // its barrier also ends the last chunk's reads of the tiles
     const int end = min(c0 + chunk, p.stop);

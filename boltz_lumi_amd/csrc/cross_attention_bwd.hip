@@ -162,7 +162,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
   cv.init(w, a.dim, a.sv[1]);
   const unsigned lds0 = lds_address(lds);
   clear_tiles<T, DP, 256>(t, lds, 4 * kTile, a.dim);
-  const int chunk = a.mask ? kMaskChunk : a.n;
+  const int chunk = a.mask ? kMaskChunk : stop - first;
   for (int c0 = first; c0 < stop; c0 += chunk) {
     words.fill(c0, stop);  // its barrier also ends the last chunk's reads of the tiles
     const int end = min(c0 + chunk, stop);
