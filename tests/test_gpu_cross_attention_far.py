@@ -131,3 +131,54 @@ def test_large_logits(gpu, dtype, shape, power, scale):
         s = torch.matmul(q.double().transpose(1, 2), k.double().permute(0, 2, 3, 1).repeat_interleave(h // hk, 1))
         want = formula(s * scale, q, k, v, scale, dout)
     compare((out.detach(), *grads), want, shape == LARGE)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_minus_infinity(gpu, dtype, shape):
+    """-inf over the same patterns: whole rows give zeros and zero gradients, whatever tiles, waves or splits hold one."""
+    print(f"bias of -inf {shape} {dtype}", flush=True)
+    b, m, n, h, hk, d = shape
+    g = torch.Generator(device=gpu).manual_seed(m + n)
+    q, k = whole(g, b, m, h, d, dtype=dtype), whole(g, b, n, hk, d, dtype=dtype)
+    v, dout = (torch.randn(b, t, x, d, generator=g, device=gpu).to(dtype) for t, x in ((n, hk), (m, h)))
+    pick = (torch.arange(h, device=gpu)[:, None] + torch.arange(m, device=gpu)) % 8
+    bias = torch.where(patterns(n, gpu)[pick], -torch.inf, whole(g, h, m, n, dtype=torch.float32) / 4).to(dtype)[None]
+    leaves = [t.requires_grad_() for t in (q, k, v, bias)]
+    out = ops.cross_attention(q, k, v, bias=bias, scale=0.125)
+    grads = torch.autograd.grad(out, leaves, dout)
+    with torch.no_grad():
+        s = torch.matmul(q.double().transpose(1, 2), k.double().permute(0, 2, 3, 1).repeat_interleave(h // hk, 1))
+        x = s * 0.125 + bias.double()
+        empty = (x == -torch.inf).all(-1, keepdim=True)
+        want = formula(torch.where(empty, 0.0, x), q, k, v, 0.125, torch.where(empty.transpose(1, 2), 0.0, dout))
+        want["out"] = [torch.where(empty.transpose(1, 2), 0.0, t) for t in want["out"]]
+    want["dbias"] = [t.sum(0, keepdim=True) for t in want["dbias"]]
+    compare((out.detach(), *grads), want, shape == LARGE)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("form", [(0, 1), (1, 1), (1, 0)])  # of the bias: per batch element, per head
+def test_a_left_out_keys_bias_is_never_looked_at(gpu, dtype, shape, form):
+    print(f"bias of left-out keys {shape} {form} {dtype}", flush=True)
+    b, m, n, h, hk, d = shape
+    g = torch.Generator(device=gpu).manual_seed(m + n)
+    q, k, v = (torch.randn(b, t, x, d, generator=g, device=gpu).to(dtype) for t, x in ((m, h), (n, hk), (n, hk)))
+    mask = torch.rand(b, n, generator=g, device=gpu) < 0.6
+    mask[:, :40] = False
+    mask[-1] &= b == 1
+    both = mask if form[0] else mask.any(0, keepdim=True)  # keys of some element that shares the bias
+    bias = torch.randn(b if form[0] else 1, h if form[1] else 1, m, n, generator=g, device=gpu).to(dtype)
+    dout = torch.randn(b, m, h, d, generator=g, device=gpu).to(dtype)
+
+    def run(bias):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, bias)]
+        out = ops.cross_attention(*leaves[:3], mask, leaves[3])
+        return out.detach(), *torch.autograd.grad(out, leaves, dout)
+
+    clean = run(bias)
+    for value in (torch.nan, torch.inf, torch.finfo(dtype).min):
+        dirty = run(torch.where(both[:, None, None], bias, value))
+        assert all(torch.equal(x, y) for x, y in zip(clean, dirty)), value
+    assert torch.isfinite(clean[-1]).all() and not clean[-1].masked_select(~both[:, None, None]).any()
