@@ -125,8 +125,8 @@ __device__ __forceinline__ void weights_of(const CrossArgs& a, f32x16& s, const 
   }
 }
 
-// dQ: four waves of 32 rows over all keys, as the forward pass runs (batch 2, 32 / 8 heads, 2048 x 4096, D = 128: 370 us,
-// 1110 TF/s).
+// dQ: four waves of 32 rows over all keys, as the forward pass runs (batch 2, 32 / 8 heads, 2048 x 4096, D = 128: 377 us,
+// 1090 TF/s; the choice of far rows costs 1 to 3%).
 template <typename T, int DP, bool kBias, bool kExact>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dq(CrossArgs a) {
   constexpr int kTile = 32 * Tile<T, DP>::kRowBytes;
@@ -226,9 +226,11 @@ __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_
 // Queries past the last repeat it with weights of zero. A wave's K, and V for narrow heads, are in registers;
 // bf16 heads past 64 channels keep V in LDS, which makes room for two waves on a SIMD.
 // A bias of its own for every head and batch element has its gradient written here, as dS is at hand (kGrad).
-// Bound by the MFMA (batch 2, 32 / 8 heads, 2048 x 4096, D = 128: 512 us, 1070 TF/s), with a bias by
+// Bound by the MFMA (batch 2, 32 / 8 heads, 2048 x 4096, D = 128: 518 us, 1060 TF/s), with a bias by
 // the work between the products at two waves a SIMD (batch 5, 16 heads, 1024 x 1531, D = 64: 116 us, 550 TF/s; its 16
-// two-byte loads a lane are not it: whole runs of keys turned through LDS took 124).
+// two-byte loads a lane are not it: whole runs of keys turned through LDS took 124). Two waves a SIMD leave 256
+// registers: bf16 with D = 128 spills 3 of them, 11 with 16-bit weights and 20 to 39 with a bias, fp32 with D = 64
+// and a shared bias 26.
 template <typename T, int DP, bool kBias, bool kGrad, bool kExact>
 __global__ __launch_bounds__(256, sizeof(T) == 4 && DP > 64 ? 1 : 2) void cross_attention_dkv(CrossArgs a) {
   constexpr bool kValuesInLds = sizeof(T) == 2 && DP > 64;

@@ -109,7 +109,7 @@ __global__ __launch_bounds__(256) void relative_bias_kernel(Relative s, const U*
 // consecutive threads in consecutive banks). Nothing is shared, so there is no atomic and the order of every
 // sum is fixed. A distance's bucket comes from a byte table where the last threshold is below kLut. The bound is the
 // read of dbias (16 heads, 2048 x 2048, fp32, 268 MB: 72 us, 3.7 TB/s, as a plain sum over it; right behind the forward
-// pass, whose result is then still on its way to HBM, 105; LDS atomics instead of own bins 350).
+// pass, whose result is then still on its way to HBM, 110; LDS atomics instead of own bins 350).
 constexpr int kLut = 2048, kAhead = 4;
 
 __device__ __forceinline__ int64_t wave_extreme(int64_t v, bool largest) {

@@ -1434,7 +1434,8 @@ def relative_bias(table, q_pos, k_pos, exact=None, max_distance=128, bidirection
     by n = |d|; otherwise all hold n = max(-d, 0).  Distances below ``exact``
     (default side // 2) have a bucket each; the others share the rest by
     logarithm, ``exact + floor(log(n / exact) / log(max_distance / exact) *
-    (side - exact))``, the last from ``max_distance`` on.  ``exact = side - 1``
+    (side - exact))``, at most the last one: it begins below ``max_distance``
+    and holds everything from there on.  ``exact = side - 1``
     is the clipped form (every distance its own bucket up to side - 1).
     Positions are int32 / int64, |pos| < 2^62, in any order.  The gradient
     reaches the table (fp32 sums, the same bits on every run)."""

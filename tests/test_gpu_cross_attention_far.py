@@ -81,7 +81,7 @@ SHAPES = [  # batch, m, n, heads, kv_heads, dim
     (1, 520, 1031, 8, 4, 64),  # bf16 weights of 8 bits
 ]
 LARGE = SHAPES[-1]
-VALUES = [-1e4, -1e6, -1e9, -1e10, -1e30, -9e37, -3.3e38, 1e6, 1e9, 1e30]
+VALUES = [-1e4, -1e6, -1e8, -4e8, -1e9, -1e10, -1e30, -9e37, -3.3e38, 1e6, 3e8, 1e9, 1e30]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
