@@ -300,7 +300,7 @@ int setup(NormRope& s, int dtype, const int64_t* shape, const int64_t* strides, 
   BMX_REQUIRE(half >= 0 && half % 4 == 0 && 2 * half <= dim,
               "qk_norm_rope: the rotated pairs must be a multiple of 4, at most half the head dim");
   BMX_REQUIRE(half == 0 || inv_freq, "qk_norm_rope: null inv_freq");
-  BMX_REQUIRE(eps > 0.f, "qk_norm_rope: eps must be positive");
+  BMX_REQUIRE(eps >= 0x1p-126f, "qk_norm_rope: eps must be positive, at least 2^-126");  // below it is flushed to zero
   BMX_REQUIRE(shape[3] < (1 << 20) && shape[4] < (1 << 20), "qk_norm_rope: too many heads");
   for (int i = 0; i < 6; ++i) BMX_REQUIRE(strides[i] % 4 == 0, "qk_norm_rope: strides must be multiples of 4");
   s.inv_freq = inv_freq, s.inv_freq64 = inv_freq64, s.pos64 = pos64, s.w_bf16 = w_dtype == kBF16;

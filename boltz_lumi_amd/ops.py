@@ -1333,7 +1333,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq, eps=1e-6, int
         q_pos, k_pos = q_pos.contiguous(), None if k_pos is None else k_pos.contiguous()
         inv_freq = inv_freq.contiguous()
     dev = _same_device(q, k, q_weight, k_weight, q_pos, k_pos, inv_freq)
-    _check(eps > 0, "eps must be positive")
+    _check(eps >= 2.0 ** -126, "eps must be positive, at least 2^-126")
     plan = _norm_rope_plan(_layout(q), _layout(k), _layout(q_weight), _layout(k_weight), _layout(q_pos), _layout(k_pos),
                            _layout(inv_freq))
     if not plan.q_ok or q.data_ptr() % plan.unit or not plan.k_ok or (k is not None and k.data_ptr() % plan.unit):

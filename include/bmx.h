@@ -411,7 +411,7 @@ int bmx_seq_attention_x3_batched_split_fwd(const float* q, const float* k, const
  * and k [batch, n, kv_heads, dim].  shape = {batch, m, n, heads, kv_heads, dim}; strides = {q's batch,
  * token, head; k's; q_pos's and k_pos's batch stride (0: shared)}, the last axis dense; x strides
  * multiples of 4.  R turns the channel pairs (i, half + i) (interleaved: (2 i, 2 i + 1)), i < half, by
- * pos * inv_freq[i] (product in 64 bits); other channels pass.  dim a multiple of 8 in [8, 256],
+ * pos * inv_freq[i] (product in 64 bits); other channels pass.  eps at least 2^-126.  dim a multiple of 8 in [8, 256],
  * half of 4.  Weights [dim] in w_dtype or NULL (1); positions int32 / int64 [m] / [n] per batch element;
  * inv_freq fp32 / fp64 [half].  Outputs and gradients dense.  Tensors aligned to 4 elements, weights
  * to 16 bytes.  n or m may be 0.  No reference kernel. */

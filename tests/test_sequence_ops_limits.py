@@ -62,3 +62,14 @@ def test_attention_scale(lib):
         assert refused(lib, fwd(scale), b"scale")
     for scale in (2.0 ** -126, 2.0 ** 127, 0.125):
         assert fwd(scale) == N.BMX_OK  # without queries nothing is launched
+
+
+def test_norm_rope_eps(lib):
+    """An eps that fp32 flushes to zero made rows of zeros NaN."""
+    def fwd(eps):
+        return lib.bmx_qk_norm_rope_fwd(FAKE, None, N.BF16, N.int64_array((1, 0, 0, 1, 0, 8)),
+                                        N.int64_array((0, 8, 8, 0, 0, 0, 0, 0)), None, None, N.BF16, None, None, 1, None, 1, 0,
+                                        0, eps, FAKE, None, None)
+
+    assert all(refused(lib, fwd(eps), b"eps") for eps in (1e-40, 2.0 ** -127, -1e-6, float("nan")))
+    assert fwd(2.0 ** -126) == N.BMX_OK and fwd(1e-6) == N.BMX_OK
