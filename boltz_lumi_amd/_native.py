@@ -25,6 +25,8 @@ _I64P = ctypes.POINTER(c_int64)
 _NORM_ROPE = [_P, _P, c_int, _I64P, _I64P, _P, _P, c_int, _P, _P, c_int, _P, c_int, c_int64, c_int, c_float]
 _RELATIVE = [_P, c_int, c_int64, c_int64, _P, _P, c_int] + [c_int64] * 5 + [_P, c_int, c_int]
 _CROSS = [_P, _P, _P, _P, _P, c_int, _I64P, _I64P, c_float]
+_FRAME = [_P, _P, _P, c_int, c_int, _I64P, _I64P, c_int, _P, _P, _P, c_int, c_int, c_int, c_float]
+_CONV = [_P, c_int, _I64P, _I64P, _P, c_int, _P, c_int, _P, _P, c_int, c_int]
 
 # name -> (restype, argtypes); mirrors include/bmx.h
 SIGNATURES = {
@@ -95,6 +97,17 @@ SIGNATURES = {
     "bmx_cross_attention_fwd": (c_int, _CROSS + [_P, _P, _P, _P, c_size_t, _P]),
     "bmx_cross_attention_bwd_workspace_bytes": (c_size_t, [c_int64] * 6),
     "bmx_cross_attention_bwd": (c_int, _CROSS + [_P] * 8 + [_I64P, _P, c_size_t, _P]),
+    "bmx_residual_norm_fwd": (c_int, _FRAME + [_P, _P, _P]),
+    "bmx_residual_norm_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int]),
+    "bmx_residual_norm_bwd": (c_int, _FRAME + [_P] * 9 + [c_size_t, _P]),
+    "bmx_causal_conv_fwd": (c_int, _CONV + [_P, _P, _P]),
+    "bmx_causal_conv_workspace_bytes": (c_size_t, [c_int64] * 4),
+    "bmx_causal_conv_bwd": (c_int, _CONV + [_P] * 7 + [c_size_t, _P]),
+    "bmx_selective_scan_saved_bytes": (c_size_t, [c_int64] * 4),
+    "bmx_selective_scan_workspace_bytes": (c_size_t, [c_int64] * 5),
+    "bmx_selective_scan_fwd": (c_int, [_P] * 10 + [c_int, c_int, _I64P, _I64P, c_int] + [_P] * 5 + [c_size_t, _P]),
+    "bmx_selective_scan_bwd_workspace_bytes": (c_size_t, [c_int64] * 5),
+    "bmx_selective_scan_bwd": (c_int, [_P] * 9 + [c_int, c_int, _I64P, _I64P, c_int] + [_P] * 14 + [c_size_t, _P]),
 }
 
 

@@ -1,0 +1,468 @@
+// The frame between two blocks of a sequence stack in one pass: RMS norm of the
+// block's result y, its gate and residual scale, the residual add and the next
+// block's RMS norm; and its gradient.
+//
+//   m = y rho_y yw,  rho_y = 1 / sqrt(mean(y^2) + eps)   (without the norm: m = y)
+//   r = x + scale s m,  s = sigmoid(gate)
+//   h = r rho_r w,  rho_r = 1 / sqrt(mean(r^2) + eps)
+//   e = dh w:  dR = dr + rho_r (e - r rho_r^2 mean(e r)) = dx;  dw = sum dh r rho_r
+//   f = dR s scale yw:  dy = rho_y (f - y rho_y^2 mean(f y))
+//   dscale = sum dR s m;  dgate = dR scale m s (1 - s);  dyw = sum dR s scale y rho_y
+//
+// A row lies in the registers of L threads, V runs of 8 channels each, from its
+// only read to its only write; the backward pass works r and both norms out
+// again instead of keeping them.  h comes from r before its rounding.  All sums
+// are fp32 and in a fixed order.
+#include <type_traits>
+
+#include "bmx_common.h"
+
+using namespace bmx;
+
+namespace {
+
+constexpr int kMaxDim = 8192;
+constexpr int kBwdBlocks = 512;  // of the gradient: each leaves a partial row per weight
+
+struct Rows {
+  const void* p;
+  int64_t sb, st;  // strides of a batch element and a token, in elements
+};
+struct Frame {
+  Rows x, y, gate;
+  const void *yw, *scale, *w, *dr, *dh;
+  void *r, *h, *dx, *dy, *dgate;
+  float *partial, *gate_partial;  // [blocks][3][dim] sums for yw, scale, w; [units][dim] for a shared gate
+  int64_t rows, tokens, units, unit_rows, splits;  // units: runs of rows, `splits` per batch element where it has its gate
+  int dim, w_bf16, post, pre, shared;
+  float eps, inv_dim;
+};
+
+// 8 consecutive values as fp32, and back.
+struct Oct {
+  f32x4 a, b;
+};
+__device__ __forceinline__ Oct load_oct(const float* p) { return {*(const f32x4*)p, *(const f32x4*)(p + 4)}; }
+__device__ __forceinline__ Oct load_oct(const bf16* p) {
+  const bf16x8 v = *(const bf16x8*)p;
+  return {f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]},
+          f32x4{(float)v[4], (float)v[5], (float)v[6], (float)v[7]}};
+}
+__device__ __forceinline__ void store_oct(float* p, const Oct& v) { *(f32x4*)p = v.a, *(f32x4*)(p + 4) = v.b; }
+__device__ __forceinline__ void store_oct(bf16* p, const Oct& v) {
+  *(bf16x8*)p = bf16x8{(bf16)v.a[0], (bf16)v.a[1], (bf16)v.a[2], (bf16)v.a[3],
+                       (bf16)v.b[0], (bf16)v.b[1], (bf16)v.b[2], (bf16)v.b[3]};
+}
+__device__ __forceinline__ Oct fill(float v) { return {f32x4{v, v, v, v}, f32x4{v, v, v, v}}; }
+__device__ __forceinline__ Oct operator*(const Oct& x, const Oct& y) { return {x.a * y.a, x.b * y.b}; }
+__device__ __forceinline__ Oct operator+(const Oct& x, const Oct& y) { return {x.a + y.a, x.b + y.b}; }
+__device__ __forceinline__ Oct operator-(const Oct& x, const Oct& y) { return {x.a - y.a, x.b - y.b}; }
+__device__ __forceinline__ Oct operator*(const Oct& x, float s) { return {x.a * s, x.b * s}; }
+__device__ __forceinline__ float dot(const Oct& x, const Oct& y) {
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v += x.a[i] * y.a[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v += x.b[i] * y.b[i];
+  return v;
+}
+__device__ __forceinline__ Oct sigmoid(const Oct& x) {
+  Oct o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o.a[i] = sigmoid_f(x.a[i]), o.b[i] = sigmoid_f(x.b[i]);
+  return o;
+}
+__device__ __forceinline__ Oct load_weight(const void* w, int w_bf16, int at) {
+  if (!w) return fill(1.f);
+  return w_bf16 ? load_oct((const bf16*)w + at) : load_oct((const float*)w + at);
+}
+
+// Sum over the L threads of a row, in every one of them.  Rows of several waves meet in LDS: `turn` alternates
+// between two buffers, so that one barrier a sum is enough.
+template <int L>
+__device__ __forceinline__ float row_sum(float v, float (&lds)[2][8], int& turn) {
+  if (L == 16) {
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    v += dpp<0x140>(v);
+    return v;
+  }
+  v = wave_sum_full(v);
+  if (L == 64) return v;
+  if (lane_id() == 0) lds[turn][threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0.f;
+#pragma unroll
+  for (int i = 0; i < L / 64; ++i) v += lds[turn][i];
+  turn ^= 1;
+  return v;
+}
+
+template <int L>
+constexpr int threads_of() {
+  return L > 256 ? L : 256;
+}
+
+__device__ __forceinline__ float rho(float sum, const Frame& s) { return 1.f / sqrtf(sum * s.inv_dim + s.eps); }
+
+template <typename X, typename Y, int L, int V>
+__global__ __launch_bounds__(threads_of<L>()) void residual_norm_kernel(Frame s) {
+  __shared__ float lds[2][8];
+  int turn = 0;
+  const int lane = threadIdx.x % L;
+  const int64_t row = (int64_t)block_index() * (threads_of<L>() / L) + threadIdx.x / L;
+  if (row >= s.rows) return;  // whole rows leave; a row of several waves is its block's only one
+  const int64_t b = row / s.tokens, t = row - b * s.tokens;
+  const X* x = (const X*)s.x.p + b * s.x.sb + t * s.x.st;
+  const Y* y = (const Y*)s.y.p + b * s.y.sb + t * s.y.st;
+  const Y* gate = s.gate.p ? (const Y*)s.gate.p + b * s.gate.sb + t * s.gate.st : nullptr;
+  Oct xv[V], m[V], g[V];
+  float sum = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = 8 * (lane + v * L);
+    const bool live = c < s.dim;
+    xv[v] = live ? load_oct(x + c) : fill(0.f);
+    m[v] = live ? load_oct(y + c) : fill(0.f);
+    g[v] = live && gate ? load_oct(gate + c) : fill(0.f);
+    sum += dot(m[v], m[v]);
+  }
+  const float ry = s.post ? rho(row_sum<L>(sum, lds, turn), s) : 1.f;
+  sum = 0.f;
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = 8 * (lane + v * L);
+    if (c >= s.dim) continue;
+    Oct k = load_weight(s.scale, s.w_bf16, c);
+    if (gate) k = k * sigmoid(g[v]);
+    xv[v] = xv[v] + m[v] * ry * load_weight(s.yw, s.w_bf16, c) * k;
+    sum += dot(xv[v], xv[v]);
+    store_oct((X*)s.r + row * s.dim + c, xv[v]);
+  }
+  if (!s.pre) return;
+  const float rr = rho(row_sum<L>(sum, lds, turn), s);
+#pragma unroll
+  for (int v = 0; v < V; ++v) {
+    const int c = 8 * (lane + v * L);
+    if (c < s.dim) store_oct((Y*)s.h + row * s.dim + c, xv[v] * rr * load_weight(s.w, s.w_bf16, c));
+  }
+}
+
+// Gradient.  A block walks units of rows, its L-thread groups taking every (256 / L)-th row of a unit; each thread
+// keeps the weights' sums of its channels over all of them, a shared gate's over the unit.
+template <typename X, typename Y, int L, int V>
+__global__ __launch_bounds__(threads_of<L>()) void residual_norm_bwd_kernel(Frame s) {
+  constexpr int groups = threads_of<L>() / L;
+  __shared__ float lds[2][8];
+  __shared__ float sums[groups > 1 ? groups : 1][groups > 1 ? 8 * L * V : 1];
+  int turn = 0;
+  const int lane = threadIdx.x % L, group = threadIdx.x / L;
+  Oct dyw[V], dscale[V], dw[V], dgate[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) dyw[v] = dscale[v] = dw[v] = dgate[v] = fill(0.f);
+
+  // The groups' sums of one quantity, added in their order, to `out` (its row of dim values).
+  auto put = [&](const Oct (&v)[V], auto* out) {
+    if constexpr (groups == 1) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (8 * (lane + i * L) < s.dim) store_oct(out + 8 * (lane + i * L), v[i]);
+      return;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i) store_oct(&sums[group][8 * (lane + i * L)], v[i]);
+    __syncthreads();
+    for (int c = threadIdx.x; c < s.dim; c += threads_of<L>()) {
+      float total = 0.f;
+#pragma unroll
+      for (int i = 0; i < groups; ++i) total += sums[i][c];
+      using Out = std::remove_pointer_t<decltype(out)>;
+      out[c] = (Out)total;
+    }
+  };
+
+  for (int64_t unit = blockIdx.x; unit < s.units; unit += gridDim.x) {
+    const int64_t element = s.shared ? unit / s.splits : 0, part = s.shared ? unit % s.splits : unit;
+    const int64_t limit = s.shared ? s.tokens : s.rows;
+    const int64_t first = part * s.unit_rows, last = min(first + s.unit_rows, limit);
+    for (int64_t i = first + group; i < last; i += groups) {
+      const int64_t row = element * s.tokens + i, b = row / s.tokens, t = row - b * s.tokens;
+      const X* x = (const X*)s.x.p + b * s.x.sb + t * s.x.st;
+      const Y* y = (const Y*)s.y.p + b * s.y.sb + t * s.y.st;
+      const Y* gate = s.gate.p ? (const Y*)s.gate.p + b * s.gate.sb + t * s.gate.st : nullptr;
+      Oct r[V], n[V], g[V], dr[V], dh[V];
+      float sum = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = 8 * (lane + v * L);
+        const bool live = c < s.dim;
+        r[v] = live ? load_oct(x + c) : fill(0.f);
+        n[v] = live ? load_oct(y + c) : fill(0.f);
+        g[v] = live && gate ? load_oct(gate + c) : fill(0.f);
+        dr[v] = live && s.dr ? load_oct((const X*)s.dr + row * s.dim + c) : fill(0.f);
+        dh[v] = live && s.dh ? load_oct((const Y*)s.dh + row * s.dim + c) : fill(0.f);
+        sum += dot(n[v], n[v]);
+      }
+      const float ry = s.post ? rho(row_sum<L>(sum, lds, turn), s) : 1.f;
+      float rr = 0.f, er = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = 8 * (lane + v * L);
+        if (c >= s.dim) continue;
+        if (gate) g[v] = sigmoid(g[v]);
+        Oct k = load_weight(s.scale, s.w_bf16, c);
+        if (gate) k = k * g[v];
+        n[v] = n[v] * ry;
+        r[v] = r[v] + n[v] * load_weight(s.yw, s.w_bf16, c) * k;
+        rr += dot(r[v], r[v]);
+        er += dot(dh[v] * load_weight(s.w, s.w_bf16, c), r[v]);
+      }
+      if (s.pre) {
+        rr = rho(row_sum<L>(rr, lds, turn), s);
+        er = row_sum<L>(er, lds, turn) * s.inv_dim * rr * rr;
+      }
+      float fn = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = 8 * (lane + v * L);
+        if (c >= s.dim) continue;
+        if (s.pre) {
+          dr[v] = dr[v] + (dh[v] * load_weight(s.w, s.w_bf16, c) - r[v] * er) * rr;
+          dw[v] = dw[v] + dh[v] * r[v] * rr;
+        }
+        if (s.dx) store_oct((X*)s.dx + row * s.dim + c, dr[v]);
+        const Oct yw = load_weight(s.yw, s.w_bf16, c), scale = load_weight(s.scale, s.w_bf16, c);
+        const Oct gated = gate ? dr[v] * g[v] : dr[v];  // dR s
+        dscale[v] = dscale[v] + gated * n[v] * yw;
+        if (gate) {
+          const Oct dg = gated * scale * n[v] * yw * (fill(1.f) - g[v]);
+          if (s.shared)
+            dgate[v] = dgate[v] + dg;
+          else if (s.dgate)
+            store_oct((Y*)s.dgate + row * s.dim + c, dg);
+        }
+        const Oct back = gated * scale;
+        dyw[v] = dyw[v] + back * n[v];
+        dr[v] = back * yw;
+        fn += dot(dr[v], n[v]);
+      }
+      if (s.post) fn = row_sum<L>(fn, lds, turn) * s.inv_dim;
+      if (s.dy) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          const int c = 8 * (lane + v * L);
+          if (c < s.dim)
+            store_oct((Y*)s.dy + row * s.dim + c, s.post ? (dr[v] - n[v] * fn) * ry : dr[v]);
+        }
+      }
+    }
+    if (s.shared && s.dgate) {
+      if (s.splits == 1)
+        put(dgate, (Y*)s.dgate + unit * s.dim);
+      else
+        put(dgate, s.gate_partial + unit * s.dim);
+#pragma unroll
+      for (int v = 0; v < V; ++v) dgate[v] = fill(0.f);
+    }
+  }
+  if (!s.partial) return;
+  float* out = s.partial + (int64_t)blockIdx.x * 3 * s.dim;
+  put(dyw, out);
+  put(dscale, out + s.dim);
+  put(dw, out + 2 * s.dim);
+}
+
+// Column sums of partial rows: a block per 16 columns of one result, 16 threads over the rows of each.
+struct ColumnSums {
+  const float* partial[4];
+  void* out[4];
+  int64_t row_stride[4], batch_stride[4];
+  int rows[4], bf16_out[4], batches[4];
+  int dim;
+};
+__global__ __launch_bounds__(256) void residual_norm_sums_kernel(ColumnSums s) {
+  __shared__ float lds[16][17];
+  const int which = blockIdx.y;
+  if (!s.out[which]) return;
+  const int col = threadIdx.x % 16, part = threadIdx.x / 16, c = (int)blockIdx.x * 16 + col;
+  for (int64_t batch = blockIdx.z; batch < s.batches[which]; batch += gridDim.z) {
+    const float* from = s.partial[which] + batch * s.batch_stride[which] + c;
+    float v = 0.f;
+    if (c < s.dim)
+      for (int row = part; row < s.rows[which]; row += 16) v += from[row * s.row_stride[which]];
+    __syncthreads();
+    lds[part][col] = v;
+    __syncthreads();
+    if (part == 0 && c < s.dim) {
+      v = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v += lds[i][col];
+      if (s.bf16_out[which])
+        ((bf16*)s.out[which])[batch * s.dim + c] = (bf16)v;
+      else
+        ((float*)s.out[which])[batch * s.dim + c] = v;
+    }
+  }
+}
+
+// A row's threads and runs of 8 channels each.
+template <typename Go>
+void with_layout(int dim, Go go) {
+  using std::integral_constant;
+  if (dim <= 128) return go(integral_constant<int, 16>(), integral_constant<int, 1>());
+  if (dim <= 512) return go(integral_constant<int, 64>(), integral_constant<int, 1>());
+  if (dim <= 1024) return go(integral_constant<int, 64>(), integral_constant<int, 2>());
+  if (dim <= 2048) return go(integral_constant<int, 256>(), integral_constant<int, 1>());
+  if (dim <= 4096) return go(integral_constant<int, 256>(), integral_constant<int, 2>());
+  return go(integral_constant<int, 512>(), integral_constant<int, 2>());
+}
+
+template <typename X, typename Y>
+void launch(bool backward, const Frame& s, int blocks, hipStream_t stream) {
+  with_layout(s.dim, [&](auto l, auto v) {
+    constexpr int L = decltype(l)::value, V = decltype(v)::value, per = threads_of<L>() / L;
+    if (backward)
+      residual_norm_bwd_kernel<X, Y, L, V><<<blocks, threads_of<L>(), 0, stream>>>(s);
+    else
+      residual_norm_kernel<X, Y, L, V><<<fold_grid((s.rows + per - 1) / per, threads_of<L>()), threads_of<L>(), 0,
+                                         stream>>>(s);
+  });
+}
+
+int rows_per_pass(int dim) {
+  int rows = 1;
+  with_layout(dim, [&](auto l, auto) { rows = threads_of<decltype(l)::value>() / decltype(l)::value; });
+  return rows;
+}
+
+// Units of the gradient's rows and the blocks that walk them.  About 8 rows a group, at most kBwdBlocks blocks; with
+// a gate per batch element, whole elements or equal parts of them.
+struct Units {
+  int64_t units, unit_rows, splits;
+  int blocks;
+};
+Units plan_units(int64_t batch, int64_t tokens, int64_t dim, bool shared) {
+  const int64_t per = 8 * rows_per_pass((int)dim), most = kBwdBlocks;
+  const int64_t rows = batch * tokens, length = shared ? tokens : rows, elements = shared ? batch : 1;
+  int64_t splits = elements >= most ? 1 : most / elements;
+  const int64_t enough = (length + per - 1) / per;
+  if (splits > enough) splits = enough;
+  if (splits < 1) splits = 1;
+  Units u;
+  u.unit_rows = (length + splits - 1) / splits;
+  u.splits = u.unit_rows ? (length + u.unit_rows - 1) / u.unit_rows : 1;
+  u.units = elements * u.splits;
+  u.blocks = (int)(u.units < most ? u.units : most);
+  return u;
+}
+
+int setup(Frame& s, int x_dtype, int dtype, const int64_t* shape, const int64_t* strides, int gate, int w_dtype, int post,
+          int pre, float eps) {
+  BMX_REQUIRE((x_dtype == kF32 || x_dtype == kBF16) && (dtype == kF32 || dtype == kBF16) &&
+                  (x_dtype == kF32 || dtype == kBF16),
+              "residual_norm: x and y must be fp32 or bf16, fp32 x where y is fp32");
+  BMX_REQUIRE(w_dtype == kF32 || w_dtype == kBF16, "residual_norm: weight dtype must be fp32 or bf16");
+  BMX_REQUIRE(shape && strides, "residual_norm: null shape or strides");
+  BMX_REQUIRE(gate >= 0 && gate <= 2, "residual_norm: gate must be 0 (none), 1 (per token) or 2 (per batch element)");
+  for (int i = 0; i < 3; ++i) BMX_REQUIRE(shape[i] >= 0, "residual_norm: negative size");
+  BMX_REQUIRE(shape[2] >= 8 && shape[2] <= kMaxDim && shape[2] % 8 == 0,
+              "residual_norm: dim must be a multiple of 8 in [8, 8192]");
+  BMX_REQUIRE(shape[0] < (1ll << 31) && shape[1] < (1ll << 31) && (shape[1] == 0 || shape[0] < (1ll << 31) / shape[1]),
+              "residual_norm: expected fewer than 2^31 rows");
+  BMX_REQUIRE(eps >= 0x1p-126f, "residual_norm: eps must be positive, at least 2^-126");
+  for (int i = 0; i < 6; ++i) BMX_REQUIRE(strides[i] % 8 == 0, "residual_norm: strides must be multiples of 8");
+  s.rows = shape[0] * shape[1], s.tokens = shape[1], s.dim = (int)shape[2];
+  s.x.sb = strides[0], s.x.st = strides[1], s.y.sb = strides[2], s.y.st = strides[3];
+  s.gate.sb = strides[4], s.gate.st = gate == 2 ? 0 : strides[5];
+  s.w_bf16 = w_dtype == kBF16, s.post = post != 0, s.pre = pre != 0, s.shared = gate == 2;
+  s.eps = eps, s.inv_dim = 1.f / (float)s.dim;
+  return BMX_OK;
+}
+
+bool aligned16(std::initializer_list<const void*> pointers) {
+  uintptr_t bits = 0;
+  for (const void* p : pointers) bits |= (uintptr_t)p;
+  return bits % 16 == 0;
+}
+
+}  // namespace
+
+extern "C" int bmx_residual_norm_fwd(const void* x, const void* y, const void* gate, int x_dtype, int dtype,
+                                     const int64_t* shape, const int64_t* strides, int gate_kind, const void* y_weight,
+                                     const void* scale, const void* weight, int w_dtype, int post_norm, int pre_norm,
+                                     float eps, void* r, void* h, void* stream) {
+  Frame s = {};
+  if (int rc = setup(s, x_dtype, dtype, shape, strides, gate_kind, w_dtype, post_norm, pre_norm, eps)) return rc;
+  if (s.rows == 0) return BMX_OK;
+  BMX_REQUIRE(x && y && r && (!s.pre || h) && (gate_kind == 0 || gate), "residual_norm: null pointer");
+  BMX_REQUIRE(aligned16({x, y, gate, y_weight, scale, weight, r, h}), "residual_norm: tensors must be 16-byte aligned");
+  s.x.p = x, s.y.p = y, s.gate.p = gate_kind ? gate : nullptr;
+  s.yw = s.post ? y_weight : nullptr, s.scale = scale, s.w = weight, s.r = r, s.h = h;
+  hipStream_t hs = (hipStream_t)stream;
+  if (dtype == kF32)
+    launch<float, float>(false, s, 0, hs);
+  else if (x_dtype == kF32)
+    launch<float, bf16>(false, s, 0, hs);
+  else
+    launch<bf16, bf16>(false, s, 0, hs);
+  return check_launch("residual_norm");
+}
+
+extern "C" size_t bmx_residual_norm_workspace_bytes(int64_t batch, int64_t tokens, int64_t dim, int gate_kind) {
+  if (batch <= 0 || tokens <= 0 || dim < 8 || dim > kMaxDim) return 0;
+  const Units u = plan_units(batch, tokens, dim, gate_kind == 2);
+  return (size_t)((int64_t)u.blocks * 3 + (gate_kind == 2 && u.splits > 1 ? u.units : 0)) * dim * sizeof(float);
+}
+
+extern "C" int bmx_residual_norm_bwd(const void* x, const void* y, const void* gate, int x_dtype, int dtype,
+                                     const int64_t* shape, const int64_t* strides, int gate_kind, const void* y_weight,
+                                     const void* scale, const void* weight, int w_dtype, int post_norm, int pre_norm,
+                                     float eps, const void* dr, const void* dh, void* dx, void* dy, void* dgate,
+                                     void* dy_weight, void* dscale, void* dweight, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  Frame s = {};
+  if (int rc = setup(s, x_dtype, dtype, shape, strides, gate_kind, w_dtype, post_norm, pre_norm, eps)) return rc;
+  BMX_REQUIRE(s.rows > 0, "residual_norm_bwd: expected rows");
+  BMX_REQUIRE(x && y && (gate_kind == 0 || gate), "residual_norm: null pointer");
+  BMX_REQUIRE(gate_kind != 0 || !dgate, "residual_norm_bwd: gradient of an absent gate");
+  BMX_REQUIRE((y_weight || !dy_weight) && (scale || !dscale) && (weight || !dweight),
+              "residual_norm_bwd: gradient of an absent weight");
+  BMX_REQUIRE(aligned16({x, y, gate, y_weight, scale, weight, dr, dh, dx, dy, dgate}),
+              "residual_norm: tensors must be 16-byte aligned");
+  const Units u = plan_units(shape[0], shape[1], s.dim, s.shared);
+  const bool weights = dy_weight || dscale || dweight, gates = s.shared && dgate && u.splits > 1;
+  if (weights || gates)
+    BMX_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&
+                    workspace_bytes >= bmx_residual_norm_workspace_bytes(shape[0], shape[1], s.dim, gate_kind),
+                "residual_norm_bwd: workspace too small or not 16-byte aligned");
+  s.x.p = x, s.y.p = y, s.gate.p = gate_kind ? gate : nullptr;
+  s.yw = s.post ? y_weight : nullptr, s.scale = scale, s.w = weight;
+  s.dr = dr, s.dh = s.pre ? dh : nullptr, s.dx = dx, s.dy = dy, s.dgate = dgate;
+  s.units = u.units, s.unit_rows = u.unit_rows, s.splits = u.splits;
+  s.partial = weights ? (float*)workspace : nullptr;
+  s.gate_partial = gates ? (float*)workspace + (int64_t)u.blocks * 3 * s.dim : nullptr;
+  hipStream_t hs = (hipStream_t)stream;
+  if (dtype == kF32)
+    launch<float, float>(true, s, u.blocks, hs);
+  else if (x_dtype == kF32)
+    launch<float, bf16>(true, s, u.blocks, hs);
+  else
+    launch<bf16, bf16>(true, s, u.blocks, hs);
+  if (weights || gates) {
+    ColumnSums c = {};
+    void* outs[3] = {dy_weight, dscale, dweight};
+    for (int i = 0; i < 3; ++i) {
+      c.partial[i] = s.partial + i * s.dim, c.out[i] = weights ? outs[i] : nullptr;
+      c.row_stride[i] = 3 * s.dim, c.rows[i] = u.blocks, c.bf16_out[i] = s.w_bf16, c.batches[i] = 1;
+    }
+    c.partial[3] = s.gate_partial, c.out[3] = gates ? dgate : nullptr;
+    c.row_stride[3] = s.dim, c.batch_stride[3] = u.splits * s.dim, c.rows[3] = (int)u.splits;
+    c.bf16_out[3] = dtype == kBF16, c.batches[3] = (int)shape[0];
+    c.dim = s.dim;
+    const int z = gates ? (int)(shape[0] < 64 ? shape[0] : 64) : 1;
+    residual_norm_sums_kernel<<<dim3((s.dim + 15) / 16, 4, z), 256, 0, hs>>>(c);
+  }
+  return check_launch("residual_norm_bwd");
+}

@@ -9,7 +9,8 @@ Three groups:
 * the fused hot-path modules (``trimul``, ``triattn``, ``pair_transition``,
   ``adaln``) that take a module with Boltz's parameter names;
 * sequence operators with gradients (``qk_norm_rope``, ``relative_bias``,
-  ``cross_attention``) for an encoder / decoder beside the pair stack.
+  ``cross_attention``; ``residual_norm``, ``causal_conv``, ``selective_scan``)
+  for an encoder / decoder beside the pair stack.
 
 Every call launches on torch's current stream of the input's device, allocates
 outputs and workspaces through torch's caching allocator and never
@@ -1554,3 +1555,354 @@ def cross_attention(q, k, v, mask=None, bias=None, scale=None):
     if _needs_grad(q, k, v, bias):
         return _CrossAttention.apply(plan, dev, q, k, v, mask, bias, scale)
     return _cross_attention_fwd(plan, dev, q, k, v, mask, bias, scale)[0]
+
+
+def _rows3_ok(t, unit) -> bool:
+    """[B, T, C] that a kernel reads in place: a dense last axis, rows at multiples of ``unit`` elements and 16 bytes."""
+    shape, stride = t.shape, t.stride()
+    return stride[2] == 1 and all(n <= 1 or st % unit == 0 for n, st in zip(shape, stride[:2])) and t.data_ptr() % 16 == 0
+
+
+def _in_place(t, unit=8):
+    """``t`` [B, T, C], copied where its layout cannot be read in place."""
+    return t if t is None or _rows3_ok(t, unit) else _aligned(t.contiguous())
+
+
+def _dense(t):
+    return None if t is None else _aligned(t.contiguous())
+
+
+def _apart(out, t) -> bool:
+    """Whether the dense ``out`` shares no memory with ``t`` (a tensor or None)."""
+    if t is None or not t.numel() or not out.numel():
+        return True
+    size, span = out.numel() * out.element_size(), 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr() >= out.data_ptr() + size or out.data_ptr() >= t.data_ptr() + span * t.element_size()
+
+
+@lru_cache(maxsize=512)
+def _frame_plan(x, y, gate, y_weight, scale, weight, post_norm, pre_norm):
+    _check(len(x[0]) == 3 and x[0] == y[0], "expected x and y of one shape [B, tokens, D]")
+    (b, t, d), x_code, code = x[0], _code(x[2]), _code(y[2])
+    _check(x_code == N.F32 or code == N.BF16, "fp32 y needs fp32 x")
+    _check(8 <= d <= 8192 and d % 8 == 0, "D must be a multiple of 8 in [8, 8192]")
+    _check(gate is None or (gate[0] in ((b, t, d), (b, 1, d)) and gate[2] == y[2]),
+           "expected a gate [B, tokens, D] or [B, 1, D] in y's dtype")
+    weights = [w for w in (y_weight, scale, weight) if w is not None]
+    for w in weights:
+        _check(w[0] == (d,) and w[2] in (torch.float32, y[2]), "expected weights of [D] in fp32 or y's dtype")
+        _check(w[2] == weights[0][2], "the weights must share a dtype")
+    _check(post_norm or y_weight is None, "y_weight needs post_norm")
+    _check(pre_norm or weight is None, "weight needs pre_norm")
+    plan = _Plan()
+    plan.kind = 0 if gate is None else 2 if gate[0][1] != t else 1
+    plan.codes, plan.w_code = (x_code, code), _code(weights[0][2]) if weights else N.F32
+    strides = _steps(x[0], x[1], 2) + _steps(y[0], y[1], 2) + ([0, 0] if gate is None else _steps(gate[0], gate[1], 2))
+    plan.shape, plan.strides, plan.rows = N.int64_array([b, t, d]), N.int64_array(strides), b * t
+    plan.norms = int(post_norm), int(pre_norm)
+    plan.ws = N.lib().bmx_residual_norm_workspace_bytes(b, t, d, plan.kind)
+    return plan
+
+
+def _frame_args(plan, x, y, gate, y_weight, scale, weight, eps):
+    return (x.data_ptr(), y.data_ptr(), _ptr(gate), *plan.codes, plan.shape, plan.strides, plan.kind, _ptr(y_weight),
+            _ptr(scale), _ptr(weight), plan.w_code, *plan.norms, eps)
+
+
+def _residual_norm_fwd(plan, dev, x, y, *rest):
+    r = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    h = torch.empty(x.shape, device=x.device, dtype=y.dtype) if plan.norms[1] else None
+    if plan.rows:
+        _launch(dev, "bmx_residual_norm_fwd", *_frame_args(plan, x, y, *rest), r.data_ptr(), _ptr(h))
+    return r, h
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, plan, dev, x, y, gate, y_weight, scale, weight, eps):
+        ctx.save_for_backward(x, y, gate, y_weight, scale, weight)
+        ctx.rest = plan, dev, eps
+        ctx.set_materialize_grads(False)
+        return _residual_norm_fwd(plan, dev, x, y, gate, y_weight, scale, weight, eps)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dr, dh):
+        plan, dev, eps = ctx.rest
+        tensors = ctx.saved_tensors
+        make = torch.empty if plan.rows else torch.zeros
+        grads = [make(t.shape, device=t.device, dtype=t.dtype) if need else None
+                 for need, t in zip(ctx.needs_input_grad[2:8], tensors)]
+        if plan.rows and any(g is not None for g in grads):
+            dr, dh = _dense(dr), _dense(dh)
+            ws = _workspace(plan.ws, tensors[0].device)
+            _launch(dev, "bmx_residual_norm_bwd", *_frame_args(plan, *tensors, eps), _ptr(dr), _ptr(dh),
+                    *map(_ptr, grads), ws.data_ptr(), plan.ws)
+        return None, None, *grads, None
+
+
+def residual_norm(x, y, gate=None, y_weight=None, scale=None, weight=None, eps=1e-6, post_norm=True, pre_norm=True):
+    """The frame between two blocks of a sequence stack, one pass (``bmx_residual_norm_fwd``): the RMS norm of a
+    block's result, its gate and residual scale, the residual add, and the next block's RMS norm:
+
+        ``m = y / sqrt(mean(y^2) + eps) * y_weight``  (``post_norm`` False: ``m = y``)
+        ``r = x + scale * sigmoid(gate) * m``
+        ``h = r / sqrt(mean(r^2) + eps) * weight``
+
+    x (the residual stream) and y (the block's result) are [B, T, D], fp32 or bf16, D a multiple of 8 up to 8192, any
+    T; an fp32 stream takes blocks of either type.  gate: logits in y's type, [B, T, D] or one per batch element
+    [B, 1, D], or None (no gate).  Weights and scale are [D] in fp32 or y's type, or None (1).  Any strides: layouts that
+    the kernel cannot read (a strided last axis, rows off 16 bytes) are copied.  Returns dense (r in x's type, h in y's
+    type, from r before its rounding), or r alone with ``pre_norm`` False.  Gradients reach every tensor (a shared gate's
+    summed over its tokens); sums are fp32 and the same bits on every run."""
+    dev = _same_device(x, y, gate, y_weight, scale, weight)
+    _check(eps >= 2.0 ** -126, "eps must be positive, at least 2^-126")
+    _check(x.dim() == 3 and y.dim() == 3 and (gate is None or gate.dim() == 3), "expected x, y and gate of three axes")
+    x, y, gate = _in_place(x), _in_place(y), _in_place(gate)
+    y_weight, scale, weight = _dense(y_weight), _dense(scale), _dense(weight)
+    plan = _frame_plan(_layout(x), _layout(y), _layout(gate), _layout(y_weight), _layout(scale), _layout(weight),
+                       bool(post_norm), bool(pre_norm))
+    args = plan, dev, x, y, gate, y_weight, scale, weight, float(eps)
+    r, h = (_ResidualNorm.apply if _needs_grad(x, y, gate, y_weight, scale, weight) else _residual_norm_fwd)(*args)
+    return (r, h) if pre_norm else r
+
+
+def _check_lengths(lengths, batch):
+    _check(lengths is None or (lengths[0] == (batch,) and lengths[2] in (torch.int32, torch.int64)),
+           "expected int32 or int64 lengths [B]")
+    return int(lengths is not None and lengths[2] == torch.int64)
+
+
+def _check_state_out(state_out, shape, dtype, state, inputs, grad):
+    """A buffer for the last state: dense, of the state's kind, apart from everything but the state that it may replace."""
+    _check(not grad, "state_out takes no gradient: use return_state")
+    _check(state_out.shape == shape and state_out.dtype == dtype and state_out.is_contiguous()
+           and state_out.data_ptr() % 16 == 0, "state_out must be a dense 16-byte aligned tensor of the state's shape and dtype")
+    same = state is not None and state.data_ptr() == state_out.data_ptr() and state.is_contiguous()
+    _check(all(_apart(state_out, t) for t in (*inputs, None if same else state)), "state_out shares memory with an input")
+
+
+def _empty_state(shape, dtype, device, state, state_out):
+    """The last state of a call without tokens: the first one."""
+    out = torch.empty(shape, device=device, dtype=dtype) if state_out is None else state_out
+    return out.zero_() if state is None else out if out is state else out.copy_(state)
+
+
+def _written(t):
+    """Tells autograd that a native call wrote into ``t``."""
+    if t is not None and not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
+@lru_cache(maxsize=512)
+def _conv_plan(x, weight, bias, state, lengths, silu):
+    _check(len(x[0]) == 3 and len(weight[0]) == 2, "expected x of shape [B, tokens, channels] and a [channels, width] weight")
+    (b, t, c), width, code = x[0], weight[0][1], _code(x[2])
+    _check(c % 8 == 0 and 8 <= c < 1 << 20, "channels must be a multiple of 8 below 2^20")
+    _check(weight[0][0] == c and 2 <= width <= 4, "expected a [channels, width] weight of width 2, 3 or 4")
+    for w in (weight, bias):
+        _check(w is None or w[2] in (torch.float32, x[2]), "expected weight and bias in fp32 or x's dtype")
+    _check(bias is None or bias[0] == (c,), "expected a bias of [channels]")
+    _check(state is None or (state[0] == (b, width - 1, c) and state[2] == x[2]),
+           "expected a state [B, width - 1, channels] in x's dtype")
+    plan = _Plan()
+    lengths64 = _check_lengths(lengths, b)
+    plan.head = code, N.int64_array([b, t, c, width]), N.int64_array(_steps(x[0], x[1], 2))
+    plan.codes, plan.tail = (_code(weight[2]), _code(bias[2]) if bias else code), (lengths64, silu)
+    plan.state, plan.empty = (b, width - 1, c), not (b and t)
+    plan.ws = N.lib().bmx_causal_conv_workspace_bytes(b, t, c, width)
+    return plan
+
+
+def _conv_args(plan, x, weight, bias, state, lengths):
+    return (x.data_ptr(), *plan.head, weight.data_ptr(), plan.codes[0], _ptr(bias), plan.codes[1], _ptr(state), _ptr(lengths),
+            *plan.tail)
+
+
+def _causal_conv_fwd(plan, dev, x, weight, bias, state, lengths, want_state, state_out):
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    if plan.empty:
+        return y, _empty_state(plan.state, x.dtype, x.device, state, state_out) if want_state else None
+    if want_state and state_out is None:
+        state_out = torch.empty(plan.state, device=x.device, dtype=x.dtype)
+    _launch(dev, "bmx_causal_conv_fwd", *_conv_args(plan, x, weight, bias, state, lengths), y.data_ptr(), _ptr(state_out))
+    return y, state_out
+
+
+class _CausalConv(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, plan, dev, x, weight, bias, state, lengths, want_state, state_out):
+        ctx.save_for_backward(x, weight, bias, state, lengths)
+        ctx.rest = plan, dev
+        ctx.set_materialize_grads(False)
+        return _causal_conv_fwd(plan, dev, x, weight, bias, state, lengths, want_state, state_out)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dnext):
+        plan, dev = ctx.rest
+        x, weight, bias, state, lengths = ctx.saved_tensors
+        make = torch.zeros if plan.empty else torch.empty
+        dx, dw, db, dstate = (make(t.shape, device=x.device, dtype=t.dtype) if need else None
+                              for need, t in zip(ctx.needs_input_grad[2:6], (x, weight, bias, state)))
+        if plan.empty:
+            dstate = dnext if dstate is not None and dnext is not None else dstate
+        elif any(g is not None for g in (dx, dw, db, dstate)):
+            dy, dnext = _dense(dy), _dense(dnext)
+            ws = _workspace(plan.ws, x.device) if dw is not None or db is not None else None
+            _launch(dev, "bmx_causal_conv_bwd", *_conv_args(plan, x, weight, bias, state, lengths), _ptr(dy), _ptr(dnext),
+                    _ptr(dx), _ptr(dw), _ptr(db), _ptr(dstate), _ptr(ws), plan.ws if ws is not None else 0)
+        return None, None, dx, dw, db, dstate, None, None, None
+
+
+def causal_conv(x, weight, bias=None, state=None, lengths=None, silu=True, return_state=False, state_out=None):
+    """Short causal convolution of every channel on its own (``bmx_causal_conv_fwd``), with SiLU (``silu`` False:
+    without): ``y[b, t, c] = silu(bias[c] + sum_j weight[c, j] x[b, t - (W - 1) + j, c])``, dense, in x's type.
+
+    x [B, T, C] is fp32 or bf16, C a multiple of 8, in any strides (layouts that the kernel cannot read are copied).
+    weight [C, W], W 2 to 4, and bias [C] are fp32 or in x's type.  state: the W - 1 inputs before the first, oldest first,
+    [B, W - 1, C] in x's type (None: zeros).  lengths: int32 or int64 [B] on the device, the tokens of each sequence (taken
+    into [0, T]); later rows are never read and give zeros.
+
+    ``return_state``: (y, the W - 1 inputs before each sequence's end): the next call's state.  ``state_out``: a
+    dense buffer that takes it instead of a new tensor, ``state`` itself included (a decoder's step in place); without
+    gradients only.  Gradients reach x, weight, bias and state, from y and the returned state; sums are fp32 and the same
+    bits on every run."""
+    want, grad = return_state or state_out is not None, _needs_grad(x, weight, bias, state)
+    dev = _same_device(x, weight, bias, state, lengths, state_out)
+    _check(x.dim() == 3, "expected x of shape [B, tokens, channels]")
+    x, weight, bias, lengths = _in_place(x, 16 // x.element_size()), _dense(weight), _dense(bias), None if lengths is None else lengths.contiguous()
+    first, state = state, _dense(state)
+    plan = _conv_plan(_layout(x), _layout(weight), _layout(bias), _layout(state), _layout(lengths), int(bool(silu)))
+    if state_out is not None:
+        _check_state_out(state_out, plan.state, x.dtype, first, (x, weight, bias, lengths), grad)
+    args = plan, dev, x, weight, bias, state, lengths, want, state_out
+    y, last = (_CausalConv.apply if grad else _causal_conv_fwd)(*args)
+    _written(state_out)
+    return (y, last) if return_state else y
+
+
+@lru_cache(maxsize=512)
+def _scan_plan(u, dt, A, B, C, D, z, dt_bias, state, lengths, softplus):
+    _check(len(u[0]) == 3 and len(A[0]) == 2 and len(B[0]) == 4, "expected u [B, tokens, channels], A [channels, states] "
+           "and B, C [B, tokens, groups, states]")
+    (b, t, c), states, groups, code = u[0], A[0][1], B[0][2], _code(u[2])
+    _check(dt[0] == u[0] and dt[2] == u[2] and (z is None or (z[0] == u[0] and z[2] == u[2])),
+           "dt and z must match u's shape and dtype")
+    _check(states in (8, 16, 32, 64), "states must be 8, 16, 32 or 64")
+    _check(B[0] == C[0] == (b, t, groups, states) and B[2] == C[2] == u[2],
+           "expected B and C [B, tokens, groups, states] in u's dtype")
+    _check(groups >= 1 and 8 <= c < 1 << 20 and c % (8 * groups) == 0, "channels must be a multiple of 8 per group, below 2^20")
+    _check(A[0][0] == c and A[2] == torch.float32, "expected A [channels, states] in fp32")
+    for w in (D, dt_bias):
+        _check(w is None or (w[0] == (c,) and w[2] == torch.float32), "expected D and dt_bias [channels] in fp32")
+    _check(state is None or (state[0] == (b, c, states) and state[2] == torch.float32),
+           "expected a state [B, channels, states] in fp32")
+    plan, unit = _Plan(), 4
+    plan.ok = tuple(m is None or (m[1][-1] == 1 and all(n <= 1 or st % unit == 0 for n, st in zip(m[0][:-1], m[1][:-1])))
+                    for m in (u, dt, B, C, z))
+    none = [0, 0]
+    strides = [st for m in (u, dt) for st in _steps(m[0], m[1], 2)] + (_steps(z[0], z[1], 2) if z else none)
+    strides += _steps(B[0], B[1], 3) + _steps(C[0], C[1], 3)
+    plan.codes = code, _check_lengths(lengths, b)
+    plan.shape, plan.strides = N.int64_array([b, t, c, states, groups]), N.int64_array(strides)
+    plan.softplus, plan.state, plan.empty = softplus, (b, c, states), not (b and t)
+    plan.unit = unit * (4 if code == N.F32 else 2)  # bytes
+    plan.ws = N.lib().bmx_selective_scan_workspace_bytes(b, t, c, states, groups)
+    plan.ws_bwd = N.lib().bmx_selective_scan_bwd_workspace_bytes(b, t, c, states, groups)
+    plan.saved = N.lib().bmx_selective_scan_saved_bytes(b, t, c, states) // 4
+    return plan
+
+
+def _selective_scan_fwd(plan, dev, u, dt, A, B, C, D, z, dt_bias, state, lengths, want_state, state_out,
+                        for_backward=False):
+    """(out, last state or None, states at the tiles' starts, out before its gate; the latter two for the gradient)."""
+    out = torch.empty(u.shape, device=u.device, dtype=u.dtype)
+    if plan.empty:
+        return out, _empty_state(plan.state, torch.float32, u.device, state, state_out) if want_state else None, None, None
+    if want_state and state_out is None:
+        state_out = torch.empty(plan.state, device=u.device, dtype=torch.float32)
+    saved = torch.empty(plan.saved, device=u.device, dtype=torch.float32) if for_backward else None
+    raw = torch.empty(u.shape, device=u.device, dtype=torch.float32) if for_backward and z is not None else None
+    ws = _workspace(plan.ws, u.device) if plan.ws else None
+    _launch(dev, "bmx_selective_scan_fwd", u.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), _ptr(D),
+            _ptr(z), _ptr(dt_bias), _ptr(state), _ptr(lengths), *plan.codes, plan.shape, plan.strides, plan.softplus,
+            out.data_ptr(), _ptr(state_out), _ptr(saved), _ptr(raw), _ptr(ws), plan.ws)
+    return out, state_out, saved, raw
+
+
+class _SelectiveScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, plan, dev, u, dt, A, B, C, D, z, dt_bias, state, lengths, want_state):
+        out, last, saved, raw = _selective_scan_fwd(plan, dev, u, dt, A, B, C, D, z, dt_bias, state, lengths, want_state, None,
+                                                    for_backward=True)
+        ctx.save_for_backward(u, dt, A, B, C, D, z, dt_bias, state, lengths, saved, raw)
+        ctx.rest = plan, dev
+        ctx.set_materialize_grads(False)
+        return out, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, dlast):
+        plan, dev = ctx.rest
+        *tensors, lengths, saved, raw = ctx.saved_tensors
+        u, dt, A, B, C, D, z, dt_bias, _ = tensors
+        make = torch.zeros if plan.empty else torch.empty
+        grads = [make(t.shape, device=u.device, dtype=t.dtype) if need else None
+                 for need, t in zip(ctx.needs_input_grad[2:11], tensors)]
+        if plan.empty:
+            if grads[8] is not None and dlast is not None:
+                grads[8] = dlast
+        elif any(g is not None for g in grads):
+            dout, dlast = torch.zeros_like(u, memory_format=torch.contiguous_format) if dout is None else _dense(dout), _dense(dlast)
+            ws = _workspace(plan.ws_bwd, u.device)
+            du, ddt, dA, dB, dC, dD, dz, dbias, dstate = map(_ptr, grads)
+            _launch(dev, "bmx_selective_scan_bwd", u.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(),
+                    _ptr(D), _ptr(z), _ptr(dt_bias), _ptr(lengths), *plan.codes, plan.shape, plan.strides, plan.softplus,
+                    saved.data_ptr(), _ptr(raw), dout.data_ptr(), _ptr(dlast), du, ddt, dA, dB, dC, dD, dz, dbias, dstate,
+                    ws.data_ptr(), plan.ws_bwd)
+        return None, None, *grads, None, None
+
+
+def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, lengths=None, softplus=True,
+                   return_state=False, state_out=None):
+    """A diagonal state space whose step and whose input and output maps depend on the token
+    (``bmx_selective_scan_fwd``), token after token for every channel c (of group g) and state n:
+
+        ``d = softplus(dt + dt_bias)``  (``softplus`` False: ``d = dt + dt_bias``)
+        ``h = exp(d A[c, n]) h + d u B[g, n]``
+        ``y = sum_n C[g, n] h + D u``,  ``out = y * silu(z)``  (z None: y)
+
+    u, dt, z [B, T, C] and B, C [B, T, G, N] are fp32 or bf16, one type; C a multiple of 8 G, N 8, 16, 32 or 64, any T
+    from one token on, in any strides (column slices of one projection are read in place; layouts that the kernel cannot
+    read are copied).  A [C, N] (finite), D and dt_bias [C] are fp32.  state: what h starts from, [B, C, N] fp32
+    (None: zeros).  lengths: int32 or int64 [B] on the device, the tokens of each sequence (taken into [0, T]); later ones
+    are never read, give zeros and leave the state alone.
+
+    Returns out, dense, in u's type; ``return_state``: (out, the last state, fp32), the next call's state.  ``state_out``:
+    a dense buffer that takes it instead of a new tensor, ``state`` itself included (a decoder's step in place); without
+    gradients only.  States and sums are fp32.  Gradients reach every tensor but lengths, from out and the returned state,
+    and are the same bits on every run."""
+    tensors = u, dt, A, B, C, D, z, dt_bias, state
+    want, grad = return_state or state_out is not None, _needs_grad(*tensors)
+    dev = _same_device(*tensors, lengths, state_out)
+    A, D, dt_bias, state, lengths = _dense(A), _dense(D), _dense(dt_bias), _dense(state), (
+        None if lengths is None else lengths.contiguous())
+    layouts = [_layout(t) for t in (A, D, dt_bias, state, lengths)]
+
+    def plan_of(u, dt, B, C, z):
+        return _scan_plan(_layout(u), _layout(dt), layouts[0], _layout(B), _layout(C), layouts[1], _layout(z), layouts[2],
+                          layouts[3], layouts[4], int(bool(softplus)))
+
+    plan = plan_of(u, dt, B, C, z)
+    moved = (u, dt, B, C, z)
+    if not all(plan.ok) or any(t is not None and t.data_ptr() % plan.unit for t in moved):
+        u, dt, B, C, z = (t if t is None or (ok and t.data_ptr() % plan.unit == 0) else _aligned(t.contiguous())
+                          for ok, t in zip(plan.ok, moved))
+        plan = plan_of(u, dt, B, C, z)
+    if state_out is not None:
+        _check_state_out(state_out, plan.state, torch.float32, tensors[8], (*tensors[:8], lengths), grad)
+    args = plan, dev, u, dt, A, B, C, D, z, dt_bias, state, lengths, want
+    out, last = _SelectiveScan.apply(*args) if grad else _selective_scan_fwd(*args, state_out)[:2]
+    _written(state_out)
+    return (out, last) if return_state else out

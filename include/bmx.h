@@ -479,6 +479,79 @@ int bmx_cross_attention_bwd(const void* q, const void* k, const void* v, const v
                             void* dbias, const int64_t* dbias_strides, void* workspace, size_t workspace_bytes,
                             bmx_stream_t stream);
 
+/* The frame between two blocks, for rows of dim channels of x and y [batch, tokens, dim]:
+ *   m = y / sqrt(mean(y^2) + eps) * y_weight (post_norm 0: m = y);  r = x + scale * sigmoid(gate) * m;
+ *   h = r / sqrt(mean(r^2) + eps) * weight (pre_norm 0: no h), from r before its rounding.
+ * shape = {batch, tokens, dim}, dim a multiple of 8 in [8, 8192], fewer than 2^31 rows; strides = {batch, token of x,
+ * of y, of gate}, multiples of 8, the last axis dense.  x and r in x_dtype, y, gate and h in dtype (both fp32 or bf16;
+ * fp32 y takes fp32 x).  gate_kind: 0 none, 1 per token, 2 one per batch element ([batch, dim], token stride unused).
+ * Weights [dim] in w_dtype or NULL (1).  eps at least 2^-126.  r, h dense.  All pointers 16-byte aligned.  No reference kernel. */
+int bmx_residual_norm_fwd(const void* x, const void* y, const void* gate, int x_dtype, int dtype, const int64_t* shape,
+                          const int64_t* strides, int gate_kind, const void* y_weight, const void* scale,
+                          const void* weight, int w_dtype, int post_norm, int pre_norm, float eps, void* r, void* h,
+                          bmx_stream_t stream);
+
+/* Gradients of bmx_residual_norm_fwd from dr and dh (dense, or NULL: zeros): dx, dy, dgate dense (a gate_kind 2 gate's
+ * summed over its tokens), dy_weight, dscale, dweight [dim] in w_dtype, each or NULL.  At least one row.  workspace
+ * (for a weight's gradient, or gate_kind 2's): bmx_residual_norm_workspace_bytes, 16-byte aligned.  No reference kernel. */
+size_t bmx_residual_norm_workspace_bytes(int64_t batch, int64_t tokens, int64_t dim, int gate_kind);
+int bmx_residual_norm_bwd(const void* x, const void* y, const void* gate, int x_dtype, int dtype, const int64_t* shape,
+                          const int64_t* strides, int gate_kind, const void* y_weight, const void* scale,
+                          const void* weight, int w_dtype, int post_norm, int pre_norm, float eps, const void* dr,
+                          const void* dh, void* dx, void* dy, void* dgate, void* dy_weight, void* dscale, void* dweight,
+                          void* workspace, size_t workspace_bytes, bmx_stream_t stream);
+
+/* y[t] = act(bias + sum_j weight[:, j] x[t - (width - 1) + j]) for x [batch, tokens, channels], act SiLU or (silu 0)
+ * nothing.  shape = {batch, tokens, channels, width}: channels a multiple of 8 below 2^20, width 2, 3 or 4, fewer than
+ * 2^31 rows; strides = {batch, token of x}, multiples of 16 bytes, the last axis dense.  weight [channels, width] in
+ * w_dtype, bias [channels] in bias_dtype or NULL.  state: the width - 1 rows before the first [batch, width - 1,
+ * channels] in dtype, dense, or NULL (zeros).  lengths: int32 / int64 [batch], taken into [0, tokens]; rows from there
+ * on are not read and give zeros; or NULL.  y dense; state_out (or NULL): the width - 1 rows before the end of each
+ * sequence, dense; it may be `state` itself.  x, y and the states 16-byte aligned.  No reference kernel. */
+int bmx_causal_conv_fwd(const void* x, int dtype, const int64_t* shape, const int64_t* strides, const void* weight,
+                        int w_dtype, const void* bias, int bias_dtype, const void* state, const void* lengths,
+                        int lengths64, int silu, void* y, void* state_out, bmx_stream_t stream);
+
+/* Gradients of bmx_causal_conv_fwd from dy and dstate_out (dense, or NULL: zeros): dx and dstate dense, dweight and
+ * dbias in the operands' dtypes, each or NULL.  At least one row.  workspace (for dweight or dbias):
+ * bmx_causal_conv_workspace_bytes, 16-byte aligned.  No reference kernel. */
+size_t bmx_causal_conv_workspace_bytes(int64_t batch, int64_t tokens, int64_t channels, int64_t width);
+int bmx_causal_conv_bwd(const void* x, int dtype, const int64_t* shape, const int64_t* strides, const void* weight,
+                        int w_dtype, const void* bias, int bias_dtype, const void* state, const void* lengths,
+                        int lengths64, int silu, const void* dy, const void* dstate_out, void* dx, void* dweight,
+                        void* dbias, void* dstate, void* workspace, size_t workspace_bytes, bmx_stream_t stream);
+
+/* A diagonal state space per channel c (of group g = c / (channels / groups)) and state n, token after token:
+ *   d = dt + dt_bias (softplus: log(1 + exp(that)));  h = exp(d A[c][n]) h + d u B[g][n];
+ *   y = sum_n C[g][n] h + D u;  out = y z sigmoid(z) (z NULL: y)
+ * u, dt, z [batch, tokens, channels] and B, C [batch, tokens, groups, states] in dtype; A [channels, states], D and
+ * dt_bias [channels] (or NULL: 0) fp32, dense; state [batch, channels, states] fp32 (NULL: zeros).  shape = {batch,
+ * tokens, channels, states, groups}: states 8, 16, 32 or 64, channels / groups a multiple of 8, channels below 2^20, fewer
+ * than 2^31 rows; strides = {batch, token of u, of dt, of z, batch, token, group of B, of C}, multiples of 4, last axes
+ * dense.  lengths as for bmx_causal_conv_fwd: later tokens give zeros and leave the state alone.  out dense; state_out
+ * (or NULL) fp32: the last state; it may be `state` itself.  For the backward pass, or NULL: saved
+ * (bmx_selective_scan_saved_bytes), and raw, out's shape in fp32, where z is given.  workspace:
+ * bmx_selective_scan_workspace_bytes.  Inputs aligned to 4 elements, the others to 16 bytes.  No reference kernel. */
+size_t bmx_selective_scan_saved_bytes(int64_t batch, int64_t tokens, int64_t channels, int64_t states);
+size_t bmx_selective_scan_workspace_bytes(int64_t batch, int64_t tokens, int64_t channels, int64_t states, int64_t groups);
+int bmx_selective_scan_fwd(const void* u, const void* dt, const float* A, const void* B, const void* C, const float* D,
+                           const void* z, const float* dt_bias, const float* state, const void* lengths, int dtype,
+                           int lengths64, const int64_t* shape, const int64_t* strides, int softplus, void* out,
+                           float* state_out, float* saved, float* raw, void* workspace, size_t workspace_bytes,
+                           bmx_stream_t stream);
+
+/* Gradients of bmx_selective_scan_fwd from dout (dense) and dstate_out (fp32, or NULL: zeros) and the forward pass's
+ * saved and (with z) raw: du, ddt, dB, dC, dz in dtype, dA, dD, ddt_bias, dstate fp32, dense, each or NULL.  At least one
+ * row.  workspace: bmx_selective_scan_bwd_workspace_bytes, 16-byte aligned.  No reference kernel. */
+size_t bmx_selective_scan_bwd_workspace_bytes(int64_t batch, int64_t tokens, int64_t channels, int64_t states,
+                                              int64_t groups);
+int bmx_selective_scan_bwd(const void* u, const void* dt, const float* A, const void* B, const void* C, const float* D,
+                           const void* z, const float* dt_bias, const void* lengths, int dtype, int lengths64,
+                           const int64_t* shape, const int64_t* strides, int softplus, const float* saved,
+                           const float* raw, const void* dout, const float* dstate_out, void* du, void* ddt, float* dA,
+                           void* dB, void* dC, float* dD, void* dz, float* ddt_bias, float* dstate, void* workspace,
+                           size_t workspace_bytes, bmx_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
