@@ -16,6 +16,7 @@
 // out on its own.  States, sums and statistics are fp32; tokens from a
 // sequence's length on take no step (d = 0), are never read and give zeros.
 #include <type_traits>
+#include <utility>
 
 #include "bmx_common.h"
 
@@ -24,7 +25,9 @@ using namespace bmx;
 namespace {
 
 constexpr int K = 32;             // tokens of a tile
-constexpr int kRow = K + 4;       // LDS row of a channel or state over a tile: 16-byte reads along the tokens, no conflicts
+constexpr int kRow = K + 4;       // LDS row of a state's map over a tile: 16-byte reads along the tokens, no conflicts
+constexpr int kChannelRow = K + 2;  // LDS row of a channel: reads without conflicts, transposing writes two on a bank
+constexpr int kWalk = 64;         // channels of a block that walks chunks, four lanes each
 constexpr int kSlice = 32;        // channels that the gradient stages at a time
 constexpr int kMaxSpan = 6144;    // channels x states of a gradient block (its dA in LDS)
 constexpr float kLog2e = 1.4426950408889634f;
@@ -59,21 +62,43 @@ __device__ __forceinline__ int64_t length_of(const Scan& s, int64_t b) {
   return n < 0 ? 0 : n < s.tokens ? n : s.tokens;
 }
 
-// softplus(x) = max(x, 0) + log1p(exp(-|x|)); `slope` is its derivative, sigmoid(x).
-__device__ __forceinline__ float step_of(float x, int softplus) {
-  return softplus ? fmaxf(x, 0.f) + log1pf(__builtin_amdgcn_exp2f(-fabsf(x) * kLog2e)) : x;
+// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|), with log(1 + e) = 2 atanh(r), r = e / (2 + e) <= 1 / 3, by the
+// series of atanh to r^13: what is left is below 2^-25 of it, however small e is.
+__device__ __forceinline__ float step_of(float x) {
+  const float e = __builtin_amdgcn_exp2f(-fabsf(x) * kLog2e);
+  const float r = e * __builtin_amdgcn_rcpf(2.f + e), q = r * r;
+  float s = 2.f / 13.f;
+  s = s * q + 2.f / 11.f;
+  s = s * q + 2.f / 9.f;
+  s = s * q + 2.f / 7.f;
+  s = s * q + 2.f / 5.f;
+  s = s * q + 2.f / 3.f;
+  s = s * q + 2.f;
+  return s * r + fmaxf(x, 0.f);
 }
 
-// Lanes of one channel: L of them share its states, in the low bits of the lane, except that eight take the bits 0, 1
-// and 3: a sum over them then is two exchanges within quads and one over 8 lanes of a row.
-template <int L>
-__device__ __forceinline__ int lane_state(int lane) {
-  return L == 8 ? (lane & 3) | (lane >> 1 & 4) : lane % L;
+// v of the lane that a DPP control word names, as an operand of the instruction that uses it.
+template <int kCtrl>
+__device__ __forceinline__ float from_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), kCtrl, 0xF, 0xF, true));
 }
-template <int L>
-__device__ __forceinline__ int lane_slot(int lane) {
-  return L == 8 ? (lane >> 2 & 1) | (lane >> 3 & 6) : lane / L;
+template <int kLane>
+__device__ __forceinline__ float from_quad(float v) {  // lane kLane of each quad
+  return from_lane<0x55 * kLane>(v);
 }
+template <int kLane>
+__device__ __forceinline__ float from_row(float v) {  // lane kLane of each 16
+  return from_lane<0x150 + kLane>(v);
+}
+template <typename F, int... I>
+__device__ __forceinline__ void unrolled(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int kCount, typename F>
+__device__ __forceinline__ void unrolled(F f) {
+  unrolled(f, std::make_integer_sequence<int, kCount>());
+}
+
 __device__ __forceinline__ float xor16(float v) {
   return __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), 0x401F));
 }
@@ -82,19 +107,40 @@ __device__ __forceinline__ float xor32_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Sums of four values over the L >= 4 lanes of a channel; lane j gets the one of value j % 4.
-template <int L>
-__device__ __forceinline__ float sum4(const f32x4& p, int lane) {
+// Sums of four values over a quad; lane j gets the one of value j.
+__device__ __forceinline__ float quad_sums(const f32x4& p, int lane) {
   const bool odd = lane & 1, high = lane & 2;
-  const float a = (odd ? p[1] : p[0]) + dpp<0xB1>(odd ? p[0] : p[1]);
-  const float b = (odd ? p[3] : p[2]) + dpp<0xB1>(odd ? p[2] : p[3]);
-  float v = (high ? b : a) + dpp<0x4E>(high ? a : b);
-  if (L == 16 || L >= 32) v += dpp<0x124>(v);  // row_ror:4
-  if (L >= 8) v += dpp<0x128>(v);              // row_ror:8
-  if (L >= 32) v += xor16(v);
-  if (L == 64) v = xor32_sum(v);
-  return v;
+  const float a = (odd ? p[1] : p[0]) + from_lane<0xB1>(odd ? p[0] : p[1]);
+  const float b = (odd ? p[3] : p[2]) + from_lane<0xB1>(odd ? p[2] : p[3]);
+  return (high ? b : a) + from_lane<0x4E>(high ? a : b);
 }
+
+// Sums of 16 values over the 16 lanes of a row, one value after another; lane j gets the one of value rev4(j), j's four
+// bits reversed.  Level by level two values become one, a lane keeping the first or the second by one of its bits; the
+// exchange partner (15 - j, 7 - j, j xor 2, j xor 1) has the other value of that bit, and the earlier ones' equal.
+__device__ __forceinline__ int rev4(int j) { return (j & 1) << 3 | (j & 2) << 1 | (j & 4) >> 1 | (j & 8) >> 3; }
+struct RowSum {
+  float held[4];
+  template <int kIndex>
+  __device__ __forceinline__ void add(float v, int lane) {  // values in the order 0 .. 15; the last leaves its sum in held[3]
+    level<kIndex, 0>(v, lane);
+  }
+  template <int kIndex, int kLevel>
+  __device__ __forceinline__ void level(float v, int lane) {
+    if constexpr (kLevel < 4) {
+      if constexpr ((kIndex >> kLevel) & 1) {
+        constexpr int ctrl[4] = {0x140, 0x141, 0x4E, 0xB1};
+        const bool second = lane & (8 >> kLevel);
+        const float sum = (second ? v : held[kLevel]) + from_lane<ctrl[kLevel]>(second ? held[kLevel] : v);
+        level<kIndex, kLevel + 1>(sum, lane);
+      } else {
+        held[kLevel] = v;
+      }
+    } else {
+      held[3] = v;
+    }
+  }
+};
 
 // Four channels of one token as fp32; zeros where they are not there.
 template <typename T>
@@ -108,95 +154,108 @@ __device__ __forceinline__ f32x4 row4(const Operand& o, int64_t b, int64_t t, in
 // chunk's end, of dy in the place of d u and of C in the place of B.
 enum Mode { kLocal, kOut, kBack };
 
-template <typename T, int N, int L, int kMode>
+template <typename T, int N, int kMode>
 __global__ __launch_bounds__(256) void scan_walk_kernel(Scan s) {
-  constexpr int S = N / L, kChannels = 256 / L, kPer = (kChannels * K / 4 + 255) / 256, kMaps = (N * K / 4 + 255) / 256;
-  __shared__ __align__(16) float sd[kChannels * kRow], sv[kChannels * kRow], sy[kMode == kOut ? kChannels * kRow : 4];
+  constexpr int S = N / 4, kPer = kWalk * K / 4 / 256, kMaps = (N * K / 4 + 255) / 256;
+  __shared__ float sd[kWalk * kChannelRow], sv[kWalk * kChannelRow], sy[kMode == kOut ? kWalk * kChannelRow : 4];
   __shared__ __align__(16) float sB[N * kRow], sC[kMode == kOut ? N * kRow : 4];
-  int64_t block = block_index();
+  uint32_t block = block_index();
   if (block >= s.blocks) return;
-  const int cblock = (int)(block % s.cblocks);
-  block /= s.cblocks;
-  const int group = (int)(block % s.groups);
-  block /= s.groups;
-  const int64_t chunk = block % s.chunks, b = block / s.chunks;
-  const int c_first = group * s.group_channels + cblock * kChannels;
-  const int c_end = min(c_first + kChannels, (group + 1) * s.group_channels);
+  const int cblock = (int)(block % (uint32_t)s.cblocks);
+  block /= (uint32_t)s.cblocks;
+  const int group = (int)(block % (uint32_t)s.groups);
+  block /= (uint32_t)s.groups;
+  const int64_t chunk = block % (uint32_t)s.chunks, b = block / (uint32_t)s.chunks;
+  const int c_first = group * s.group_channels + cblock * kWalk;
+  const int c_end = min(c_first + kWalk, (group + 1) * s.group_channels);
   const int64_t length = length_of(s, b);
-  const int lane = lane_id(), j = lane_state<L>(lane);
-  const int c_local = (threadIdx.x >> 6) * (64 / L) + lane_slot<L>(lane), c = c_first + c_local;
+  const int lane = lane_id(), j = threadIdx.x & 3, c_local = threadIdx.x >> 2, c = c_first + c_local;
   const bool live = c < c_end;
 
-  float A2[S], h[S], total = 0.f;
-#pragma unroll
-  for (int i = 0; i < S; ++i) {
-    A2[i] = live ? s.A[(int64_t)c * N + j * S + i] * kLog2e : 0.f;
-    h[i] = 0.f;
-  }
-  if (kMode == kOut && live) {
-    const float* from = s.chunks > 1 ? s.carry + ((b * s.chunks + chunk) * s.channels + c) * N
-                        : s.state    ? s.state + (b * s.channels + c) * N
-                                     : nullptr;
-#pragma unroll
-    for (int i = 0; i < S; ++i) h[i] = from ? from[j * S + i] : 0.f;
-  }
-
   const int64_t tile0 = chunk * s.chunk_tiles, tile1 = min(tile0 + s.chunk_tiles, s.tiles);
-  // this thread's elements of a tile: four channels of one token
+  const int64_t start = kMode == kBack ? tile1 - 1 : tile0;
+  // this thread's elements of a tile: four channels of kPer tokens, and of the maps four states of kMaps tokens
+  const int e = threadIdx.x % (kWalk / 4) * 4, et = threadIdx.x / (kWalk / 4), cc = c_first + e;
+  const int en = threadIdx.x % (N / 4) * 4, ent = threadIdx.x / (N / 4);
+  const bool mine = cc < c_end;
+  const int64_t dense = (b * s.tokens + start * K + et) * s.channels + cc;
+  const T *dt = (const T*)s.dt.p + b * s.dt.sb + (start * K + et) * s.dt.st + cc, *u = (const T*)s.u.p, *z = (const T*)s.z.p;
+  u = kMode == kBack ? (const T*)s.dout + dense : u + b * s.u.sb + (start * K + et) * s.u.st + cc;
+  z = z ? z + b * s.z.sb + (start * K + et) * s.z.st + cc : nullptr;
+  const int64_t u_st = kMode == kBack ? s.channels : s.u.st;
+  const T* B = (const T*)s.B.p + b * s.B.sb + (start * K + ent) * s.B.st + group * s.B.sg + en;
+  const T* C = (const T*)s.C.p + b * s.C.sb + (start * K + ent) * s.C.st + group * s.C.sg + en;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   f32x4 ru[kPer], rdt[kPer], rz[kPer], rB[kMaps], rC[kMaps];
   auto fetch = [&](int64_t tile) {
+    const int64_t left = length - tile * K;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int at = threadIdx.x + 256 * i, e = at % (kChannels / 4) * 4, cc = c_first + e;
-      const int64_t t = tile * K + at / (kChannels / 4);
-      const bool there = at < kChannels / 4 * K && t < length && cc < c_end;
-      rdt[i] = row4<T>(s.dt, b, t, cc, there);
-      if (kMode == kBack)
-        ru[i] = there ? load4((const T*)s.dout + (b * s.tokens + t) * s.channels + cc) : f32x4{0.f, 0.f, 0.f, 0.f};
-      else
-        ru[i] = row4<T>(s.u, b, t, cc, there);
-      if (kMode != kLocal) rz[i] = row4<T>(s.z, b, t, cc, there && s.z.p);
+      const int t = i * (K / kPer);
+      const bool there = mine && et + t < left;
+      rdt[i] = there ? load4(dt + t * s.dt.st) : zero;
+      ru[i] = there ? load4(u + t * u_st) : zero;
+      if (kMode != kLocal) rz[i] = there && z ? load4(z + t * s.z.st) : zero;
     }
 #pragma unroll
     for (int i = 0; i < kMaps; ++i) {
-      const int at = threadIdx.x + 256 * i, n = at % (N / 4) * 4;
-      const int64_t t = tile * K + at / (N / 4);
-      const bool there = at < N / 4 * K && t < length;
-      rB[i] = there && kMode != kBack ? load4((const T*)s.B.p + b * s.B.sb + t * s.B.st + group * s.B.sg + n)
-                                      : f32x4{0.f, 0.f, 0.f, 0.f};
-      rC[i] = there && kMode != kLocal ? load4((const T*)s.C.p + b * s.C.sb + t * s.C.st + group * s.C.sg + n)
-                                       : f32x4{0.f, 0.f, 0.f, 0.f};
+      const int t = i * (1024 / N);
+      const bool there = ent + t < K && ent + t < left;
+      if (kMode != kBack) rB[i] = there ? load4(B + t * s.B.st) : zero;
+      if (kMode != kLocal) rC[i] = there ? load4(C + t * s.C.st) : zero;
     }
+    const int64_t step = kMode == kBack ? -K : K;
+    dt += step * s.dt.st, u += step * u_st, B += step * s.B.st, C += step * s.C.st;
+    if (z) z += step * s.z.st;
   };
+  fetch(start);
 
-  fetch(kMode == kBack ? tile1 - 1 : tile0);
+  f32x4 bias = zero, skip = zero;
+  if (mine && s.dt_bias) bias = load4(s.dt_bias + cc);
+  if (kMode == kOut && mine && s.D) skip = load4(s.D + cc);
+  float A2[S], h[S], total = 0.f;
+  const float* from = nullptr;
+  if (kMode == kOut)
+    from = s.chunks > 1 ? s.carry + ((b * s.chunks + chunk) * s.channels + c) * N
+           : s.state    ? s.state + (b * s.channels + c) * N
+                        : nullptr;
+#pragma unroll
+  for (int i = 0; i < S; ++i) {
+    A2[i] = live ? s.A[(int64_t)c * N + j * S + i] * kLog2e : 0.f;
+    h[i] = live && from ? from[j * S + i] : 0.f;
+  }
+
   for (int64_t k = tile0; k < tile1; ++k) {
-    const int64_t tile = kMode == kBack ? tile0 + tile1 - 1 - k : k;
+    const int64_t tile = kMode == kBack ? tile0 + tile1 - 1 - k : k, left = length - tile * K;
     // d, and d u (kBack: dy), of the tile to LDS, along the tokens; a token that is not there takes no step
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int at = threadIdx.x + 256 * i, e = at % (kChannels / 4) * 4, t = at / (kChannels / 4);
-      if (at >= kChannels / 4 * K) continue;
-      const bool there = tile * K + t < length && c_first + e < c_end;
+      const int t = et + i * (K / kPer);
+      f32x4 d = rdt[i] + bias;
+      if (s.softplus) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) d[q] = step_of(d[q]);
+      }
+      d = d * (mine && t < left ? 1.f : 0.f);
+      f32x4 v = kMode == kBack ? ru[i] : d * ru[i];
+      if (kMode == kBack && s.z.p) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] *= silu_f(rz[i][q]);
+      }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float bias = s.dt_bias && there ? s.dt_bias[c_first + e + q] : 0.f;
-        const float d = there ? step_of(rdt[i][q] + bias, s.softplus) : 0.f;
-        sd[(e + q) * kRow + t] = d;
-        if (kMode == kBack)
-          sv[(e + q) * kRow + t] = s.z.p ? ru[i][q] * silu_f(rz[i][q]) : ru[i][q];
-        else
-          sv[(e + q) * kRow + t] = d * ru[i][q];
+        sd[(e + q) * kChannelRow + t] = d[q];
+        sv[(e + q) * kChannelRow + t] = v[q];
       }
     }
 #pragma unroll
     for (int i = 0; i < kMaps; ++i) {
-      const int at = threadIdx.x + 256 * i, n = at % (N / 4) * 4, t = at / (N / 4);
-      if (at >= N / 4 * K) continue;
+      const int t = ent + i * (1024 / N);
+      if (t >= K) continue;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        sB[(n + q) * kRow + t] = kMode == kBack ? rC[i][q] : rB[i][q];
-        if (kMode == kOut) sC[(n + q) * kRow + t] = rC[i][q];
+        sB[(en + q) * kRow + t] = kMode == kBack ? rC[i][q] : rB[i][q];
+        if (kMode == kOut) sC[(en + q) * kRow + t] = rC[i][q];
       }
     }
     __syncthreads();
@@ -207,51 +266,51 @@ __global__ __launch_bounds__(256) void scan_walk_kernel(Scan s) {
     }
     if (k + 1 < tile1) fetch(kMode == kBack ? tile - 1 : tile + 1);
     if (kMode == kOut && s.saved && live) {
+      float* to = s.saved + ((b * s.tiles + tile) * s.channels + c) * N + j * S;
 #pragma unroll
-      for (int i = 0; i < S; ++i) s.saved[((b * s.tiles + tile) * s.channels + c) * N + j * S + i] = h[i];
+      for (int i = 0; i < S; ++i) to[i] = h[i];
     }
 
+    // Four tokens at a time: lane j of a channel's quad holds token j's d and d u, which the others take from it.
 #pragma unroll 2
     for (int step = 0; step < K; step += 4) {
       const int t = kMode == kBack ? K - 4 - step : step;
-      const f32x4 d = *(const f32x4*)(sd + c_local * kRow + t), v = *(const f32x4*)(sv + c_local * kRow + t);
-      f32x4 p = {0.f, 0.f, 0.f, 0.f};
+      const float d = sd[c_local * kChannelRow + t + j], v = sv[c_local * kChannelRow + t + j];
+      f32x4 p = zero;
 #pragma unroll
       for (int i = 0; i < S; ++i) {
         const f32x4 m = *(const f32x4*)(sB + (j * S + i) * kRow + t);
-        if (kMode == kBack) {
-#pragma unroll
-          for (int q = 3; q >= 0; --q) h[i] = __builtin_amdgcn_exp2f(d[q] * A2[i]) * (m[q] * v[q] + h[i]);
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            h[i] = __builtin_amdgcn_exp2f(d[q] * A2[i]) * h[i] + m[q] * v[q];
-            if (kMode == kOut) p[q] += sC[(j * S + i) * kRow + t + q] * h[i];
+        f32x4 r = zero;
+        if (kMode == kOut) r = *(const f32x4*)(sC + (j * S + i) * kRow + t);
+        unrolled<4>([&](auto index) {
+          constexpr int q = kMode == kBack ? 3 - decltype(index)::value : decltype(index)::value;
+          const float a = __builtin_amdgcn_exp2f(from_quad<q>(d) * A2[i]);
+          if (kMode == kBack) {
+            h[i] = a * __builtin_fmaf(from_quad<q>(v), m[q], h[i]);
+          } else {
+            h[i] = __builtin_fmaf(from_quad<q>(v), m[q], a * h[i]);
+            if (kMode == kOut) p[q] = __builtin_fmaf(r[q], h[i], p[q]);
           }
-        }
+        });
       }
-      if (kMode != kOut) {
-        total += (d[0] + d[1]) + (d[2] + d[3]);
-      } else {
-        const float y = sum4<L>(p, lane);
-        if (j < 4) sy[c_local * kRow + t + j] = y;
-      }
+      if (kMode != kOut)
+        total += d;
+      else
+        sy[c_local * kChannelRow + t + j] = quad_sums(p, lane);
     }
     __syncthreads();
     if (kMode == kOut) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const int at = threadIdx.x + 256 * i, e = at % (kChannels / 4) * 4, t = at / (kChannels / 4);
+        const int t = et + i * (K / kPer);
         const int64_t token = tile * K + t;
-        if (at >= kChannels / 4 * K || token >= s.tokens || c_first + e >= c_end) continue;
-        const bool there = token < length;
+        if (!mine || token >= s.tokens) continue;
+        const bool there = t < left;
         f32x4 y;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          y[q] = sy[(e + q) * kRow + t] + (s.D ? s.D[c_first + e + q] * keep_u[i][q] : 0.f);
-          if (!there) y[q] = 0.f;
-        }
-        const int64_t to = (b * s.tokens + token) * s.channels + c_first + e;
+        for (int q = 0; q < 4; ++q)
+          y[q] = there ? sy[(e + q) * kChannelRow + t] + skip[q] * keep_u[i][q] : 0.f;
+        const int64_t to = (b * s.tokens + token) * s.channels + cc;
         if (s.raw) store4(s.raw + to, y);
         if (s.z.p) {
 #pragma unroll
@@ -261,14 +320,16 @@ __global__ __launch_bounds__(256) void scan_walk_kernel(Scan s) {
       }
     }
   }
-  if (!live) return;
   if (kMode == kOut) {
-    if (s.state_out && chunk == s.chunks - 1) {
+    if (live && s.state_out && chunk == s.chunks - 1) {
 #pragma unroll
       for (int i = 0; i < S; ++i) s.state_out[(b * s.channels + c) * N + j * S + i] = h[i];
     }
     return;
   }
+  total += from_lane<0xB1>(total);
+  total += from_lane<0x4E>(total);
+  if (!live) return;
   const int64_t at = (b * s.chunks + chunk) * s.channels + c;
 #pragma unroll
   for (int i = 0; i < S; ++i) s.carry[at * N + j * S + i] = h[i];
@@ -320,7 +381,8 @@ __global__ __launch_bounds__(256) void scan_step_kernel(Scan s) {
     const f32x4 B = load4((const T*)s.B.p + b * s.B.sb + group * s.B.sg + n);
     const f32x4 C = load4((const T*)s.C.p + b * s.C.sb + group * s.C.sg + n);
     u = (float)((const T*)s.u.p)[b * s.u.sb + c];
-    const float d = step_of((float)((const T*)s.dt.p)[b * s.dt.sb + c] + (s.dt_bias ? s.dt_bias[c] : 0.f), s.softplus);
+    float d = (float)((const T*)s.dt.p)[b * s.dt.sb + c] + (s.dt_bias ? s.dt_bias[c] : 0.f);
+    if (s.softplus) d = step_of(d);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       h[i] = __builtin_amdgcn_exp2f(d * (A[i] * kLog2e)) * h[i] + d * u * B[i];
@@ -342,36 +404,40 @@ __global__ __launch_bounds__(256) void scan_step_kernel(Scan s) {
 
 // ------------------------------------------------------------------ gradient
 
-// A block takes a span of a group's channels and a range of tiles.  A lane has one state and, wave by wave, channel
-// after channel: B, C and the sums dB, dC of its state stay in its registers over a tile, h and a of a channel over its
-// 32 tokens.  dA, dD and the bias's sums stay in LDS over the range.
+// A block takes a span of a group's channels and a range of tiles.  A lane has one state (of 8 states every second lane
+// none) and, pass by pass, channel after channel: the sums dB, dC of its state stay in its registers over a tile, h and a
+// of a channel over its 32 tokens.  A token's d, d u and dy stay with lane t % 16 of each row of 16, from where the others
+// take them.  dA, dD and the bias's sums stay in LDS over the range.
 template <typename T, int N>
 __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(Scan s) {
-  constexpr int kSlots = 64 / N, kPasses = kSlice / (4 * kSlots);
+  constexpr int NP = N < 16 ? 16 : N, kSlots = 64 / NP, kPasses = kSlice / (4 * kSlots);
   constexpr int kStage = 5 * kSlice * kRow, kJoin = 4 * K * N;
   __shared__ __align__(16) float lds[kStage > kJoin ? kStage : kJoin];
+  __shared__ __align__(16) float sB[NP * kRow], sC[NP * kRow];
   extern __shared__ __align__(16) float span_sums[];  // dA [span][N], dD [span], dbias [span]
   float *sd = lds, *sv = sd + kSlice * kRow, *sy = sv + kSlice * kRow, *s1 = sy + kSlice * kRow, *s2 = s1 + kSlice * kRow;
   float *aA = span_sums, *aD = aA + s.span * N, *ab = aD + s.span;
-  int64_t block = block_index();
+  uint32_t block = block_index();
   if (block >= s.blocks) return;
-  const int span = (int)(block % s.spans);
-  block /= s.spans;
-  const int group = (int)(block % s.groups);
-  block /= s.groups;
-  const int range = (int)(block % s.ranges);
-  const int64_t b = block / s.ranges, length = length_of(s, b);
+  const int span = (int)(block % (uint32_t)s.spans);
+  block /= (uint32_t)s.spans;
+  const int group = (int)(block % (uint32_t)s.groups);
+  block /= (uint32_t)s.groups;
+  const int range = (int)(block % (uint32_t)s.ranges);
+  const int64_t b = block / (uint32_t)s.ranges, length = length_of(s, b);
   const int c_first = group * s.group_channels + span * s.span;
   const int c_end = min(c_first + s.span, (group + 1) * s.group_channels);
-  const int lane = lane_id(), wave = threadIdx.x >> 6, n = lane_state<N>(lane), slot = lane_slot<N>(lane);
+  const int lane = lane_id(), wave = threadIdx.x >> 6, n = lane % NP, slot = lane / NP, r = lane & 15;
+  const bool held = n < N;
   for (int i = threadIdx.x; i < s.span * (N + 2); i += 256) span_sums[i] = 0.f;
 
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   const int e = threadIdx.x % (kSlice / 4) * 4, et = threadIdx.x / (kSlice / 4);  // this thread's element of a slice
   const int64_t tile0 = (int64_t)range * s.range_tiles, tile1 = min(tile0 + s.range_tiles, s.tiles);
   for (int64_t tile = tile0; tile < tile1; ++tile) {
     const int64_t token = tile * K + et;
+    const int64_t maps = (((int64_t)(s.whole ? 0 : span) * s.batch + b) * s.tokens + tile * K) * s.groups * N + group * N;
     if (tile * K >= length) {  // nothing here depends on anything
-      const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
       if (token < s.tokens) {
         for (int cc = c_first + e; cc < c_end; cc += kSlice) {
           const int64_t at = (b * s.tokens + token) * s.channels + cc;
@@ -381,9 +447,8 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(Scan s) {
         }
       }
       for (int i = threadIdx.x; i < K * N; i += 256) {
-        const int64_t t = tile * K + i / N;
-        if (t >= s.tokens) continue;
-        const int64_t at = (((int64_t)(s.whole ? 0 : span) * s.batch + b) * s.tokens + t) * s.groups * N + group * N + i % N;
+        if (tile * K + i / N >= s.tokens) continue;
+        const int64_t at = maps + (int64_t)(i / N) * s.groups * N + i % N;
         if (s.whole) {
           if (s.dB_out) ((T*)s.dB_out)[at] = (T)0.f;
           if (s.dC_out) ((T*)s.dC_out)[at] = (T)0.f;
@@ -393,103 +458,143 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(Scan s) {
       }
       continue;
     }
-    float Bm[K], Cm[K], accB[K], accC[K];
-#pragma unroll
-    for (int t = 0; t < K; ++t) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < K * NP; i += 256) {
+      const int t = i / NP, m = i % NP;
       const int64_t at = tile * K + t;
-      const bool there = at < length;
-      Bm[t] = there ? load_f((const T*)s.B.p + b * s.B.sb + at * s.B.st + group * s.B.sg + n) : 0.f;
-      Cm[t] = there ? load_f((const T*)s.C.p + b * s.C.sb + at * s.C.st + group * s.C.sg + n) : 0.f;
-      accB[t] = accC[t] = 0.f;
+      const bool there = at < length && m < N;
+      sB[m * kRow + t] = there ? load_f((const T*)s.B.p + b * s.B.sb + at * s.B.st + group * s.B.sg + m) : 0.f;
+      sC[m * kRow + t] = there ? load_f((const T*)s.C.p + b * s.C.sb + at * s.C.st + group * s.C.sg + m) : 0.f;
     }
-    for (int c0 = c_first; c0 < c_end; c0 += kSlice) {
-      const bool there = token < length && c0 + e < c_end, inside = token < s.tokens && c0 + e < c_end;
-      const int64_t at = (b * s.tokens + token) * s.channels + c0 + e;
-      const f32x4 u = row4<T>(s.u, b, token, c0 + e, there), z = row4<T>(s.z, b, token, c0 + e, there && s.z.p);
-      f32x4 x = row4<T>(s.dt, b, token, c0 + e, there), d, dy, dz;
-      dy = there && s.dout ? load4((const T*)s.dout + at) : f32x4{0.f, 0.f, 0.f, 0.f};
-      const f32x4 raw = there && s.z.p ? load4(s.raw + at) : f32x4{0.f, 0.f, 0.f, 0.f};
+    float accB[K], accC[K];
+#pragma unroll
+    for (int t = 0; t < K; ++t) accB[t] = accC[t] = 0.f;
+    // uniform addresses of the tile and this thread's offsets from them (a token's stride is below 2^26 elements)
+    const int64_t first = b * s.tokens + tile * K;
+    const T *u_at = (const T*)s.u.p + b * s.u.sb + tile * K * s.u.st + c_first;
+    const T *dt_at = (const T*)s.dt.p + b * s.dt.sb + tile * K * s.dt.st + c_first;
+    const T *z_at = (const T*)s.z.p + b * s.z.sb + tile * K * s.z.st + c_first;
+    const uint32_t u_of = (uint32_t)et * (uint32_t)s.u.st + e, dt_of = (uint32_t)et * (uint32_t)s.dt.st + e;
+    const uint32_t z_of = (uint32_t)et * (uint32_t)s.z.st + e, of = (uint32_t)et * (uint32_t)s.channels + e;
+    const bool here = token < length;
+    for (int c0 = 0; c0 < c_end - c_first; c0 += kSlice) {
+      const bool mine = c0 + e < c_end - c_first, there = here && mine, inside = token < s.tokens && mine;
+      const int64_t row = first * s.channels + c_first + c0;
+      f32x4 u = zero, x = zero, dy = zero, z = zero, raw = zero, bias = zero;
+      if (there) {
+        u = load4(u_at + c0 + u_of), x = load4(dt_at + c0 + dt_of), dy = load4((const T*)s.dout + row + of);
+        if (s.dt_bias) bias = load4(s.dt_bias + c_first + c0 + e);
+        if (s.z.p) z = load4(z_at + c0 + z_of), raw = load4(s.raw + row + of);
+      }
       __syncthreads();
+      // a token that is not there has u, dy and z zero, and takes no step
+      x += bias;
+      f32x4 d = x;
+      if (s.softplus) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) d[q] = step_of(x[q]);
+      }
+      d = d * (there ? 1.f : 0.f);
+      if (s.z.p) {
+        f32x4 dz;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const float sg = sigmoid_f(z[q]);
+          dz[q] = dy[q] * raw[q] * (sg + z[q] * sg * (1.f - sg));
+          dy[q] = dy[q] * z[q] * sg;
+        }
+        if (s.dz && inside) store4((T*)s.dz + row + of, dz);
+      }
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        x[q] += there && s.dt_bias ? s.dt_bias[c0 + e + q] : 0.f;
-        d[q] = there ? step_of(x[q], s.softplus) : 0.f;
-        if (s.z.p) {
-          const float sg = sigmoid_f(z[q]);
-          dz[q] = there ? dy[q] * raw[q] * (sg + z[q] * sg * (1.f - sg)) : 0.f;
-          dy[q] = there ? dy[q] * z[q] * sg : 0.f;
-        }
         sd[(e + q) * kRow + et] = d[q];
         sv[(e + q) * kRow + et] = d[q] * u[q];
         sy[(e + q) * kRow + et] = dy[q];
       }
-      if (s.dz && inside) store4((T*)s.dz + at, dz);
       __syncthreads();
       for (int pass = 0; pass < kPasses; ++pass) {
-        const int cl = (pass * 4 + wave) * kSlots + slot, c = c0 + cl;
-        const bool live = c < c_end;
+        const int cl = (pass * 4 + wave) * kSlots + slot, c = c_first + c0 + cl;
+        const bool live = c < c_end && held;
         const int64_t from = ((b * s.tiles + tile) * s.channels + c) * N + n;
         const float A = live ? s.A[(int64_t)c * N + n] : 0.f, A2 = A * kLog2e;
         const float h0 = live ? s.h_in[from] : 0.f;
         float X = live ? s.x_in[from] : 0.f, dA = 0.f;
-        float h[K], a[K];
-#pragma unroll
-        for (int t = 0; t < K; t += 4) {
-          const f32x4 dl = *(const f32x4*)(sd + cl * kRow + t), vl = *(const f32x4*)(sv + cl * kRow + t);
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            a[t + q] = __builtin_amdgcn_exp2f(dl[q] * A2);
-            h[t + q] = a[t + q] * (t + q ? h[t + q ? t + q - 1 : 0] : h0) + Bm[t + q] * vl[q];
+        // d as an operand from the lanes of a row in the exponent; in multiply-adds, which take none, from LDS
+        const float dl[2] = {sd[cl * kRow + r], sd[cl * kRow + 16 + r]};
+        float h[K], a[K], last = h0;
+        unrolled<K / 4>([&](auto quad) {
+          constexpr int t0 = decltype(quad)::value * 4;
+          const f32x4 v = *(const f32x4*)(sv + cl * kRow + t0), m = *(const f32x4*)(sB + n * kRow + t0);
+          unrolled<4>([&](auto index) {
+            constexpr int q = decltype(index)::value, t = t0 + q;
+            a[t] = __builtin_amdgcn_exp2f(from_row<t % 16>(dl[t / 16]) * A2);
+            h[t] = last = __builtin_fmaf(v[q], m[q], a[t] * last);
+          });
+          __builtin_amdgcn_sched_barrier(0);
+        });
+        RowSum sum1, sum2;
+        unrolled<K / 4>([&](auto quad) {
+          constexpr int t0 = K - 4 - decltype(quad)::value * 4;
+          const f32x4 m = *(const f32x4*)(sB + n * kRow + t0), o = *(const f32x4*)(sC + n * kRow + t0);
+          const f32x4 d = *(const f32x4*)(sd + cl * kRow + t0), v = *(const f32x4*)(sv + cl * kRow + t0);
+          const f32x4 y = *(const f32x4*)(sy + cl * kRow + t0);
+          unrolled<4>([&](auto index) {
+            constexpr int q = 3 - decltype(index)::value, t = t0 + q, in = t % 16;
+            const float G = __builtin_fmaf(y[q], o[q], X);
+            accC[t] = __builtin_fmaf(y[q], h[t], accC[t]);
+            accB[t] = __builtin_fmaf(v[q], G, accB[t]);
+            asm volatile("" : "+v"(accB[t]), "+v"(accC[t]));  // here, not sunk behind the pass with all that they need
+            X = a[t] * G;
+            const float back = X * (t ? h[t ? t - 1 : 0] : h0);
+            dA = __builtin_fmaf(d[q], back, dA);
+            sum1.add<15 - in>(G * m[q], lane);
+            sum2.add<15 - in>(A * back, lane);
+          });
+          if constexpr (t0 % 16 == 0) {
+            float r1 = sum1.held[3], r2 = sum2.held[3];
+            if (N >= 32) r1 += xor16(r1), r2 += xor16(r2);
+            if (N == 64) r1 = xor32_sum(r1), r2 = xor32_sum(r2);
+            if (N <= 16 || n < 16) {
+              s1[cl * kRow + t0 + 15 - rev4(r)] = r1;
+              s2[cl * kRow + t0 + 15 - rev4(r)] = r2;
+            }
           }
-        }
-#pragma unroll
-        for (int t = K - 4; t >= 0; t -= 4) {
-          const f32x4 dl = *(const f32x4*)(sd + cl * kRow + t), vl = *(const f32x4*)(sv + cl * kRow + t);
-          const f32x4 yl = *(const f32x4*)(sy + cl * kRow + t);
-          f32x4 p1, p2;
-#pragma unroll
-          for (int q = 3; q >= 0; --q) {
-            const float G = Cm[t + q] * yl[q] + X;
-            accC[t + q] += yl[q] * h[t + q];
-            accB[t + q] += G * vl[q];
-            p1[q] = G * Bm[t + q];
-            X = a[t + q] * G;
-            const float back = X * (t + q ? h[t + q ? t + q - 1 : 0] : h0);
-            dA += dl[q] * back;
-            p2[q] = A * back;
-          }
-          const float r1 = sum4<N>(p1, lane), r2 = sum4<N>(p2, lane);
-          if (n < 4) {
-            s1[cl * kRow + t + n] = r1;
-            s2[cl * kRow + t + n] = r2;
-          }
-        }
+          __builtin_amdgcn_sched_barrier(0);
+        });
         if (live) aA[(c - c_first) * N + n] += dA;
       }
       __syncthreads();
-      f32x4 du, ddt;
+      {
+        f32x4 du, ddt, skip = zero;
+        if (s.D && mine) skip = load4(s.D + c_first + c0 + e);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float g = s1[(e + q) * kRow + et], D = s.D && inside ? s.D[c0 + e + q] : 0.f;
-        du[q] = there ? d[q] * g + D * dy[q] : 0.f;
-        float slope = 1.f;
-        if (s.softplus) slope = sigmoid_f(x[q]);
-        ddt[q] = there ? (u[q] * g + s2[(e + q) * kRow + et]) * slope : 0.f;
-        s1[(e + q) * kRow + et] = there ? dy[q] * u[q] : 0.f;
-        s2[(e + q) * kRow + et] = ddt[q];
+        for (int q = 0; q < 4; ++q) {
+          const int i = (e + q) * kRow + et;
+          const float g = s1[i], y = sy[i];
+          du[q] = there ? sd[i] * g + skip[q] * y : 0.f;
+          ddt[q] = there ? u[q] * g + s2[i] : 0.f;
+          s1[i] = there ? y * u[q] : 0.f;
+        }
+        if (s.softplus) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) ddt[q] *= sigmoid_f(x[q]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s2[(e + q) * kRow + et] = ddt[q];
+        if (inside && s.du) store4((T*)s.du + row + of, du);
+        if (inside && s.ddt) store4((T*)s.ddt + row + of, ddt);
       }
-      if (inside && s.du) store4((T*)s.du + at, du);
-      if (inside && s.ddt) store4((T*)s.ddt + at, ddt);
       __syncthreads();
       // sums over the tile's tokens: four lanes a channel, 8 tokens each; dD by the first two waves, the bias's by the others
       {
         const int which = threadIdx.x >> 7, cl = threadIdx.x % 128 / 4, quarter = threadIdx.x % 4;
         const float* from = (which ? s2 : s1) + cl * kRow + 8 * quarter;
-        const f32x4 p = *(const f32x4*)from, q = *(const f32x4*)(from + 4);
-        float v = ((p[0] + p[1]) + (p[2] + p[3])) + ((q[0] + q[1]) + (q[2] + q[3]));
-        v += dpp<0xB1>(v);
-        v += dpp<0x4E>(v);
-        if (quarter == 0 && c0 + cl < c_end) (which ? ab : aD)[c0 - c_first + cl] += v;
+        float v = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v += from[i];
+        v += from_lane<0xB1>(v);
+        v += from_lane<0x4E>(v);
+        if (quarter == 0 && c_first + c0 + cl < c_end) (which ? ab : aD)[c0 + cl] += v;
       }
     }
     // the slots' and waves' sums of dB, then dC
@@ -499,21 +604,19 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(Scan s) {
 #pragma unroll
       for (int t = 0; t < K; ++t) {
         float v = which ? accC[t] : accB[t];
-        if (N == 8) v += __int_as_float(__builtin_amdgcn_ds_swizzle(__float_as_int(v), 0x101F));  // xor 4
-        if (N <= 16) v += xor16(v);
-        if (N <= 32) v = xor32_sum(v);
-        if (slot == 0) lds[(wave * K + t) * N + n] = v;
+        if (NP == 16) v += xor16(v);
+        if (NP <= 32) v = xor32_sum(v);
+        if (slot == 0 && held) lds[(wave * K + t) * N + n] = v;
       }
       __syncthreads();
       for (int i = threadIdx.x; i < K * N; i += 256) {
         const float v = (lds[i] + lds[K * N + i]) + (lds[2 * K * N + i] + lds[3 * K * N + i]);
-        const int64_t t = tile * K + i / N;
-        if (t >= s.tokens) continue;
-        const int64_t to = (((int64_t)(s.whole ? 0 : span) * s.batch + b) * s.tokens + t) * s.groups * N + group * N + i % N;
+        if (tile * K + i / N >= s.tokens) continue;
+        const int64_t at = maps + (int64_t)(i / N) * s.groups * N + i % N;
         if (!s.whole)
-          (which ? s.dC : s.dB)[to] = v;
+          (which ? s.dC : s.dB)[at] = v;
         else if (which ? s.dC_out : s.dB_out)
-          ((T*)(which ? s.dC_out : s.dB_out))[to] = (T)v;
+          ((T*)(which ? s.dC_out : s.dB_out))[at] = (T)v;
       }
     }
   }
@@ -567,16 +670,12 @@ void with_states(int64_t states, Go go) {
   return go(integral_constant<int, 64>());
 }
 
-// Lanes of a channel where chunks are walked: four states each (of eight states two).
-constexpr int walk_lanes(int states) { return states <= 16 ? 4 : states / 4; }
-
 struct Chunks {
   int64_t chunks, tiles;  // tiles of a chunk
 };
 // One chunk where the channels alone make 768 blocks (three waves a SIMD), else about 1536 blocks.
 Chunks plan_chunks(int64_t batch, int64_t tokens, int64_t channels, int64_t states, int64_t groups) {
-  const int64_t per = 256 / walk_lanes((int)states), tiles = (tokens + K - 1) / K;
-  const int64_t blocks = batch * groups * ((channels / groups + per - 1) / per);
+  const int64_t tiles = (tokens + K - 1) / K, blocks = batch * groups * ((channels / groups + kWalk - 1) / kWalk);
   if (blocks >= 768 || tiles <= 2) return {1, tiles};
   int64_t chunks = (1536 + blocks - 1) / blocks;
   if (chunks > tiles) chunks = tiles;
@@ -644,14 +743,14 @@ template <typename T, int kMode>
 int walk(Scan s, hipStream_t stream) {
   int rc = BMX_OK;
   with_states(s.states, [&](auto n) {
-    constexpr int N = decltype(n)::value, L = walk_lanes(N);
-    s.cblocks = (s.group_channels + 256 / L - 1) / (256 / L);
+    constexpr int N = decltype(n)::value;
+    s.cblocks = (s.group_channels + kWalk - 1) / kWalk;
     s.blocks = s.batch * s.chunks * s.groups * s.cblocks;
     if (s.blocks >= (1ll << 31)) {
       rc = set_error(BMX_EINVAL, "selective_scan: too many rows");
       return;
     }
-    scan_walk_kernel<T, N, L, kMode><<<fold_grid(s.blocks, 256), 256, 0, stream>>>(s);
+    scan_walk_kernel<T, N, kMode><<<fold_grid(s.blocks, 256), 256, 0, stream>>>(s);
   });
   return rc ? rc : check_launch("selective_scan");
 }
