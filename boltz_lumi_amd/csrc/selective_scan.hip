@@ -11,9 +11,9 @@
 // sum of its steps d (its decay is exp(A sum d)), a second carries states from
 // chunk to chunk, a third walks the chunks again from where they really start.
 // Where channels alone fill the card there is one chunk and only the third.
-// Backward, X goes through the first two passes from the end, a tile a chunk; a
-// tile then has its entering h (kept by the forward pass) and X and is worked
-// out on its own.  States, sums and statistics are fp32; tokens from a
+// Backward, X goes through the first two passes from the end; a chunk then has the
+// X that comes to it and, tile by tile, the h that the forward pass kept, and is
+// worked out on its own.  States, sums and statistics are fp32; tokens from a
 // sequence's length on take no step (d = 0), are never read and give zeros.
 #include <type_traits>
 #include <utility>
@@ -26,10 +26,11 @@ namespace {
 
 constexpr int K = 32;             // tokens of a tile
 constexpr int kRow = K + 4;       // LDS row of a state's map over a tile: 16-byte reads along the tokens, no conflicts
+constexpr int KG = 16;            // tokens of a tile of the gradient, which keeps that many states and decays in registers
+constexpr int kGradRow = KG + 4;
 constexpr int kChannelRow = K + 2;  // LDS row of a channel: reads without conflicts, transposing writes two on a bank
-constexpr int kWalk = 64;         // channels of a block that walks chunks, four lanes each
-constexpr int kSlice = 32;        // channels that the gradient stages at a time
-constexpr int kMaxSpan = 6144;    // channels x states of a gradient block (its dA in LDS)
+constexpr int kSlice = 16;        // channels that a wave of the gradient stages at a time
+constexpr int kMaxSpan = 2048;    // channels x states of a gradient block (X and dA in LDS), but at least 64 channels
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Operand {
@@ -43,13 +44,14 @@ struct Scan {
   void* out;
   float *state_out, *raw;   // raw: y before its gate, for the gradient
   float *carry, *steps;     // [batch][chunks][channels][states] and [batch][chunks][channels]
-  float* saved;             // [batch][tiles][channels][states]: h at every tile's start
+  float* saved;             // [batch][grad_tiles][channels][states]: h where every tile of the gradient begins
   const float *h_in, *x_in;
   void *du, *ddt, *dz;
   float *dB, *dC;           // [spans][batch][tokens][groups][states], or the results where there is one span
   void *dB_out, *dC_out;
   float *dA, *dD, *dbias;   // partial sums, [batch * ranges][channels]([states])
-  int64_t batch, tokens, tiles, chunks, chunk_tiles, blocks;
+  int64_t batch, tokens, tiles, grad_tiles, chunks, chunk_tiles, blocks;
+  uint32_t eighth;  // blocks of an XCD
   int channels, groups, group_channels, states, cblocks, lengths64, softplus;
   int span, spans, ranges, range_tiles, whole;
 };
@@ -62,17 +64,16 @@ __device__ __forceinline__ int64_t length_of(const Scan& s, int64_t b) {
   return n < 0 ? 0 : n < s.tokens ? n : s.tokens;
 }
 
-// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|), with log(1 + e) = 2 atanh(r), r = e / (2 + e) <= 1 / 3, by the
-// series of atanh to r^13: what is left is below 2^-25 of it, however small e is.
+// softplus(x) = max(x, 0) + log1p(e), e = exp(-|x|), with log(1 + e) = 2 atanh(r), r = e / (2 + e) <= 1 / 3, and
+// 2 atanh(r) / r a polynomial of degree four in r^2, within 4.0e-09 of it on [0, 1 / 9]: relative to log1p(e) itself,
+// however small e is.
 __device__ __forceinline__ float step_of(float x) {
   const float e = __builtin_amdgcn_exp2f(-fabsf(x) * kLog2e);
   const float r = e * __builtin_amdgcn_rcpf(2.f + e), q = r * r;
-  float s = 2.f / 13.f;
-  s = s * q + 2.f / 11.f;
-  s = s * q + 2.f / 9.f;
-  s = s * q + 2.f / 7.f;
-  s = s * q + 2.f / 5.f;
-  s = s * q + 2.f / 3.f;
+  float s = 0.281783193f;
+  s = s * q + 0.279606074f;
+  s = s * q + 0.400249094f;
+  s = s * q + 0.66666317f;
   s = s * q + 2.f;
   return s * r + fmaxf(x, 0.f);
 }
@@ -107,12 +108,29 @@ __device__ __forceinline__ float xor32_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Sums of four values over a quad; lane j gets the one of value j.
-__device__ __forceinline__ float quad_sums(const f32x4& p, int lane) {
+// L lanes of a channel share its states, in the low bits of the lane, except that eight take the bits 0, 1 and 3: a sum
+// over them then is two exchanges within quads and one over 8 lanes of a row.
+template <int L>
+__device__ __forceinline__ int lane_state(int lane) {
+  return L == 8 ? (lane & 3) | (lane >> 1 & 4) : lane % L;
+}
+template <int L>
+__device__ __forceinline__ int lane_slot(int lane) {
+  return L == 8 ? (lane >> 2 & 1) | (lane >> 3 & 6) : lane / L;
+}
+
+// Sums of four values over the L >= 4 lanes of a channel; lane j gets the one of value j % 4.
+template <int L>
+__device__ __forceinline__ float sum4(const f32x4& p, int lane) {
   const bool odd = lane & 1, high = lane & 2;
   const float a = (odd ? p[1] : p[0]) + from_lane<0xB1>(odd ? p[0] : p[1]);
   const float b = (odd ? p[3] : p[2]) + from_lane<0xB1>(odd ? p[2] : p[3]);
-  return (high ? b : a) + from_lane<0x4E>(high ? a : b);
+  float v = (high ? b : a) + from_lane<0x4E>(high ? a : b);
+  if (L >= 16) v += from_lane<0x124>(v);  // row_ror:4
+  if (L >= 8) v += from_lane<0x128>(v);   // row_ror:8
+  if (L >= 32) v += xor16(v);
+  if (L == 64) v = xor32_sum(v);
+  return v;
 }
 
 // Sums of 16 values over the 16 lanes of a row, one value after another; lane j gets the one of value rev4(j), j's four
@@ -142,10 +160,35 @@ struct RowSum {
   }
 };
 
-// Four channels of one token as fp32; zeros where they are not there.
+// Four values as they lie in memory: a load in flight holds no more registers than it has bytes.  Addresses are a uniform
+// base and a lane's bytes from it, which fit 32 bits (a token's stride is below 2^25 elements, a tile 32 tokens).
 template <typename T>
-__device__ __forceinline__ f32x4 row4(const Operand& o, int64_t b, int64_t t, int c, bool there) {
-  return there ? load4((const T*)o.p + b * o.sb + t * o.st + c) : f32x4{0.f, 0.f, 0.f, 0.f};
+struct Four;
+template <>
+struct Four<float> {
+  f32x4 v;
+  __device__ __forceinline__ f32x4 wide() const { return v; }
+};
+template <>
+struct Four<bf16> {
+  bf16x4 v;
+  __device__ __forceinline__ f32x4 wide() const { return f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]}; }
+};
+template <typename T>
+__device__ __forceinline__ Four<T> four(const T* base, uint32_t bytes, bool there) {
+  Four<T> o = {};
+  if (there) o = *(const Four<T>*)((const char*)base + bytes);
+  return o;
+}
+template <typename T>
+__device__ __forceinline__ void put4(T* base, uint32_t bytes, const f32x4& v) {
+  store4((T*)((char*)base + bytes), v);
+}
+
+// Between a wave's LDS writes and its other lanes' reads: the LDS keeps a wave's order, the compiler has to.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 // ------------------------------------------------------------ walking chunks
@@ -154,12 +197,15 @@ __device__ __forceinline__ f32x4 row4(const Operand& o, int64_t b, int64_t t, in
 // chunk's end, of dy in the place of d u and of C in the place of B.
 enum Mode { kLocal, kOut, kBack };
 
-template <typename T, int N, int kMode>
-__global__ __launch_bounds__(256) void scan_walk_kernel(Scan s) {
-  constexpr int S = N / 4, kPer = kWalk * K / 4 / 256, kMaps = (N * K / 4 + 255) / 256;
+template <typename T, int N, int L, int kMode>
+__global__ __launch_bounds__(256, 4) void scan_walk_kernel(Scan s) {
+  constexpr int S = N / L, kWalk = 256 / L, kPer = (kWalk * K / 4 + 255) / 256, kMaps = (N * K / 4 + 255) / 256;
+  constexpr int kStep = K / kPer, kMapStep = 1024 / N;  // tokens between a thread's elements, and between its maps'
   __shared__ float sd[kWalk * kChannelRow], sv[kWalk * kChannelRow], sy[kMode == kOut ? kWalk * kChannelRow : 4];
   __shared__ __align__(16) float sB[N * kRow], sC[kMode == kOut ? N * kRow : 4];
+  // Neighbours in channels read the same lines: they are dealt to one XCD, one after another.
   uint32_t block = block_index();
+  block = block % 8 * s.eighth + block / 8;
   if (block >= s.blocks) return;
   const int cblock = (int)(block % (uint32_t)s.cblocks);
   block /= (uint32_t)s.cblocks;
@@ -169,46 +215,51 @@ __global__ __launch_bounds__(256) void scan_walk_kernel(Scan s) {
   const int c_first = group * s.group_channels + cblock * kWalk;
   const int c_end = min(c_first + kWalk, (group + 1) * s.group_channels);
   const int64_t length = length_of(s, b);
-  const int lane = lane_id(), j = threadIdx.x & 3, c_local = threadIdx.x >> 2, c = c_first + c_local;
+  const int lane = lane_id(), j = lane_state<L>(lane), jq = lane & 3;
+  const int c_local = (threadIdx.x >> 6) * (64 / L) + lane_slot<L>(lane), c = c_first + c_local;
   const bool live = c < c_end;
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 
+  // tiles of this chunk that have tokens, and those behind them, which states pass
   const int64_t tile0 = chunk * s.chunk_tiles, tile1 = min(tile0 + s.chunk_tiles, s.tiles);
-  const int64_t start = kMode == kBack ? tile1 - 1 : tile0;
+  const int64_t tile_end = max(tile0, min(tile1, (length + K - 1) / K));
+
   // this thread's elements of a tile: four channels of kPer tokens, and of the maps four states of kMaps tokens
   const int e = threadIdx.x % (kWalk / 4) * 4, et = threadIdx.x / (kWalk / 4), cc = c_first + e;
   const int en = threadIdx.x % (N / 4) * 4, ent = threadIdx.x / (N / 4);
-  const bool mine = cc < c_end;
-  const int64_t dense = (b * s.tokens + start * K + et) * s.channels + cc;
-  const T *dt = (const T*)s.dt.p + b * s.dt.sb + (start * K + et) * s.dt.st + cc, *u = (const T*)s.u.p, *z = (const T*)s.z.p;
-  u = kMode == kBack ? (const T*)s.dout + dense : u + b * s.u.sb + (start * K + et) * s.u.st + cc;
-  z = z ? z + b * s.z.sb + (start * K + et) * s.z.st + cc : nullptr;
-  const int64_t u_st = kMode == kBack ? s.channels : s.u.st;
-  const T* B = (const T*)s.B.p + b * s.B.sb + (start * K + ent) * s.B.st + group * s.B.sg + en;
-  const T* C = (const T*)s.C.p + b * s.C.sb + (start * K + ent) * s.C.st + group * s.C.sg + en;
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  f32x4 ru[kPer], rdt[kPer], rz[kPer], rB[kMaps], rC[kMaps];
+  const bool mine = cc < c_end && et < K;
+  const uint32_t size = sizeof(T), u_st = kMode == kBack ? s.channels : (uint32_t)s.u.st;
+  const uint32_t u_of = (et * u_st + e) * size, dt_of = (et * (uint32_t)s.dt.st + e) * size;
+  const uint32_t z_of = (et * (uint32_t)s.z.st + e) * size, of = et * (uint32_t)s.channels + e;
+  const uint32_t B_of = (ent * (uint32_t)s.B.st + en) * size, C_of = (ent * (uint32_t)s.C.st + en) * size;
+  const bool gate_grad = kMode == kBack && s.dz;
+  Four<T> ru[kPer], rdt[kPer], rz[kPer], rB[kMaps], rC[kMaps];
+  f32x4 rraw[kPer];
   auto fetch = [&](int64_t tile) {
-    const int64_t left = length - tile * K;
+    const int left = (int)min(length - tile * K, (int64_t)K);
+    const int64_t row = (b * s.tokens + tile * K) * s.channels + c_first;
+    const T* u = kMode == kBack ? (const T*)s.dout + row : (const T*)s.u.p + b * s.u.sb + tile * K * s.u.st + c_first;
+    const T* dt = (const T*)s.dt.p + b * s.dt.sb + tile * K * s.dt.st + c_first;
+    const T* z = (const T*)s.z.p + b * s.z.sb + tile * K * s.z.st + c_first;
+    const T* B = (const T*)s.B.p + b * s.B.sb + tile * K * s.B.st + group * s.B.sg;
+    const T* C = (const T*)s.C.p + b * s.C.sb + tile * K * s.C.st + group * s.C.sg;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int t = i * (K / kPer);
-      const bool there = mine && et + t < left;
-      rdt[i] = there ? load4(dt + t * s.dt.st) : zero;
-      ru[i] = there ? load4(u + t * u_st) : zero;
-      if (kMode != kLocal) rz[i] = there && z ? load4(z + t * s.z.st) : zero;
+      const bool there = mine && et + i * kStep < left;
+      rdt[i] = four(dt + i * kStep * s.dt.st, dt_of, there);
+      ru[i] = four(u + (int64_t)(i * kStep) * u_st, u_of, there);
+      if (kMode != kLocal) rz[i] = four(z + i * kStep * s.z.st, z_of, there && s.z.p);
+      if (kMode == kBack)
+        rraw[i] = four(s.raw + row + (int64_t)(i * kStep) * s.channels, of * 4, there && gate_grad).wide();
     }
 #pragma unroll
     for (int i = 0; i < kMaps; ++i) {
-      const int t = i * (1024 / N);
-      const bool there = ent + t < K && ent + t < left;
-      if (kMode != kBack) rB[i] = there ? load4(B + t * s.B.st) : zero;
-      if (kMode != kLocal) rC[i] = there ? load4(C + t * s.C.st) : zero;
+      const bool there = ent + i * kMapStep < left;
+      if (kMode != kBack) rB[i] = four(B + i * kMapStep * s.B.st, B_of, there);
+      if (kMode != kLocal) rC[i] = four(C + i * kMapStep * s.C.st, C_of, there);
     }
-    const int64_t step = kMode == kBack ? -K : K;
-    dt += step * s.dt.st, u += step * u_st, B += step * s.B.st, C += step * s.C.st;
-    if (z) z += step * s.z.st;
   };
-  fetch(start);
+  if (tile_end > tile0) fetch(kMode == kBack ? tile_end - 1 : tile0);
 
   f32x4 bias = zero, skip = zero;
   if (mine && s.dt_bias) bias = load4(s.dt_bias + cc);
@@ -224,24 +275,43 @@ __global__ __launch_bounds__(256) void scan_walk_kernel(Scan s) {
     A2[i] = live ? s.A[(int64_t)c * N + j * S + i] * kLog2e : 0.f;
     h[i] = live && from ? from[j * S + i] : 0.f;
   }
+  auto save = [&](int64_t tile, int part) {  // h where a tile of the gradient begins
+    const int64_t at = tile * (K / KG) + part;
+    if (kMode != kOut || !s.saved || !live || at >= s.grad_tiles) return;
+    float* to = s.saved + ((b * s.grad_tiles + at) * s.channels + c) * N + j * S;
+#pragma unroll
+    for (int i = 0; i < S; ++i) to[i] = h[i];
+  };
 
-  for (int64_t k = tile0; k < tile1; ++k) {
-    const int64_t tile = kMode == kBack ? tile0 + tile1 - 1 - k : k, left = length - tile * K;
+  for (int64_t k = tile0; k < tile_end; ++k) {
+    const int64_t tile = kMode == kBack ? tile0 + tile_end - 1 - k : k;
+    const int64_t row = (b * s.tokens + tile * K) * s.channels + c_first;
+    const int left = (int)min(length - tile * K, (int64_t)K), inside = (int)min(s.tokens - tile * K, (int64_t)K);
     // d, and d u (kBack: dy), of the tile to LDS, along the tokens; a token that is not there takes no step
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int t = et + i * (K / kPer);
-      f32x4 d = rdt[i] + bias;
+      const int t = et + i * kStep;
+      f32x4 d = rdt[i].wide() + bias, v = ru[i].wide();
       if (s.softplus) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) d[q] = step_of(d[q]);
       }
       d = d * (mine && t < left ? 1.f : 0.f);
-      f32x4 v = kMode == kBack ? ru[i] : d * ru[i];
-      if (kMode == kBack && s.z.p) {
+      if (kMode != kBack) {
+        v = v * d;
+      } else if (s.z.p) {
+        const f32x4 z = rz[i].wide();
+        f32x4 dz;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] *= silu_f(rz[i][q]);
+        for (int q = 0; q < 4; ++q) {
+          const float sg = sigmoid_f(z[q]);
+          dz[q] = v[q] * rraw[i][q] * (sg + z[q] * sg * (1.f - sg));
+          v[q] *= z[q] * sg;
+        }
+        if (gate_grad && mine && t < inside)
+          put4((T*)s.dz + row + (int64_t)(i * kStep) * s.channels, of * size, dz);
       }
+      if (kPer * 256 > kWalk * K / 4 && et >= K) continue;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         sd[(e + q) * kChannelRow + t] = d[q];
@@ -250,32 +320,29 @@ __global__ __launch_bounds__(256) void scan_walk_kernel(Scan s) {
     }
 #pragma unroll
     for (int i = 0; i < kMaps; ++i) {
-      const int t = ent + i * (1024 / N);
+      const int t = ent + i * kMapStep;
       if (t >= K) continue;
+      const f32x4 m = (kMode == kBack ? rC[i] : rB[i]).wide();
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        sB[(en + q) * kRow + t] = kMode == kBack ? rC[i][q] : rB[i][q];
-        if (kMode == kOut) sC[(en + q) * kRow + t] = rC[i][q];
+        sB[(en + q) * kRow + t] = m[q];
+        if (kMode == kOut) sC[(en + q) * kRow + t] = rC[i].wide()[q];
       }
     }
     __syncthreads();
-    f32x4 keep_u[kPer], keep_z[kPer];
+    Four<T> keep_u[kPer], keep_z[kPer];
     if (kMode == kOut) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) keep_u[i] = ru[i], keep_z[i] = rz[i];
     }
-    if (k + 1 < tile1) fetch(kMode == kBack ? tile - 1 : tile + 1);
-    if (kMode == kOut && s.saved && live) {
-      float* to = s.saved + ((b * s.tiles + tile) * s.channels + c) * N + j * S;
-#pragma unroll
-      for (int i = 0; i < S; ++i) to[i] = h[i];
-    }
+    if (k + 1 < tile_end) fetch(kMode == kBack ? tile - 1 : tile + 1);
 
-    // Four tokens at a time: lane j of a channel's quad holds token j's d and d u, which the others take from it.
+    // Four tokens at a time: lane i of a quad holds token i's d and d u, which the others take from it as an operand.
 #pragma unroll 2
     for (int step = 0; step < K; step += 4) {
+      if (step % KG == 0) save(tile, step / KG);
       const int t = kMode == kBack ? K - 4 - step : step;
-      const float d = sd[c_local * kChannelRow + t + j], v = sv[c_local * kChannelRow + t + j];
+      const float d = sd[c_local * kChannelRow + t + jq], v = sv[c_local * kChannelRow + t + jq];
       f32x4 p = zero;
 #pragma unroll
       for (int i = 0; i < S; ++i) {
@@ -285,39 +352,55 @@ __global__ __launch_bounds__(256) void scan_walk_kernel(Scan s) {
         unrolled<4>([&](auto index) {
           constexpr int q = kMode == kBack ? 3 - decltype(index)::value : decltype(index)::value;
           const float a = __builtin_amdgcn_exp2f(from_quad<q>(d) * A2[i]);
+          const float into = from_quad<q>(v) * m[q];  // not fused: a multiply-add takes no other lane's operand
           if (kMode == kBack) {
-            h[i] = a * __builtin_fmaf(from_quad<q>(v), m[q], h[i]);
+            h[i] = a * (into + h[i]);
           } else {
-            h[i] = __builtin_fmaf(from_quad<q>(v), m[q], a * h[i]);
+            h[i] = __builtin_fmaf(a, h[i], into);
             if (kMode == kOut) p[q] = __builtin_fmaf(r[q], h[i], p[q]);
           }
         });
       }
-      if (kMode != kOut)
+      if (kMode != kOut) {
         total += d;
-      else
-        sy[c_local * kChannelRow + t + j] = quad_sums(p, lane);
+      } else {
+        const float y = sum4<L>(p, lane);
+        if (L == 4 || j < 4) sy[c_local * kChannelRow + t + jq] = y;
+      }
     }
     __syncthreads();
     if (kMode == kOut) {
 #pragma unroll
       for (int i = 0; i < kPer; ++i) {
-        const int t = et + i * (K / kPer);
-        const int64_t token = tile * K + t;
-        if (!mine || token >= s.tokens) continue;
+        const int t = et + i * kStep;
+        if (!mine || t >= inside) continue;
         const bool there = t < left;
+        const f32x4 u = keep_u[i].wide();
         f32x4 y;
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          y[q] = there ? sy[(e + q) * kChannelRow + t] + skip[q] * keep_u[i][q] : 0.f;
-        const int64_t to = (b * s.tokens + token) * s.channels + cc;
-        if (s.raw) store4(s.raw + to, y);
+        for (int q = 0; q < 4; ++q) y[q] = there ? sy[(e + q) * kChannelRow + t] + skip[q] * u[q] : 0.f;
+        const int64_t to = row + (int64_t)(i * kStep) * s.channels;
+        if (s.raw) put4(s.raw + to, of * 4, y);
         if (s.z.p) {
+          const f32x4 z = keep_z[i].wide();
 #pragma unroll
-          for (int q = 0; q < 4; ++q) y[q] = there ? y[q] * silu_f(keep_z[i][q]) : 0.f;
+          for (int q = 0; q < 4; ++q) y[q] = there ? y[q] * silu_f(z[q]) : 0.f;
         }
-        store4((T*)s.out + to, y);
+        put4((T*)s.out + to, of * size, y);
       }
+    }
+  }
+
+  for (int64_t tile = tile_end; tile < tile1; ++tile) {
+    if (kMode == kLocal || (kMode == kBack && !gate_grad)) continue;
+    const int64_t row = (b * s.tokens + tile * K) * s.channels + c_first;
+    const int inside = (int)min(s.tokens - tile * K, (int64_t)K);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      if (!mine || et + i * kStep >= inside) continue;
+      const int64_t to = row + (int64_t)(i * kStep) * s.channels;
+      if (kMode == kOut && s.raw) put4(s.raw + to, of * 4, zero);
+      put4((T*)(kMode == kOut ? s.out : s.dz) + to, of * size, zero);
     }
   }
   if (kMode == kOut) {
@@ -337,32 +420,55 @@ __global__ __launch_bounds__(256) void scan_walk_kernel(Scan s) {
 }
 
 // The second pass: from each chunk's own states and the sum of its steps to what enters it, in place; forward from the
-// given state (or zeros), backward from the gradient of the last one.
-template <bool kReverse>
+// given state (or zeros), backward from the gradient of the last one.  A block takes 256 states one chunk after
+// another or, where they are few, 32 by eight runs of chunks: each run's own states and decay first, then from what the
+// runs before it make of `first` (3072 states, 251 chunks: 32 -> 8.5 us; 98304 states, 16 chunks: 5.5 -> 11.5, so not there).
+template <bool kReverse, int kRuns>
 __global__ __launch_bounds__(256) void scan_carry_kernel(Scan s, const float* first, float* last) {
-  const int64_t item = (int64_t)block_index() * 256 + threadIdx.x, per = (int64_t)s.channels * s.states;
-  if (item >= s.batch * per) return;
+  constexpr int kAhead = 8, kColumns = 256 / kRuns;
+  __shared__ float decay[kRuns][kColumns], state[kRuns][kColumns];
+  const int col = threadIdx.x % kColumns, run = threadIdx.x / kColumns;
+  const int64_t item = (int64_t)block_index() * kColumns + col, per = (int64_t)s.channels * s.states;  // a multiple of 64
+  if (item >= s.batch * per) return;  // whole blocks leave where there are runs
   const int64_t b = item / per, cn = item - b * per, c = cn / s.states;
   const float A2 = s.A[cn] * kLog2e;
-  float carry = first ? first[item] : 0.f;
-  constexpr int kAhead = 8;
-  for (int64_t k0 = 0; k0 < s.chunks; k0 += kAhead) {
-    float own[kAhead], d[kAhead];
+  const int64_t each = (s.chunks + kRuns - 1) / kRuns, k_first = run * each, k_last = min(k_first + each, s.chunks);
+  float own[kAhead], d[kAhead];
+  auto at = [&](int64_t k) { return b * s.chunks + (kReverse ? s.chunks - 1 - k : k); };
+  auto load = [&](int64_t k0) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int64_t k = min(k0 + i, s.chunks - 1), at = b * s.chunks + (kReverse ? s.chunks - 1 - k : k);
-      own[i] = s.carry[at * per + cn];
-      d[i] = s.steps[at * s.channels + c];
+      const bool there = k0 + i < k_last;
+      own[i] = there ? s.carry[at(k0 + i) * per + cn] : 0.f;
+      d[i] = there ? s.steps[at(k0 + i) * s.channels + c] : 0.f;  // no step: the state passes
     }
+  };
+  float carry = first ? first[item] : 0.f;
+  if (kRuns > 1) {
+    float total = 0.f, mine = 0.f;
+    for (int64_t k0 = k_first; k0 < k_last; k0 += kAhead) {
+      load(k0);
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        mine = __builtin_amdgcn_exp2f(A2 * d[i]) * mine + own[i];
+        total += d[i];
+      }
+    }
+    decay[run][col] = __builtin_amdgcn_exp2f(A2 * total);
+    state[run][col] = mine;
+    __syncthreads();
+    for (int i = 0; i < run; ++i) carry = decay[i][col] * carry + state[i][col];
+  }
+  for (int64_t k0 = k_first; k0 < k_last; k0 += kAhead) {
+    if (kRuns == 1 || each > kAhead) load(k0);  // else they are still there
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      if (k0 + i >= s.chunks) break;
-      const int64_t at = b * s.chunks + (kReverse ? s.chunks - 1 - (k0 + i) : k0 + i);
-      s.carry[at * per + cn] = carry;
+      if (k0 + i >= k_last) break;
+      s.carry[at(k0 + i) * per + cn] = carry;
       carry = __builtin_amdgcn_exp2f(A2 * d[i]) * carry + own[i];
     }
   }
-  if (last) last[item] = carry;
+  if (last && run == kRuns - 1) last[item] = carry;
 }
 
 // One token: four states a thread.
@@ -404,19 +510,25 @@ __global__ __launch_bounds__(256) void scan_step_kernel(Scan s) {
 
 // ------------------------------------------------------------------ gradient
 
-// A block takes a span of a group's channels and a range of tiles.  A lane has one state (of 8 states every second lane
-// none) and, pass by pass, channel after channel: the sums dB, dC of its state stay in its registers over a tile, h and a
-// of a channel over its 32 tokens.  A token's d, d u and dy stay with lane t % 16 of each row of 16, from where the others
-// take them.  dA, dD and the bias's sums stay in LDS over the range.
+// v, as a value that the compiler does not know: what is worked out of it is not kept in registers over the loops around.
+__device__ __forceinline__ int again(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
+// A block takes a span of a group's channels and a range of tiles; its waves take slices of 16 channels in turn, each in
+// its own part of LDS, and wait for each other only at a tile's ends.  The range's tiles go from the last to the first, X
+// handed on in LDS.  A lane has one state (of 8 states every second
+// lane none) and, pass by pass, channel after channel: the sums dB, dC of its state stay in its registers over a tile, h
+// and a of a channel over its 32 tokens.  dA, dD and the bias's sums stay in LDS over the range.
 template <typename T, int N>
-__global__ __launch_bounds__(256, 2) void scan_bwd_kernel(Scan s) {
-  constexpr int NP = N < 16 ? 16 : N, kSlots = 64 / NP, kPasses = kSlice / (4 * kSlots);
-  constexpr int kStage = 5 * kSlice * kRow, kJoin = 4 * K * N;
+__global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
+  constexpr int NP = N < 16 ? 16 : N, kSlots = 64 / NP, kPasses = kSlice / kSlots, R = kGradRow;
+  constexpr int kPart = kSlice * R, kStage = 4 * 4 * kPart, kJoin = 256 * KG;
   __shared__ __align__(16) float lds[kStage > kJoin ? kStage : kJoin];
-  __shared__ __align__(16) float sB[NP * kRow], sC[NP * kRow];
-  extern __shared__ __align__(16) float span_sums[];  // dA [span][N], dD [span], dbias [span]
-  float *sd = lds, *sv = sd + kSlice * kRow, *sy = sv + kSlice * kRow, *s1 = sy + kSlice * kRow, *s2 = s1 + kSlice * kRow;
-  float *aA = span_sums, *aD = aA + s.span * N, *ab = aD + s.span;
+  __shared__ __align__(16) float sB[NP * R], sC[NP * R];
+  extern __shared__ __align__(16) float span_sums[];  // X [span][N], dA [span][N], dD [span], dbias [span]
+  float *aX = span_sums, *aA = aX + s.span * N, *aD = aA + s.span * N, *ab = aD + s.span;
   uint32_t block = block_index();
   if (block >= s.blocks) return;
   const int span = (int)(block % (uint32_t)s.spans);
@@ -429,117 +541,120 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(Scan s) {
   const int c_end = min(c_first + s.span, (group + 1) * s.group_channels);
   const int lane = lane_id(), wave = threadIdx.x >> 6, n = lane % NP, slot = lane / NP, r = lane & 15;
   const bool held = n < N;
-  for (int i = threadIdx.x; i < s.span * (N + 2); i += 256) span_sums[i] = 0.f;
+  // d, d u, dy and the sums G B of a slice; the sums A X h take the place of the d u that they have used
+  float *sd = lds + wave * 4 * kPart, *sv = sd + kPart, *sy = sv + kPart, *s1 = sy + kPart, *s2 = sv;
+  const float* x_at = s.x_in + ((b * s.ranges + range) * s.channels + c_first) * N;
+  for (int i = threadIdx.x; i < s.span * N; i += 256) aX[i] = i < (c_end - c_first) * N ? x_at[i] : 0.f;
+  for (int i = threadIdx.x; i < s.span * (N + 2); i += 256) aA[i] = 0.f;
 
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  const int e = threadIdx.x % (kSlice / 4) * 4, et = threadIdx.x / (kSlice / 4);  // this thread's element of a slice
-  const int64_t tile0 = (int64_t)range * s.range_tiles, tile1 = min(tile0 + s.range_tiles, s.tiles);
-  for (int64_t tile = tile0; tile < tile1; ++tile) {
-    const int64_t token = tile * K + et;
-    const int64_t maps = (((int64_t)(s.whole ? 0 : span) * s.batch + b) * s.tokens + tile * K) * s.groups * N + group * N;
-    if (tile * K >= length) {  // nothing here depends on anything
-      if (token < s.tokens) {
-        for (int cc = c_first + e; cc < c_end; cc += kSlice) {
-          const int64_t at = (b * s.tokens + token) * s.channels + cc;
-          if (s.du) store4((T*)s.du + at, zero);
-          if (s.ddt) store4((T*)s.ddt + at, zero);
-          if (s.dz) store4((T*)s.dz + at, zero);
-        }
+  const int e = lane % (kSlice / 4) * 4, et = lane / (kSlice / 4);  // a lane's element of a slice
+  const uint32_t size = sizeof(T), u_of = (et * (uint32_t)s.u.st + e) * size, dt_of = (et * (uint32_t)s.dt.st + e) * size;
+  const uint32_t z_of = (et * (uint32_t)s.z.st + e) * size, of = et * (uint32_t)s.channels + e;
+  const int64_t tile0 = (int64_t)range * s.range_tiles * (K / KG);
+  const int64_t tile1 = min(tile0 + (int64_t)s.range_tiles * (K / KG), s.grad_tiles);
+  for (int64_t tile = tile1 - 1; tile >= tile0; --tile) {
+    const int64_t first = b * s.tokens + tile * KG, map_row = s.whole ? first : (span * s.batch + b) * s.tokens + tile * KG;
+    const int left = (int)min(length - tile * KG, (int64_t)KG), inside = (int)min(s.tokens - tile * KG, (int64_t)KG);
+    if (left <= 0) {  // nothing here depends on anything
+      for (int cc = again(c_first + wave * kSlice + e); et < inside && cc < c_end; cc += 4 * kSlice) {
+        if (s.du) store4((T*)s.du + (first + et) * s.channels + cc, zero);
+        if (s.ddt) store4((T*)s.ddt + (first + et) * s.channels + cc, zero);
       }
-      for (int i = threadIdx.x; i < K * N; i += 256) {
-        if (tile * K + i / N >= s.tokens) continue;
-        const int64_t at = maps + (int64_t)(i / N) * s.groups * N + i % N;
-        if (s.whole) {
-          if (s.dB_out) ((T*)s.dB_out)[at] = (T)0.f;
-          if (s.dC_out) ((T*)s.dC_out)[at] = (T)0.f;
-        } else {
-          s.dB[at] = 0.f, s.dC[at] = 0.f;
-        }
+      for (int i = again(threadIdx.x); i < inside * N; i += 256) {
+        const int64_t at = ((map_row + i / N) * s.groups + group) * N + i % N;
+        if (!s.whole) s.dB[at] = 0.f, s.dC[at] = 0.f;
+        if (s.whole && s.dB_out) ((T*)s.dB_out)[at] = (T)0.f;
+        if (s.whole && s.dC_out) ((T*)s.dC_out)[at] = (T)0.f;
       }
       continue;
     }
+    const int64_t row = first * s.channels;
+    const T* u_at = (const T*)s.u.p + b * s.u.sb + tile * KG * s.u.st;
+    const T* dt_at = (const T*)s.dt.p + b * s.dt.sb + tile * KG * s.dt.st;
+    const T* z_at = (const T*)s.z.p + b * s.z.sb + tile * KG * s.z.st;
+    const float* h_at = s.h_in + (b * s.grad_tiles + tile) * s.channels * N;
+    // a slice's elements, and a pass's A and entering h, are asked for a slice and a pass before
+    Four<T> u, x, dy, z;
+    auto ask_slice = [&](int c0) {
+      const bool there = c0 + e < c_end && et < left;
+      u = four(u_at + c0, u_of, there), x = four(dt_at + c0, dt_of, there);
+      dy = four((const T*)s.dout + row + c0, of * size, there), z = four(z_at + c0, z_of, there && s.z.p);
+    };
+    float nA = 0.f, nh = 0.f;
+    auto ask = [&](int c) {
+      const bool live = c < c_end && held;
+      const uint32_t at = (uint32_t)c * N + n;
+      nA = live ? s.A[at] : 0.f, nh = live ? h_at[at] : 0.f;
+    };
+    ask_slice(c_first + wave * kSlice);
+    ask(c_first + wave * kSlice + slot);
     __syncthreads();
-    for (int i = threadIdx.x; i < K * NP; i += 256) {
+    for (int i = again(threadIdx.x); i < KG * NP; i += 256) {
       const int t = i / NP, m = i % NP;
-      const int64_t at = tile * K + t;
-      const bool there = at < length && m < N;
-      sB[m * kRow + t] = there ? load_f((const T*)s.B.p + b * s.B.sb + at * s.B.st + group * s.B.sg + m) : 0.f;
-      sC[m * kRow + t] = there ? load_f((const T*)s.C.p + b * s.C.sb + at * s.C.st + group * s.C.sg + m) : 0.f;
+      const int64_t at = tile * KG + t;
+      const bool there = t < left && m < N;
+      sB[m * R + t] = there ? load_f((const T*)s.B.p + b * s.B.sb + at * s.B.st + group * s.B.sg + m) : 0.f;
+      sC[m * R + t] = there ? load_f((const T*)s.C.p + b * s.C.sb + at * s.C.st + group * s.C.sg + m) : 0.f;
     }
-    float accB[K], accC[K];
+    __syncthreads();
+    float accB[KG], accC[KG];
 #pragma unroll
-    for (int t = 0; t < K; ++t) accB[t] = accC[t] = 0.f;
-    // uniform addresses of the tile and this thread's offsets from them (a token's stride is below 2^26 elements)
-    const int64_t first = b * s.tokens + tile * K;
-    const T *u_at = (const T*)s.u.p + b * s.u.sb + tile * K * s.u.st + c_first;
-    const T *dt_at = (const T*)s.dt.p + b * s.dt.sb + tile * K * s.dt.st + c_first;
-    const T *z_at = (const T*)s.z.p + b * s.z.sb + tile * K * s.z.st + c_first;
-    const uint32_t u_of = (uint32_t)et * (uint32_t)s.u.st + e, dt_of = (uint32_t)et * (uint32_t)s.dt.st + e;
-    const uint32_t z_of = (uint32_t)et * (uint32_t)s.z.st + e, of = (uint32_t)et * (uint32_t)s.channels + e;
-    const bool here = token < length;
-    for (int c0 = 0; c0 < c_end - c_first; c0 += kSlice) {
-      const bool mine = c0 + e < c_end - c_first, there = here && mine, inside = token < s.tokens && mine;
-      const int64_t row = first * s.channels + c_first + c0;
-      f32x4 u = zero, x = zero, dy = zero, z = zero, raw = zero, bias = zero;
-      if (there) {
-        u = load4(u_at + c0 + u_of), x = load4(dt_at + c0 + dt_of), dy = load4((const T*)s.dout + row + of);
-        if (s.dt_bias) bias = load4(s.dt_bias + c_first + c0 + e);
-        if (s.z.p) z = load4(z_at + c0 + z_of), raw = load4(s.raw + row + of);
-      }
-      __syncthreads();
-      // a token that is not there has u, dy and z zero, and takes no step
-      x += bias;
-      f32x4 d = x;
-      if (s.softplus) {
+    for (int t = 0; t < KG; ++t) accB[t] = accC[t] = 0.f;
+    for (int c0 = c_first + wave * kSlice; c0 < c_end; c0 += 4 * kSlice) {
+      const bool mine = c0 + e < c_end, there = mine && et < left;
+      f32x4 bias = zero;
+      if (mine && s.dt_bias) bias = load4(s.dt_bias + c0 + e);
+      const Four<T> u_kept = u, x_kept = x;
+      {
+        // a token that is not there has u, dy and z zero, and takes no step
+        f32x4 d = x.wide() + bias, y = dy.wide();
+        const f32x4 uw = u.wide(), zw = z.wide();
+        if (s.softplus) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) d[q] = step_of(x[q]);
-      }
-      d = d * (there ? 1.f : 0.f);
-      if (s.z.p) {
-        f32x4 dz;
+          for (int q = 0; q < 4; ++q) d[q] = step_of(d[q]);
+        }
+        d = d * (there ? 1.f : 0.f);
+        if (s.z.p) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) y[q] *= silu_f(zw[q]);
+        }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float sg = sigmoid_f(z[q]);
-          dz[q] = dy[q] * raw[q] * (sg + z[q] * sg * (1.f - sg));
-          dy[q] = dy[q] * z[q] * sg;
+          sd[(e + q) * R + et] = d[q];
+          sv[(e + q) * R + et] = d[q] * uw[q];
+          sy[(e + q) * R + et] = y[q];
         }
-        if (s.dz && inside) store4((T*)s.dz + row + of, dz);
       }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        sd[(e + q) * kRow + et] = d[q];
-        sv[(e + q) * kRow + et] = d[q] * u[q];
-        sy[(e + q) * kRow + et] = dy[q];
-      }
-      __syncthreads();
+      ask_slice(c0 + 4 * kSlice);
+      wave_fence();
       for (int pass = 0; pass < kPasses; ++pass) {
-        const int cl = (pass * 4 + wave) * kSlots + slot, c = c_first + c0 + cl;
+        const int cl = pass * kSlots + slot, c = c0 + cl;
         const bool live = c < c_end && held;
-        const int64_t from = ((b * s.tiles + tile) * s.channels + c) * N + n;
-        const float A = live ? s.A[(int64_t)c * N + n] : 0.f, A2 = A * kLog2e;
-        const float h0 = live ? s.h_in[from] : 0.f;
-        float X = live ? s.x_in[from] : 0.f, dA = 0.f;
+        const float A = nA, A2 = A * kLog2e, h0 = nh;
+        float X = live ? aX[(c - c_first) * N + n] : 0.f, dA = 0.f;
+        ask(pass + 1 < kPasses ? c + kSlots : c0 + 4 * kSlice + slot);
         // d as an operand from the lanes of a row in the exponent; in multiply-adds, which take none, from LDS
-        const float dl[2] = {sd[cl * kRow + r], sd[cl * kRow + 16 + r]};
-        float h[K], a[K], last = h0;
-        unrolled<K / 4>([&](auto quad) {
+        const float dl = sd[cl * R + r];
+        float h[KG], a[KG], last = h0;
+        unrolled<KG / 4>([&](auto quad) {
           constexpr int t0 = decltype(quad)::value * 4;
-          const f32x4 v = *(const f32x4*)(sv + cl * kRow + t0), m = *(const f32x4*)(sB + n * kRow + t0);
+          const f32x4 v = *(const f32x4*)(sv + cl * R + t0), m = *(const f32x4*)(sB + n * R + t0);
           unrolled<4>([&](auto index) {
             constexpr int q = decltype(index)::value, t = t0 + q;
-            a[t] = __builtin_amdgcn_exp2f(from_row<t % 16>(dl[t / 16]) * A2);
+            a[t] = __builtin_amdgcn_exp2f(from_row<t>(dl) * A2);
             h[t] = last = __builtin_fmaf(v[q], m[q], a[t] * last);
           });
           __builtin_amdgcn_sched_barrier(0);
         });
         RowSum sum1, sum2;
-        unrolled<K / 4>([&](auto quad) {
-          constexpr int t0 = K - 4 - decltype(quad)::value * 4;
-          const f32x4 m = *(const f32x4*)(sB + n * kRow + t0), o = *(const f32x4*)(sC + n * kRow + t0);
-          const f32x4 d = *(const f32x4*)(sd + cl * kRow + t0), v = *(const f32x4*)(sv + cl * kRow + t0);
-          const f32x4 y = *(const f32x4*)(sy + cl * kRow + t0);
+        unrolled<KG / 4>([&](auto quad) {
+          constexpr int t0 = KG - 4 - decltype(quad)::value * 4;
+          const f32x4 m = *(const f32x4*)(sB + n * R + t0), o = *(const f32x4*)(sC + n * R + t0);
+          const f32x4 d = *(const f32x4*)(sd + cl * R + t0), v = *(const f32x4*)(sv + cl * R + t0);
+          const f32x4 y = *(const f32x4*)(sy + cl * R + t0);
           unrolled<4>([&](auto index) {
-            constexpr int q = 3 - decltype(index)::value, t = t0 + q, in = t % 16;
+            constexpr int q = 3 - decltype(index)::value, t = t0 + q;
             const float G = __builtin_fmaf(y[q], o[q], X);
             accC[t] = __builtin_fmaf(y[q], h[t], accC[t]);
             accB[t] = __builtin_fmaf(v[q], G, accB[t]);
@@ -547,72 +662,73 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(Scan s) {
             X = a[t] * G;
             const float back = X * (t ? h[t ? t - 1 : 0] : h0);
             dA = __builtin_fmaf(d[q], back, dA);
-            sum1.add<15 - in>(G * m[q], lane);
-            sum2.add<15 - in>(A * back, lane);
+            sum1.add<15 - t>(G * m[q], lane);
+            sum2.add<15 - t>(A * back, lane);
           });
-          if constexpr (t0 % 16 == 0) {
-            float r1 = sum1.held[3], r2 = sum2.held[3];
-            if (N >= 32) r1 += xor16(r1), r2 += xor16(r2);
-            if (N == 64) r1 = xor32_sum(r1), r2 = xor32_sum(r2);
-            if (N <= 16 || n < 16) {
-              s1[cl * kRow + t0 + 15 - rev4(r)] = r1;
-              s2[cl * kRow + t0 + 15 - rev4(r)] = r2;
-            }
-          }
           __builtin_amdgcn_sched_barrier(0);
         });
-        if (live) aA[(c - c_first) * N + n] += dA;
+        float r1 = sum1.held[3], r2 = sum2.held[3];
+        if (N >= 32) r1 += xor16(r1), r2 += xor16(r2);
+        if (N == 64) r1 = xor32_sum(r1), r2 = xor32_sum(r2);
+        if (N <= 16 || n < 16) {
+          s1[cl * R + 15 - rev4(r)] = r1;
+          s2[cl * R + 15 - rev4(r)] = r2;
+        }
+        if (live) {
+          aA[(c - c_first) * N + n] += dA;
+          aX[(c - c_first) * N + n] = X;
+        }
       }
-      __syncthreads();
+      wave_fence();
       {
-        f32x4 du, ddt, skip = zero;
-        if (s.D && mine) skip = load4(s.D + c_first + c0 + e);
+        f32x4 skip = zero, du, ddt;
+        if (mine && s.D) skip = load4(s.D + c0 + e);
+        const f32x4 uw = u_kept.wide(), xw = x_kept.wide() + bias;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const int i = (e + q) * kRow + et;
-          const float g = s1[i], y = sy[i];
-          du[q] = there ? sd[i] * g + skip[q] * y : 0.f;
-          ddt[q] = there ? u[q] * g + s2[i] : 0.f;
-          s1[i] = there ? y * u[q] : 0.f;
+          const int at = (e + q) * R + et;
+          const float g = s1[at], y = sy[at];
+          du[q] = there ? sd[at] * g + skip[q] * y : 0.f;
+          ddt[q] = there ? uw[q] * g + s2[at] : 0.f;
+          s1[at] = there ? y * uw[q] : 0.f;
         }
         if (s.softplus) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) ddt[q] *= sigmoid_f(x[q]);
+          for (int q = 0; q < 4; ++q) ddt[q] *= sigmoid_f(xw[q]);
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) s2[(e + q) * kRow + et] = ddt[q];
-        if (inside && s.du) store4((T*)s.du + row + of, du);
-        if (inside && s.ddt) store4((T*)s.ddt + row + of, ddt);
+        for (int q = 0; q < 4; ++q) s2[(e + q) * R + et] = ddt[q];
+        if (mine && et < inside) {
+          if (s.du) put4((T*)s.du + row + c0, of * size, du);
+          if (s.ddt) put4((T*)s.ddt + row + c0, of * size, ddt);
+        }
       }
-      __syncthreads();
-      // sums over the tile's tokens: four lanes a channel, 8 tokens each; dD by the first two waves, the bias's by the others
+      wave_fence();
+      // sums over the tile's tokens: two lanes a channel, 8 tokens each; dD by the lower half of the wave, the bias's by
+      // the upper
       {
-        const int which = threadIdx.x >> 7, cl = threadIdx.x % 128 / 4, quarter = threadIdx.x % 4;
-        const float* from = (which ? s2 : s1) + cl * kRow + 8 * quarter;
-        float v = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v += from[i];
-        v += from_lane<0xB1>(v);
-        v += from_lane<0x4E>(v);
-        if (quarter == 0 && c_first + c0 + cl < c_end) (which ? ab : aD)[c0 + cl] += v;
+        const int cl = (lane & 31) >> 1;
+        const float* from = (lane & 32 ? s2 : s1) + cl * R + 8 * (lane & 1);
+        const f32x4 v = *(const f32x4*)from + *(const f32x4*)(from + 4);
+        float total = (v[0] + v[1]) + (v[2] + v[3]);
+        total += from_lane<0xB1>(total);
+        if (!(lane & 1) && c0 + cl < c_end) (lane & 32 ? ab : aD)[c0 - c_first + cl] += total;
       }
+      wave_fence();
     }
     // the slots' and waves' sums of dB, then dC
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       __syncthreads();
 #pragma unroll
-      for (int t = 0; t < K; ++t) {
-        float v = which ? accC[t] : accB[t];
-        if (NP == 16) v += xor16(v);
-        if (NP <= 32) v = xor32_sum(v);
-        if (slot == 0 && held) lds[(wave * K + t) * N + n] = v;
-      }
+      for (int t = 0; t < KG; ++t) lds[t * 256 + threadIdx.x] = which ? accC[t] : accB[t];
       __syncthreads();
-      for (int i = threadIdx.x; i < K * N; i += 256) {
-        const float v = (lds[i] + lds[K * N + i]) + (lds[2 * K * N + i] + lds[3 * K * N + i]);
-        if (tile * K + i / N >= s.tokens) continue;
-        const int64_t at = maps + (int64_t)(i / N) * s.groups * N + i % N;
+      for (int i = again(threadIdx.x); i < inside * N; i += 256) {
+        const float* from = lds + i / N * 256 + i % N;
+        float v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 4 * kSlots; ++k) v += from[k * NP];
+        const int64_t at = ((map_row + i / N) * s.groups + group) * N + i % N;
         if (!s.whole)
           (which ? s.dC : s.dB)[at] = v;
         else if (which ? s.dC_out : s.dB_out)
@@ -622,40 +738,42 @@ __global__ __launch_bounds__(256, 2) void scan_bwd_kernel(Scan s) {
   }
   __syncthreads();
   const int64_t part = b * s.ranges + range;
-  for (int i = threadIdx.x; i < (c_end - c_first) * N; i += 256) s.dA[(part * s.channels + c_first) * N + i] = aA[i];
-  for (int i = threadIdx.x; i < c_end - c_first; i += 256) {
+  for (int i = again(threadIdx.x); i < (c_end - c_first) * N; i += 256) s.dA[(part * s.channels + c_first) * N + i] = aA[i];
+  for (int i = again(threadIdx.x); i < c_end - c_first; i += 256) {
     s.dD[part * s.channels + c_first + i] = aD[i];
     s.dbias[part * s.channels + c_first + i] = ab[i];
   }
 }
 
-// Sums of partial rows, 16 columns by 16 slices of the rows a block: out[i] = sum over r of from[r * columns + i].
+// Sums of partial rows, 64 columns by 16 slices of the rows a block: out[i] = sum over r of from[r * columns + i].
 struct RowSums {
   const float* from[5];
   void* out[5];
-  int64_t columns[5], rows[5];
+  int64_t columns[5], rows[5];  // columns are multiples of 4
   int bf16_out[5];
 };
 __global__ __launch_bounds__(256) void scan_sums_kernel(RowSums s) {
-  __shared__ float lds[16][17];
+  __shared__ f32x4 lds[16][17];
   const int which = blockIdx.y, col = threadIdx.x % 16, slice = threadIdx.x / 16;
   if (!s.out[which]) return;
-  for (int64_t first = (int64_t)blockIdx.x * 16; first < s.columns[which]; first += (int64_t)gridDim.x * 16) {
-    const int64_t i = first + col;
-    float v = 0.f;
-    if (i < s.columns[which])
-      for (int64_t r = slice; r < s.rows[which]; r += 16) v += s.from[which][r * s.columns[which] + i];
+  const int64_t columns = s.columns[which], rows = s.rows[which];
+  for (int64_t first = (int64_t)blockIdx.x * 64; first < columns; first += (int64_t)gridDim.x * 64) {
+    const int64_t i = first + 4 * col;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (i < columns) {
+#pragma unroll 4
+      for (int64_t r = slice; r < rows; r += 16) v += *(const f32x4*)(s.from[which] + r * columns + i);
+    }
     __syncthreads();
     lds[slice][col] = v;
     __syncthreads();
-    if (slice || i >= s.columns[which]) continue;
-    v = 0.f;
+    if (slice || i >= columns) continue;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) v += lds[k][col];
+    for (int k = 1; k < 16; ++k) v += lds[k][col];
     if (s.bf16_out[which])
-      ((bf16*)s.out[which])[i] = (bf16)v;
+      store4((bf16*)s.out[which] + i, v);
     else
-      ((float*)s.out[which])[i] = v;
+      store4((float*)s.out[which] + i, v);
   }
 }
 
@@ -670,12 +788,14 @@ void with_states(int64_t states, Go go) {
   return go(integral_constant<int, 64>());
 }
 
+// Lanes of a channel where chunks are walked: four states each (of eight states two).
+constexpr int walk_lanes(int states) { return states <= 16 ? 4 : states / 4; }
 struct Chunks {
   int64_t chunks, tiles;  // tiles of a chunk
 };
-// One chunk where the channels alone make 768 blocks (three waves a SIMD), else about 1536 blocks.
 Chunks plan_chunks(int64_t batch, int64_t tokens, int64_t channels, int64_t states, int64_t groups) {
-  const int64_t tiles = (tokens + K - 1) / K, blocks = batch * groups * ((channels / groups + kWalk - 1) / kWalk);
+  const int64_t tiles = (tokens + K - 1) / K, per = 256 / walk_lanes((int)states);
+  const int64_t blocks = batch * groups * ((channels / groups + per - 1) / per);
   if (blocks >= 768 || tiles <= 2) return {1, tiles};
   int64_t chunks = (1536 + blocks - 1) / blocks;
   if (chunks > tiles) chunks = tiles;
@@ -686,17 +806,16 @@ Chunks plan_chunks(int64_t batch, int64_t tokens, int64_t channels, int64_t stat
 struct Spans {
   int64_t span, spans, ranges, range_tiles, whole;
 };
-// Spans of a group's channels and ranges of tiles of the gradient's blocks: about 1024 blocks.
+// Spans of a group's channels and ranges of tiles of the gradient's blocks: two tiles (of 32) where that leaves enough
+// blocks, four rounds of the three that a compute unit holds; one halves what a wave waits for in the small calls.
 Spans plan_spans(int64_t batch, int64_t tokens, int64_t channels, int64_t states, int64_t groups) {
-  const int64_t tiles = (tokens + K - 1) / K, group = channels / groups;
-  const int64_t most = kMaxSpan / states / kSlice * kSlice;
+  const int64_t tiles = (tokens + K - 1) / K, group = channels / groups, unit = 4 * kSlice;
+  const int64_t most = kMaxSpan / states < unit ? unit : kMaxSpan / states / unit * unit;
   Spans p;
   p.spans = (group + most - 1) / most;
-  p.span = ((group + p.spans - 1) / p.spans + kSlice - 1) / kSlice * kSlice;
+  p.span = ((group + p.spans - 1) / p.spans + unit - 1) / unit * unit;
   p.spans = (group + p.span - 1) / p.span;
-  const int64_t blocks = batch * groups * p.spans;
-  int64_t ranges = (1024 + blocks - 1) / blocks;
-  if (ranges > tiles) ranges = tiles;
+  const int64_t m = batch * groups * p.spans * tiles >= 3072 ? 2 : 1, ranges = (tiles + m - 1) / m;
   p.range_tiles = (tiles + ranges - 1) / ranges;
   p.ranges = (tiles + p.range_tiles - 1) / p.range_tiles;
   p.whole = p.spans == 1;
@@ -717,11 +836,14 @@ int setup(Scan& s, const void* u, const void* dt, const float* A, const void* B,
               "selective_scan: expected fewer than 2^31 rows");
   for (int i = 0; i < 12; ++i)
     BMX_REQUIRE(strides[i] % 4 == 0, "selective_scan: strides must be multiples of 4");
+  for (int i : {1, 3, 5, 7, 10})
+    BMX_REQUIRE(strides[i] >= 0 && strides[i] < (1 << 25), "selective_scan: a token's stride must be below 2^25");
   s.u = {u, strides[0], strides[1], 0}, s.dt = {dt, strides[2], strides[3], 0}, s.z = {z, strides[4], strides[5], 0};
   s.B = {B, strides[6], strides[7], strides[8]}, s.C = {C, strides[9], strides[10], strides[11]};
   s.A = A, s.D = D, s.dt_bias = dt_bias, s.lengths = lengths, s.lengths64 = lengths64, s.softplus = softplus != 0;
   s.batch = shape[0], s.tokens = shape[1], s.channels = (int)channels, s.states = (int)states, s.groups = (int)groups;
   s.group_channels = (int)(channels / groups), s.tiles = (s.tokens + K - 1) / K;
+  s.grad_tiles = (s.tokens + KG - 1) / KG;
   return BMX_OK;
 }
 
@@ -743,23 +865,27 @@ template <typename T, int kMode>
 int walk(Scan s, hipStream_t stream) {
   int rc = BMX_OK;
   with_states(s.states, [&](auto n) {
-    constexpr int N = decltype(n)::value;
-    s.cblocks = (s.group_channels + kWalk - 1) / kWalk;
+    constexpr int N = decltype(n)::value, L = walk_lanes(N);
+    s.cblocks = (s.group_channels + 256 / L - 1) / (256 / L);
     s.blocks = s.batch * s.chunks * s.groups * s.cblocks;
-    if (s.blocks >= (1ll << 31)) {
+    if (s.blocks >= (1ll << 31) - 8) {
       rc = set_error(BMX_EINVAL, "selective_scan: too many rows");
       return;
     }
-    scan_walk_kernel<T, N, kMode><<<fold_grid(s.blocks, 256), 256, 0, stream>>>(s);
+    s.eighth = (uint32_t)((s.blocks + 7) / 8);
+    scan_walk_kernel<T, N, L, kMode><<<fold_grid((int64_t)s.eighth * 8, 256), 256, 0, stream>>>(s);
   });
   return rc ? rc : check_launch("selective_scan");
 }
 
 template <bool kReverse>
 int carry(const Scan& s, const float* first, float* last, hipStream_t stream) {
-  const int64_t blocks = (s.batch * s.channels * s.states + 255) / 256;
-  BMX_REQUIRE(blocks < (1ll << 31), "selective_scan: too many states");
-  scan_carry_kernel<kReverse><<<fold_grid(blocks, 256), 256, 0, stream>>>(s, first, last);
+  const int64_t states = s.batch * s.channels * s.states;
+  BMX_REQUIRE(states / 32 < (1ll << 31), "selective_scan: too many states");
+  if (states >= 65536)
+    scan_carry_kernel<kReverse, 1><<<fold_grid((states + 255) / 256, 256), 256, 0, stream>>>(s, first, last);
+  else
+    scan_carry_kernel<kReverse, 8><<<fold_grid(states / 32, 256), 256, 0, stream>>>(s, first, last);
   return check_launch("selective_scan carry");
 }
 
@@ -786,7 +912,7 @@ int gradient(Scan& s, const float* dstate_out, float* dstate, hipStream_t stream
   if (int rc = carry<true>(s, dstate_out, dstate, stream)) return rc;
   with_states(s.states, [&](auto n) {
     constexpr int N = decltype(n)::value;
-    scan_bwd_kernel<T, N><<<fold_grid(s.blocks, 256), 256, s.span * (N + 2) * sizeof(float), stream>>>(s);
+    scan_bwd_kernel<T, N><<<fold_grid(s.blocks, 256), 256, s.span * (2 * N + 2) * sizeof(float), stream>>>(s);
   });
   return check_launch("selective_scan_bwd");
 }
@@ -795,8 +921,8 @@ int gradient(Scan& s, const float* dstate_out, float* dstate, hipStream_t stream
 struct BackSpace {
   int64_t carry, steps, maps, dA, dD;
   BackSpace(int64_t batch, int64_t tokens, int64_t channels, int64_t states, int64_t groups, const Spans& p) {
-    const int64_t tiles = (tokens + K - 1) / K, parts = batch * p.ranges;
-    carry = batch * tiles * channels * states, steps = batch * tiles * channels;
+    const int64_t parts = batch * p.ranges;
+    carry = parts * channels * states, steps = parts * channels;
     maps = p.whole ? 0 : p.spans * batch * tokens * groups * states;
     dA = parts * channels * states, dD = parts * channels;
   }
@@ -811,7 +937,7 @@ bool sizes_ok(int64_t batch, int64_t tokens, int64_t channels, int64_t states, i
 
 extern "C" size_t bmx_selective_scan_saved_bytes(int64_t batch, int64_t tokens, int64_t channels, int64_t states) {
   if (batch <= 0 || tokens <= 0 || channels <= 0 || states <= 0) return 0;
-  return (size_t)(batch * ((tokens + K - 1) / K) * channels * states) * sizeof(float);
+  return (size_t)(batch * ((tokens + KG - 1) / KG) * channels * states) * sizeof(float);
 }
 
 extern "C" size_t bmx_selective_scan_workspace_bytes(int64_t batch, int64_t tokens, int64_t channels, int64_t states,
@@ -869,7 +995,7 @@ extern "C" int bmx_selective_scan_bwd(const void* u, const void* dt, const float
   if (int rc = check_inputs(s, dtype)) return rc;
   BMX_REQUIRE(saved && dout && (!z || raw), "selective_scan_bwd: null pointer");
   BMX_REQUIRE((D || !dD) && (z || !dz) && (dt_bias || !ddt_bias), "selective_scan_bwd: gradient of an absent operand");
-  BMX_REQUIRE(aligned(16, {saved, raw, dout, du, ddt, dz}), "selective_scan: tensors must be 16-byte aligned");
+  BMX_REQUIRE(aligned(16, {saved, raw, dout, du, ddt, dz, dA, dB, dC, dD, ddt_bias}), "selective_scan: tensors must be 16-byte aligned");
   const Spans p = plan_spans(s.batch, s.tokens, s.channels, s.states, s.groups);
   const BackSpace space(s.batch, s.tokens, s.channels, s.states, s.groups, p);
   BMX_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= (size_t)space.floats() * sizeof(float),
@@ -878,7 +1004,7 @@ extern "C" int bmx_selective_scan_bwd(const void* u, const void* dt, const float
   s.carry = (float*)workspace, s.steps = s.carry + space.carry, s.x_in = s.carry;
   s.dB = s.steps + space.steps, s.dC = s.dB + space.maps, s.dB_out = dB, s.dC_out = dC;
   s.dA = s.dC + space.maps, s.dD = s.dA + space.dA, s.dbias = s.dD + space.dD;
-  s.chunks = s.tiles, s.chunk_tiles = 1;
+  s.chunks = p.ranges, s.chunk_tiles = p.range_tiles;
   s.span = (int)p.span, s.spans = (int)p.spans, s.ranges = (int)p.ranges, s.range_tiles = (int)p.range_tiles;
   s.whole = (int)p.whole;
   s.blocks = s.batch * s.groups * p.spans * p.ranges;
@@ -894,7 +1020,7 @@ extern "C" int bmx_selective_scan_bwd(const void* u, const void* dt, const float
                         {0, 0, 0, dtype == kBF16, dtype == kBF16}};
   int64_t columns = (int64_t)s.channels * s.states;
   if (!p.whole && maps > columns) columns = maps;
-  const int64_t blocks = (columns + 15) / 16;
+  const int64_t blocks = (columns + 63) / 64;
   scan_sums_kernel<<<dim3((unsigned)(blocks < 16384 ? blocks : 16384), 5), 256, 0, hs>>>(sums);
   return check_launch("selective_scan_bwd sums");
 }

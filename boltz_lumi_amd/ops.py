@@ -1572,12 +1572,22 @@ def _dense(t):
     return None if t is None else _aligned(t.contiguous())
 
 
-def _apart(out, t) -> bool:
-    """Whether the dense ``out`` shares no memory with ``t`` (a tensor or None)."""
-    if t is None or not t.numel() or not out.numel():
-        return True
-    size, span = out.numel() * out.element_size(), 1 + sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
-    return t.data_ptr() >= out.data_ptr() + size or out.data_ptr() >= t.data_ptr() + span * t.element_size()
+def _span(layout, size):
+    """Bytes from a tensor's first element to behind its last."""
+    shape, stride, _ = layout
+    return 0 if 0 in shape else size * (1 + sum((n - 1) * st for n, st in zip(shape, stride)))
+
+
+def _like(t):
+    """A dense tensor of ``t``'s shape, to be written."""
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
+def _grads(needed, tensors, empty):
+    """Room for the gradients that are needed; zeros where nothing is there to be computed."""
+    if empty:
+        return [torch.zeros(t.shape, device=t.device, dtype=t.dtype) if need else None for need, t in zip(needed, tensors)]
+    return [_like(t) if need else None for need, t in zip(needed, tensors)]
 
 
 @lru_cache(maxsize=512)
@@ -1610,8 +1620,7 @@ def _frame_args(plan, x, y, gate, y_weight, scale, weight, eps):
 
 
 def _residual_norm_fwd(plan, dev, x, y, *rest):
-    r = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    h = torch.empty(x.shape, device=x.device, dtype=y.dtype) if plan.norms[1] else None
+    r, h = _like(x), _like(y) if plan.norms[1] else None
     if plan.rows:
         _launch(dev, "bmx_residual_norm_fwd", *_frame_args(plan, x, y, *rest), r.data_ptr(), _ptr(h))
     return r, h
@@ -1630,9 +1639,7 @@ class _ResidualNorm(torch.autograd.Function):
     def backward(ctx, dr, dh):
         plan, dev, eps = ctx.rest
         tensors = ctx.saved_tensors
-        make = torch.empty if plan.rows else torch.zeros
-        grads = [make(t.shape, device=t.device, dtype=t.dtype) if need else None
-                 for need, t in zip(ctx.needs_input_grad[2:8], tensors)]
+        grads = _grads(ctx.needs_input_grad[2:8], tensors, not plan.rows)
         if plan.rows and any(g is not None for g in grads):
             dr, dh = _dense(dr), _dense(dh)
             ws = _workspace(plan.ws, tensors[0].device)
@@ -1673,13 +1680,20 @@ def _check_lengths(lengths, batch):
     return int(lengths is not None and lengths[2] == torch.int64)
 
 
-def _check_state_out(state_out, shape, dtype, state, inputs, grad):
+def _check_state_out(state_out, plan, dtype, state, inputs, grad):
     """A buffer for the last state: dense, of the state's kind, apart from everything but the state that it may replace."""
     _check(not grad, "state_out takes no gradient: use return_state")
-    _check(state_out.shape == shape and state_out.dtype == dtype and state_out.is_contiguous()
-           and state_out.data_ptr() % 16 == 0, "state_out must be a dense 16-byte aligned tensor of the state's shape and dtype")
-    same = state is not None and state.data_ptr() == state_out.data_ptr() and state.is_contiguous()
-    _check(all(_apart(state_out, t) for t in (*inputs, None if same else state)), "state_out shares memory with an input")
+    lo = state_out.data_ptr()
+    _check(state_out.shape == plan.state and state_out.dtype == dtype and state_out.is_contiguous() and lo % 16 == 0,
+           "state_out must be a dense 16-byte aligned tensor of the state's shape and dtype")
+    hi = lo + plan.state_bytes
+    for t, span in zip(inputs, plan.spans):
+        if t is not None and span:
+            at = t.data_ptr()
+            _check(at >= hi or lo >= at + span, "state_out shares memory with an input")
+    if state is not None:
+        at = state.data_ptr()
+        _check(at == lo or at >= hi or lo >= at + plan.state_bytes, "state_out shares memory with an input")
 
 
 def _empty_state(shape, dtype, device, state, state_out):
@@ -1710,6 +1724,8 @@ def _conv_plan(x, weight, bias, state, lengths, silu):
     plan.head = code, N.int64_array([b, t, c, width]), N.int64_array(_steps(x[0], x[1], 2))
     plan.codes, plan.tail = (_code(weight[2]), _code(bias[2]) if bias else code), (lengths64, silu)
     plan.state, plan.empty = (b, width - 1, c), not (b and t)
+    plan.state_bytes = b * (width - 1) * c * x[2].itemsize
+    plan.spans = [0 if w is None else _span(w, w[2].itemsize) for w in (x, weight, bias, lengths)]
     plan.ws = N.lib().bmx_causal_conv_workspace_bytes(b, t, c, width)
     return plan
 
@@ -1720,7 +1736,7 @@ def _conv_args(plan, x, weight, bias, state, lengths):
 
 
 def _causal_conv_fwd(plan, dev, x, weight, bias, state, lengths, want_state, state_out):
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    y = _like(x)
     if plan.empty:
         return y, _empty_state(plan.state, x.dtype, x.device, state, state_out) if want_state else None
     if want_state and state_out is None:
@@ -1742,9 +1758,7 @@ class _CausalConv(torch.autograd.Function):
     def backward(ctx, dy, dnext):
         plan, dev = ctx.rest
         x, weight, bias, state, lengths = ctx.saved_tensors
-        make = torch.zeros if plan.empty else torch.empty
-        dx, dw, db, dstate = (make(t.shape, device=x.device, dtype=t.dtype) if need else None
-                              for need, t in zip(ctx.needs_input_grad[2:6], (x, weight, bias, state)))
+        dx, dw, db, dstate = _grads(ctx.needs_input_grad[2:6], (x, weight, bias, state), plan.empty)
         if plan.empty:
             dstate = dnext if dstate is not None and dnext is not None else dstate
         elif any(g is not None for g in (dx, dw, db, dstate)):
@@ -1772,14 +1786,17 @@ def causal_conv(x, weight, bias=None, state=None, lengths=None, silu=True, retur
     dev = _same_device(x, weight, bias, state, lengths, state_out)
     _check(x.dim() == 3, "expected x of shape [B, tokens, channels]")
     x, weight, bias, lengths = _in_place(x, 16 // x.element_size()), _dense(weight), _dense(bias), None if lengths is None else lengths.contiguous()
-    first, state = state, _dense(state)
+    state = _dense(state)
     plan = _conv_plan(_layout(x), _layout(weight), _layout(bias), _layout(state), _layout(lengths), int(bool(silu)))
     if state_out is not None:
-        _check_state_out(state_out, plan.state, x.dtype, first, (x, weight, bias, lengths), grad)
+        _check_state_out(state_out, plan, x.dtype, state, (x, weight, bias, lengths), grad)
     args = plan, dev, x, weight, bias, state, lengths, want, state_out
     y, last = (_CausalConv.apply if grad else _causal_conv_fwd)(*args)
     _written(state_out)
     return (y, last) if return_state else y
+
+
+MAX_SCAN_STRIDE = 1 << 25  # elements, of a token of selective_scan's operands
 
 
 @lru_cache(maxsize=512)
@@ -1799,14 +1816,16 @@ def _scan_plan(u, dt, A, B, C, D, z, dt_bias, state, lengths, softplus):
     _check(state is None or (state[0] == (b, c, states) and state[2] == torch.float32),
            "expected a state [B, channels, states] in fp32")
     plan, unit = _Plan(), 4
-    plan.ok = tuple(m is None or (m[1][-1] == 1 and all(n <= 1 or st % unit == 0 for n, st in zip(m[0][:-1], m[1][:-1])))
-                    for m in (u, dt, B, C, z))
+    plan.ok = tuple(m is None or (m[1][-1] == 1 and all(n <= 1 or st % unit == 0 for n, st in zip(m[0][:-1], m[1][:-1]))
+                                  and (t <= 1 or m[1][1] < MAX_SCAN_STRIDE)) for m in (u, dt, B, C, z))
     none = [0, 0]
     strides = [st for m in (u, dt) for st in _steps(m[0], m[1], 2)] + (_steps(z[0], z[1], 2) if z else none)
     strides += _steps(B[0], B[1], 3) + _steps(C[0], C[1], 3)
     plan.codes = code, _check_lengths(lengths, b)
     plan.shape, plan.strides = N.int64_array([b, t, c, states, groups]), N.int64_array(strides)
     plan.softplus, plan.state, plan.empty = softplus, (b, c, states), not (b and t)
+    plan.state_bytes = b * c * states * 4
+    plan.spans = [0 if w is None else _span(w, w[2].itemsize) for w in (u, dt, A, B, C, D, z, dt_bias, lengths)]
     plan.unit = unit * (4 if code == N.F32 else 2)  # bytes
     plan.ws = N.lib().bmx_selective_scan_workspace_bytes(b, t, c, states, groups)
     plan.ws_bwd = N.lib().bmx_selective_scan_bwd_workspace_bytes(b, t, c, states, groups)
@@ -1817,7 +1836,7 @@ def _scan_plan(u, dt, A, B, C, D, z, dt_bias, state, lengths, softplus):
 def _selective_scan_fwd(plan, dev, u, dt, A, B, C, D, z, dt_bias, state, lengths, want_state, state_out,
                         for_backward=False):
     """(out, last state or None, states at the tiles' starts, out before its gate; the latter two for the gradient)."""
-    out = torch.empty(u.shape, device=u.device, dtype=u.dtype)
+    out = _like(u)
     if plan.empty:
         return out, _empty_state(plan.state, torch.float32, u.device, state, state_out) if want_state else None, None, None
     if want_state and state_out is None:
@@ -1847,9 +1866,7 @@ class _SelectiveScan(torch.autograd.Function):
         plan, dev = ctx.rest
         *tensors, lengths, saved, raw = ctx.saved_tensors
         u, dt, A, B, C, D, z, dt_bias, _ = tensors
-        make = torch.zeros if plan.empty else torch.empty
-        grads = [make(t.shape, device=u.device, dtype=t.dtype) if need else None
-                 for need, t in zip(ctx.needs_input_grad[2:11], tensors)]
+        grads = _grads(ctx.needs_input_grad[2:11], tensors, plan.empty)
         if plan.empty:
             if grads[8] is not None and dlast is not None:
                 grads[8] = dlast
@@ -1901,7 +1918,7 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, len
                           for ok, t in zip(plan.ok, moved))
         plan = plan_of(u, dt, B, C, z)
     if state_out is not None:
-        _check_state_out(state_out, plan.state, torch.float32, tensors[8], (*tensors[:8], lengths), grad)
+        _check_state_out(state_out, plan, torch.float32, state, (u, dt, A, B, C, D, z, dt_bias, lengths), grad)
     args = plan, dev, u, dt, A, B, C, D, z, dt_bias, state, lengths, want
     out, last = _SelectiveScan.apply(*args) if grad else _selective_scan_fwd(*args, state_out)[:2]
     _written(state_out)

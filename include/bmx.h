@@ -527,8 +527,8 @@ int bmx_causal_conv_bwd(const void* x, int dtype, const int64_t* shape, const in
  * u, dt, z [batch, tokens, channels] and B, C [batch, tokens, groups, states] in dtype; A [channels, states], D and
  * dt_bias [channels] (or NULL: 0) fp32, dense; state [batch, channels, states] fp32 (NULL: zeros).  shape = {batch,
  * tokens, channels, states, groups}: states 8, 16, 32 or 64, channels / groups a multiple of 8, channels below 2^20, fewer
- * than 2^31 rows; strides = {batch, token of u, of dt, of z, batch, token, group of B, of C}, multiples of 4, last axes
- * dense.  lengths as for bmx_causal_conv_fwd: later tokens give zeros and leave the state alone.  out dense; state_out
+ * than 2^31 rows; strides = {batch, token of u, of dt, of z, batch, token, group of B, of C}, multiples of 4, a token's
+ * in [0, 2^25), last axes dense.  lengths as for bmx_causal_conv_fwd: later tokens give zeros and leave the state alone.  out dense; state_out
  * (or NULL) fp32: the last state; it may be `state` itself.  For the backward pass, or NULL: saved
  * (bmx_selective_scan_saved_bytes), and raw, out's shape in fp32, where z is given.  workspace:
  * bmx_selective_scan_workspace_bytes.  Inputs aligned to 4 elements, the others to 16 bytes.  No reference kernel. */

@@ -110,7 +110,7 @@ def test_selective_scan_rejects_bad_arguments(lib):
     assert refused(lib, fwd(shape=long, ws=None), b"workspace")
     assert fwd(shape=(0, 5, 64, 16, 1), u=None, out=None) == N.BMX_OK
     assert lib.bmx_selective_scan_workspace_bytes(1, 1, 64, 16, 1) == 0
-    assert lib.bmx_selective_scan_saved_bytes(2, 33, 64, 16) == 2 * 2 * 64 * 16 * 4
+    assert lib.bmx_selective_scan_saved_bytes(2, 33, 64, 16) == 2 * 3 * 64 * 16 * 4
     size = lib.bmx_selective_scan_bwd_workspace_bytes(2, 5, 64, 16, 1)
 
     def bwd(D=FAKE, z=FAKE, bias=FAKE, saved=FAKE, raw=FAKE, du=FAKE, ws=FAKE, size=size, rows=5):
@@ -180,20 +180,22 @@ def test_state_buffers():
     state, x = memory[:2], torch.zeros(2, 5, 64, dtype=BF16)
 
     def check(out, state=state, x=x, grad=False):
-        ops._check_state_out(out, (2, 3, 64), BF16, state, (x,), grad)
+        plan = ops._conv_plan(*layouts(x, e(64, 4), None, state, None), 1)
+        ops._check_state_out(out, plan, BF16, state, (x, None, None, None), grad)
 
     check(state)
     check(memory[2:])
     check(state.view(2, 3, 64))
+    check(memory[1:3], x=memory.flatten()[:128].view(1, 2, 64).expand(2, 2, 64), state=None)  # in front of it
     for out, text in ((memory[1:3], "shares memory"), (torch.zeros(2, 3, 64), "dense"), (torch.zeros(2, 3, 128, dtype=BF16)
                       [..., :64], "dense"), (memory.flatten()[4:4 + 384].view(2, 3, 64), "aligned"),
                       (torch.zeros(1, 3, 64, dtype=BF16).expand(2, 3, 64), "dense")):
         with pytest.raises(RuntimeError, match=text):
             check(out)
     with pytest.raises(RuntimeError, match="shares memory"):
-        check(memory[:2], state=None, x=memory[:1])
+        check(memory[:2], state=None, x=memory[1:].flatten()[:256].view(2, 2, 64))
     with pytest.raises(RuntimeError, match="shares memory"):
-        check(memory[:2], state=memory[::2])
+        check(memory[:2], state=None, x=memory[:2])  # the inputs themselves are not the state
     with pytest.raises(RuntimeError, match="return_state"):
         check(state, grad=True)
 
