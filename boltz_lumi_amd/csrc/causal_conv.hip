@@ -13,6 +13,7 @@
 // with all its rows in flight at once; the W - 1 rows before (backward: and
 // behind) a run come from the neighbours' cache lines.  Sums are fp32.
 #include <type_traits>
+#include <utility>
 
 #include "bmx_common.h"
 
@@ -20,9 +21,18 @@ using namespace bmx;
 
 namespace {
 
-constexpr int kRun = 16;      // tokens of a thread
-constexpr int kBwdRun = 8;
+constexpr int kRun = 8;       // tokens of a thread
+constexpr int kBwdVec = 4, kBwdRun = 8;
 constexpr int kBwdVecs = 32;  // a gradient's block: 32 runs of channels by 8 runs of tokens
+
+template <typename F, int... I>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>()), ...);
+}
+template <int kCount, typename F>
+__device__ __forceinline__ void each_of(F f) {
+  each_of(f, std::make_integer_sequence<int, kCount>());
+}
 
 struct Conv {
   const void *x, *w, *bias, *state, *lengths, *dy, *dnext;
@@ -33,36 +43,23 @@ struct Conv {
   int channels, vecs, runs, lengths64, silu, w_bf16, b_bf16;
 };
 
-template <typename T>
-constexpr int kVec = 16 / sizeof(T);
-
+// V channels of one token as they lie in memory, and as fp32.
+template <typename T, int V>
+struct Run {
+  typedef T Vec __attribute__((ext_vector_type(V)));
+  Vec v;
+  __device__ __forceinline__ float operator[](int i) const { return (float)v[i]; }
+};
 template <int V>
 struct Vals {
   float v[V];
 };
-template <typename T>
-__device__ __forceinline__ Vals<kVec<T>> unpack(const f32x4& raw) {
-  Vals<kVec<T>> o;
-  if constexpr (sizeof(T) == 4) {
+template <typename T, int V>
+__device__ __forceinline__ void put(T* p, const Vals<V>& a) {
+  Run<T, V> o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o.v[i] = raw[i];
-  } else {
-    const bf16x8 h = __builtin_bit_cast(bf16x8, raw);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) o.v[i] = (float)h[i];
-  }
-  return o;
-}
-template <typename T>
-__device__ __forceinline__ f32x4 pack(const Vals<kVec<T>>& a) {
-  if constexpr (sizeof(T) == 4) {
-    return f32x4{a.v[0], a.v[1], a.v[2], a.v[3]};
-  } else {
-    bf16x8 h;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = (bf16)a.v[i];
-    return __builtin_bit_cast(f32x4, h);
-  }
+  for (int i = 0; i < V; ++i) o.v[i] = (T)a.v[i];
+  *(Run<T, V>*)p = o;
 }
 
 __device__ __forceinline__ int64_t length_of(const void* lengths, int lengths64, int64_t b, int64_t tokens) {
@@ -71,79 +68,85 @@ __device__ __forceinline__ int64_t length_of(const void* lengths, int lengths64,
   return n < 0 ? 0 : n < tokens ? n : tokens;
 }
 
-// The taps of a thread's channels and the bias: weight is [channels][W].
-template <typename T, int W>
+// The taps of a thread's channels and the bias: weight is [channels][W], V W values in a row.
+template <int W, int V>
 struct Taps {
-  float w[kVec<T>][W], b[kVec<T>];
-  __device__ __forceinline__ Taps(const Conv& s, int c) {
+  float w[V][W], b[V];
+  template <typename T, int kCount>
+  static __device__ __forceinline__ void load(const void* from, int at, float* to) {
 #pragma unroll
-    for (int i = 0; i < kVec<T>; ++i) {
+    for (int i = 0; i < kCount; i += 4) {
+      const f32x4 q = load4((const T*)from + at + i);
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const int at = (c + i) * W + j;
-        w[i][j] = s.w_bf16 ? (float)((const bf16*)s.w)[at] : ((const float*)s.w)[at];
-      }
-      b[i] = !s.bias ? 0.f : s.b_bf16 ? (float)((const bf16*)s.bias)[c + i] : ((const float*)s.bias)[c + i];
+      for (int k = 0; k < 4; ++k) to[i + k] = q[k];
     }
+  }
+  __device__ __forceinline__ Taps(const Conv& s, int c) {
+    if (s.w_bf16)
+      load<bf16, V * W>(s.w, c * W, &w[0][0]);
+    else
+      load<float, V * W>(s.w, c * W, &w[0][0]);
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] = 0.f;
+    if (s.bias) s.b_bf16 ? load<bf16, V>(s.bias, c, b) : load<float, V>(s.bias, c, b);
   }
 };
 
 // Row t of a sequence: the state's rows before token 0, zeros from its length on.
-template <typename T, int W>
-__device__ __forceinline__ f32x4 input_row(const Conv& s, int64_t b, int64_t t, int64_t length, int c) {
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  if (t >= length) return zero;
-  if (t >= 0) return *(const f32x4*)((const T*)s.x + b * s.sb + t * s.st + c);
-  return s.state ? *(const f32x4*)((const T*)s.state + (b * (W - 1) + t + W - 1) * s.channels + c) : zero;
+template <typename T, int W, int V>
+__device__ __forceinline__ Run<T, V> input_row(const Conv& s, int64_t b, int64_t t, int64_t length, int c) {
+  Run<T, V> o = {};
+  if (t >= length) return o;
+  if (t >= 0)
+    o = *(const Run<T, V>*)((const T*)s.x + b * s.sb + t * s.st + c);
+  else if (s.state)
+    o = *(const Run<T, V>*)((const T*)s.state + (b * (W - 1) + t + W - 1) * s.channels + c);
+  return o;
 }
 
-template <typename T, int W, int R>
+template <typename T, int W, int V, int R>
 __global__ __launch_bounds__(256) void causal_conv_kernel(Conv s) {
   const int64_t item = (int64_t)block_index() * 256 + threadIdx.x;
   const int64_t row = item / s.vecs, b = row / s.runs;
   if (b >= s.batch) return;
-  const int c = (int)(item - row * s.vecs) * kVec<T>;
+  const int c = (int)(item - row * s.vecs) * V;
   const int64_t t0 = (row - b * s.runs) * R, length = length_of(s.lengths, s.lengths64, b, s.tokens);
-  f32x4 raw[R + W - 1];
+  Run<T, V> raw[R + W - 1];
 #pragma unroll
-  for (int i = 0; i < R + W - 1; ++i) raw[i] = input_row<T, W>(s, b, t0 + i - (W - 1), length, c);
+  for (int i = 0; i < R + W - 1; ++i) raw[i] = input_row<T, W, V>(s, b, t0 + i - (W - 1), length, c);
   if (s.next && t0 == 0) {
     // The thread of the first tokens alone looks at the state, so that the next one may take its place.
-    f32x4 last[W - 1];
+    Run<T, V> last[W - 1];
 #pragma unroll
-    for (int i = 0; i < W - 1; ++i) last[i] = input_row<T, W>(s, b, length + i - (W - 1), length, c);
+    for (int i = 0; i < W - 1; ++i) last[i] = input_row<T, W, V>(s, b, length + i - (W - 1), length, c);
 #pragma unroll
-    for (int i = 0; i < W - 1; ++i) *(f32x4*)((T*)s.next + (b * (W - 1) + i) * s.channels + c) = last[i];
+    for (int i = 0; i < W - 1; ++i) *(Run<T, V>*)((T*)s.next + (b * (W - 1) + i) * s.channels + c) = last[i];
   }
-  const Taps<T, W> taps(s, c);
+  const Taps<W, V> taps(s, c);
   T* y = (T*)s.y + (b * s.tokens + t0) * s.channels + c;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     if (t0 + i >= s.tokens) break;
-    Vals<kVec<T>> p;
+    Vals<V> p;
 #pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) p.v[e] = taps.b[e];
+    for (int e = 0; e < V; ++e) {
+      p.v[e] = taps.b[e];
 #pragma unroll
-    for (int j = 0; j < W; ++j) {
-      const Vals<kVec<T>> x = unpack<T>(raw[i + j]);
-#pragma unroll
-      for (int e = 0; e < kVec<T>; ++e) p.v[e] += taps.w[e][j] * x.v[e];
-    }
-#pragma unroll
-    for (int e = 0; e < kVec<T>; ++e) {
+      for (int j = 0; j < W; ++j) p.v[e] += taps.w[e][j] * raw[i + j][e];
       if (s.silu) p.v[e] = silu_f(p.v[e]);
       if (t0 + i >= length) p.v[e] = 0.f;
     }
-    *(f32x4*)(y + (int64_t)i * s.channels) = pack<T>(p);
+    put<T, V>(y + (int64_t)i * s.channels, p);
   }
 }
 
-// Gradient: a thread works dp out for its run and the W - 1 tokens behind it.  Its eight token-run neighbours add
-// their sums for the weights in LDS; a block leaves one partial row per weight.
+// Gradient: a thread works dp out for its run and the W - 1 tokens behind it, four channels (eight of bf16 need more
+// registers than two waves a SIMD have: 50 us for 16 at 4 x 2048 x 1536).  Its eight token-run neighbours add their sums
+// for the weights in LDS; a block leaves one partial row per weight.
 template <typename T, int W>
 __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(Conv s) {
-  constexpr int V = kVec<T>, R = kBwdRun, kRows = 256 / kBwdVecs;
-  __shared__ float sums[kRows][kBwdVecs][V + 1];
+  constexpr int V = kBwdVec, R = kBwdRun, kRows = 256 / kBwdVecs;
+  __shared__ __align__(16) f32x4 sums[kRows][kBwdVecs];
   const int64_t block = block_index();
   if (block >= s.blocks) return;
   const int cblocks = (s.vecs + kBwdVecs - 1) / kBwdVecs, tblocks = (s.runs + kRows - 1) / kRows;
@@ -154,95 +157,81 @@ __global__ __launch_bounds__(256) void causal_conv_bwd_kernel(Conv s) {
   const bool live = vec < s.vecs && t0 < s.tokens;
   const int c = live ? vec * V : 0;
   const int64_t length = live ? length_of(s.lengths, s.lengths64, b, s.tokens) : 0;
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  f32x4 raw[R + 2 * (W - 1)], back[R + W - 1];
+  Run<T, V> raw[R + 2 * (W - 1)], back[R + W - 1];
 #pragma unroll
-  for (int i = 0; i < R + 2 * (W - 1); ++i) raw[i] = input_row<T, W>(s, b, t0 + i - (W - 1), length, c);
+  for (int i = 0; i < R + 2 * (W - 1); ++i) raw[i] = input_row<T, W, V>(s, b, t0 + i - (W - 1), length, c);
 #pragma unroll
-  for (int i = 0; i < R + W - 1; ++i)
-    back[i] = s.dy && t0 + i < length ? *(const f32x4*)((const T*)s.dy + (b * s.tokens + t0 + i) * s.channels + c) : zero;
-  const Taps<T, W> taps(s, c);
-  float dw[W + 1][V];
+  for (int i = 0; i < R + W - 1; ++i) {
+    back[i] = {};
+    if (s.dy && t0 + i < length) back[i] = *(const Run<T, V>*)((const T*)s.dy + (b * s.tokens + t0 + i) * s.channels + c);
+  }
+  const Taps<W, V> taps(s, c);
+  f32x4 dw[W + 1];
 #pragma unroll
-  for (int j = 0; j <= W; ++j)
-#pragma unroll
-    for (int e = 0; e < V; ++e) dw[j][e] = 0.f;
+  for (int j = 0; j <= W; ++j) dw[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   Vals<V> dp[R + W - 1];
 #pragma unroll
   for (int i = 0; i < R + W - 1; ++i) {
-    dp[i] = unpack<T>(back[i]);
-    if (s.silu) {
-      Vals<V> p;
+    const bool there = t0 + i < length;  // a row that is not there has dp 0, whatever an infinite p does
 #pragma unroll
-      for (int e = 0; e < V; ++e) p.v[e] = taps.b[e];
+    for (int e = 0; e < V; ++e) {
+      float d = back[i][e];
+      if (s.silu) {
+        float p = taps.b[e];
 #pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const Vals<V> x = unpack<T>(raw[i + j]);
-#pragma unroll
-        for (int e = 0; e < V; ++e) p.v[e] += taps.w[e][j] * x.v[e];
+        for (int j = 0; j < W; ++j) p += taps.w[e][j] * raw[i + j][e];
+        const float sg = sigmoid_f(p);
+        d *= sg + p * sg * (1.f - sg);
       }
+      dp[i].v[e] = there ? d : 0.f;
+      if (i < R) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float sg = sigmoid_f(p.v[e]);
-        // a row that is not there has dp 0, whatever the sigmoid of an infinite p does
-        dp[i].v[e] = t0 + i < length ? dp[i].v[e] * (sg + p.v[e] * sg * (1.f - sg)) : 0.f;
+        for (int j = 0; j < W; ++j) dw[j][e] += there ? d * raw[i + j][e] : 0.f;
+        dw[W][e] += dp[i].v[e];
       }
-    }
-    if (i < R) {
-#pragma unroll
-      for (int j = 0; j < W; ++j) {
-        const Vals<V> x = unpack<T>(raw[i + j]);
-#pragma unroll
-        for (int e = 0; e < V; ++e) dw[j][e] += t0 + i < length ? dp[i].v[e] * x.v[e] : 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < V; ++e) dw[W][e] += dp[i].v[e];
     }
   }
   // dx of row t (the state's rows where t < 0): the taps that it went into, and its place in the next state.
-  auto dx_row = [&](int i, int64_t t) {  // i: dp's index of row t
+  auto dx_row = [&](auto index, int64_t t, T* to) {  // index: dp's of row t
+    constexpr int i = decltype(index)::value;
     Vals<V> dx;
 #pragma unroll
-    for (int e = 0; e < V; ++e) dx.v[e] = 0.f;
+    for (int e = 0; e < V; ++e) {
+      dx.v[e] = 0.f;
 #pragma unroll
-    for (int j = 0; j < W; ++j)
-      if (i + W - 1 - j >= 0) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) dx.v[e] += taps.w[e][j] * dp[i + W - 1 - j].v[e];
-      }
+      for (int j = 0; j < W; ++j)
+        if (i + W - 1 - j >= 0) dx.v[e] += taps.w[e][j] * dp[i + W - 1 - j >= 0 ? i + W - 1 - j : 0].v[e];
+    }
     const int64_t at = t - (length - (W - 1));
     if (s.dnext && at >= 0 && at < W - 1) {
-      const Vals<V> d = unpack<T>(*(const f32x4*)((const T*)s.dnext + (b * (W - 1) + at) * s.channels + c));
+      const Run<T, V> d = *(const Run<T, V>*)((const T*)s.dnext + (b * (W - 1) + at) * s.channels + c);
 #pragma unroll
-      for (int e = 0; e < V; ++e) dx.v[e] += d.v[e];
+      for (int e = 0; e < V; ++e) dx.v[e] += d[e];
     }
-    return pack<T>(dx);
+    put<T, V>(to, dx);
   };
   if (live && s.dx) {
     T* dx = (T*)s.dx + (b * s.tokens + t0) * s.channels + c;
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-      if (t0 + i < s.tokens) *(f32x4*)(dx + (int64_t)i * s.channels) = dx_row(i, t0 + i);
+    each_of<R>([&](auto i) {
+      if (t0 + i < s.tokens) dx_row(i, t0 + i, dx + (int64_t)i * s.channels);
+    });
   }
-  if (live && s.dstate && t0 == 0) {
-#pragma unroll
-    for (int i = 0; i < W - 1; ++i)
-      *(f32x4*)((T*)s.dstate + (b * (W - 1) + i) * s.channels + c) = dx_row(i - (W - 1), i - (W - 1));
-  }
+  if (live && s.dstate && t0 == 0)
+    each_of<W - 1>([&](auto i) {
+      dx_row(std::integral_constant<int, decltype(i)::value - (W - 1)>(), i - (W - 1),
+             (T*)s.dstate + (b * (W - 1) + i) * s.channels + c);
+    });
   if (!s.partial) return;
 #pragma unroll
   for (int j = 0; j <= W; ++j) {
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < V; ++e) sums[group][v][e] = live ? dw[j][e] : 0.f;
+    sums[group][v] = live ? dw[j] : f32x4{0.f, 0.f, 0.f, 0.f};
     __syncthreads();
-    const int e = threadIdx.x % V, u = threadIdx.x / V;
-    const int at = (int)(block % cblocks) * kBwdVecs + u;
-    if (u < kBwdVecs && at < s.vecs) {
-      float total = 0.f;
+    if (group == 0 && vec < s.vecs) {
+      f32x4 total = sums[0][v];
 #pragma unroll
-      for (int g = 0; g < kRows; ++g) total += sums[g][u][e];
-      s.partial[(part * (W + 1) + j) * s.channels + at * V + e] = total;
+      for (int g = 1; g < kRows; ++g) total += sums[g][v];
+      *(f32x4*)(s.partial + (part * (W + 1) + j) * s.channels + vec * V) = total;
     }
   }
 }
@@ -275,6 +264,9 @@ __global__ __launch_bounds__(256) void causal_conv_sums_kernel(ConvSums s) {
     ((float*)out)[at] = v;
 }
 
+template <typename T>
+constexpr int kVec = 16 / sizeof(T);  // channels of a thread, forward
+
 template <typename Go>
 int with_width(int64_t width, Go go) {
   using std::integral_constant;
@@ -296,11 +288,11 @@ int forward(Conv& s, int64_t width, hipStream_t stream) {
   return with_width(width, [&](auto w) {
     constexpr int W = decltype(w)::value;
     if (run == 1)
-      causal_conv_kernel<T, W, 1><<<fold_grid(blocks, 256), 256, 0, stream>>>(s);
+      causal_conv_kernel<T, W, kVec<T>, 1><<<fold_grid(blocks, 256), 256, 0, stream>>>(s);
     else if (run == 4)
-      causal_conv_kernel<T, W, 4><<<fold_grid(blocks, 256), 256, 0, stream>>>(s);
+      causal_conv_kernel<T, W, kVec<T>, 4><<<fold_grid(blocks, 256), 256, 0, stream>>>(s);
     else
-      causal_conv_kernel<T, W, kRun><<<fold_grid(blocks, 256), 256, 0, stream>>>(s);
+      causal_conv_kernel<T, W, kVec<T>, kRun><<<fold_grid(blocks, 256), 256, 0, stream>>>(s);
     return check_launch("causal_conv");
   });
 }
@@ -312,7 +304,7 @@ int64_t bwd_parts(int64_t batch, int64_t tokens) {
 
 template <typename T>
 int backward(Conv& s, int64_t width, hipStream_t stream) {
-  s.vecs = s.channels / kVec<T>;
+  s.vecs = s.channels / kBwdVec;
   s.runs = (int)((s.tokens + kBwdRun - 1) / kBwdRun);
   s.blocks = bwd_parts(s.batch, s.tokens) * ((s.vecs + kBwdVecs - 1) / kBwdVecs);
   BMX_REQUIRE(s.blocks < (1ll << 31), "causal_conv: too many rows");
@@ -361,7 +353,7 @@ extern "C" int bmx_causal_conv_fwd(const void* x, int dtype, const int64_t* shap
     return BMX_OK;
   }
   BMX_REQUIRE(x && weight && y, "causal_conv: null pointer");
-  BMX_REQUIRE(aligned16({x, state, y, state_out}), "causal_conv: tensors must be 16-byte aligned");
+  BMX_REQUIRE(aligned16({x, weight, bias, state, y, state_out}), "causal_conv: tensors must be 16-byte aligned");
   s.y = y, s.next = state_out;
   return dtype == kF32 ? forward<float>(s, shape[3], (hipStream_t)stream) : forward<bf16>(s, shape[3], (hipStream_t)stream);
 }
@@ -382,7 +374,7 @@ extern "C" int bmx_causal_conv_bwd(const void* x, int dtype, const int64_t* shap
   BMX_REQUIRE(s.batch > 0 && s.tokens > 0, "causal_conv_bwd: expected rows");
   BMX_REQUIRE(x && weight, "causal_conv: null pointer");
   BMX_REQUIRE((bias || !dbias) && (state || !dstate), "causal_conv_bwd: gradient of an absent bias or state");
-  BMX_REQUIRE(aligned16({x, state, dy, dstate_out, dx, dstate}), "causal_conv: tensors must be 16-byte aligned");
+  BMX_REQUIRE(aligned16({x, weight, bias, state, dy, dstate_out, dx, dstate}), "causal_conv: tensors must be 16-byte aligned");
   s.dy = dy, s.dnext = dstate_out, s.dx = dx, s.dstate = dstate;
   if (dweight || dbias) {
     BMX_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 &&

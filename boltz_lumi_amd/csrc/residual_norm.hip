@@ -22,7 +22,7 @@ using namespace bmx;
 namespace {
 
 constexpr int kMaxDim = 8192;
-constexpr int kBwdBlocks = 512;  // of the gradient: each leaves a partial row per weight
+constexpr int kBwdThreads = 512 * 256;  // of the gradient at most: two waves a SIMD; a block leaves a partial row per weight
 
 struct Rows {
   const void* p;
@@ -53,6 +53,28 @@ __device__ __forceinline__ void store_oct(bf16* p, const Oct& v) {
   *(bf16x8*)p = bf16x8{(bf16)v.a[0], (bf16)v.a[1], (bf16)v.a[2], (bf16)v.a[3],
                        (bf16)v.b[0], (bf16)v.b[1], (bf16)v.b[2], (bf16)v.b[3]};
 }
+// The same as they lie in memory: a row that is on its way holds no more registers than it has bytes.
+template <typename T>
+struct RawOct;
+template <>
+struct RawOct<float> {
+  Oct v;
+  __device__ __forceinline__ Oct wide() const { return v; }
+};
+template <>
+struct RawOct<bf16> {
+  bf16x8 v;
+  __device__ __forceinline__ Oct wide() const {
+    return {f32x4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]},
+            f32x4{(float)v[4], (float)v[5], (float)v[6], (float)v[7]}};
+  }
+};
+template <typename T>
+__device__ __forceinline__ RawOct<T> load_raw(const T* p, bool there) {
+  RawOct<T> o = {};
+  if (there) o = *(const RawOct<T>*)p;
+  return o;
+}
 __device__ __forceinline__ Oct fill(float v) { return {f32x4{v, v, v, v}, f32x4{v, v, v, v}}; }
 __device__ __forceinline__ Oct operator*(const Oct& x, const Oct& y) { return {x.a * y.a, x.b * y.b}; }
 __device__ __forceinline__ Oct operator+(const Oct& x, const Oct& y) { return {x.a + y.a, x.b + y.b}; }
@@ -80,7 +102,7 @@ __device__ __forceinline__ Oct load_weight(const void* w, int w_bf16, int at) {
 // Sum over the L threads of a row, in every one of them.  Rows of several waves meet in LDS: `turn` alternates
 // between two buffers, so that one barrier a sum is enough.
 template <int L>
-__device__ __forceinline__ float row_sum(float v, float (&lds)[2][8], int& turn) {
+__device__ __forceinline__ float row_sum(float v, float (&lds)[2][16], int& turn) {
   if (L == 16) {
     v += dpp<0xB1>(v);
     v += dpp<0x4E>(v);
@@ -99,16 +121,33 @@ __device__ __forceinline__ float row_sum(float v, float (&lds)[2][8], int& turn)
   return v;
 }
 
+// The same for two values, one barrier for both.
+template <int L>
+__device__ __forceinline__ void row_sums(float& v, float& w, float (&lds)[2][16], int& turn) {
+  if (L <= 64) {
+    v = row_sum<L>(v, lds, turn), w = row_sum<L>(w, lds, turn);
+    return;
+  }
+  v = wave_sum_full(v), w = wave_sum_full(w);
+  if (lane_id() == 0) lds[turn][threadIdx.x >> 6] = v, lds[turn][8 + (threadIdx.x >> 6)] = w;
+  __syncthreads();
+  v = w = 0.f;
+#pragma unroll
+  for (int i = 0; i < L / 64; ++i) v += lds[turn][i], w += lds[turn][8 + i];
+  turn ^= 1;
+}
+
+// Threads of a block: rows of up to a wave share one, others have one of their own (they meet at barriers).
 template <int L>
 constexpr int threads_of() {
-  return L > 256 ? L : 256;
+  return L > 64 ? L : 256;
 }
 
 __device__ __forceinline__ float rho(float sum, const Frame& s) { return 1.f / sqrtf(sum * s.inv_dim + s.eps); }
 
 template <typename X, typename Y, int L, int V>
 __global__ __launch_bounds__(threads_of<L>()) void residual_norm_kernel(Frame s) {
-  __shared__ float lds[2][8];
+  __shared__ float lds[2][16];
   int turn = 0;
   const int lane = threadIdx.x % L;
   const int64_t row = (int64_t)block_index() * (threads_of<L>() / L) + threadIdx.x / L;
@@ -154,13 +193,24 @@ __global__ __launch_bounds__(threads_of<L>()) void residual_norm_kernel(Frame s)
 template <typename X, typename Y, int L, int V>
 __global__ __launch_bounds__(threads_of<L>()) void residual_norm_bwd_kernel(Frame s) {
   constexpr int groups = threads_of<L>() / L;
-  __shared__ float lds[2][8];
+  __shared__ float lds[2][16];
   __shared__ float sums[groups > 1 ? groups : 1][groups > 1 ? 8 * L * V : 1];
   int turn = 0;
   const int lane = threadIdx.x % L, group = threadIdx.x / L;
   Oct dyw[V], dscale[V], dw[V], dgate[V];
 #pragma unroll
   for (int v = 0; v < V; ++v) dyw[v] = dscale[v] = dw[v] = dgate[v] = fill(0.f);
+  // the weights stay in registers where there is room; channels that are not there have no part in a row's sums
+  Oct kept[3] = {fill(0.f), fill(0.f), fill(0.f)};
+  if (V == 1 && 8 * lane < s.dim) {
+    kept[0] = load_weight(s.yw, s.w_bf16, 8 * lane), kept[1] = load_weight(s.scale, s.w_bf16, 8 * lane);
+    kept[2] = load_weight(s.w, s.w_bf16, 8 * lane);
+  }
+  auto weight = [&](int which, int v) {
+    const int c = 8 * (lane + v * L);
+    if (V == 1) return kept[which];
+    return c < s.dim ? load_weight(which == 0 ? s.yw : which == 1 ? s.scale : s.w, s.w_bf16, c) : fill(0.f);
+  };
 
   // The groups' sums of one quantity, added in their order, to `out` (its row of dim values).
   auto put = [&](const Oct (&v)[V], auto* out) {
@@ -187,65 +237,74 @@ __global__ __launch_bounds__(threads_of<L>()) void residual_norm_bwd_kernel(Fram
     const int64_t element = s.shared ? unit / s.splits : 0, part = s.shared ? unit % s.splits : unit;
     const int64_t limit = s.shared ? s.tokens : s.rows;
     const int64_t first = part * s.unit_rows, last = min(first + s.unit_rows, limit);
-    for (int64_t i = first + group; i < last; i += groups) {
+    // a row's operands are asked for while the row before is worked on (with two runs a thread there is no room)
+    RawOct<X> nx[V], ndr[V];
+    RawOct<Y> ny[V], ng[V], ndh[V];
+    auto ask = [&](int64_t i) {
       const int64_t row = element * s.tokens + i, b = row / s.tokens, t = row - b * s.tokens;
-      const X* x = (const X*)s.x.p + b * s.x.sb + t * s.x.st;
-      const Y* y = (const Y*)s.y.p + b * s.y.sb + t * s.y.st;
-      const Y* gate = s.gate.p ? (const Y*)s.gate.p + b * s.gate.sb + t * s.gate.st : nullptr;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int c = 8 * (lane + v * L);
+        const bool live = c < s.dim && i < last;
+        nx[v] = load_raw((const X*)s.x.p + b * s.x.sb + t * s.x.st + c, live);
+        ny[v] = load_raw((const Y*)s.y.p + b * s.y.sb + t * s.y.st + c, live);
+        ng[v] = load_raw((const Y*)s.gate.p + b * s.gate.sb + t * s.gate.st + c, live && s.gate.p);
+        ndr[v] = load_raw((const X*)s.dr + row * s.dim + c, live && s.dr);
+        ndh[v] = load_raw((const Y*)s.dh + row * s.dim + c, live && s.dh);
+      }
+    };
+    if (V == 1) ask(first + group);
+    for (int64_t i = first + group; i < last; i += groups) {
+      const int64_t row = element * s.tokens + i;
+      const bool gate = s.gate.p;
+      if (V > 1) ask(i);
       Oct r[V], n[V], g[V], dr[V], dh[V];
       float sum = 0.f;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int c = 8 * (lane + v * L);
-        const bool live = c < s.dim;
-        r[v] = live ? load_oct(x + c) : fill(0.f);
-        n[v] = live ? load_oct(y + c) : fill(0.f);
-        g[v] = live && gate ? load_oct(gate + c) : fill(0.f);
-        dr[v] = live && s.dr ? load_oct((const X*)s.dr + row * s.dim + c) : fill(0.f);
-        dh[v] = live && s.dh ? load_oct((const Y*)s.dh + row * s.dim + c) : fill(0.f);
+        r[v] = nx[v].wide(), n[v] = ny[v].wide(), g[v] = ng[v].wide(), dr[v] = ndr[v].wide(), dh[v] = ndh[v].wide();
         sum += dot(n[v], n[v]);
       }
+      if (V == 1) ask(i + groups);
       const float ry = s.post ? rho(row_sum<L>(sum, lds, turn), s) : 1.f;
       float rr = 0.f, er = 0.f;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        const int c = 8 * (lane + v * L);
-        if (c >= s.dim) continue;
         if (gate) g[v] = sigmoid(g[v]);
-        Oct k = load_weight(s.scale, s.w_bf16, c);
+        Oct k = weight(1, v);
         if (gate) k = k * g[v];
         n[v] = n[v] * ry;
-        r[v] = r[v] + n[v] * load_weight(s.yw, s.w_bf16, c) * k;
+        r[v] = r[v] + n[v] * weight(0, v) * k;
         rr += dot(r[v], r[v]);
-        er += dot(dh[v] * load_weight(s.w, s.w_bf16, c), r[v]);
+        er += dot(dh[v] * weight(2, v), r[v]);
       }
       if (s.pre) {
-        rr = rho(row_sum<L>(rr, lds, turn), s);
-        er = row_sum<L>(er, lds, turn) * s.inv_dim * rr * rr;
+        row_sums<L>(rr, er, lds, turn);
+        rr = rho(rr, s), er *= s.inv_dim * rr * rr;
       }
       float fn = 0.f;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         const int c = 8 * (lane + v * L);
-        if (c >= s.dim) continue;
+        const bool live = c < s.dim;
         if (s.pre) {
-          dr[v] = dr[v] + (dh[v] * load_weight(s.w, s.w_bf16, c) - r[v] * er) * rr;
+          dr[v] = dr[v] + (dh[v] * weight(2, v) - r[v] * er) * rr;
           dw[v] = dw[v] + dh[v] * r[v] * rr;
         }
-        if (s.dx) store_oct((X*)s.dx + row * s.dim + c, dr[v]);
-        const Oct yw = load_weight(s.yw, s.w_bf16, c), scale = load_weight(s.scale, s.w_bf16, c);
+        if (s.dx && live) store_oct((X*)s.dx + row * s.dim + c, dr[v]);
         const Oct gated = gate ? dr[v] * g[v] : dr[v];  // dR s
-        dscale[v] = dscale[v] + gated * n[v] * yw;
+        const Oct block = gated * n[v];
+        dscale[v] = dscale[v] + block * weight(0, v);
+        const Oct back = gated * weight(1, v);
+        dyw[v] = dyw[v] + back * n[v];
+        dr[v] = back * weight(0, v);
         if (gate) {
-          const Oct dg = gated * scale * n[v] * yw * (fill(1.f) - g[v]);
+          const Oct dg = dr[v] * n[v] * (fill(1.f) - g[v]);
           if (s.shared)
             dgate[v] = dgate[v] + dg;
-          else if (s.dgate)
+          else if (s.dgate && live)
             store_oct((Y*)s.dgate + row * s.dim + c, dg);
         }
-        const Oct back = gated * scale;
-        dyw[v] = dyw[v] + back * n[v];
-        dr[v] = back * yw;
         fn += dot(dr[v], n[v]);
       }
       if (s.post) fn = row_sum<L>(fn, lds, turn) * s.inv_dim;
@@ -253,8 +312,7 @@ __global__ __launch_bounds__(threads_of<L>()) void residual_norm_bwd_kernel(Fram
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const int c = 8 * (lane + v * L);
-          if (c < s.dim)
-            store_oct((Y*)s.dy + row * s.dim + c, s.post ? (dr[v] - n[v] * fn) * ry : dr[v]);
+          if (c < s.dim) store_oct((Y*)s.dy + row * s.dim + c, s.post ? (dr[v] - n[v] * fn) * ry : dr[v]);
         }
       }
     }
@@ -274,7 +332,7 @@ __global__ __launch_bounds__(threads_of<L>()) void residual_norm_bwd_kernel(Fram
   put(dw, out + 2 * s.dim);
 }
 
-// Column sums of partial rows: a block per 16 columns of one result, 16 threads over the rows of each.
+// Column sums of partial rows: a block per 32 columns of one result, 32 slices of the rows, four columns a thread.
 struct ColumnSums {
   const float* partial[4];
   void* out[4];
@@ -283,68 +341,71 @@ struct ColumnSums {
   int dim;
 };
 __global__ __launch_bounds__(256) void residual_norm_sums_kernel(ColumnSums s) {
-  __shared__ float lds[16][17];
+  __shared__ f32x4 lds[32][9];
   const int which = blockIdx.y;
   if (!s.out[which]) return;
-  const int col = threadIdx.x % 16, part = threadIdx.x / 16, c = (int)blockIdx.x * 16 + col;
+  const int col = threadIdx.x % 8, part = threadIdx.x / 8, c = (int)blockIdx.x * 32 + 4 * col;
   for (int64_t batch = blockIdx.z; batch < s.batches[which]; batch += gridDim.z) {
     const float* from = s.partial[which] + batch * s.batch_stride[which] + c;
-    float v = 0.f;
-    if (c < s.dim)
-      for (int row = part; row < s.rows[which]; row += 16) v += from[row * s.row_stride[which]];
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (c < s.dim) {
+#pragma unroll 8
+      for (int row = part; row < s.rows[which]; row += 32) v += *(const f32x4*)(from + row * s.row_stride[which]);
+    }
     __syncthreads();
     lds[part][col] = v;
     __syncthreads();
     if (part == 0 && c < s.dim) {
-      v = 0.f;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) v += lds[i][col];
+      for (int i = 1; i < 32; ++i) v += lds[i][col];
       if (s.bf16_out[which])
-        ((bf16*)s.out[which])[batch * s.dim + c] = (bf16)v;
+        store4((bf16*)s.out[which] + batch * s.dim + c, v);
       else
-        ((float*)s.out[which])[batch * s.dim + c] = v;
+        store4((float*)s.out[which] + batch * s.dim + c, v);
     }
   }
 }
 
-// A row's threads and runs of 8 channels each.
-template <typename Go>
+// A row's threads and runs of 8 channels each.  The gradient has one run a thread where it can: with two its registers
+// leave one wave a SIMD.
+template <bool kBackward, typename Go>
 void with_layout(int dim, Go go) {
   using std::integral_constant;
   if (dim <= 128) return go(integral_constant<int, 16>(), integral_constant<int, 1>());
   if (dim <= 512) return go(integral_constant<int, 64>(), integral_constant<int, 1>());
-  if (dim <= 1024) return go(integral_constant<int, 64>(), integral_constant<int, 2>());
+  if (dim <= 1024) return go(integral_constant<int, kBackward ? 128 : 64>(), integral_constant<int, kBackward ? 1 : 2>());
   if (dim <= 2048) return go(integral_constant<int, 256>(), integral_constant<int, 1>());
-  if (dim <= 4096) return go(integral_constant<int, 256>(), integral_constant<int, 2>());
+  if (dim <= 4096) return go(integral_constant<int, kBackward ? 512 : 256>(), integral_constant<int, kBackward ? 1 : 2>());
   return go(integral_constant<int, 512>(), integral_constant<int, 2>());
 }
 
 template <typename X, typename Y>
-void launch(bool backward, const Frame& s, int blocks, hipStream_t stream) {
-  with_layout(s.dim, [&](auto l, auto v) {
-    constexpr int L = decltype(l)::value, V = decltype(v)::value, per = threads_of<L>() / L;
-    if (backward)
-      residual_norm_bwd_kernel<X, Y, L, V><<<blocks, threads_of<L>(), 0, stream>>>(s);
-    else
-      residual_norm_kernel<X, Y, L, V><<<fold_grid((s.rows + per - 1) / per, threads_of<L>()), threads_of<L>(), 0,
-                                         stream>>>(s);
+void launch(const Frame& s, hipStream_t stream) {
+  with_layout<false>(s.dim, [&](auto l, auto v) {
+    constexpr int L = decltype(l)::value, V = decltype(v)::value, threads = threads_of<L>(), per = threads / L;
+    residual_norm_kernel<X, Y, L, V><<<fold_grid((s.rows + per - 1) / per, threads), threads, 0, stream>>>(s);
+  });
+}
+template <typename X, typename Y>
+void launch_bwd(const Frame& s, int blocks, hipStream_t stream) {
+  with_layout<true>(s.dim, [&](auto l, auto v) {
+    constexpr int L = decltype(l)::value, V = decltype(v)::value;
+    residual_norm_bwd_kernel<X, Y, L, V><<<blocks, threads_of<L>(), 0, stream>>>(s);
   });
 }
 
-int rows_per_pass(int dim) {
-  int rows = 1;
-  with_layout(dim, [&](auto l, auto) { rows = threads_of<decltype(l)::value>() / decltype(l)::value; });
-  return rows;
-}
-
-// Units of the gradient's rows and the blocks that walk them.  About 8 rows a group, at most kBwdBlocks blocks; with
+// Units of the gradient's rows and the blocks that walk them.  About 8 rows a group, at most kBwdThreads threads; with
 // a gate per batch element, whole elements or equal parts of them.
 struct Units {
   int64_t units, unit_rows, splits;
   int blocks;
 };
 Units plan_units(int64_t batch, int64_t tokens, int64_t dim, bool shared) {
-  const int64_t per = 8 * rows_per_pass((int)dim), most = kBwdBlocks;
+  int64_t per = 1, most = 1;
+  with_layout<true>((int)dim, [&](auto l, auto) {
+    constexpr int L = decltype(l)::value, threads = threads_of<L>();
+    per = 8 * (threads / L), most = kBwdThreads / threads;
+  });
   const int64_t rows = batch * tokens, length = shared ? tokens : rows, elements = shared ? batch : 1;
   int64_t splits = elements >= most ? 1 : most / elements;
   const int64_t enough = (length + per - 1) / per;
@@ -402,11 +463,11 @@ extern "C" int bmx_residual_norm_fwd(const void* x, const void* y, const void* g
   s.yw = s.post ? y_weight : nullptr, s.scale = scale, s.w = weight, s.r = r, s.h = h;
   hipStream_t hs = (hipStream_t)stream;
   if (dtype == kF32)
-    launch<float, float>(false, s, 0, hs);
+    launch<float, float>(s, hs);
   else if (x_dtype == kF32)
-    launch<float, bf16>(false, s, 0, hs);
+    launch<float, bf16>(s, hs);
   else
-    launch<bf16, bf16>(false, s, 0, hs);
+    launch<bf16, bf16>(s, hs);
   return check_launch("residual_norm");
 }
 
@@ -429,7 +490,7 @@ extern "C" int bmx_residual_norm_bwd(const void* x, const void* y, const void* g
   BMX_REQUIRE(gate_kind != 0 || !dgate, "residual_norm_bwd: gradient of an absent gate");
   BMX_REQUIRE((y_weight || !dy_weight) && (scale || !dscale) && (weight || !dweight),
               "residual_norm_bwd: gradient of an absent weight");
-  BMX_REQUIRE(aligned16({x, y, gate, y_weight, scale, weight, dr, dh, dx, dy, dgate}),
+  BMX_REQUIRE(aligned16({x, y, gate, y_weight, scale, weight, dr, dh, dx, dy, dgate, dy_weight, dscale, dweight}),
               "residual_norm: tensors must be 16-byte aligned");
   const Units u = plan_units(shape[0], shape[1], s.dim, s.shared);
   const bool weights = dy_weight || dscale || dweight, gates = s.shared && dgate && u.splits > 1;
@@ -445,11 +506,11 @@ extern "C" int bmx_residual_norm_bwd(const void* x, const void* y, const void* g
   s.gate_partial = gates ? (float*)workspace + (int64_t)u.blocks * 3 * s.dim : nullptr;
   hipStream_t hs = (hipStream_t)stream;
   if (dtype == kF32)
-    launch<float, float>(true, s, u.blocks, hs);
+    launch_bwd<float, float>(s, u.blocks, hs);
   else if (x_dtype == kF32)
-    launch<float, bf16>(true, s, u.blocks, hs);
+    launch_bwd<float, bf16>(s, u.blocks, hs);
   else
-    launch<bf16, bf16>(true, s, u.blocks, hs);
+    launch_bwd<bf16, bf16>(s, u.blocks, hs);
   if (weights || gates) {
     ColumnSums c = {};
     void* outs[3] = {dy_weight, dscale, dweight};
@@ -462,7 +523,7 @@ extern "C" int bmx_residual_norm_bwd(const void* x, const void* y, const void* g
     c.bf16_out[3] = dtype == kBF16, c.batches[3] = (int)shape[0];
     c.dim = s.dim;
     const int z = gates ? (int)(shape[0] < 64 ? shape[0] : 64) : 1;
-    residual_norm_sums_kernel<<<dim3((s.dim + 15) / 16, 4, z), 256, 0, hs>>>(c);
+    residual_norm_sums_kernel<<<dim3((s.dim + 31) / 32, 4, z), 256, 0, hs>>>(c);
   }
   return check_launch("residual_norm_bwd");
 }

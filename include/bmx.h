@@ -507,7 +507,7 @@ int bmx_residual_norm_bwd(const void* x, const void* y, const void* gate, int x_
  * w_dtype, bias [channels] in bias_dtype or NULL.  state: the width - 1 rows before the first [batch, width - 1,
  * channels] in dtype, dense, or NULL (zeros).  lengths: int32 / int64 [batch], taken into [0, tokens]; rows from there
  * on are not read and give zeros; or NULL.  y dense; state_out (or NULL): the width - 1 rows before the end of each
- * sequence, dense; it may be `state` itself.  x, y and the states 16-byte aligned.  No reference kernel. */
+ * sequence, dense; it may be `state` itself.  All pointers but lengths 16-byte aligned.  No reference kernel. */
 int bmx_causal_conv_fwd(const void* x, int dtype, const int64_t* shape, const int64_t* strides, const void* weight,
                         int w_dtype, const void* bias, int bias_dtype, const void* state, const void* lengths,
                         int lengths64, int silu, void* y, void* state_out, bmx_stream_t stream);
