@@ -51,7 +51,6 @@ struct Scan {
   void *dB_out, *dC_out;
   float *dA, *dD, *dbias;   // partial sums, [batch * ranges][channels]([states])
   int64_t batch, tokens, tiles, grad_tiles, chunks, chunk_tiles, blocks;
-  uint32_t eighth;  // blocks of an XCD
   int channels, groups, group_channels, states, cblocks, lengths64, softplus;
   int span, spans, ranges, range_tiles, whole;
 };
@@ -75,7 +74,7 @@ __device__ __forceinline__ float step_of(float x) {
   s = s * q + 0.400249094f;
   s = s * q + 0.66666317f;
   s = s * q + 2.f;
-  return s * r + fmaxf(x, 0.f);
+  return s * r + __builtin_amdgcn_fmed3f(x, 0.f, __builtin_inff());
 }
 
 // v of the lane that a DPP control word names, as an operand of the instruction that uses it.
@@ -191,6 +190,12 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_wave_barrier();
 }
 
+// v, as a value that the compiler does not know: what is worked out of it is not kept in registers over the loops around.
+__device__ __forceinline__ int again(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
+
 // ------------------------------------------------------------ walking chunks
 
 // kLocal: from zero states to each chunk's own, forward; kOut: the outputs; kBack: the same as kLocal for X, from the
@@ -203,9 +208,10 @@ __global__ __launch_bounds__(256, 4) void scan_walk_kernel(Scan s) {
   constexpr int kStep = K / kPer, kMapStep = 1024 / N;  // tokens between a thread's elements, and between its maps'
   __shared__ float sd[kWalk * kChannelRow], sv[kWalk * kChannelRow], sy[kMode == kOut ? kWalk * kChannelRow : 4];
   __shared__ __align__(16) float sB[N * kRow], sC[kMode == kOut ? N * kRow : 4];
-  // Neighbours in channels read the same lines: they are dealt to one XCD, one after another.
+  // Neighbours in channels read the same lines (below 64 bf16 channels a block): four at a time are dealt to an XCD.
+  // Longer runs would give an XCD whole sequences, whose lengths differ.
   uint32_t block = block_index();
-  block = block % 8 * s.eighth + block / 8;
+  block = (block / 32 * 8 + block % 8) * 4 + block / 8 % 4;
   if (block >= s.blocks) return;
   const int cblock = (int)(block % (uint32_t)s.cblocks);
   block /= (uint32_t)s.cblocks;
@@ -275,6 +281,9 @@ __global__ __launch_bounds__(256, 4) void scan_walk_kernel(Scan s) {
     A2[i] = live ? s.A[(int64_t)c * N + j * S + i] * kLog2e : 0.f;
     h[i] = live && from ? from[j * S + i] : 0.f;
   }
+  int own[S];
+#pragma unroll
+  for (int i = 0; i < S; ++i) own[i] = again(c_local * kChannelRow + jq);
   auto save = [&](int64_t tile, int part) {  // h where a tile of the gradient begins
     const int64_t at = tile * (K / KG) + part;
     if (kMode != kOut || !s.saved || !live || at >= s.grad_tiles) return;
@@ -338,14 +347,16 @@ __global__ __launch_bounds__(256, 4) void scan_walk_kernel(Scan s) {
     if (k + 1 < tile_end) fetch(kMode == kBack ? tile - 1 : tile + 1);
 
     // Four tokens at a time: lane i of a quad holds token i's d and d u, which the others take from it as an operand.
+    // Each state reads them for itself: were they one value, it would be moved to every lane by an instruction of its own.
 #pragma unroll 2
     for (int step = 0; step < K; step += 4) {
       if (step % KG == 0) save(tile, step / KG);
       const int t = kMode == kBack ? K - 4 - step : step;
-      const float d = sd[c_local * kChannelRow + t + jq], v = sv[c_local * kChannelRow + t + jq];
       f32x4 p = zero;
 #pragma unroll
       for (int i = 0; i < S; ++i) {
+        const float d = sd[own[i] + t], v = sv[own[i] + t];
+        if (kMode != kOut && i == 0) total += d;
         const f32x4 m = *(const f32x4*)(sB + (j * S + i) * kRow + t);
         f32x4 r = zero;
         if (kMode == kOut) r = *(const f32x4*)(sC + (j * S + i) * kRow + t);
@@ -361,11 +372,9 @@ __global__ __launch_bounds__(256, 4) void scan_walk_kernel(Scan s) {
           }
         });
       }
-      if (kMode != kOut) {
-        total += d;
-      } else {
+      if (kMode == kOut) {
         const float y = sum4<L>(p, lane);
-        if (L == 4 || j < 4) sy[c_local * kChannelRow + t + jq] = y;
+        if (L == 4 || j < 4) sy[own[0] + t] = y;
       }
     }
     __syncthreads();
@@ -510,12 +519,6 @@ __global__ __launch_bounds__(256) void scan_step_kernel(Scan s) {
 
 // ------------------------------------------------------------------ gradient
 
-// v, as a value that the compiler does not know: what is worked out of it is not kept in registers over the loops around.
-__device__ __forceinline__ int again(int v) {
-  asm volatile("" : "+v"(v));
-  return v;
-}
-
 // A block takes a span of a group's channels and a range of tiles; its waves take slices of 16 channels in turn, each in
 // its own part of LDS, and wait for each other only at a tile's ends.  The range's tiles go from the last to the first, X
 // handed on in LDS.  A lane has one state (of 8 states every second
@@ -552,50 +555,62 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
   const uint32_t size = sizeof(T), u_of = (et * (uint32_t)s.u.st + e) * size, dt_of = (et * (uint32_t)s.dt.st + e) * size;
   const uint32_t z_of = (et * (uint32_t)s.z.st + e) * size, of = et * (uint32_t)s.channels + e;
   const int64_t tile0 = (int64_t)range * s.range_tiles * (K / KG);
-  const int64_t tile1 = min(tile0 + (int64_t)s.range_tiles * (K / KG), s.grad_tiles);
-  for (int64_t tile = tile1 - 1; tile >= tile0; --tile) {
-    const int64_t first = b * s.tokens + tile * KG, map_row = s.whole ? first : (span * s.batch + b) * s.tokens + tile * KG;
-    const int left = (int)min(length - tile * KG, (int64_t)KG), inside = (int)min(s.tokens - tile * KG, (int64_t)KG);
-    if (left <= 0) {  // nothing here depends on anything
-      for (int cc = again(c_first + wave * kSlice + e); et < inside && cc < c_end; cc += 4 * kSlice) {
-        if (s.du) store4((T*)s.du + (first + et) * s.channels + cc, zero);
-        if (s.ddt) store4((T*)s.ddt + (first + et) * s.channels + cc, zero);
-      }
-      for (int i = again(threadIdx.x); i < inside * N; i += 256) {
-        const int64_t at = ((map_row + i / N) * s.groups + group) * N + i % N;
-        if (!s.whole) s.dB[at] = 0.f, s.dC[at] = 0.f;
-        if (s.whole && s.dB_out) ((T*)s.dB_out)[at] = (T)0.f;
-        if (s.whole && s.dC_out) ((T*)s.dC_out)[at] = (T)0.f;
-      }
-      continue;
+  int64_t tile1 = min(tile0 + (int64_t)s.range_tiles * (K / KG), s.grad_tiles);
+  const int64_t map_row = (s.whole ? 0 : (int64_t)span * s.batch + b) * s.tokens + (s.whole ? b * s.tokens : 0);
+  for (; tile1 > tile0 && (tile1 - 1) * KG >= length; --tile1) {  // nothing there depends on anything
+    const int64_t token = (tile1 - 1) * KG, first = b * s.tokens + token;
+    const int inside = (int)min(s.tokens - token, (int64_t)KG);
+    for (int cc = again(c_first + wave * kSlice + e); et < inside && cc < c_end; cc += 4 * kSlice) {
+      if (s.du) store4((T*)s.du + (first + et) * s.channels + cc, zero);
+      if (s.ddt) store4((T*)s.ddt + (first + et) * s.channels + cc, zero);
     }
-    const int64_t row = first * s.channels;
-    const T* u_at = (const T*)s.u.p + b * s.u.sb + tile * KG * s.u.st;
-    const T* dt_at = (const T*)s.dt.p + b * s.dt.sb + tile * KG * s.dt.st;
-    const T* z_at = (const T*)s.z.p + b * s.z.sb + tile * KG * s.z.st;
-    const float* h_at = s.h_in + (b * s.grad_tiles + tile) * s.channels * N;
-    // a slice's elements, and a pass's A and entering h, are asked for a slice and a pass before
-    Four<T> u, x, dy, z;
-    auto ask_slice = [&](int c0) {
-      const bool there = c0 + e < c_end && et < left;
-      u = four(u_at + c0, u_of, there), x = four(dt_at + c0, dt_of, there);
-      dy = four((const T*)s.dout + row + c0, of * size, there), z = four(z_at + c0, z_of, there && s.z.p);
-    };
-    float nA = 0.f, nh = 0.f;
-    auto ask = [&](int c) {
-      const bool live = c < c_end && held;
-      const uint32_t at = (uint32_t)c * N + n;
-      nA = live ? s.A[at] : 0.f, nh = live ? h_at[at] : 0.f;
-    };
-    ask_slice(c_first + wave * kSlice);
-    ask(c_first + wave * kSlice + slot);
+    for (int i = again(threadIdx.x); i < inside * N; i += 256) {
+      const int64_t at = ((map_row + token + i / N) * s.groups + group) * N + i % N;
+      if (!s.whole) s.dB[at] = 0.f, s.dC[at] = 0.f;
+      if (s.whole && s.dB_out) ((T*)s.dB_out)[at] = (T)0.f;
+      if (s.whole && s.dC_out) ((T*)s.dC_out)[at] = (T)0.f;
+    }
+  }
+
+  // a slice's elements, and a pass's A and entering h, are asked for a slice and a pass before, a tile's maps and its
+  // first slice before the tile behind it is summed up
+  Four<T> u, x, dy, z;
+  auto ask_slice = [&](int64_t tile, int c0) {
+    const bool there = c0 + e < c_end && et < length - tile * KG;
+    u = four((const T*)s.u.p + b * s.u.sb + tile * KG * s.u.st + c0, u_of, there);
+    x = four((const T*)s.dt.p + b * s.dt.sb + tile * KG * s.dt.st + c0, dt_of, there);
+    dy = four((const T*)s.dout + (b * s.tokens + tile * KG) * s.channels + c0, of * size, there);
+    z = four((const T*)s.z.p + b * s.z.sb + tile * KG * s.z.st + c0, z_of, there && s.z.p);
+  };
+  float nA = 0.f, nh = 0.f;
+  auto ask = [&](int64_t tile, int c) {
+    const bool live = c < c_end && held;
+    const uint32_t at = (uint32_t)c * N + n;
+    nA = live ? s.A[at] : 0.f, nh = live ? s.h_in[(b * s.grad_tiles + tile) * s.channels * N + at] : 0.f;
+  };
+  constexpr int kMaps = KG * NP / 256;
+  T map_B[kMaps], map_C[kMaps];
+  auto ask_tile = [&](int64_t tile) {
+    for (int i = 0; i < kMaps; ++i) {
+      const int at = again(threadIdx.x) + 256 * i, m = at % NP;
+      const int64_t t = tile * KG + at / NP;
+      const bool there = t < length && m < N;
+      map_B[i] = there ? ((const T*)s.B.p)[b * s.B.sb + t * s.B.st + group * s.B.sg + m] : (T)0.f;
+      map_C[i] = there ? ((const T*)s.C.p)[b * s.C.sb + t * s.C.st + group * s.C.sg + m] : (T)0.f;
+    }
+    ask_slice(tile, c_first + wave * kSlice);
+    ask(tile, c_first + wave * kSlice + slot);
+  };
+  if (tile1 > tile0) ask_tile(tile1 - 1);
+  for (int64_t tile = tile1 - 1; tile >= tile0; --tile) {
+    const int left = (int)min(length - tile * KG, (int64_t)KG), inside = (int)min(s.tokens - tile * KG, (int64_t)KG);
+    const int64_t row = (b * s.tokens + tile * KG) * s.channels;
     __syncthreads();
-    for (int i = again(threadIdx.x); i < KG * NP; i += 256) {
-      const int t = i / NP, m = i % NP;
-      const int64_t at = tile * KG + t;
-      const bool there = t < left && m < N;
-      sB[m * R + t] = there ? load_f((const T*)s.B.p + b * s.B.sb + at * s.B.st + group * s.B.sg + m) : 0.f;
-      sC[m * R + t] = there ? load_f((const T*)s.C.p + b * s.C.sb + at * s.C.st + group * s.C.sg + m) : 0.f;
+#pragma unroll
+    for (int i = 0; i < kMaps; ++i) {
+      const int at = threadIdx.x + 256 * i;
+      sB[at % NP * R + at / NP] = (float)map_B[i];
+      sC[at % NP * R + at / NP] = (float)map_C[i];
     }
     __syncthreads();
     float accB[KG], accC[KG];
@@ -626,14 +641,14 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
           sy[(e + q) * R + et] = y[q];
         }
       }
-      ask_slice(c0 + 4 * kSlice);
+      ask_slice(tile, c0 + 4 * kSlice);
       wave_fence();
       for (int pass = 0; pass < kPasses; ++pass) {
         const int cl = pass * kSlots + slot, c = c0 + cl;
         const bool live = c < c_end && held;
         const float A = nA, A2 = A * kLog2e, h0 = nh;
         float X = live ? aX[(c - c_first) * N + n] : 0.f, dA = 0.f;
-        ask(pass + 1 < kPasses ? c + kSlots : c0 + 4 * kSlice + slot);
+        ask(tile, pass + 1 < kPasses ? c + kSlots : c0 + 4 * kSlice + slot);
         // d as an operand from the lanes of a row in the exponent; in multiply-adds, which take none, from LDS
         const float dl = sd[cl * R + r];
         float h[KG], a[KG], last = h0;
@@ -716,6 +731,7 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
       }
       wave_fence();
     }
+    if (tile > tile0) ask_tile(tile - 1);
     // the slots' and waves' sums of dB, then dC
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
@@ -728,7 +744,7 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
         float v = 0.f;
 #pragma unroll
         for (int k = 0; k < 4 * kSlots; ++k) v += from[k * NP];
-        const int64_t at = ((map_row + i / N) * s.groups + group) * N + i % N;
+        const int64_t at = ((map_row + tile * KG + i / N) * s.groups + group) * N + i % N;
         if (!s.whole)
           (which ? s.dC : s.dB)[at] = v;
         else if (which ? s.dC_out : s.dB_out)
@@ -797,8 +813,8 @@ Chunks plan_chunks(int64_t batch, int64_t tokens, int64_t channels, int64_t stat
   const int64_t tiles = (tokens + K - 1) / K, per = 256 / walk_lanes((int)states);
   const int64_t blocks = batch * groups * ((channels / groups + per - 1) / per);
   if (blocks >= 768 || tiles <= 2) return {1, tiles};
-  int64_t chunks = (1536 + blocks - 1) / blocks;
-  if (chunks > tiles) chunks = tiles;
+  int64_t chunks = (3072 + blocks - 1) / blocks;
+  if (chunks > tiles / 2) chunks = tiles / 2;
   const int64_t each = (tiles + chunks - 1) / chunks;
   return {(tiles + each - 1) / each, each};
 }
@@ -868,12 +884,11 @@ int walk(Scan s, hipStream_t stream) {
     constexpr int N = decltype(n)::value, L = walk_lanes(N);
     s.cblocks = (s.group_channels + 256 / L - 1) / (256 / L);
     s.blocks = s.batch * s.chunks * s.groups * s.cblocks;
-    if (s.blocks >= (1ll << 31) - 8) {
+    if (s.blocks >= (1ll << 31) - 32) {
       rc = set_error(BMX_EINVAL, "selective_scan: too many rows");
       return;
     }
-    s.eighth = (uint32_t)((s.blocks + 7) / 8);
-    scan_walk_kernel<T, N, L, kMode><<<fold_grid((int64_t)s.eighth * 8, 256), 256, 0, stream>>>(s);
+    scan_walk_kernel<T, N, L, kMode><<<fold_grid((s.blocks + 31) / 32 * 32, 256), 256, 0, stream>>>(s);
   });
   return rc ? rc : check_launch("selective_scan");
 }
