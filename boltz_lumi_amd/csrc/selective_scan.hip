@@ -432,6 +432,12 @@ __global__ __launch_bounds__(256, 4) void scan_walk_kernel(Scan s) {
 // given state (or zeros), backward from the gradient of the last one.  A block takes 256 states one chunk after
 // another or, where they are few, 32 by eight runs of chunks: each run's own states and decay first, then from what the
 // runs before it make of `first` (3072 states, 251 chunks: 32 -> 8.5 us; 98304 states, 16 chunks: 5.5 -> 11.5, so not there).
+// A state after a run of tokens that decays by 2^x and adds `own`.  The power is taken in halves: a growing state (A > 0)
+// may be finite behind a run whose own power is not, and one that is zero stays so.
+__device__ __forceinline__ float after_run(float state, float x, float own) {
+  const float half = __builtin_amdgcn_exp2f(0.5f * x);
+  return state == 0.f ? own : state * half * half + own;
+}
 template <bool kReverse, int kRuns>
 __global__ __launch_bounds__(256) void scan_carry_kernel(Scan s, const float* first, float* last) {
   constexpr int kAhead = 8, kColumns = 256 / kRuns;
@@ -459,14 +465,14 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(Scan s, const float* fi
       load(k0);
 #pragma unroll
       for (int i = 0; i < kAhead; ++i) {
-        mine = __builtin_amdgcn_exp2f(A2 * d[i]) * mine + own[i];
+        mine = after_run(mine, A2 * d[i], own[i]);
         total += d[i];
       }
     }
-    decay[run][col] = __builtin_amdgcn_exp2f(A2 * total);
+    decay[run][col] = A2 * total;
     state[run][col] = mine;
     __syncthreads();
-    for (int i = 0; i < run; ++i) carry = decay[i][col] * carry + state[i][col];
+    for (int i = 0; i < run; ++i) carry = after_run(carry, decay[i][col], state[i][col]);
   }
   for (int64_t k0 = k_first; k0 < k_last; k0 += kAhead) {
     if (kRuns == 1 || each > kAhead) load(k0);  // else they are still there
@@ -474,7 +480,7 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(Scan s, const float* fi
     for (int i = 0; i < kAhead; ++i) {
       if (k0 + i >= k_last) break;
       s.carry[at(k0 + i) * per + cn] = carry;
-      carry = __builtin_amdgcn_exp2f(A2 * d[i]) * carry + own[i];
+      carry = after_run(carry, A2 * d[i], own[i]);
     }
   }
   if (last && run == kRuns - 1) last[item] = carry;

@@ -1789,7 +1789,7 @@ def causal_conv(x, weight, bias=None, state=None, lengths=None, silu=True, retur
     state = _dense(state)
     plan = _conv_plan(_layout(x), _layout(weight), _layout(bias), _layout(state), _layout(lengths), int(bool(silu)))
     if state_out is not None:
-        _check_state_out(state_out, plan, x.dtype, state, (x, weight, bias, lengths), grad)
+        _check_state_out(state_out, plan, x.dtype, state, (x, weight, bias, lengths), grad or _needs_grad(state_out))
     args = plan, dev, x, weight, bias, state, lengths, want, state_out
     y, last = (_CausalConv.apply if grad else _causal_conv_fwd)(*args)
     _written(state_out)
@@ -1918,7 +1918,8 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, len
                           for ok, t in zip(plan.ok, moved))
         plan = plan_of(u, dt, B, C, z)
     if state_out is not None:
-        _check_state_out(state_out, plan, torch.float32, state, (u, dt, A, B, C, D, z, dt_bias, lengths), grad)
+        _check_state_out(state_out, plan, torch.float32, state, (u, dt, A, B, C, D, z, dt_bias, lengths),
+                         grad or _needs_grad(state_out))
     args = plan, dev, u, dt, A, B, C, D, z, dt_bias, state, lengths, want
     out, last = _SelectiveScan.apply(*args) if grad else _selective_scan_fwd(*args, state_out)[:2]
     _written(state_out)

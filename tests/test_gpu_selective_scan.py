@@ -267,3 +267,41 @@ def test_differences(gpu):
         want = (ends[0] - ends[1]) / (2 * h)
         scale = (grad.double() * step).abs().sum() + 10
         assert abs((grad.double() * step).sum() - want) <= 2e-3 * scale, i
+
+
+def test_growing_states(gpu):
+    """Decays above one: a state that is zero stays so, and a small one is finite where the power of a whole chunk is not."""
+    b, t, c, n = 1, 400, 8, 8
+    zeros = torch.zeros(b, t, c, device=gpu)
+    dt, A = torch.full((b, t, c), 1.0, device=gpu), torch.full((c, n), 0.5, device=gpu)  # exp(200) over the call
+    maps = torch.ones(b, t, 1, n, device=gpu)
+    out, last = ops.selective_scan(zeros, dt, A, maps, maps, softplus=False, return_state=True)
+    assert not out.any() and not last.any()
+    first = torch.full((b, c, n), 1e-37, device=gpu)
+    out, last = ops.selective_scan(zeros[:, :340], dt[:, :340], A, maps[:, :340], maps[:, :340], state=first, softplus=False,
+                                   return_state=True)
+    want = 1e-37 * torch.exp(torch.tensor(170.0, dtype=torch.float64))  # 6.6e36
+    # 340 decays of 2 roundings and 2 of their exponent, as many products
+    assert (last.double().cpu() - want).abs().max() <= 5 * 340 * 2.0 ** -24 * want
+    leaves = [zeros.clone().requires_grad_(), first.clone().requires_grad_()]
+    out = ops.selective_scan(leaves[0], dt, A, maps, maps, state=leaves[1], softplus=False)
+    du, ds = torch.autograd.grad(out, leaves, torch.zeros_like(out))
+    assert not du.any() and not ds.any()
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+def test_state_in_place(gpu, mode):
+    """A decoder's state, made inside or outside the mode, moves on in place; writing over a leaf is refused."""
+    inputs, _ = make(2, 3, 16, 8, 1, FP32)
+    outside = [x.to(gpu) for x in inputs]
+    with mode():
+        inside = [x.to(gpu) for x in inputs]
+        for v in (outside, inside):
+            want = call(v, return_state=True)[1].clone()
+            call(v, state_out=v[8])
+            assert torch.equal(v[8], want)
+    fresh = outside[8].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="return_state"):
+        call([*outside[:8], None], state_out=fresh)
+    with pytest.raises(RuntimeError, match="return_state"):
+        call([x.requires_grad_() if i == 0 else x for i, x in enumerate(outside)], state_out=outside[8].clone())
