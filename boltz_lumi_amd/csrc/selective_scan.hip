@@ -196,6 +196,14 @@ __device__ __forceinline__ int again(int v) {
   return v;
 }
 
+// The same for a value that all lanes share, in a scalar register: an address of it and a lane's constant offset takes
+// no vector registers of its own.
+__device__ __forceinline__ int uniform(int v) {
+  v = __builtin_amdgcn_readfirstlane(v);
+  asm volatile("" : "+s"(v));
+  return v;
+}
+
 // ------------------------------------------------------------ walking chunks
 
 // kLocal: from zero states to each chunk's own, forward; kOut: the outputs; kBack: the same as kLocal for X, from the
@@ -536,8 +544,9 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
   constexpr int kPart = kSlice * R, kStage = 4 * 4 * kPart, kJoin = 256 * KG;
   __shared__ __align__(16) float lds[kStage > kJoin ? kStage : kJoin];
   __shared__ __align__(16) float sB[NP * R], sC[NP * R];
-  extern __shared__ __align__(16) float span_sums[];  // X [span][N], dA [span][N], dD [span], dbias [span]
-  float *aX = span_sums, *aA = aX + s.span * N, *aD = aA + s.span * N, *ab = aD + s.span;
+  extern __shared__ __align__(16) float span_sums[];  // X [span][N], dA [span][N], dD, dbias, D and the bias [span]
+  float *aX = span_sums, *aA = aX + s.span * N, *aD = aA + s.span * N, *ab = aD + s.span, *skips = ab + s.span;
+  float* biases = skips + s.span;
   uint32_t block = block_index();
   if (block >= s.blocks) return;
   const int span = (int)(block % (uint32_t)s.spans);
@@ -548,13 +557,18 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
   const int64_t b = block / (uint32_t)s.ranges, length = length_of(s, b);
   const int c_first = group * s.group_channels + span * s.span;
   const int c_end = min(c_first + s.span, (group + 1) * s.group_channels);
-  const int lane = lane_id(), wave = threadIdx.x >> 6, n = lane % NP, slot = lane / NP, r = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // uniform, as what is worked out of it
+  const int lane = lane_id(), n = lane % NP, slot = lane / NP, r = lane & 15;
   const bool held = n < N;
   // d, d u, dy and the sums G B of a slice; the sums A X h take the place of the d u that they have used
   float *sd = lds + wave * 4 * kPart, *sv = sd + kPart, *sy = sv + kPart, *s1 = sy + kPart, *s2 = sv;
   const float* x_at = s.x_in + ((b * s.ranges + range) * s.channels + c_first) * N;
   for (int i = threadIdx.x; i < s.span * N; i += 256) aX[i] = i < (c_end - c_first) * N ? x_at[i] : 0.f;
   for (int i = threadIdx.x; i < s.span * (N + 2); i += 256) aA[i] = 0.f;
+  for (int i = threadIdx.x; i < s.span; i += 256) {
+    skips[i] = s.D && c_first + i < c_end ? s.D[c_first + i] : 0.f;
+    biases[i] = s.dt_bias && c_first + i < c_end ? s.dt_bias[c_first + i] : 0.f;
+  }
 
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
   const int e = lane % (kSlice / 4) * 4, et = lane / (kSlice / 4);  // a lane's element of a slice
@@ -581,7 +595,9 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
   // a slice's elements, and a pass's A and entering h, are asked for a slice and a pass before, a tile's maps and its
   // first slice before the tile behind it is summed up
   Four<T> u, x, dy, z;
-  auto ask_slice = [&](int64_t tile, int c0) {
+  auto ask_slice = [&](int64_t tile_of, int c_of) {
+    const int64_t tile = uniform((int)tile_of);
+    const int c0 = uniform(c_of);
     const bool there = c0 + e < c_end && et < length - tile * KG;
     u = four((const T*)s.u.p + b * s.u.sb + tile * KG * s.u.st + c0, u_of, there);
     x = four((const T*)s.dt.p + b * s.dt.sb + tile * KG * s.dt.st + c0, dt_of, there);
@@ -589,23 +605,32 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
     z = four((const T*)s.z.p + b * s.z.sb + tile * KG * s.z.st + c0, z_of, there && s.z.p);
   };
   float nA = 0.f, nh = 0.f;
-  auto ask = [&](int64_t tile, int c) {
-    const bool live = c < c_end && held;
-    const uint32_t at = (uint32_t)c * N + n;
-    nA = live ? s.A[at] : 0.f, nh = live ? s.h_in[(b * s.grad_tiles + tile) * s.channels * N + at] : 0.f;
+  const uint32_t state_of = slot * N + n;
+  auto ask = [&](int64_t tile_of, int c_of) {  // of the channels from c_of on, a slot each
+    const int64_t tile = uniform((int)tile_of);
+    const int c0 = uniform(c_of);
+    const bool live = c0 + slot < c_end && held;
+    const float* A = s.A + (int64_t)c0 * N;
+    const float* h = s.h_in + ((b * s.grad_tiles + tile) * s.channels + c0) * N;
+    nA = nh = 0.f;
+    if (live) nA = A[state_of], nh = h[state_of];
   };
   constexpr int kMaps = KG * NP / 256;
   T map_B[kMaps], map_C[kMaps];
-  auto ask_tile = [&](int64_t tile) {
+  const uint32_t map_m = threadIdx.x % NP, map_t = threadIdx.x / NP;
+  auto ask_tile = [&](int64_t tile_of) {
+    const int64_t tile = uniform((int)tile_of);
+    const T* B = (const T*)s.B.p + b * s.B.sb + tile * KG * s.B.st + group * s.B.sg;
+    const T* C = (const T*)s.C.p + b * s.C.sb + tile * KG * s.C.st + group * s.C.sg;
+#pragma unroll
     for (int i = 0; i < kMaps; ++i) {
-      const int at = again(threadIdx.x) + 256 * i, m = at % NP;
-      const int64_t t = tile * KG + at / NP;
-      const bool there = t < length && m < N;
-      map_B[i] = there ? ((const T*)s.B.p)[b * s.B.sb + t * s.B.st + group * s.B.sg + m] : (T)0.f;
-      map_C[i] = there ? ((const T*)s.C.p)[b * s.C.sb + t * s.C.st + group * s.C.sg + m] : (T)0.f;
+      const uint32_t t = map_t + i * (256 / NP);
+      const bool there = t < length - tile * KG && map_m < N;
+      map_B[i] = map_C[i] = (T)0.f;
+      if (there) map_B[i] = B[t * (uint32_t)s.B.st + map_m], map_C[i] = C[t * (uint32_t)s.C.st + map_m];
     }
     ask_slice(tile, c_first + wave * kSlice);
-    ask(tile, c_first + wave * kSlice + slot);
+    ask(tile, c_first + wave * kSlice);
   };
   if (tile1 > tile0) ask_tile(tile1 - 1);
   for (int64_t tile = tile1 - 1; tile >= tile0; --tile) {
@@ -614,18 +639,18 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kMaps; ++i) {
-      const int at = threadIdx.x + 256 * i;
-      sB[at % NP * R + at / NP] = (float)map_B[i];
-      sC[at % NP * R + at / NP] = (float)map_C[i];
+      const int at = map_m * R + map_t + i * (256 / NP);
+      sB[at] = (float)map_B[i];
+      sC[at] = (float)map_C[i];
     }
     __syncthreads();
     float accB[KG], accC[KG];
 #pragma unroll
     for (int t = 0; t < KG; ++t) accB[t] = accC[t] = 0.f;
-    for (int c0 = c_first + wave * kSlice; c0 < c_end; c0 += 4 * kSlice) {
+    for (int c_of = c_first + wave * kSlice; c_of < c_end; c_of += 4 * kSlice) {
+      const int c0 = uniform(c_of);
       const bool mine = c0 + e < c_end, there = mine && et < left;
-      f32x4 bias = zero;
-      if (mine && s.dt_bias) bias = load4(s.dt_bias + c0 + e);
+      const f32x4 bias = *(const f32x4*)(biases + c0 - c_first + e);
       const Four<T> u_kept = u, x_kept = x;
       {
         // a token that is not there has u, dy and z zero, and takes no step
@@ -647,14 +672,18 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
           sy[(e + q) * R + et] = y[q];
         }
       }
-      ask_slice(tile, c0 + 4 * kSlice);
       wave_fence();
       for (int pass = 0; pass < kPasses; ++pass) {
         const int cl = pass * kSlots + slot, c = c0 + cl;
         const bool live = c < c_end && held;
-        const float A = nA, A2 = A * kLog2e, h0 = nh;
+        float A = nA, h0 = nh;
+        asm volatile("" : "+v"(A), "+v"(h0));
+        const float A2 = A * kLog2e;
         float X = live ? aX[(c - c_first) * N + n] : 0.f, dA = 0.f;
-        ask(tile, pass + 1 < kPasses ? c + kSlots : c0 + 4 * kSlice + slot);
+        // behind the use of what was asked for before: loads come back in their order, and a pass waits for all of them
+        __builtin_amdgcn_sched_barrier(0);
+        if (pass == 0) ask_slice(tile, c0 + 4 * kSlice);
+        ask(tile, pass + 1 < kPasses ? c0 + (pass + 1) * kSlots : c0 + 4 * kSlice);
         // d as an operand from the lanes of a row in the exponent; in multiply-adds, which take none, from LDS
         const float dl = sd[cl * R + r];
         float h[KG], a[KG], last = h0;
@@ -702,8 +731,8 @@ __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
       }
       wave_fence();
       {
-        f32x4 skip = zero, du, ddt;
-        if (mine && s.D) skip = load4(s.D + c0 + e);
+        const f32x4 skip = *(const f32x4*)(skips + c0 - c_first + e);
+        f32x4 du, ddt;
         const f32x4 uw = u_kept.wide(), xw = x_kept.wide() + bias;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
@@ -933,7 +962,7 @@ int gradient(Scan& s, const float* dstate_out, float* dstate, hipStream_t stream
   if (int rc = carry<true>(s, dstate_out, dstate, stream)) return rc;
   with_states(s.states, [&](auto n) {
     constexpr int N = decltype(n)::value;
-    scan_bwd_kernel<T, N><<<fold_grid(s.blocks, 256), 256, s.span * (2 * N + 2) * sizeof(float), stream>>>(s);
+    scan_bwd_kernel<T, N><<<fold_grid(s.blocks, 256), 256, s.span * (2 * N + 4) * sizeof(float), stream>>>(s);
   });
   return check_launch("selective_scan_bwd");
 }
