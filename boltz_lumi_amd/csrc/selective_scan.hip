@@ -278,26 +278,24 @@ __global__ __launch_bounds__(256, 4) void scan_walk_kernel(Scan s) {
   f32x4 bias = zero, skip = zero;
   if (mine && s.dt_bias) bias = load4(s.dt_bias + cc);
   if (kMode == kOut && mine && s.D) skip = load4(s.D + cc);
-  float A2[S], h[S], total = 0.f;
+  typedef float States __attribute__((ext_vector_type(S)));
   const float* from = nullptr;
   if (kMode == kOut)
     from = s.chunks > 1 ? s.carry + ((b * s.chunks + chunk) * s.channels + c) * N
            : s.state    ? s.state + (b * s.channels + c) * N
                         : nullptr;
-#pragma unroll
-  for (int i = 0; i < S; ++i) {
-    A2[i] = live ? s.A[(int64_t)c * N + j * S + i] * kLog2e : 0.f;
-    h[i] = live && from ? from[j * S + i] : 0.f;
-  }
+  States A = {}, h = {};
+  if (live) A = *(const States*)(s.A + (int64_t)c * N + j * S);
+  if (live && from) h = *(const States*)(from + j * S);
+  const States A2 = A * kLog2e;
+  float total = 0.f;
   int own[S];
 #pragma unroll
   for (int i = 0; i < S; ++i) own[i] = again(c_local * kChannelRow + jq);
   auto save = [&](int64_t tile, int part) {  // h where a tile of the gradient begins
     const int64_t at = tile * (K / KG) + part;
     if (kMode != kOut || !s.saved || !live || at >= s.grad_tiles) return;
-    float* to = s.saved + ((b * s.grad_tiles + at) * s.channels + c) * N + j * S;
-#pragma unroll
-    for (int i = 0; i < S; ++i) to[i] = h[i];
+    *(States*)(s.saved + ((b * s.grad_tiles + at) * s.channels + c) * N + j * S) = h;
   };
 
   for (int64_t k = tile0; k < tile_end; ++k) {
@@ -421,18 +419,15 @@ __global__ __launch_bounds__(256, 4) void scan_walk_kernel(Scan s) {
     }
   }
   if (kMode == kOut) {
-    if (live && s.state_out && chunk == s.chunks - 1) {
-#pragma unroll
-      for (int i = 0; i < S; ++i) s.state_out[(b * s.channels + c) * N + j * S + i] = h[i];
-    }
+    if (live && s.state_out && chunk == s.chunks - 1)
+      *(States*)(s.state_out + (b * s.channels + c) * N + j * S) = h;
     return;
   }
   total += from_lane<0xB1>(total);
   total += from_lane<0x4E>(total);
   if (!live) return;
   const int64_t at = (b * s.chunks + chunk) * s.channels + c;
-#pragma unroll
-  for (int i = 0; i < S; ++i) s.carry[at * N + j * S + i] = h[i];
+  *(States*)(s.carry + at * N + j * S) = h;
   if (j == 0) s.steps[at] = total;
 }
 
