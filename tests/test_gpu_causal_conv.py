@@ -108,7 +108,7 @@ def test_parts_of_a_sequence(gpu, parts):
 
 
 def test_long_rows_and_many_runs(gpu):
-    """Runs of 16 tokens a thread (from 2^18 of them on), whose outputs are those of short calls, bit for bit."""
+    """Runs of 8 tokens a thread (from 2^18 runs of channels on), whose outputs are those of short calls, bit for bit."""
     (x, w, b, first), _ = make(2, 8200, 128, 4, BF16)
     x, w, b, first = (t.to(gpu) for t in (x, w, b, first))
     lengths = torch.tensor([8200, 4097], device=gpu)
