@@ -22,7 +22,9 @@ using namespace bmx;
 namespace {
 
 constexpr int kMaxDim = 8192;
-constexpr int kBwdThreads = 512 * 256;  // of the gradient at most: two waves a SIMD; a block leaves a partial row per weight
+// Threads of the gradient at most: two waves a SIMD.  A block leaves a partial row per weight, so not twice as many (2^24
+// values of 4096 a row, both ways: 114 us, 119); with half of them 157.
+constexpr int kBwdThreads = 512 * 256;
 
 struct Rows {
   const void* p;
@@ -366,14 +368,17 @@ __global__ __launch_bounds__(256) void residual_norm_sums_kernel(ColumnSums s) {
   }
 }
 
-// A row's threads and runs of 8 channels each.  The gradient has one run a thread where it can: with two its registers
-// leave one wave a SIMD.
+// A row's threads and runs of 8 channels each: as few threads as hold it with one run each (a wave for 128 channels
+// instead of 16 lanes: 79 us for 36 at 131072 rows), as a row of several waves meets at a barrier a sum, but two runs
+// cost as much (64 rows of 1024: 128 threads 3.4 us, 64 with two runs 4.2) and in the gradient, where they leave one
+// wave a SIMD, more (2^24 values, both ways: 1024 106 and 125 us, 4096 114 and 143).  Forward, rows past 2048 lose
+// more to idle threads (8160 rows of 2056: 512 threads 50 us, 256 with two runs 42; of 4096: 38 and 37).
 template <bool kBackward, typename Go>
 void with_layout(int dim, Go go) {
   using std::integral_constant;
   if (dim <= 128) return go(integral_constant<int, 16>(), integral_constant<int, 1>());
   if (dim <= 512) return go(integral_constant<int, 64>(), integral_constant<int, 1>());
-  if (dim <= 1024) return go(integral_constant<int, kBackward ? 128 : 64>(), integral_constant<int, kBackward ? 1 : 2>());
+  if (dim <= 1024) return go(integral_constant<int, 128>(), integral_constant<int, 1>());
   if (dim <= 2048) return go(integral_constant<int, 256>(), integral_constant<int, 1>());
   if (dim <= 4096) return go(integral_constant<int, kBackward ? 512 : 256>(), integral_constant<int, kBackward ? 1 : 2>());
   return go(integral_constant<int, 512>(), integral_constant<int, 2>());

@@ -836,15 +836,23 @@ void with_states(int64_t states, Go go) {
 
 // Lanes of a channel where chunks are walked: four states each (of eight states two).
 constexpr int walk_lanes(int states) { return states <= 16 ? 4 : states / 4; }
+// Chunks of a forward call.  One where its blocks keep the card busy (a round of them takes as long with 288 as with 480;
+// us at 1536 channels of 16 states, 512 tokens, one chunk against several: 384 blocks 96 and 104, 480 97 and 139, 288 97
+// and 87) or where there is little to walk (96 tokens: 17 and 19; 128: 21 and 20).  Else about three rounds of the four
+// blocks that a compute unit holds: 2 x 4096 tokens take 111 with 3072 or 4096 blocks, 118 with 2048, 115 to 122 with
+// 1024.  Two tiles a chunk at least, as the carry is read and written per chunk (2 x 4096: 102, with one 107; 16001 x 384
+// of 8 states: 47 and 55), but one where all tiles are a round's blocks (1 x 512 x 768: 23 with two, 16 with one;
+// 1 x 2048: 31 and 27; at 1536 blocks equal).
 struct Chunks {
   int64_t chunks, tiles;  // tiles of a chunk
 };
 Chunks plan_chunks(int64_t batch, int64_t tokens, int64_t channels, int64_t states, int64_t groups) {
   const int64_t tiles = (tokens + K - 1) / K, per = 256 / walk_lanes((int)states);
   const int64_t blocks = batch * groups * ((channels / groups + per - 1) / per);
-  if (blocks >= 768 || tiles <= 2) return {1, tiles};
+  if (blocks >= 384 || tiles <= 3) return {1, tiles};
+  const int64_t most = blocks * tiles <= 1024 ? tiles : tiles / 2;
   int64_t chunks = (3072 + blocks - 1) / blocks;
-  if (chunks > tiles / 2) chunks = tiles / 2;
+  if (chunks > most) chunks = most;
   const int64_t each = (tiles + chunks - 1) / chunks;
   return {(tiles + each - 1) / each, each};
 }
