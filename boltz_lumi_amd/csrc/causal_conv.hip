@@ -12,6 +12,11 @@
 // A thread takes 16 bytes of channels (8 bf16, 4 fp32) of a run of kRun tokens
 // with all its rows in flight at once; the W - 1 rows before (backward: and
 // behind) a run come from the neighbours' cache lines.  Sums are fp32.
+//
+// Bound by HBM forward (16001 x 768 in fp32: 17 us, 5.7 TB/s, part of it cached;
+// 4 x 2048 x 1536 in bf16, ragged: 15 us) and by the loads that the gradient's
+// registers let be in flight backward (the same: 32 us, 25 rows asked for per 16
+// that are needed, and 4 for the partial rows).  32 single tokens: 4 us.
 #include <type_traits>
 #include <utility>
 
@@ -21,7 +26,7 @@ using namespace bmx;
 
 namespace {
 
-constexpr int kRun = 8;       // tokens of a thread
+constexpr int kRun = 8;       // tokens of a thread (4 x 2048 x 1536: 15 us; with 16 23, with 4 15.5)
 constexpr int kBwdVec = 4, kBwdRun = 8;
 constexpr int kBwdVecs = 32;  // a gradient's block: 32 runs of channels by 8 runs of tokens
 
@@ -278,18 +283,17 @@ int with_width(int64_t width, Go go) {
 template <typename T>
 int forward(Conv& s, int64_t width, hipStream_t stream) {
   s.vecs = s.channels / kVec<T>;
-  // Few rows go in short runs, for the latency of one.  A run of several tokens covers the W - 1 that read the state,
-  // so that one thread reads it and may write the next one over it.
-  const bool few = s.batch * s.tokens * s.vecs < 256 * 1024;
-  const int run = s.tokens == 1 ? 1 : few ? 4 : kRun;
+  // Few rows go in short runs, for the latency of one (1 x 1024 x 1536: 5.0 us, with kRun 6.5; 1 x 2048: 6.6 and 7.3;
+  // 4 x 2048: 15.5 and 14.8).  Either covers the W - 1 tokens that read the state, so that one thread reads it and may
+  // write the next one over it.
+  const bool few = s.tokens <= 4 || s.batch * s.tokens * s.vecs < 512 * 1024;
+  const int run = few ? 4 : kRun;
   s.runs = (int)((s.tokens + run - 1) / run);
   const int64_t blocks = (s.batch * s.runs * s.vecs + 255) / 256;
   BMX_REQUIRE(blocks < (1ll << 31), "causal_conv: too many rows");
   return with_width(width, [&](auto w) {
     constexpr int W = decltype(w)::value;
-    if (run == 1)
-      causal_conv_kernel<T, W, kVec<T>, 1><<<fold_grid(blocks, 256), 256, 0, stream>>>(s);
-    else if (run == 4)
+    if (few)
       causal_conv_kernel<T, W, kVec<T>, 4><<<fold_grid(blocks, 256), 256, 0, stream>>>(s);
     else
       causal_conv_kernel<T, W, kVec<T>, kRun><<<fold_grid(blocks, 256), 256, 0, stream>>>(s);

@@ -15,6 +15,14 @@
 // X that comes to it and, tile by tile, the h that the forward pass kept, and is
 // worked out on its own.  States, sums and statistics are fp32; tokens from a
 // sequence's length on take no step (d = 0), are never read and give zeros.
+//
+// What bounds it is vector instructions, an exp (2.2 slots of the 38.5e12 lanes
+// a second) per state and token and four around it in a walk, 20 in the
+// gradient, so that a second walk costs more than its bytes.  bf16, four ragged
+// sequences of up to 2048 tokens, 1536 channels of 16 states, us (its
+// instructions alone): kLocal 41 (30), kOut 60 (41), kBack 48 (34), gradient 155
+// to 162 (106), both carries 15, sums 7; 45 would be the bytes of all.  A walk
+// that has no chunks to spread (16 lanes a channel instead of four) takes 166.
 #include <type_traits>
 #include <utility>
 
@@ -30,7 +38,9 @@ constexpr int KG = 16;            // tokens of a tile of the gradient, which kee
 constexpr int kGradRow = KG + 4;
 constexpr int kChannelRow = K + 2;  // LDS row of a channel: reads without conflicts, transposing writes two on a bank
 constexpr int kSlice = 16;        // channels that a wave of the gradient stages at a time
-constexpr int kMaxSpan = 2048;    // channels x states of a gradient block (X and dA in LDS), but at least 64 channels
+// Channels x states of a gradient block (X and dA in LDS), but at least 64 channels.  4 x 2048 tokens, 1536 channels of 16
+// states, both ways: 324 us; with 4096 368 (one block less a compute unit), with 1024 347 (more partial sums dB, dC).
+constexpr int kMaxSpan = 2048;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Operand {
@@ -47,8 +57,8 @@ struct Scan {
   float* saved;             // [batch][grad_tiles][channels][states]: h where every tile of the gradient begins
   const float *h_in, *x_in;
   void *du, *ddt, *dz;
-  float *dB, *dC;           // [spans][batch][tokens][groups][states], or the results where there is one span
-  void *dB_out, *dC_out;
+  float *dB, *dC;           // partial sums, [spans][batch][tokens][groups][states]; unused where there is one span
+  void *dB_out, *dC_out;    // the results
   float *dA, *dD, *dbias;   // partial sums, [batch * ranges][channels]([states])
   int64_t batch, tokens, tiles, grad_tiles, chunks, chunk_tiles, blocks;
   int channels, groups, group_channels, states, cblocks, lengths64, softplus;
@@ -489,7 +499,7 @@ __global__ __launch_bounds__(256) void scan_carry_kernel(Scan s, const float* fi
   if (last && run == kRuns - 1) last[item] = carry;
 }
 
-// One token: four states a thread.
+// One token: four states a thread (64 x 1536 channels of 16 states: 5.1 us; a walk would take 17.6).
 template <typename T, int N>
 __global__ __launch_bounds__(256) void scan_step_kernel(Scan s) {
   constexpr int L = N / 4;
@@ -530,9 +540,10 @@ __global__ __launch_bounds__(256) void scan_step_kernel(Scan s) {
 
 // A block takes a span of a group's channels and a range of tiles; its waves take slices of 16 channels in turn, each in
 // its own part of LDS, and wait for each other only at a tile's ends.  The range's tiles go from the last to the first, X
-// handed on in LDS.  A lane has one state (of 8 states every second
-// lane none) and, pass by pass, channel after channel: the sums dB, dC of its state stay in its registers over a tile, h
-// and a of a channel over its 32 tokens.  dA, dD and the bias's sums stay in LDS over the range.
+// handed on in LDS.  A lane has one state (of 8 states every second lane none) and, pass by pass, channel after channel:
+// the sums dB, dC of its state stay in its registers over a tile, h and a of a channel over its 16 tokens.  dA, dD and the
+// bias's sums stay in LDS over the range.  Three waves a SIMD: 159 us at 4 x 2048 x 1536 x 16; two, without spills, 189,
+// four, with the sums spilled, 263.
 template <typename T, int N>
 __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
   constexpr int NP = N < 16 ? 16 : N, kSlots = 64 / NP, kPasses = kSlice / kSlots, R = kGradRow;
@@ -860,8 +871,10 @@ Chunks plan_chunks(int64_t batch, int64_t tokens, int64_t channels, int64_t stat
 struct Spans {
   int64_t span, spans, ranges, range_tiles, whole;
 };
-// Spans of a group's channels and ranges of tiles of the gradient's blocks: two tiles (of 32) where that leaves enough
-// blocks, four rounds of the three that a compute unit holds; one halves what a wave waits for in the small calls.
+// Spans of a group's channels and ranges of tiles of the gradient's blocks: two tiles (of 32) a range where that leaves
+// four rounds of blocks at least, for half the states to carry (4 x 2048 x 1536 x 16, 1536 blocks a tile column: kernel
+// 160 us and carry 7.7 with two, 154 and 12.8 with one, both ways 325 with two and 338 with four); one where there are
+// fewer, as a wave then waits for every tile.
 Spans plan_spans(int64_t batch, int64_t tokens, int64_t channels, int64_t states, int64_t groups) {
   const int64_t tiles = (tokens + K - 1) / K, group = channels / groups, unit = 4 * kSlice;
   const int64_t most = kMaxSpan / states < unit ? unit : kMaxSpan / states / unit * unit;

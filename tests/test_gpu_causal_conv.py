@@ -108,15 +108,15 @@ def test_parts_of_a_sequence(gpu, parts):
 
 
 def test_long_rows_and_many_runs(gpu):
-    """Runs of 8 tokens a thread (from 2^18 runs of channels on), whose outputs are those of short calls, bit for bit."""
-    (x, w, b, first), _ = make(2, 8200, 128, 4, BF16)
+    """Runs of 8 tokens a thread (from 2^19 runs of channels on), whose outputs are those of short calls, bit for bit."""
+    (x, w, b, first), _ = make(2, 16400, 128, 4, BF16)
     x, w, b, first = (t.to(gpu) for t in (x, w, b, first))
-    lengths = torch.tensor([8200, 4097], device=gpu)
+    lengths = torch.tensor([16400, 4097], device=gpu)
     whole, last = ops.causal_conv(x, w, b, state=first, lengths=lengths, return_state=True)
-    for at in (0, 15, 16, 4090, 8190):
+    for at in (0, 7, 8, 4090, 16390):
         before = first if at == 0 else torch.cat([first, x], 1)[:, at:at + 3].contiguous()
         part = ops.causal_conv(x[:, at:at + 10], w, b, state=before)
-        keep = (torch.arange(at, min(at + 10, 8200), device=gpu) < lengths[:, None])[..., None]
+        keep = (torch.arange(at, at + 10, device=gpu) < lengths[:, None])[..., None]
         assert torch.equal(torch.where(keep, part, torch.zeros_like(part)), whole[:, at:at + 10])
     assert torch.equal(last, torch.stack([x[0, -3:], x[1, 4094:4097]]))
 
