@@ -924,7 +924,8 @@ int check_inputs(const Scan& s, int dtype) {
   BMX_REQUIRE(s.u.p && s.dt.p && s.A && s.B.p && s.C.p, "selective_scan: null pointer");
   BMX_REQUIRE(aligned(dtype == kF32 ? 16 : 8, {s.u.p, s.dt.p, s.z.p, s.B.p, s.C.p}),
               "selective_scan: tensors must be aligned to four elements");
-  BMX_REQUIRE(aligned(16, {s.A, s.state, s.state_out, s.raw, s.saved}), "selective_scan: fp32 tensors must be 16-byte aligned");
+  BMX_REQUIRE(aligned(16, {s.A, s.D, s.dt_bias, s.state, s.state_out, s.raw, s.saved}),
+              "selective_scan: fp32 tensors must be 16-byte aligned");
   return BMX_OK;
 }
 
@@ -1061,7 +1062,8 @@ extern "C" int bmx_selective_scan_bwd(const void* u, const void* dt, const float
   if (int rc = check_inputs(s, dtype)) return rc;
   BMX_REQUIRE(saved && dout && (!z || raw), "selective_scan_bwd: null pointer");
   BMX_REQUIRE((D || !dD) && (z || !dz) && (dt_bias || !ddt_bias), "selective_scan_bwd: gradient of an absent operand");
-  BMX_REQUIRE(aligned(16, {saved, raw, dout, du, ddt, dz, dA, dB, dC, dD, ddt_bias}), "selective_scan: tensors must be 16-byte aligned");
+  BMX_REQUIRE(aligned(16, {saved, raw, dout, du, ddt, dz, dA, dB, dC, dD, ddt_bias}),
+              "selective_scan: tensors must be 16-byte aligned");
   const Spans p = plan_spans(s.batch, s.tokens, s.channels, s.states, s.groups);
   const BackSpace space(s.batch, s.tokens, s.channels, s.states, s.groups, p);
   BMX_REQUIRE(workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= (size_t)space.floats() * sizeof(float),

@@ -164,7 +164,7 @@ def test_parts_of_a_sequence(gpu, parts):
     assert_close("state", kept, results[1], sizes[1], 96 + 8 * at)
 
 
-@pytest.mark.parametrize("c,t,b", [(8, 4099, 1), (8, 300, 5), (512, 1100, 2)])
+@pytest.mark.parametrize("c,t,b", [(8, 4099, 1), (8, 300, 5), (512, 1100, 2), (512, 4200, 2)])
 def test_chunks(gpu, c, t, b):
     """Few channels and many tokens: chunks side by side, with decays slow enough that states cross several.  Against the
     same call in parts that are one chunk each."""

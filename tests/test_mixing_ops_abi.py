@@ -123,6 +123,7 @@ def test_selective_scan_rejects_bad_arguments(lib):
     assert refused(lib, bwd(bias=None), b"absent") and refused(lib, bwd(saved=None), b"null pointer")
     assert refused(lib, bwd(raw=None), b"null pointer") and refused(lib, bwd(du=ODD), b"aligned")
     assert refused(lib, bwd(rows=0), b"rows")
+    assert refused(lib, bwd(D=ODD), b"aligned") and refused(lib, bwd(bias=ODD), b"aligned")
 
 
 def layouts(*tensors):
