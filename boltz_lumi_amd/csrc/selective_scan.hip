@@ -16,13 +16,13 @@
 // worked out on its own.  States, sums and statistics are fp32; tokens from a
 // sequence's length on take no step (d = 0), are never read and give zeros.
 //
-// What bounds it is vector instructions, an exp (2.2 slots of the 38.5e12 lanes
-// a second) per state and token and four around it in a walk, 20 in the
+// What bounds it is vector instructions, an exp (2.6 slots of the 38.5e12 lanes
+// a second) per state and token and four around it in a walk, 16 to 20 in the
 // gradient, so that a second walk costs more than its bytes.  bf16, four ragged
 // sequences of up to 2048 tokens, 1536 channels of 16 states, us (its
-// instructions alone): kLocal 41 (30), kOut 60 (41), kBack 48 (34), gradient 155
-// to 162 (106), both carries 15, sums 7; 45 would be the bytes of all.  A walk
-// that has no chunks to spread (16 lanes a channel instead of four) takes 166.
+// instructions alone): kLocal 41 (30), kOut 58 (41), kBack 47 (34), gradient 160
+// (106), both carries 15, sums 7; 45 would be the bytes of all.  With 16 lanes a
+// channel instead of four and no chunks the outputs take 166.
 #include <type_traits>
 #include <utility>
 
