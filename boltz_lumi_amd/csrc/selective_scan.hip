@@ -41,6 +41,7 @@ constexpr int kSlice = 16;        // channels that a wave of the gradient stages
 // Channels x states of a gradient block (X and dA in LDS), but at least 64 channels.  4 x 2048 tokens, 1536 channels of 16
 // states, both ways: 324 us; with 4096 368 (one block less a compute unit), with 1024 347 (more partial sums dB, dC).
 constexpr int kMaxSpan = 2048;
+constexpr int64_t kRound = 4 * 256, kGradRound = 3 * 256;  // blocks of a walk and of the gradient that the card holds
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Operand {
@@ -149,7 +150,7 @@ __device__ __forceinline__ int rev4(int j) { return (j & 1) << 3 | (j & 2) << 1 
 struct RowSum {
   float held[4];
   template <int kIndex>
-  __device__ __forceinline__ void add(float v, int lane) {  // values in the order 0 .. 15; the last leaves its sum in held[3]
+  __device__ __forceinline__ void add(float v, int lane) {  // in the order 0 .. 15; the last leaves its sum in held[3]
     level<kIndex, 0>(v, lane);
   }
   template <int kIndex, int kLevel>
@@ -444,7 +445,8 @@ __global__ __launch_bounds__(256, 4) void scan_walk_kernel(Scan s) {
 // The second pass: from each chunk's own states and the sum of its steps to what enters it, in place; forward from the
 // given state (or zeros), backward from the gradient of the last one.  A block takes 256 states one chunk after
 // another or, where they are few, 32 by eight runs of chunks: each run's own states and decay first, then from what the
-// runs before it make of `first` (3072 states, 251 chunks: 32 -> 8.5 us; 98304 states, 16 chunks: 5.5 -> 11.5, so not there).
+// runs before it make of `first` (384 channels of 8 states, 251 chunks: 32 -> 8.5 us; 98304 states, 16 chunks: 5.5 ->
+// 11.5, so not there).
 // A state after a run of tokens that decays by 2^x and adds `own`.  The power is taken in halves: a growing state (A > 0)
 // may be finite behind a run whose own power is not, and one that is zero stays so.
 __device__ __forceinline__ float after_run(float state, float x, float own) {
@@ -847,13 +849,14 @@ void with_states(int64_t states, Go go) {
 
 // Lanes of a channel where chunks are walked: four states each (of eight states two).
 constexpr int walk_lanes(int states) { return states <= 16 ? 4 : states / 4; }
+
 // Chunks of a forward call.  One where its blocks keep the card busy (a round of them takes as long with 288 as with 480;
 // us at 1536 channels of 16 states, 512 tokens, one chunk against several: 384 blocks 96 and 104, 480 97 and 139, 288 97
 // and 87) or where there is little to walk (96 tokens: 17 and 19; 128: 21 and 20).  Else about three rounds of the four
-// blocks that a compute unit holds: 2 x 4096 tokens take 111 with 3072 or 4096 blocks, 118 with 2048, 115 to 122 with
-// 1024.  Two tiles a chunk at least, as the carry is read and written per chunk (2 x 4096: 102, with one 107; 16001 x 384
-// of 8 states: 47 and 55), but one where all tiles are a round's blocks (1 x 512 x 768: 23 with two, 16 with one;
-// 1 x 2048: 31 and 27; at 1536 blocks equal).
+// blocks that a compute unit holds: 2 x 4096 tokens take 111 with three or four rounds, 118 with two, 115 to 122 with one.
+// Two tiles a chunk at least, as the carry is read and written per chunk (2 x 4096: 102, with one 107; 16001 x 384 of 8
+// states: 47 and 55), but one where all tiles are a round's blocks (1 x 512 x 768: 23 with two, 16 with one; 1 x 2048: 31
+// and 27; at 1536 blocks equal).
 struct Chunks {
   int64_t chunks, tiles;  // tiles of a chunk
 };
@@ -861,8 +864,8 @@ Chunks plan_chunks(int64_t batch, int64_t tokens, int64_t channels, int64_t stat
   const int64_t tiles = (tokens + K - 1) / K, per = 256 / walk_lanes((int)states);
   const int64_t blocks = batch * groups * ((channels / groups + per - 1) / per);
   if (blocks >= 384 || tiles <= 3) return {1, tiles};
-  const int64_t most = blocks * tiles <= 1024 ? tiles : tiles / 2;
-  int64_t chunks = (3072 + blocks - 1) / blocks;
+  const int64_t most = blocks * tiles <= kRound ? tiles : tiles / 2;
+  int64_t chunks = (3 * kRound + blocks - 1) / blocks;
   if (chunks > most) chunks = most;
   const int64_t each = (tiles + chunks - 1) / chunks;
   return {(tiles + each - 1) / each, each};
@@ -871,10 +874,9 @@ Chunks plan_chunks(int64_t batch, int64_t tokens, int64_t channels, int64_t stat
 struct Spans {
   int64_t span, spans, ranges, range_tiles, whole;
 };
-// Spans of a group's channels and ranges of tiles of the gradient's blocks: two tiles (of 32) a range where that leaves
-// four rounds of blocks at least, for half the states to carry (4 x 2048 x 1536 x 16, 1536 blocks a tile column: kernel
-// 160 us and carry 7.7 with two, 154 and 12.8 with one, both ways 325 with two and 338 with four); one where there are
-// fewer, as a wave then waits for every tile.
+// Spans of a group's channels and ranges of tiles of the gradient's blocks: two tiles (of 32) a range, for half the states
+// to carry, where that still is a round of blocks (both ways, us at 2048 tokens x 1536 channels of 16 states with two and
+// one: batch 8 655 and 690, 2 204 and 211, 1 142 and 125, as a wave then waits for every tile; with four 338 for 325).
 Spans plan_spans(int64_t batch, int64_t tokens, int64_t channels, int64_t states, int64_t groups) {
   const int64_t tiles = (tokens + K - 1) / K, group = channels / groups, unit = 4 * kSlice;
   const int64_t most = kMaxSpan / states < unit ? unit : kMaxSpan / states / unit * unit;
@@ -882,7 +884,7 @@ Spans plan_spans(int64_t batch, int64_t tokens, int64_t channels, int64_t states
   p.spans = (group + most - 1) / most;
   p.span = ((group + p.spans - 1) / p.spans + unit - 1) / unit * unit;
   p.spans = (group + p.span - 1) / p.span;
-  const int64_t m = batch * groups * p.spans * tiles >= 3072 ? 2 : 1, ranges = (tiles + m - 1) / m;
+  const int64_t m = batch * groups * p.spans * tiles >= 2 * kGradRound ? 2 : 1, ranges = (tiles + m - 1) / m;
   p.range_tiles = (tiles + ranges - 1) / ranges;
   p.ranges = (tiles + p.range_tiles - 1) / p.range_tiles;
   p.whole = p.spans == 1;
