@@ -1557,15 +1557,35 @@ def cross_attention(q, k, v, mask=None, bias=None, scale=None):
     return _cross_attention_fwd(plan, dev, q, k, v, mask, bias, scale)[0]
 
 
-def _rows3_ok(t, unit) -> bool:
-    """[B, T, C] that a kernel reads in place: a dense last axis, rows at multiples of ``unit`` elements and 16 bytes."""
-    shape, stride = t.shape, t.stride()
-    return stride[2] == 1 and all(n <= 1 or st % unit == 0 for n, st in zip(shape, stride[:2])) and t.data_ptr() % 16 == 0
+def _rows_in_place(layout, unit) -> bool:
+    """[..., C] that a kernel reads in place: a dense last axis, the others at multiples of ``unit`` elements."""
+    return layout is None or (layout[1][-1] == 1
+                              and all(n <= 1 or st % unit == 0 for n, st in zip(layout[0][:-1], layout[1][:-1])))
 
 
-def _in_place(t, unit=8):
-    """``t`` [B, T, C], copied where its layout cannot be read in place."""
-    return t if t is None or _rows3_ok(t, unit) else _aligned(t.contiguous())
+def _is_dense(layout) -> bool:
+    if layout is None or 0 in layout[0]:
+        return True
+    step = 1
+    for n, st in zip(reversed(layout[0]), reversed(layout[1])):
+        if n != 1 and st != step:
+            return False
+        step *= n
+    return True
+
+
+def _bits(*tensors) -> int:
+    """The addresses' bits, for a look at what all are aligned to."""
+    bits = 0
+    for t in tensors:
+        if t is not None:
+            bits |= t.data_ptr()
+    return bits
+
+
+def _readable(t, ok, unit=16):
+    """``t``, copied where its layout (``ok``) or its address cannot be read in place."""
+    return t if t is None or (ok and t.data_ptr() % unit == 0) else _aligned(t.contiguous())
 
 
 def _dense(t):
@@ -1610,6 +1630,8 @@ def _frame_plan(x, y, gate, y_weight, scale, weight, post_norm, pre_norm):
     strides = _steps(x[0], x[1], 2) + _steps(y[0], y[1], 2) + ([0, 0] if gate is None else _steps(gate[0], gate[1], 2))
     plan.shape, plan.strides, plan.rows = N.int64_array([b, t, d]), N.int64_array(strides), b * t
     plan.norms = int(post_norm), int(pre_norm)
+    plan.ok = tuple(_rows_in_place(m, 8) for m in (x, y, gate)) + tuple(map(_is_dense, (y_weight, scale, weight)))
+    plan.in_place = all(plan.ok)
     plan.ws = N.lib().bmx_residual_norm_workspace_bytes(b, t, d, plan.kind)
     return plan
 
@@ -1664,11 +1686,11 @@ def residual_norm(x, y, gate=None, y_weight=None, scale=None, weight=None, eps=1
     summed over its tokens); sums are fp32 and the same bits on every run."""
     dev = _same_device(x, y, gate, y_weight, scale, weight)
     _check(eps >= 2.0 ** -126, "eps must be positive, at least 2^-126")
-    _check(x.dim() == 3 and y.dim() == 3 and (gate is None or gate.dim() == 3), "expected x, y and gate of three axes")
-    x, y, gate = _in_place(x), _in_place(y), _in_place(gate)
-    y_weight, scale, weight = _dense(y_weight), _dense(scale), _dense(weight)
-    plan = _frame_plan(_layout(x), _layout(y), _layout(gate), _layout(y_weight), _layout(scale), _layout(weight),
-                       bool(post_norm), bool(pre_norm))
+    norms = bool(post_norm), bool(pre_norm)
+    plan = _frame_plan(_layout(x), _layout(y), _layout(gate), _layout(y_weight), _layout(scale), _layout(weight), *norms)
+    if not plan.in_place or _bits(x, y, gate, y_weight, scale, weight) % 16:
+        x, y, gate, y_weight, scale, weight = map(_readable, (x, y, gate, y_weight, scale, weight), plan.ok)
+        plan = _frame_plan(_layout(x), _layout(y), _layout(gate), _layout(y_weight), _layout(scale), _layout(weight), *norms)
     args = plan, dev, x, y, gate, y_weight, scale, weight, float(eps)
     r, h = (_ResidualNorm.apply if _needs_grad(x, y, gate, y_weight, scale, weight) else _residual_norm_fwd)(*args)
     return (r, h) if pre_norm else r
@@ -1723,6 +1745,8 @@ def _conv_plan(x, weight, bias, state, lengths, silu):
     lengths64 = _check_lengths(lengths, b)
     plan.head = code, N.int64_array([b, t, c, width]), N.int64_array(_steps(x[0], x[1], 2))
     plan.codes, plan.tail = (_code(weight[2]), _code(bias[2]) if bias else code), (lengths64, silu)
+    plan.ok = (_rows_in_place(x, 16 // x[2].itemsize), *map(_is_dense, (weight, bias, state)))
+    plan.in_place = all(plan.ok) and _is_dense(lengths)
     plan.state, plan.empty = (b, width - 1, c), not (b and t)
     plan.state_bytes = b * (width - 1) * c * x[2].itemsize
     plan.spans = [0 if w is None else _span(w, w[2].itemsize) for w in (x, weight, bias, lengths)]
@@ -1784,10 +1808,12 @@ def causal_conv(x, weight, bias=None, state=None, lengths=None, silu=True, retur
     bits on every run."""
     want, grad = return_state or state_out is not None, _needs_grad(x, weight, bias, state)
     dev = _same_device(x, weight, bias, state, lengths, state_out)
-    _check(x.dim() == 3, "expected x of shape [B, tokens, channels]")
-    x, weight, bias, lengths = _in_place(x, 16 // x.element_size()), _dense(weight), _dense(bias), None if lengths is None else lengths.contiguous()
-    state = _dense(state)
-    plan = _conv_plan(_layout(x), _layout(weight), _layout(bias), _layout(state), _layout(lengths), int(bool(silu)))
+    silu = int(bool(silu))
+    plan = _conv_plan(_layout(x), _layout(weight), _layout(bias), _layout(state), _layout(lengths), silu)
+    if not plan.in_place or _bits(x, weight, bias, state) % 16:
+        x, weight, bias, state = map(_readable, (x, weight, bias, state), plan.ok)
+        lengths = None if lengths is None else lengths.contiguous()
+        plan = _conv_plan(_layout(x), _layout(weight), _layout(bias), _layout(state), _layout(lengths), silu)
     if state_out is not None:
         _check_state_out(state_out, plan, x.dtype, state, (x, weight, bias, lengths), grad or _needs_grad(state_out))
     args = plan, dev, x, weight, bias, state, lengths, want, state_out
@@ -1815,9 +1841,10 @@ def _scan_plan(u, dt, A, B, C, D, z, dt_bias, state, lengths, softplus):
         _check(w is None or (w[0] == (c,) and w[2] == torch.float32), "expected D and dt_bias [channels] in fp32")
     _check(state is None or (state[0] == (b, c, states) and state[2] == torch.float32),
            "expected a state [B, channels, states] in fp32")
-    plan, unit = _Plan(), 4
-    plan.ok = tuple(m is None or (m[1][-1] == 1 and all(n <= 1 or st % unit == 0 for n, st in zip(m[0][:-1], m[1][:-1]))
-                                  and (t <= 1 or m[1][1] < MAX_SCAN_STRIDE)) for m in (u, dt, B, C, z))
+    plan = _Plan()
+    plan.ok = tuple(_rows_in_place(m, 4) and (t <= 1 or m is None or m[1][1] < MAX_SCAN_STRIDE) for m in (u, dt, B, C, z))
+    plan.dense = tuple(map(_is_dense, (A, D, dt_bias, state)))
+    plan.in_place = all(plan.ok) and all(plan.dense) and _is_dense(lengths)
     none = [0, 0]
     strides = [st for m in (u, dt) for st in _steps(m[0], m[1], 2)] + (_steps(z[0], z[1], 2) if z else none)
     strides += _steps(B[0], B[1], 3) + _steps(C[0], C[1], 3)
@@ -1826,7 +1853,7 @@ def _scan_plan(u, dt, A, B, C, D, z, dt_bias, state, lengths, softplus):
     plan.softplus, plan.state, plan.empty = softplus, (b, c, states), not (b and t)
     plan.state_bytes = b * c * states * 4
     plan.spans = [0 if w is None else _span(w, w[2].itemsize) for w in (u, dt, A, B, C, D, z, dt_bias, lengths)]
-    plan.unit = unit * (4 if code == N.F32 else 2)  # bytes
+    plan.unit = 4 * u[2].itemsize  # bytes that activations are aligned to
     plan.ws = N.lib().bmx_selective_scan_workspace_bytes(b, t, c, states, groups)
     plan.ws_bwd = N.lib().bmx_selective_scan_bwd_workspace_bytes(b, t, c, states, groups)
     plan.saved = N.lib().bmx_selective_scan_saved_bytes(b, t, c, states) // 4
@@ -1903,20 +1930,18 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, len
     tensors = u, dt, A, B, C, D, z, dt_bias, state
     want, grad = return_state or state_out is not None, _needs_grad(*tensors)
     dev = _same_device(*tensors, lengths, state_out)
-    A, D, dt_bias, state, lengths = _dense(A), _dense(D), _dense(dt_bias), _dense(state), (
-        None if lengths is None else lengths.contiguous())
-    layouts = [_layout(t) for t in (A, D, dt_bias, state, lengths)]
+    softplus = int(bool(softplus))
 
-    def plan_of(u, dt, B, C, z):
-        return _scan_plan(_layout(u), _layout(dt), layouts[0], _layout(B), _layout(C), layouts[1], _layout(z), layouts[2],
-                          layouts[3], layouts[4], int(bool(softplus)))
+    def plan_of(u, dt, A, B, C, D, z, dt_bias, state, lengths):
+        return _scan_plan(_layout(u), _layout(dt), _layout(A), _layout(B), _layout(C), _layout(D), _layout(z), _layout(dt_bias),
+                          _layout(state), _layout(lengths), softplus)
 
-    plan = plan_of(u, dt, B, C, z)
-    moved = (u, dt, B, C, z)
-    if not all(plan.ok) or any(t is not None and t.data_ptr() % plan.unit for t in moved):
-        u, dt, B, C, z = (t if t is None or (ok and t.data_ptr() % plan.unit == 0) else _aligned(t.contiguous())
-                          for ok, t in zip(plan.ok, moved))
-        plan = plan_of(u, dt, B, C, z)
+    plan = plan_of(*tensors, lengths)
+    if not plan.in_place or _bits(u, dt, B, C, z) % plan.unit or _bits(A, D, dt_bias, state) % 16:
+        u, dt, B, C, z = map(_readable, (u, dt, B, C, z), plan.ok, [plan.unit] * 5)
+        A, D, dt_bias, state = map(_readable, (A, D, dt_bias, state), plan.dense)
+        lengths = None if lengths is None else lengths.contiguous()
+        plan = plan_of(u, dt, A, B, C, D, z, dt_bias, state, lengths)
     if state_out is not None:
         _check_state_out(state_out, plan, torch.float32, state, (u, dt, A, B, C, D, z, dt_bias, lengths),
                          grad or _needs_grad(state_out))
