@@ -100,6 +100,17 @@ __device__ __forceinline__ Oct sigmoid(const Oct& x) {
   for (int i = 0; i < 4; ++i) o.a[i] = sigmoid_f(x.a[i]), o.b[i] = sigmoid_f(x.b[i]);
   return o;
 }
+// 1 - s of a gate's s = sigmoid(x), relative to itself, as a factor of s (1 - s): exp(-x) s.  Of 1 less an s that is
+// rounded to nearly 1 little or (from x = 17 on) nothing would be left.  Where exp(-x) is infinite, s is zero.
+__device__ __forceinline__ Oct shut(const Oct& x, const Oct& s) {
+  Oct o;
+  auto one = [](float x, float s) {
+    return __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(x * -1.4426950408889634f), 0.f, 0x1p126f) * s;
+  };
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o.a[i] = one(x.a[i], s.a[i]), o.b[i] = one(x.b[i], s.b[i]);
+  return o;
+}
 __device__ __forceinline__ Oct load_weight(const void* w, int w_bf16, int at) {
   if (!w) return fill(1.f);
   return w_bf16 ? load_oct((const bf16*)w + at) : load_oct((const float*)w + at);
@@ -276,9 +287,8 @@ __global__ __launch_bounds__(threads_of<L>()) void residual_norm_bwd_kernel(Fram
       float rr = 0.f, er = 0.f;
 #pragma unroll
       for (int v = 0; v < V; ++v) {
-        if (gate) g[v] = sigmoid(g[v]);
         Oct k = weight(1, v);
-        if (gate) k = k * g[v];
+        if (gate) k = k * sigmoid(g[v]);
         n[v] = n[v] * ry;
         r[v] = r[v] + n[v] * weight(0, v) * k;
         rr += dot(r[v], r[v]);
@@ -298,14 +308,14 @@ __global__ __launch_bounds__(threads_of<L>()) void residual_norm_bwd_kernel(Fram
           dw[v] = dw[v] + dh[v] * r[v] * rr;
         }
         if (s.dx && live) store_oct((X*)s.dx + row * s.dim + c, dr[v]);
-        const Oct gated = gate ? dr[v] * g[v] : dr[v];  // dR s
+        const Oct gated = gate ? dr[v] * sigmoid(g[v]) : dr[v];  // dR s
         const Oct block = gated * n[v];
         dscale[v] = dscale[v] + block * weight(0, v);
         const Oct back = gated * weight(1, v);
         dyw[v] = dyw[v] + back * n[v];
         dr[v] = back * weight(0, v);
         if (gate) {
-          const Oct dg = dr[v] * n[v] * (fill(1.f) - g[v]);
+          const Oct dg = dr[v] * n[v] * shut(g[v], sigmoid(g[v]));
           if (s.shared)
             dgate[v] = dgate[v] + dg;
           else if (s.dgate && live)
