@@ -1882,7 +1882,8 @@ class _SelectiveScan(torch.autograd.Function):
     def forward(ctx, plan, dev, u, dt, A, B, C, D, z, dt_bias, state, lengths, want_state):
         out, last, saved, raw = _selective_scan_fwd(plan, dev, u, dt, A, B, C, D, z, dt_bias, state, lengths, want_state, None,
                                                     for_backward=True)
-        ctx.save_for_backward(u, dt, A, B, C, D, z, dt_bias, state, lengths, saved, raw)
+        # not the first state, which the gradient does not read (`saved` has it): it may move on in place before then
+        ctx.save_for_backward(u, dt, A, B, C, D, z, dt_bias, lengths, saved, raw)
         ctx.rest = plan, dev
         ctx.set_materialize_grads(False)
         return out, last
@@ -1892,11 +1893,12 @@ class _SelectiveScan(torch.autograd.Function):
     def backward(ctx, dout, dlast):
         plan, dev = ctx.rest
         *tensors, lengths, saved, raw = ctx.saved_tensors
-        u, dt, A, B, C, D, z, dt_bias, _ = tensors
-        grads = _grads(ctx.needs_input_grad[2:11], tensors, plan.empty)
+        u, dt, A, B, C, D, z, dt_bias = tensors
+        grads = _grads(ctx.needs_input_grad[2:10], tensors, plan.empty)
+        grads.append(torch.empty(plan.state, device=u.device, dtype=torch.float32) if ctx.needs_input_grad[10] else None)
         if plan.empty:
-            if grads[8] is not None and dlast is not None:
-                grads[8] = dlast
+            if grads[8] is not None:
+                grads[8] = grads[8].zero_() if dlast is None else dlast
         elif any(g is not None for g in grads):
             dout, dlast = torch.zeros_like(u, memory_format=torch.contiguous_format) if dout is None else _dense(dout), _dense(dlast)
             ws = _workspace(plan.ws_bwd, u.device)
