@@ -41,7 +41,7 @@ constexpr int kSlice = 16;        // channels that a wave of the gradient stages
 // Channels x states of a gradient block (X and dA in LDS), but at least 64 channels.  4 x 2048 tokens, 1536 channels of 16
 // states, both ways: 324 us; with 4096 368 (one block less a compute unit), with 1024 347 (more partial sums dB, dC).
 constexpr int kMaxSpan = 2048;
-constexpr int64_t kRound = 4 * 256, kGradRound = 3 * 256;  // blocks of a walk and of the gradient that the card holds
+constexpr int64_t kRound = 4 * 256;  // blocks of a walk that the card holds
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Operand {
@@ -540,6 +540,25 @@ __global__ __launch_bounds__(256) void scan_step_kernel(Scan s) {
 
 // ------------------------------------------------------------------ gradient
 
+// LDS of a block in floats: four parts of a slice for each wave, or the tile's sums that meet there; the maps; and what
+// is kept for the span, of at most grad_span() channels.
+constexpr int kGradStage = 4 * 4 * kSlice * kGradRow > 256 * KG ? 4 * 4 * kSlice * kGradRow : 256 * KG;
+constexpr int grad_span(int states) {
+  constexpr int unit = 4 * kSlice;
+  return kMaxSpan / states < unit ? unit : kMaxSpan / states / unit * unit;
+}
+constexpr int grad_span_floats(int states) { return 2 * states + 4; }  // of a channel
+constexpr int grad_lds_bytes(int states) {
+  return (kGradStage + 2 * (states < 16 ? 16 : states) * kGradRow + grad_span(states) * grad_span_floats(states)) * 4;
+}
+static_assert(grad_lds_bytes(8) <= 65536 && grad_lds_bytes(16) <= 65536 && grad_lds_bytes(32) <= 65536 &&
+                  grad_lds_bytes(64) <= 65536,
+              "a launch gets no more LDS than this");
+// Blocks that the card holds: three a compute unit by their registers; by their LDS too, but two of 64 states (64512 bytes).
+constexpr int64_t grad_round(int states) {
+  return 256 * (163840 / grad_lds_bytes(states) < 3 ? 163840 / grad_lds_bytes(states) : 3);
+}
+
 // A block takes a span of a group's channels and a range of tiles; its waves take slices of 16 channels in turn, each in
 // its own part of LDS, and wait for each other only at a tile's ends.  The range's tiles go from the last to the first, X
 // handed on in LDS.  A lane has one state (of 8 states every second lane none) and, pass by pass, channel after channel:
@@ -549,8 +568,8 @@ __global__ __launch_bounds__(256) void scan_step_kernel(Scan s) {
 template <typename T, int N>
 __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
   constexpr int NP = N < 16 ? 16 : N, kSlots = 64 / NP, kPasses = kSlice / kSlots, R = kGradRow;
-  constexpr int kPart = kSlice * R, kStage = 4 * 4 * kPart, kJoin = 256 * KG;
-  __shared__ __align__(16) float lds[kStage > kJoin ? kStage : kJoin];
+  constexpr int kPart = kSlice * R;
+  __shared__ __align__(16) float lds[kGradStage];
   __shared__ __align__(16) float sB[NP * R], sC[NP * R];
   extern __shared__ __align__(16) float span_sums[];  // X [span][N], dA [span][N], dD, dbias, D and the bias [span]
   float *aX = span_sums, *aA = aX + s.span * N, *aD = aA + s.span * N, *ab = aD + s.span, *skips = ab + s.span;
@@ -876,15 +895,16 @@ struct Spans {
 };
 // Spans of a group's channels and ranges of tiles of the gradient's blocks: two tiles (of 32) a range, for half the states
 // to carry, where that still is a round of blocks (both ways, us at 2048 tokens x 1536 channels of 16 states with two and
-// one: batch 8 655 and 690, 2 204 and 211, 1 142 and 125, as a wave then waits for every tile; with four 338 for 325).
+// one: batch 8 655 and 690, 2 204 and 211, 1 142 and 125, as a wave then waits for every tile; with four 338 for 325;
+// backward, 512 channels of 64 states in 8 groups, where a round is 512 blocks: 1024 of them 160 and 170, 768 151 and 142).
 Spans plan_spans(int64_t batch, int64_t tokens, int64_t channels, int64_t states, int64_t groups) {
   const int64_t tiles = (tokens + K - 1) / K, group = channels / groups, unit = 4 * kSlice;
-  const int64_t most = kMaxSpan / states < unit ? unit : kMaxSpan / states / unit * unit;
+  const int64_t most = grad_span((int)states);
   Spans p;
   p.spans = (group + most - 1) / most;
   p.span = ((group + p.spans - 1) / p.spans + unit - 1) / unit * unit;
   p.spans = (group + p.span - 1) / p.span;
-  const int64_t m = batch * groups * p.spans * tiles >= 2 * kGradRound ? 2 : 1, ranges = (tiles + m - 1) / m;
+  const int64_t m = batch * groups * p.spans * tiles >= 2 * grad_round((int)states) ? 2 : 1, ranges = (tiles + m - 1) / m;
   p.range_tiles = (tiles + ranges - 1) / ranges;
   p.ranges = (tiles + p.range_tiles - 1) / p.range_tiles;
   p.whole = p.spans == 1;
@@ -981,7 +1001,7 @@ int gradient(Scan& s, const float* dstate_out, float* dstate, hipStream_t stream
   if (int rc = carry<true>(s, dstate_out, dstate, stream)) return rc;
   with_states(s.states, [&](auto n) {
     constexpr int N = decltype(n)::value;
-    scan_bwd_kernel<T, N><<<fold_grid(s.blocks, 256), 256, s.span * (2 * N + 4) * sizeof(float), stream>>>(s);
+    scan_bwd_kernel<T, N><<<fold_grid(s.blocks, 256), 256, s.span * grad_span_floats(N) * sizeof(float), stream>>>(s);
   });
   return check_launch("selective_scan_bwd");
 }

@@ -63,6 +63,11 @@ def test_two_tiles_a_range(gpu, n, t):
     check(12, t, 256, n, 32, FP32, lengths, gpu)
 
 
+def test_two_tiles_a_range_of_64_states(gpu):
+    """Two blocks a compute unit, so from 1024 tiles on."""
+    check(8, 100, 256, 64, 32, FP32, [100, 99, 97, 96, 64, 33, 1, 0], gpu)
+
+
 def test_two_tiles_a_range_of_several_spans(gpu):
     """Maps' gradients added over spans of channels, of two groups."""
     check(64, 130, 512, 16, 2, BF16, [130 - 2 * i for i in range(64)], gpu)
