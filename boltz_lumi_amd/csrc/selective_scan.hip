@@ -564,8 +564,9 @@ constexpr int64_t grad_round(int states) {
 // its own part of LDS, and wait for each other only at a tile's ends.  The range's tiles go from the last to the first, X
 // handed on in LDS.  A lane has one state (of 8 states every second lane none) and, pass by pass, channel after channel:
 // the sums dB, dC of its state stay in its registers over a tile, h and a of a channel over its 16 tokens.  dA, dD and the
-// bias's sums stay in LDS over the range.  Three waves a SIMD: 159 us at 4 x 2048 x 1536 x 16; two, without spills, 189,
-// four, with the sums spilled, 263.
+// bias's sums stay in LDS over the range.  Three waves a SIMD, at which a few registers are spilled (bf16 2 at 8 and 16
+// states, 12 at 32; fp32 10 and 17): 159 us at 4 x 2048 x 1536 x 16; two, without spills, 189, four, with the sums spilled,
+// 263.  Of 64 states the LDS holds two; the 28 (bf16 20) registers that three would have to spill are spilled there too.
 template <typename T, int N>
 __global__ __launch_bounds__(256, 3) void scan_bwd_kernel(Scan s) {
   constexpr int NP = N < 16 ? 16 : N, kSlots = 64 / NP, kPasses = kSlice / kSlots, R = kGradRow;
@@ -876,7 +877,9 @@ constexpr int walk_lanes(int states) { return states <= 16 ? 4 : states / 4; }
 // blocks that a compute unit holds: 2 x 4096 tokens take 111 with three or four rounds, 118 with two, 115 to 122 with one.
 // Two tiles a chunk at least, as the carry is read and written per chunk (2 x 4096: 102, with one 107; 16001 x 384 of 8
 // states: 47 and 55), but one where all tiles are a round's blocks (1 x 512 x 768: 23 with two, 16 with one; 1 x 2048: 31
-// and 27; at 1536 blocks equal).
+// and 27; at 1536 blocks equal).  Longer calls draw the same line, with a few per cent lost on it (one chunk against
+// several: 8192 tokens, 384 blocks 1483 and 1426, 480 1486 and 1851, 768 1938 and 2877; 2048 tokens 375 and 368, 375 and 483,
+// 483 and 722).
 struct Chunks {
   int64_t chunks, tiles;  // tiles of a chunk
 };

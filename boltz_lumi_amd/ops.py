@@ -1928,7 +1928,8 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, len
     Returns out, dense, in u's type; ``return_state``: (out, the last state, fp32), the next call's state.  ``state_out``:
     a dense buffer that takes it instead of a new tensor, ``state`` itself included (a decoder's step in place); without
     gradients only.  States and sums are fp32.  Gradients reach every tensor but lengths, from out and the returned state,
-    and are the same bits on every run."""
+    and are the same bits on every run.  For them a call keeps, beside its operands but the first state, N / 4 bytes for every
+    token and channel (states every 16 tokens) and with z four more (y)."""
     tensors = u, dt, A, B, C, D, z, dt_bias, state
     want, grad = return_state or state_out is not None, _needs_grad(*tensors)
     dev = _same_device(*tensors, lengths, state_out)
